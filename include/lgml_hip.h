@@ -106,6 +106,43 @@ int lgmlh_set_rows_f16(uint16_t *dst, int64_t dst_rows, int64_t row, const float
     const int64_t *ids, const int64_t *h_ids, int64_t n, void *stream);
 
 /* ===================================================================== *
+ * The KV pool in Q8_0: 8 bits a value and an f16 scale per 32 values of a head
+ * (cache types q8_0, lua/lgml/kv.lua:14-20, without its rotation of the
+ * rows), 17/32 of the f16 pool's bytes. The same blocks, cell ids, plans and
+ * bookkeeping; head sizes 64, 128 and 256. A block of one layer's K (or V) is
+ * 68 * Hkv * D bytes, blocks one after the other, so whole blocks are copied,
+ * spilled and grown as bytes. Within a (block, KV head) tile of 68 * D bytes:
+ * 64 * D int8 values, then f16 scales [D / 32][64 cells]; values of K
+ * [D / 64][cell][4][2][8] with dim 64 j + 32 b + 8 q + e at (j, cell, q, b,
+ * e), of V [D][4][2][8] with cell 32 b + 8 q + e at (d, q, b, e).
+ * ===================================================================== */
+/* Bytes of one layer's K (or V); -1 for an unsupported shape. */
+int64_t lgmlh_kv_q8_layer_bytes(int64_t n_cells, int n_head_kv, int head_dim);
+/* lgmlh_kv_store into Q8_0 pools, the rows quantized as ggml's
+ * quantize_row_q8_0 does: per 32 values d = max|x| / 127, q = x (1 / d)
+ * rounded with halves away from zero, d kept as f16. Rows are finite and below
+ * 127 * 65504 (d is f16; above it reads back as infinite). Cells of one call
+ * are distinct: a cell twice, which would mix two rows, is LGMLH_EINVAL. */
+int lgmlh_kv_store_q8(void *kpool, void *vpool, int64_t n_cells, int n_head_kv, int head_dim,
+    const float *k_src, const float *v_src, const int64_t *cells, const int64_t *h_cells,
+    int64_t n, void *stream);
+/* Read cells back as (n, Hkv*D) rows of the values d q they stand for
+ * (which = 0: K, 1: V; out_type LGMLH_F32, or LGMLH_F16 rounded to nearest
+ * even). Cells may repeat; one outside [0, n_cells) gives a row of zeros. */
+int lgmlh_kv_gather_q8(const void *pool, int which, int64_t n_cells, int n_head_kv, int head_dim,
+    const int64_t *cells, int64_t n, void *out, int out_type, void *stream);
+/* Move cells in every pool tensor at once: dst[j] takes what src[j] held
+ * before the call, for all j (a cell may be a source and a target). For the
+ * accepted tokens of a verified tree (lgmlh_plan_tree), which go to the slots
+ * behind the context. type LGMLH_F16 or LGMLH_Q8_0; pools a DEVICE array of
+ * n_pools tensor addresses, K and V of each layer in turn
+ * (lgmlh_kv_block_host's). n up to 1024; h_src and h_dst are host copies for
+ * the checks (LGMLH_ERANGE; a target twice is LGMLH_EINVAL). */
+int lgmlh_kv_move(int type, void *const *pools, int n_pools, int64_t n_cells, int n_head_kv,
+    int head_dim, const int64_t *src, const int64_t *dst, const int64_t *h_src,
+    const int64_t *h_dst, int64_t n, void *stream);
+
+/* ===================================================================== *
  * Pool bookkeeping (host): lua/lgml/kvpool.lua in C. All state lives in
  * one caller buffer of lgmlh_kvpool_bytes(blocks, size) bytes. Block ids
  * count from 0; priorities are LOW 0, NORMAL 1, HIGH 2 (kvpool.lua:25).
@@ -168,7 +205,8 @@ typedef struct {
 	/* byte offsets of the arrays inside the plan buffer */
 	int64_t off_ids, off_pos, off_cells, off_seq_off, off_npast, off_block_tab, off_logit_rows,
 	    off_items, off_merge;
-	int32_t window, ring;  /* a ring plan (lgmlh_plan_ring): window, ring blocks; else 0 */
+	int32_t window, ring;  /* a ring plan (lgmlh_plan_ring): window, ring blocks; a tree plan
+	                        * (lgmlh_plan_tree): mask words, LGMLH_PLAN_TREE; else 0 */
 	/* items [0, n_single) are query groups on their own; the rest come in
 	 * shared runs of consecutive items, {first item, count} at off_shared */
 	int32_t n_single, n_shared;
@@ -188,7 +226,7 @@ typedef struct {
 	const int32_t *logit_rows; /* [n_seq] off + n - 1 (batch_inputs :2540-2545) */
 	const int32_t *items;      /* [n_items * 4] attention work items */
 	const int32_t *merge;      /* [n_merge * 4] split-merge groups */
-	int32_t window, ring;      /* ring plans: the window and the ring's blocks; else 0 */
+	int32_t window, ring;      /* as in lgmlh_plan_info */
 	int32_t n_single, n_shared;
 	const int32_t *shared;     /* [n_shared * 2] {first item, count} of each shared run */
 	/* [n_single] the items on their own in the order the attention kernel
@@ -226,6 +264,28 @@ int lgmlh_plan_ring(int n_seq, const int32_t *seq_n, const int32_t *seq_npast,
     const int32_t *ring_tab, int ring_blocks, int64_t pool_blocks, int window, const int32_t *ids,
     int n_head, int n_head_kv, int blocks_per_split, void *buf, size_t buf_bytes,
     lgmlh_plan_info *info);
+/* The plan of a pass over drafted tokens that form a tree: several guesses of
+ * how a sequence goes on, verified at once. It has no counterpart in the
+ * reference, whose drafts are one line (lua/lgml/spec.lua:1-12).
+ * parents[t] of token t is the index, within its sequence's tokens of the
+ * pass, of the token that it follows (a smaller index), or -1 when it follows
+ * the cached context directly. Token j of sequence s is stored in the slot
+ * seq_npast[s] + j of the block table, as in lgmlh_plan, and has position
+ * seq_npast[s] + its depth (pos; rope). It sees the seq_npast[s] cached
+ * cells, the tokens it follows and itself. A line of tokens (parents[t] = j -
+ * 1) sees what lgmlh_plan's tokens see. Up to LGMLH_TREE_MAX tokens a sequence.
+ * lgmlh_paged_attention, lgmlh_paged_attention_q8 and lgmlh_forward (of models
+ * without sliding layers) take the bound plan as any other; logit_rows are the
+ * last tokens, so pass the wanted rows as out_rows. After a verification the
+ * accepted tokens' cells go to the slots behind the context with
+ * lgmlh_kv_move. info->ring is LGMLH_PLAN_TREE, info->window the 64-bit words
+ * of a token's mask (the masks stand last in the buffer).
+ * Errors: as lgmlh_plan; LGMLH_ERANGE for a parent that is no earlier token. */
+enum { LGMLH_PLAN_TREE = -1, LGMLH_TREE_MAX = 1024 };
+int lgmlh_plan_tree(int n_seq, const int32_t *seq_n, const int32_t *seq_npast,
+    const int32_t *parents, const int32_t *block_tab, int max_blocks, int64_t pool_blocks,
+    const int32_t *ids, int n_head, int n_head_kv, int blocks_per_split, void *buf,
+    size_t buf_bytes, lgmlh_plan_info *info);
 /* Device views of a plan buffer at dev (a device copy of buf). */
 int lgmlh_plan_bind(const lgmlh_plan_info *info, const void *dev, lgmlh_ubatch *ub);
 
@@ -243,6 +303,14 @@ int lgmlh_plan_bind(const lgmlh_plan_info *info, const void *dev, lgmlh_ubatch *
  * ===================================================================== */
 size_t lgmlh_attention_workspace(const lgmlh_plan_info *info, int head_dim);
 int lgmlh_paged_attention(const float *q, int n_head, int n_head_kv, int head_dim, float scale,
+    const void *kpool, const void *vpool, const lgmlh_ubatch *ub, float *out, void *workspace,
+    size_t workspace_bytes, void *stream);
+
+/* lgmlh_paged_attention over Q8_0 pools (lgmlh_kv_store_q8): the same
+ * plans, workspace and outputs, products accurate to f32 (q is not
+ * quantized). Head sizes 64, 128 and 256. Cells that a row does not see
+ * change nothing in it, whatever their bytes. */
+int lgmlh_paged_attention_q8(const float *q, int n_head, int n_head_kv, int head_dim, float scale,
     const void *kpool, const void *vpool, const lgmlh_ubatch *ub, float *out, void *workspace,
     size_t workspace_bytes, void *stream);
 
@@ -413,6 +481,21 @@ int lgmlh_geglu(const float *gu, int64_t n, int64_t F, void *out, int out_type, 
 int lgmlh_softcap(float *x, int64_t n, float cap, void *stream);
 /* Greedy id of each row: the first index of the maximum (src/sample.c:914-925). */
 int lgmlh_argmax(const float *x, int64_t n_rows, int64_t n_cols, int32_t *out, void *stream);
+
+/* Log probabilities of rows of logits (n_rows, n_cols) f32, n_cols <= 2^20
+ * (the sampler's logprobs, src/sample.c:1-1266, on the device): log p(i) = x_i -
+ * log sum_j e^x_j. id_lp (n_rows, n_ids): of the given tokens ids (n_rows,
+ * n_ids), up to 64 a row; -inf for an id outside the row. entropy (n_rows):
+ * -sum p log p, or NULL. top_ids, top_lp (n_rows, n_top): the n_top <= 64 most
+ * likely tokens and their log p, largest first, ties to the smaller id (either
+ * may be NULL). A -inf logit is a token of probability 0; a row of nothing else
+ * gives -inf, entropy 0 and the first ids. A NaN makes the row's log p and
+ * entropy NaN and ranks as -inf. The workspace (16-byte aligned) needs no
+ * initialisation. */
+size_t lgmlh_log_probs_workspace(int64_t n_rows, int64_t n_cols, int n_top);
+int lgmlh_log_probs(const float *logits, int64_t n_rows, int64_t n_cols, const int32_t *ids,
+    int n_ids, float *id_lp, float *entropy, int n_top, int32_t *top_ids, float *top_lp,
+    void *workspace, size_t ws_bytes, void *stream);
 
 /* Seeded random-init weights in a ggml layout (rows x cols of `type`,
  * F32 / Q4_K / Q6_K / Q8_0): N(mean, sd) values of tensor:fill("normal")

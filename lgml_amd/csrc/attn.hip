@@ -34,44 +34,20 @@
 
 #include <type_traits>
 
-#include "common.h"
-#include "split.h"
+#include "attn.h"
 
 namespace lgmlh {
-
-constexpr int ROWS = 16;      // MFMA rows per wave
-constexpr float LOG2E = 1.4426950408889634f;
-constexpr float ATTN_P = 32768.0f;  // the scale of P
-
-__device__ __forceinline__ f32x4 mfma16(f16x8 a, f16x8 b, f32x4 c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
-}
-
-__device__ __forceinline__ f16x8 load_f16x8(const uint16_t *p) {
-  return __builtin_bit_cast(f16x8, *(const u32x4 *)p);
-}
-
-// The cells of the S^T tiles. MFMA row r of tile ct is cell 32 (ct / 2) + 8 (r /
-// 4) + 4 (ct % 2) + r % 4 of the block: the 4 values that lane quad q holds of
-// tiles 2j and 2j + 1 are then cells 32 j + 8 q .. + 7, the B operand of the
-// second product over the V^T tile's own order of cells, and P never leaves
-// the registers. (With P through LDS and K and V fragments read as they were
-// needed, a 512-token chunk after 1024 tokens, 32 / 8 heads of 128, took 65.7
-// us; 59.6 here. 300 tokens beside 16 sequences, 8 / 4 heads of 64: 42.0 and
-// 34.6.)
-__device__ __forceinline__ int s_cell(int ct, int r) {
-  return 32 * (ct >> 1) + 8 * (r >> 2) + 4 * (ct & 1) + (r & 3);
-}
 
 // Scores of one block (scaled, in units of log2) -> P, the running max and
 // sum, and the rescale of O^T: the online softmax of a row (a lane owns one;
 // its quads hold the cells). masked: cells past p_row (RING: before the window)
-// are dropped; rows past the group hold zeros and are never stored.
+// are dropped (TREE: cells whose bit of vis is off); rows past the group hold
+// zeros and are never stored.
 typedef float f32x2 __attribute__((ext_vector_type(2)));
-template <int DT>
+template <int DT, bool TREE = false>
 __device__ __forceinline__ void softmax_block(f32x4 (&st)[4], float scale_log2, bool full,
                                               int cbase, int quad, int p_row, int p_lo, bool rvalid,
-                                              float &m, float &l, f32x4 (&o)[DT], f16x8 (&ph)[2],
+                                              uint64_t vis, float &m, float &l, f32x4 (&o)[DT], f16x8 (&ph)[2],
                                               f16x8 (&pl)[2]) {
 #pragma unroll
   for (int ct = 0; ct < 4; ct++) st[ct] *= scale_log2;
@@ -80,8 +56,12 @@ __device__ __forceinline__ void softmax_block(f32x4 (&st)[4], float scale_log2, 
     for (int ct = 0; ct < 4; ct++)
 #pragma unroll
       for (int i = 0; i < 4; i++) {
-        const int p = cbase + s_cell(ct, 4 * quad + i);
-        if (!rvalid || p > p_row || p < p_lo) st[ct][i] = -INFINITY;
+        if constexpr (TREE) {
+          if (!(vis >> s_cell(ct, 4 * quad + i) & 1)) st[ct][i] = -INFINITY;
+        } else {
+          const int p = cbase + s_cell(ct, 4 * quad + i);
+          if (!rvalid || p > p_row || p < p_lo) st[ct][i] = -INFINITY;
+        }
       }
   }
   float mx = -INFINITY;
@@ -129,179 +109,54 @@ __device__ __forceinline__ void softmax_block(f32x4 (&st)[4], float scale_log2, 
     }
 }
 
-// Partial state of one (item, kv head): O^T rows then m, l per row.
-template <int D>
-struct Partial {
-  static constexpr int floats = ROWS * D + 2 * ROWS;
-};
-
-// The Q8_K blocks of the output product's X (ggml's arithmetic) from the
-// rows of an item in one run: a block (256 values) is 256 / D heads of one
-// token, rows row .. of one row group and all four quads: value
-// (row % HB) D + 16 dt + 4 quad + i of the block. The same steps as
-// q8k_block8 (largest |x| and its first occurrence, iscale = -127 / max,
-// q = min(127, nearest-even(iscale x)), d = 1 / iscale, the 16 sums of 16
-// q); every lane takes part in the reductions, lanes of rows past the
-// item's store nothing.
-template <int D>
-__device__ __forceinline__ void finish_q8k(const f32x4 (&o)[D / 16], float l, bool rvalid,
-                                           int64_t n, int rhead, int H, int row, int quad,
-                                           f16 *__restrict__ planes, int64_t npad) {
-  constexpr int DT = D / 16, HB = 256 / D;
-  const int64_t K = (int64_t)H * D;
-  f32x4 y[DT];
-  float amax = 0.0f, mx = 0.0f;
-  int at = 1 << 30;
-  const int kb = (row % HB) * D + quad * 4;
+// The second product of a block where rows see different cells of a tree's
+// nodes and a node's V may be infinite or NaN: 0 times it would be NaN for the
+// rows that do not see it. Row by row, with the V of the cells the row does not
+// see as zeros, keeping that row's column only. Taken where a lane's V of the
+// block is not finite.
+__device__ __forceinline__ bool not_finite(f16x8 v) {
+  const u32x4 w = __builtin_bit_cast(u32x4, v);
+  bool bad = false;
 #pragma unroll
-  for (int dt = 0; dt < DT; dt++) {
-    y[dt] = o[dt] / l;
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const float a = fabsf(y[dt][i]);
-      if (a > amax) {
-        amax = a;
-        mx = y[dt][i];
-        at = kb + dt * 16 + i;
-      }
-    }
-  }
-#pragma unroll
-  for (int s = 1; s < HB; s <<= 1) q8k_amax_step(amax, mx, at, s);
-  q8k_amax_step(amax, mx, at, 16);
-  q8k_amax_step(amax, mx, at, 32);
-  const float iscale = amax == 0.0f ? 0.0f : -127.0f / mx;
-  const int64_t col = (int64_t)rhead * D + quad * 4;
-  f16 *qrow = planes + n * K;
-  f16 *bsrow = planes + q8_bs_off(npad, K) + n * (K / 16);
-#pragma unroll
-  for (int dt = 0; dt < DT; dt++) {
-    float qv[4], s = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      qv[i] = amax == 0.0f ? 0.0f : fminf(127.0f, __builtin_rintf(iscale * y[dt][i]));
-      s += qv[i];
-    }
-    s += __shfl_xor(s, 16);
-    s += __shfl_xor(s, 32);
-    if (rvalid) {
-      *(f16x4 *)(qrow + col + dt * 16) = f16x4{(f16)qv[0], (f16)qv[1], (f16)qv[2], (f16)qv[3]};
-      if (quad == 0) bsrow[(col + dt * 16) >> 4] = (f16)s;
-    }
-  }
-  if (rvalid && quad == 0 && row % HB == 0) {
-    float *dp = (float *)((char *)planes + q8_d_off(npad, K));
-    dp[n * (K / 256) + (int64_t)rhead * D / 256] = amax == 0.0f ? 0.0f : 1.0f / iscale;
-  }
+  for (int i = 0; i < 4; i++)
+    bad |= (w[i] & 0x7c00u) == 0x7c00u || (w[i] & 0x7c000000u) == 0x7c000000u;
+  return bad;
 }
-
-// The Q8_0 blocks of the output product's X (ggml's arithmetic, a Q8_0
-// output matrix) from the rows of an item in one run: block g of a head is
-// its d tiles 2g and 2g + 1, held by the row's four quads; the steps of
-// q80_block8 (d = amax / 127, q = roundf(x / d), d kept as f16).
-template <int D>
-__device__ __forceinline__ void finish_q80(const f32x4 (&o)[D / 16], float l, bool rvalid,
-                                           int64_t n, int rhead, int H, int quad,
-                                           f16 *__restrict__ planes, int64_t npad) {
-  constexpr int DT = D / 16;
-  const int64_t K = (int64_t)H * D;
-  float *dp = (float *)((char *)planes + q8_d_off(npad, K));
+// The cells 32 kc + 8 quad .. + 7 of a V fragment that row r's word leaves.
+__device__ __forceinline__ f16x8 seen_cells(f16x8 v, uint64_t word, int kc, int quad) {
+  const uint32_t bits = (uint32_t)(word >> (32 * kc + 8 * quad)) & 0xff;
 #pragma unroll
-  for (int g = 0; g < DT / 2; g++) {
-    const f32x4 y0 = o[2 * g] / l, y1 = o[2 * g + 1] / l;
-    float amax = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 4; i++) amax = fmaxf(amax, fmaxf(fabsf(y0[i]), fabsf(y1[i])));
-    amax = fmaxf(amax, __shfl_xor(amax, 16));
-    amax = fmaxf(amax, __shfl_xor(amax, 32));
-    const float dd = amax / 127.0f;
-    const float id = dd != 0.0f ? 1.0f / dd : 0.0f;
-    if (rvalid) {
-      const int64_t col = (int64_t)rhead * D + 32 * g + quad * 4;
-      f16x4 h0, h1;
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        h0[i] = (f16)__builtin_roundf(y0[i] * id);
-        h1[i] = (f16)__builtin_roundf(y1[i] * id);
-      }
-      *(f16x4 *)(planes + n * K + col) = h0;
-      *(f16x4 *)(planes + n * K + col + 16) = h1;
-      if (quad == 0) dp[n * (K / 32) + (col >> 5)] = (float)(f16)dd;
-    }
-  }
+  for (int e = 0; e < 8; e++)
+    if (!(bits >> e & 1)) v[e] = (f16)0.0f;
+  return v;
 }
-
-// The end of a work item: lane holds O^T[d = dt*16 + quad*4 + i][row].
-// A group in one run writes o / l (as the merge divides: a token's output
-// does not depend on whether its group was split) to out or, with planes,
-// to the output product's X in the form xf (split planes, or Q8_K blocks);
-// a run of a split group writes its partial state (rows in use only) for
-// the merge.
-template <int D>
-__device__ __forceinline__ void finish_item(const f32x4 (&o)[D / 16], float m, float l, int mg,
-                                            bool rvalid, int tok0, int rtok, int rhead, int ntok,
-                                            int G, int row, int quad, int item, int kvh, int Hkv,
-                                            int H, float *__restrict__ out,
-                                            f16 *__restrict__ planes, int64_t npad, int xf,
-                                            float *__restrict__ part) {
-  constexpr int DT = D / 16;
-  if (mg < 0) {
-    if constexpr (D >= 64) {
-      if (planes && xf == XF_Q8K) {  // wave-uniform
-        finish_q8k<D>(o, l, rvalid, tok0 + rtok, rhead, H, row, quad, planes, npad);
-        return;
+template <int D, typename V>
+__device__ __forceinline__ void product_by_rows(f32x4 (&o)[D / 16], const f16x8 (&ph)[2],
+                                                const f16x8 (&pl)[2], uint64_t vis, int row,
+                                                int quad, V frag) {
+#pragma unroll
+  for (int dt = 0; dt < D / 16; dt++) {
+#pragma unroll 1
+    for (int r = 0; r < ROWS; r++) {
+      const uint64_t word = __shfl(vis, r);  // lane r holds row r's
+      f32x4 acc = o[dt];
+#pragma unroll
+      for (int kc = 0; kc < 2; kc++) {
+        const f16x8 v = seen_cells(frag(dt, kc), word, kc, quad);
+        acc = mfma16(v, ph[kc], acc);
+        acc = mfma16(v, pl[kc], acc);
       }
-    }
-    if constexpr (D >= 32) {
-      if (planes && xf == XF_Q80) {
-        finish_q80<D>(o, l, rvalid, tok0 + rtok, rhead, H, quad, planes, npad);
-        return;
-      }
-    }
-    if (rvalid) {
-      const int64_t n = tok0 + rtok;
-      if (planes) {
-        // split planes of the output product's X: the lanes of a row hold
-        // 8 values of each 32-value group (d tiles 2g and 2g + 1)
-        const int64_t K = (int64_t)H * D, k0 = (int64_t)rhead * D;
-#pragma unroll
-        for (int g = 0; g < DT / 2; g++) {
-          float s = 0.0f;
-#pragma unroll
-          for (int h2 = 0; h2 < 2; h2++) {
-            const f32x4 y = o[2 * g + h2] / l;
-            const float v[4] = {y[0], y[1], y[2], y[3]};
-            split_store4(planes, npad, K, n, k0 + (2 * g + h2) * 16 + quad * 4, v);
-            s += v[0] + v[1] + v[2] + v[3];
-          }
-          s += __shfl_xor(s, 16);
-          s += __shfl_xor(s, 32);
-          if (quad == 0) split_store_gsum(planes, npad, K, n, (k0 >> 5) + g, s);
-        }
-      } else {
-        float *orow = out + (n * H + rhead) * D;
-#pragma unroll
-        for (int dt = 0; dt < DT; dt++) *(f32x4 *)(orow + dt * 16 + quad * 4) = o[dt] / l;
-      }
-    }
-    return;
-  }
-  const int nrows = ntok * G;
-  float *pp = part + ((int64_t)item * Hkv + kvh) * Partial<D>::floats;
-  if (row < nrows) {
-#pragma unroll
-    for (int dt = 0; dt < DT; dt++) *(f32x4 *)(pp + row * D + dt * 16 + quad * 4) = o[dt];
-    if (quad == 0) {
-      pp[ROWS * D + row] = m;
-      pp[ROWS * D + ROWS + row] = l;
+      if (row == r) o[dt] = acc;
     }
   }
 }
 
 // RING: a sliding-window plan. Items hold logical block ranges; logical
 // block b of sequence s is ring entry b % ring, and row position p sees
-// positions p - window + 1 .. p only.
-template <int D, bool RING>
+// positions p - window + 1 .. p only. TREE: the plan of drafted trees
+// (lgmlh_plan_tree). Blocks before npast / 64 are visible to every token; from
+// there a token sees the cells of its words in vis (vis_words a token).
+template <int D, bool RING, bool TREE = false>
 __global__ void __launch_bounds__(64, D <= 128 ? 2 : 1)
 paged_attn_kernel(const float *__restrict__ q, int H, int Hkv, float scale_log2,
                   const uint16_t *__restrict__ kpool, const uint16_t *__restrict__ vpool,
@@ -309,7 +164,8 @@ paged_attn_kernel(const float *__restrict__ q, int H, int Hkv, float scale_log2,
                   const int32_t *__restrict__ seq_npast, const int32_t *__restrict__ block_tab,
                   int max_blocks, int ring, int window, float *__restrict__ out,
                   f16 *__restrict__ planes, int64_t npad, int xf, float *__restrict__ part,
-                  const int32_t *__restrict__ order, int n_order) {
+                  const int32_t *__restrict__ order, int n_order, const uint64_t *__restrict__ vis,
+                  int vis_words) {
   // MFMA k-steps over D; a head of 16 takes one step of 32 whose upper
   // half is zero in K and Q (the lanes of quads 2 and 3 load nothing)
   constexpr int KS = D >= 32 ? D / 32 : 1;
@@ -338,6 +194,9 @@ paged_attn_kernel(const float *__restrict__ q, int H, int Hkv, float scale_log2,
   const bool rvalid = rtok < ntok;
   const int p_first = seq_npast[s] + (tok0 - seq_off[s]);
   const int p_row = p_first + rtok;  // last visible position of the row
+
+  const int b_tree = TREE ? seq_npast[s] / KV_BLOCK : 0;  // the first block that vis speaks of
+  const uint64_t *vrow = TREE ? vis + (int64_t)(tok0 + (rvalid ? rtok : 0)) * vis_words : nullptr;
 
   const int32_t *bt = block_tab + (int64_t)s * max_blocks;
   auto phys = [&](int blk) -> int64_t { return RING ? bt[blk % ring] : bt[blk]; };
@@ -435,11 +294,18 @@ paged_attn_kernel(const float *__restrict__ q, int H, int Hkv, float scale_log2,
     // window, starts inside the window of its last) is visible to every
     // valid row.
     const int cbase = blk * 64;
-    const bool full = cbase + 63 <= p_first &&
-                      (!RING || cbase > p_first + ntok - 1 - window);
+    bool full = cbase + 63 <= p_first && (!RING || cbase > p_first + ntok - 1 - window);
+    if constexpr (TREE) {
+      // every block here; not known when compiled, so that the scores are rounded
+      // before the maximum is taken off as in the other plans (a line of tokens
+      // has the bits of the causal plan)
+      int all = 1;
+      asm volatile("" : "+s"(all));
+      full = all != 0;
+    }
     f16x8 pfh[2], pfl[2];
     softmax_block<DT>(st, scale_log2, full, cbase, quad, p_row, RING ? p_row - window + 1 : 0,
-                      rvalid, m, l, o, pfh, pfl);
+                      rvalid, 0, m, l, o, pfh, pfl);
     if constexpr (!PEEL) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int dt = 0; dt < DT; dt++)
@@ -450,9 +316,57 @@ paged_attn_kernel(const float *__restrict__ q, int H, int Hkv, float scale_log2,
       }
     if constexpr (NEXT) load_v(vtile(nxt));
   };
-  for (int blk = blo; blk + (PEEL ? 1 : 0) < bhi; blk++) block(blk, std::true_type{});
+  // A block with tokens of the pass (TREE), its tiles loaded: nothing is loaded
+  // ahead, so that the tiles in flight and the rows of product_by_rows do not
+  // want registers at once. A sequence has one or two.
+  auto tree_block = [&](int blk) __attribute__((always_inline)) {
+    f32x4 st[4];
+#pragma unroll
+    for (int ct = 0; ct < 4; ct++) {
+      st[ct] = f32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int ks = 0; ks < KS; ks++) {
+        st[ct] = mfma16(kf[ct][ks], qsh[ks * 64 + lane], st[ct]);
+        st[ct] = mfma16(kf[ct][ks], qsl[ks * 64 + lane], st[ct]);
+      }
+    }
+    const uint64_t word = rvalid ? vrow[blk - b_tree] : 0;
+    f16x8 pfh[2], pfl[2];
+    softmax_block<DT, true>(st, scale_log2, false, blk * 64, quad, 0, 0, rvalid, word, m, l, o, pfh,
+                            pfl);
+    bool bad = false;
+#pragma unroll
+    for (int dt = 0; dt < DT; dt++) bad |= not_finite(vf[dt][0]) || not_finite(vf[dt][1]);
+    if (__builtin_amdgcn_ballot_w64(bad)) {
+      const uint16_t *vt = vtile(blk);  // read again: the fragments are addressed by row here
+      product_by_rows<D>(o, pfh, pfl, word, row, quad, [&](int dt, int kc) {
+        int at = (dt * 16 + row) * 64 + kc * 32 + quad * 8;
+        asm volatile("" : "+v"(at));  // made here, not ahead of the loops for every dt and kc
+        return load_f16x8(vt + at);
+      });
+    } else {
+#pragma unroll
+      for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+        for (int kc = 0; kc < 2; kc++) {
+          o[dt] = mfma16(vf[dt][kc], pfh[kc], o[dt]);
+          o[dt] = mfma16(vf[dt][kc], pfl[kc], o[dt]);
+        }
+    }
+  };
+  const int bend = TREE && b_tree < bhi ? b_tree : bhi;  // blocks from here on are a tree's
+  int blk = blo;
+  for (; blk + (PEEL && bend == bhi ? 1 : 0) < bend; blk++) block(blk, std::true_type{});
   if constexpr (PEEL)
-    if (blo < bhi) block(bhi - 1, std::false_type{});
+    if (blk < bend) block(blk, std::false_type{});
+  if constexpr (TREE)
+    for (blk = blo > b_tree ? blo : b_tree; blk < bhi; blk++) {
+      tree_block(blk);
+      if (blk + 1 < bhi) {
+        load_k(ktile(blk + 1));
+        load_v(vtile(blk + 1));
+      }
+    }
 
   finish_item<D>(o, m, l * ATTN_P, mg, rvalid, tok0, rtok, rhead, ntok, G, row, quad, item, kvh, Hkv, H,
                  out, planes, npad, xf, part);
@@ -479,7 +393,7 @@ __device__ __forceinline__ int swk(int r) {  // distinct over the 16 rows of a t
 }
 __device__ __forceinline__ int swv(int r) { return (r >> 1) & 7; }
 
-template <int D>
+template <int D, bool TREE = false>
 __global__ void __launch_bounds__(64 * SHARED_WAVES)
 paged_attn_shared_kernel(const float *__restrict__ q, int H, int Hkv, float scale_log2,
                          const uint16_t *__restrict__ kpool, const uint16_t *__restrict__ vpool,
@@ -487,7 +401,8 @@ paged_attn_shared_kernel(const float *__restrict__ q, int H, int Hkv, float scal
                          const int32_t *__restrict__ seq_off, const int32_t *__restrict__ seq_npast,
                          const int32_t *__restrict__ block_tab, int max_blocks,
                          float *__restrict__ out, f16 *__restrict__ planes, int64_t npad,
-                         int xf, float *__restrict__ part) {
+                         int xf, float *__restrict__ part, const uint64_t *__restrict__ vis,
+                         int vis_words) {
   constexpr int KS = D / 32, DT = D / 16;
   constexpr int TILE = 64 * D;             // f16 of one K (or V) tile
   constexpr int KC = D / 8;                // 16-byte chunks per K row
@@ -516,6 +431,8 @@ paged_attn_shared_kernel(const float *__restrict__ q, int H, int Hkv, float scal
   const int p_first = seq_npast[s] + (tok0 - seq_off[s]);
   const int p_row = p_first + rtok;
   const int p_last = p_first + ntok - 1;  // the wave's last position
+  const int b_tree = TREE ? seq_npast[s] / KV_BLOCK : 0;
+  const uint64_t *vrow = TREE ? vis + (int64_t)(tok0 + (rvalid ? rtok : 0)) * vis_words : nullptr;
 
   // Q fragments in registers: Q[row][ks*32 + quad*8 .. +7] as f16 hi + lo
   f16x8 qh[KS], ql[KS];
@@ -593,8 +510,25 @@ paged_attn_shared_kernel(const float *__restrict__ q, int H, int Hkv, float scal
         __builtin_amdgcn_sched_barrier(0);
       }
       f16x8 pfh[2], pfl[2];
-      softmax_block<DT>(st, scale_log2, cbase + 63 <= p_first, cbase, quad, p_row, 0, rvalid, m, l,
-                        o, pfh, pfl);
+      const bool full = TREE ? blk < b_tree : cbase + 63 <= p_first;
+      uint64_t word = 0;
+      if (TREE && !full && rvalid) word = vrow[blk - b_tree];
+      softmax_block<DT, TREE>(st, scale_log2, full, cbase, quad, p_row, 0, rvalid, word, m, l, o, pfh,
+                              pfl);
+      bool by_rows = false;
+      if constexpr (TREE) {
+        if (!full) {
+          auto frag = [&](int dt, int kc) {
+            const int r = dt * 16 + row;
+            return load_f16x8(vt + (r * 8 + ((kc * 4 + quad) ^ swv(r))) * 8);
+          };
+          bool bad = false;
+#pragma unroll 1
+          for (int dt = 0; dt < DT; dt++) bad |= not_finite(frag(dt, 0)) || not_finite(frag(dt, 1));
+          by_rows = __builtin_amdgcn_ballot_w64(bad) != 0;
+          if (by_rows) product_by_rows<D>(o, pfh, pfl, word, row, quad, frag);
+        }
+      }
       // O^T += V^T P^T, two d tiles at a time, the next two read meanwhile
       f16x8 vf[2][2][2];
       auto read_v = [&](int dt, f16x8(&f)[2][2]) __attribute__((always_inline)) {
@@ -606,20 +540,22 @@ paged_attn_shared_kernel(const float *__restrict__ q, int H, int Hkv, float scal
             f[t][kc] = load_f16x8(vt + (r * 8 + ((kc * 4 + quad) ^ swv(r))) * 8);
           }
       };
-      read_v(0, vf[0]);
+      if (!TREE || !by_rows) {
+        read_v(0, vf[0]);
 #pragma unroll
-      for (int dt = 0; dt < DT; dt += 2) {
-        const int b = dt >> 1 & 1;
-        if (dt + 2 < DT) read_v(dt + 2, vf[b ^ 1]);
-        __builtin_amdgcn_sched_barrier(0);
+        for (int dt = 0; dt < DT; dt += 2) {
+          const int b = dt >> 1 & 1;
+          if (dt + 2 < DT) read_v(dt + 2, vf[b ^ 1]);
+          __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int kc = 0; kc < 2; kc++) {
-          o[dt] = mfma16(vf[b][0][kc], pfh[kc], o[dt]);
-          o[dt + 1] = mfma16(vf[b][1][kc], pfh[kc], o[dt + 1]);
-          o[dt] = mfma16(vf[b][0][kc], pfl[kc], o[dt]);
-          o[dt + 1] = mfma16(vf[b][1][kc], pfl[kc], o[dt + 1]);
+          for (int kc = 0; kc < 2; kc++) {
+            o[dt] = mfma16(vf[b][0][kc], pfh[kc], o[dt]);
+            o[dt + 1] = mfma16(vf[b][1][kc], pfh[kc], o[dt + 1]);
+            o[dt] = mfma16(vf[b][0][kc], pfl[kc], o[dt]);
+            o[dt + 1] = mfma16(vf[b][1][kc], pfl[kc], o[dt + 1]);
+          }
+          __builtin_amdgcn_sched_barrier(0);
         }
-        __builtin_amdgcn_sched_barrier(0);
       }
     }
     __builtin_amdgcn_s_waitcnt(0);  // this wave's loads of blk + 1 have landed
@@ -780,9 +716,30 @@ extern "C" size_t lgmlh_attention_workspace(const lgmlh_plan_info *info, int hea
 }
 
 template <int D>
+static void launch_merge(const lgmlh_ubatch *ub, int H, int Hkv, const float *part, float *out,
+                         f16 *planes, int64_t npad, int xf, hipStream_t st) {
+  hipLaunchKernelGGL(merge_kernel<D>, dim3(ub->n_merge, Hkv), dim3(MERGE_THREADS), 0, st, ub->merge,
+                     H, Hkv, part, out, planes, npad, xf);
+}
+
+void lgmlh::merge_dev(int head_dim, const lgmlh_ubatch *ub, int H, int Hkv, const float *part,
+                      float *out, f16 *planes, int64_t npad, int xf, hipStream_t st) {
+  if (ub->n_merge <= 0) return;
+  switch (head_dim) {
+    case 16: launch_merge<16>(ub, H, Hkv, part, out, planes, npad, xf, st); break;
+    case 32: launch_merge<32>(ub, H, Hkv, part, out, planes, npad, xf, st); break;
+    case 64: launch_merge<64>(ub, H, Hkv, part, out, planes, npad, xf, st); break;
+    case 128: launch_merge<128>(ub, H, Hkv, part, out, planes, npad, xf, st); break;
+    case 256: launch_merge<256>(ub, H, Hkv, part, out, planes, npad, xf, st); break;
+  }
+}
+
+template <int D>
 static void launch_attn(const float *q, int H, int Hkv, float scale_log2, const void *kp,
                         const void *vp, const lgmlh_ubatch *ub, float *out, f16 *planes,
                         int64_t npad, int xf, float *part, hipStream_t st) {
+  const bool tree = ub->ring == LGMLH_PLAN_TREE;
+  const uint64_t *vis = tree ? plan_vis(ub->order, ub->n_single) : nullptr;
   // one workgroup per (item, KV head), the items on their own in the
   // plan's order
   if (ub->ring > 0)
@@ -790,25 +747,26 @@ static void launch_attn(const float *q, int H, int Hkv, float scale_log2, const 
                        dim3(64), 0, st, q, H, Hkv, scale_log2, (const uint16_t *)kp,
                        (const uint16_t *)vp, ub->items, ub->seq_off, ub->seq_npast, ub->block_tab,
                        ub->max_blocks, ub->ring, ub->window, out, planes, npad, xf, part,
-                       ub->order, ub->n_single);
+                       ub->order, ub->n_single, nullptr, 0);
   // heads of 256, and of 32 or less, run the shared runs' items with the
   // per-item kernel too
-  else if (const int n1 = D <= 128 && D >= 64 ? ub->n_single : ub->n_items; n1 > 0)
-    hipLaunchKernelGGL((paged_attn_kernel<D, false>), dim3((uint32_t)n1 * Hkv), dim3(64), 0, st,
-                       q, H, Hkv, scale_log2, (const uint16_t *)kp, (const uint16_t *)vp,
-                       ub->items, ub->seq_off, ub->seq_npast, ub->block_tab, ub->max_blocks, 0,
-                       0, out, planes, npad, xf, part, ub->order, ub->n_single);
-  if (ub->ring == 0 && ub->n_shared > 0) {
-    if constexpr (D <= 128 && D >= 64)
-      hipLaunchKernelGGL(paged_attn_shared_kernel<D>, dim3(ub->n_shared, Hkv),
-                         dim3(64 * SHARED_WAVES), 0, st, q, H, Hkv, scale_log2,
-                         (const uint16_t *)kp, (const uint16_t *)vp, ub->items, ub->shared,
-                         ub->seq_off, ub->seq_npast, ub->block_tab, ub->max_blocks, out, planes,
-                         npad, xf, part);
+  else if (const int n1 = D <= 128 && D >= 64 ? ub->n_single : ub->n_items; n1 > 0) {
+    const auto kern = tree ? paged_attn_kernel<D, false, true> : paged_attn_kernel<D, false, false>;
+    hipLaunchKernelGGL(kern, dim3((uint32_t)n1 * Hkv), dim3(64), 0, st, q, H, Hkv, scale_log2,
+                       (const uint16_t *)kp, (const uint16_t *)vp, ub->items, ub->seq_off,
+                       ub->seq_npast, ub->block_tab, ub->max_blocks, 0, 0, out, planes, npad, xf,
+                       part, ub->order, ub->n_single, vis, ub->window);
   }
-  if (ub->n_merge > 0)
-    hipLaunchKernelGGL(merge_kernel<D>, dim3(ub->n_merge, Hkv), dim3(MERGE_THREADS), 0, st, ub->merge, H,
-                       Hkv, part, out, planes, npad, xf);
+  if (ub->ring <= 0 && ub->n_shared > 0) {
+    if constexpr (D <= 128 && D >= 64) {
+      const auto kern = tree ? paged_attn_shared_kernel<D, true> : paged_attn_shared_kernel<D, false>;
+      hipLaunchKernelGGL(kern, dim3(ub->n_shared, Hkv), dim3(64 * SHARED_WAVES), 0, st, q, H, Hkv,
+                         scale_log2, (const uint16_t *)kp, (const uint16_t *)vp, ub->items,
+                         ub->shared, ub->seq_off, ub->seq_npast, ub->block_tab, ub->max_blocks, out,
+                         planes, npad, xf, part, vis, ub->window);
+    }
+  }
+  merge_dev(D, ub, H, Hkv, part, out, planes, npad, xf, st);
 }
 
 namespace lgmlh {
@@ -821,35 +779,47 @@ bool attn_q8k_fits(int head_dim, int G) {
   return head_dim >= 64 && head_dim <= 256 && G % (256 / head_dim) == 0;
 }
 
-int paged_attention_dev(const float *q, int n_head, int n_head_kv, int head_dim, float scale,
-                        const void *kpool, const void *vpool, const lgmlh_ubatch *ub, float *out,
-                        f16 *planes, int64_t npad, void *workspace, size_t workspace_bytes,
-                        hipStream_t st, int xf) {
+// The checks of an attention call (16 rows a wave); *run: there is work.
+int attn_check(const char *what, const float *q, int n_head, int n_head_kv, int head_dim,
+               const void *kpool, const void *vpool, const lgmlh_ubatch *ub, const float *out,
+               const f16 *planes, int xf, const void *workspace, size_t workspace_bytes, int *run) {
   if (!q || !kpool || !vpool || !ub || !(out || planes) || n_head_kv <= 0 ||
-      n_head % n_head_kv) {
-    set_error("paged_attention: bad arguments");
+      n_head <= 0 || n_head % n_head_kv) {
+    set_error("%s: bad arguments", what);
     return LGMLH_EINVAL;
   }
   int G = n_head / n_head_kv;
   if (G > ROWS || ROWS % G || ub->rows != ROWS || ub->n_head_kv != n_head_kv) {
-    set_error("paged_attention: %d query heads per KV head does not match the plan", G);
+    set_error("%s: %d query heads per KV head does not match the plan", what, G);
     return LGMLH_EINVAL;
   }
   size_t need = (size_t)ub->n_items * n_head_kv * (ROWS * head_dim + 2 * ROWS) * sizeof(float);
   if (ub->n_merge > 0 && (!workspace || workspace_bytes < need)) {
-    set_error("paged_attention: workspace of %zu bytes, need %zu", workspace_bytes, need);
+    set_error("%s: workspace of %zu bytes, need %zu", what, workspace_bytes, need);
     return LGMLH_ENOMEM;
   }
-  if (ub->n_items == 0) return LGMLH_OK;
+  *run = ub->n_items > 0;
+  if (!*run) return LGMLH_OK;
   if ((int64_t)ub->n_items * n_head_kv > (int64_t)1 << 25) {  // the per-item grid's threads
-    set_error("paged_attention: %d items x %d KV heads in one launch", ub->n_items, n_head_kv);
+    set_error("%s: %d items x %d KV heads in one launch", what, ub->n_items, n_head_kv);
     return LGMLH_EINVAL;
   }
   if (planes && (xf == XF_Q8K ? !attn_q8k_fits(head_dim, G) : head_dim < 32)) {
-    set_error("paged_attention: heads of %d (%d per KV head) cannot write X form %d", head_dim,
+    set_error("%s: heads of %d (%d per KV head) cannot write X form %d", what, head_dim,
               G, xf);
     return LGMLH_EINVAL;
   }
+  return LGMLH_OK;
+}
+
+int paged_attention_dev(const float *q, int n_head, int n_head_kv, int head_dim, float scale,
+                        const void *kpool, const void *vpool, const lgmlh_ubatch *ub, float *out,
+                        f16 *planes, int64_t npad, void *workspace, size_t workspace_bytes,
+                        hipStream_t st, int xf) {
+  int run = 0;
+  LGMLH_TRY(attn_check("paged_attention", q, n_head, n_head_kv, head_dim, kpool, vpool, ub, out,
+                       planes, xf, workspace, workspace_bytes, &run));
+  if (!run) return LGMLH_OK;
   float sl = scale * LOG2E;
   float *part = (float *)workspace;
   switch (head_dim) {

@@ -334,6 +334,10 @@ extern "C" int lgmlh_forward(const lgmlh_model *m, const lgmlh_ubatch *ub,
   }
   for (int il = 0; il < m->n_layer; il++) {
     const lgmlh_layer &L = m->layers[il];
+    if (L.swa && ub->ring == LGMLH_PLAN_TREE) {
+      set_error("forward: layer %d slides; a tree plan has no sliding-window form", il);
+      return LGMLH_EINVAL;
+    }
     if (L.swa && (!ub_ring || ub_ring->ring <= 0 || ub_ring->n_tokens != ub->n_tokens)) {
       set_error("forward: layer %d slides and needs the pass's ring plan", il);
       return LGMLH_EINVAL;

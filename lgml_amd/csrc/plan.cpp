@@ -22,6 +22,10 @@
 // their own are started longest run first (`order`): every item runs as
 // one wave, all at once, so the waves that share a SIMD once the SIMDs
 // are full are the shortest ones, and they end early.
+//
+// A tree plan (parents given) has the same work list over the tokens' slots
+// n_past + j, and a bit mask per token of what it sees in the blocks that hold
+// the sequence's tokens of the pass; its positions are n_past + depth.
 #include <string.h>
 
 #include <utility>
@@ -36,19 +40,23 @@ constexpr int SHARED = ATTN_SHARED;  // query groups per shared set
 using namespace lgmlh;
 
 // The plan of a pass; ring > 0 makes the sliding-window plan of
-// lgmlh_plan_ring (block_tab = the ring tables, max_blocks = ring).
+// lgmlh_plan_ring (block_tab = the ring tables, max_blocks = ring), ring =
+// LGMLH_PLAN_TREE the plan of lgmlh_plan_tree.
 static int plan_impl(int n_seq, const int32_t *seq_n, const int32_t *seq_npast,
                      const int32_t *block_tab, int max_blocks, int64_t pool_blocks,
                      const int32_t *ids, int n_head, int n_head_kv, int blocks_per_split,
-                     int window, int ring, void *buf, size_t buf_bytes, lgmlh_plan_info *info) {
+                     int window, int plan_ring, const int32_t *parents, void *buf, size_t buf_bytes, lgmlh_plan_info *info) {
   if (n_seq < 0 || !seq_n || !seq_npast || !block_tab || max_blocks <= 0 || !info ||
-      n_head_kv <= 0 || n_head % n_head_kv || n_head / n_head_kv > 16 ||
-      16 % (n_head / n_head_kv) || blocks_per_split < 0 || (ring > 0 && window < 1)) {
+      n_head_kv <= 0 || n_head <= 0 || n_head % n_head_kv || n_head / n_head_kv > 16 ||
+      16 % (n_head / n_head_kv) || blocks_per_split < 0 || (plan_ring > 0 && window < 1)) {
     set_error("plan: bad arguments");
     return LGMLH_EINVAL;
   }
+  const bool tree = plan_ring == LGMLH_PLAN_TREE;
+  const int ring = tree ? 0 : plan_ring;
   const int G = n_head / n_head_kv, T = 16 / G, B = KV_BLOCK;
   int64_t N = 0;
+  int words = 0;  // of a token's mask (tree plans)
   for (int s = 0; s < n_seq; s++) {
     if (seq_n[s] < 0 || seq_npast[s] < 0) {
       set_error("plan: negative count");
@@ -77,6 +85,20 @@ static int plan_impl(int n_seq, const int32_t *seq_n, const int32_t *seq_npast,
                   (long long)(i * B), s, b, (long long)pool_blocks);
         return LGMLH_ERANGE;
       }
+    }
+    if (tree) {
+      if (seq_n[s] > LGMLH_TREE_MAX) {
+        set_error("plan_tree: %d tokens in a tree (at most %d)", seq_n[s], LGMLH_TREE_MAX);
+        return LGMLH_EINVAL;
+      }
+      for (int j = 0; j < seq_n[s]; j++)
+        if (parents[N + j] < -1 || parents[N + j] >= j) {
+          set_error("plan_tree: token %d of sequence %d has parent %d (-1 or a token before it)",
+                    j, s, parents[N + j]);
+          return LGMLH_ERANGE;
+        }
+      const int w = (seq_npast[s] % B + seq_n[s] + B - 1) / B;
+      words = words > w ? words : w;
     }
     N += seq_n[s];
   }
@@ -158,8 +180,8 @@ static int plan_impl(int n_seq, const int32_t *seq_n, const int32_t *seq_npast,
   in.n_shared = (int32_t)counts.shared;
   in.rows = 16;
   in.n_head_kv = n_head_kv;
-  in.window = ring ? window : 0;
-  in.ring = ring;
+  in.window = ring ? window : words;
+  in.ring = plan_ring;
   int64_t o = 0;
   in.off_ids = o;          o = align16(o + 4 * N);
   in.off_pos = o;          o = align16(o + 4 * N);
@@ -172,6 +194,8 @@ static int plan_impl(int n_seq, const int32_t *seq_n, const int32_t *seq_npast,
   in.off_merge = o;        o = align16(o + 16 * (int64_t)in.n_merge);
   in.off_shared = o;       o = align16(o + 8 * (int64_t)in.n_shared);
   in.off_order = o;        o = align16(o + 4 * (int64_t)in.n_single);
+  const int64_t off_vis = o;
+  o += align16(8 * N * words);  // plan_vis
   in.bytes = o;
   *info = in;
   if (!buf) return LGMLH_OK;
@@ -185,6 +209,7 @@ static int plan_impl(int n_seq, const int32_t *seq_n, const int32_t *seq_npast,
   int64_t *pcell = (int64_t *)(b + in.off_cells);
   int32_t *psoff = (int32_t *)(b + in.off_seq_off), *pnp = (int32_t *)(b + in.off_npast);
   int32_t *plr = (int32_t *)(b + in.off_logit_rows);
+  uint64_t *pvis = (uint64_t *)(b + off_vis);
   int64_t t = 0;
   for (int s = 0; s < n_seq; s++) {
     psoff[s] = (int32_t)t;
@@ -195,6 +220,20 @@ static int plan_impl(int n_seq, const int32_t *seq_n, const int32_t *seq_npast,
       ppos[t] = p;
       const int bi = ring ? (p / B) % ring : p / B;
       pcell[t] = (int64_t)block_tab[(int64_t)s * max_blocks + bi] * B + p % B;
+      if (tree) {
+        // a token sees what its parent sees (without one the cells before
+        // the pass) and itself; it is one position after its parent
+        const int par = parents[t], slot = seq_npast[s] % B + j;
+        uint64_t *v = pvis + t * words;
+        if (par >= 0) {
+          memcpy(v, v - (int64_t)(j - par) * words, 8 * (size_t)words);
+          ppos[t] = ppos[t - (j - par)] + 1;
+        } else {
+          v[0] = ((uint64_t)1 << seq_npast[s] % B) - 1;
+          ppos[t] = seq_npast[s];
+        }
+        v[slot / B] |= (uint64_t)1 << slot % B;
+      }
     }
     plr[s] = (int32_t)t - 1;
   }
@@ -229,7 +268,20 @@ extern "C" int lgmlh_plan(int n_seq, const int32_t *seq_n, const int32_t *seq_np
                           const int32_t *ids, int n_head, int n_head_kv, int blocks_per_split,
                           void *buf, size_t buf_bytes, lgmlh_plan_info *info) {
   return plan_impl(n_seq, seq_n, seq_npast, block_tab, max_blocks, pool_blocks, ids, n_head,
-                   n_head_kv, blocks_per_split, 0, 0, buf, buf_bytes, info);
+                   n_head_kv, blocks_per_split, 0, 0, nullptr, buf, buf_bytes, info);
+}
+
+extern "C" int lgmlh_plan_tree(int n_seq, const int32_t *seq_n, const int32_t *seq_npast,
+                               const int32_t *parents, const int32_t *block_tab, int max_blocks,
+                               int64_t pool_blocks, const int32_t *ids, int n_head, int n_head_kv,
+                               int blocks_per_split, void *buf, size_t buf_bytes,
+                               lgmlh_plan_info *info) {
+  if (!parents) {
+    set_error("plan_tree: the tokens' parents are required");
+    return LGMLH_EINVAL;
+  }
+  return plan_impl(n_seq, seq_n, seq_npast, block_tab, max_blocks, pool_blocks, ids, n_head,
+                   n_head_kv, blocks_per_split, 0, LGMLH_PLAN_TREE, parents, buf, buf_bytes, info);
 }
 
 extern "C" int lgmlh_plan_ring(int n_seq, const int32_t *seq_n, const int32_t *seq_npast,
@@ -242,7 +294,7 @@ extern "C" int lgmlh_plan_ring(int n_seq, const int32_t *seq_n, const int32_t *s
     return LGMLH_EINVAL;
   }
   return plan_impl(n_seq, seq_n, seq_npast, ring_tab, ring_blocks, pool_blocks, ids, n_head,
-                   n_head_kv, blocks_per_split, window, ring_blocks, buf, buf_bytes, info);
+                   n_head_kv, blocks_per_split, window, ring_blocks, nullptr, buf, buf_bytes, info);
 }
 
 extern "C" int lgmlh_plan_bind(const lgmlh_plan_info *info, const void *dev, lgmlh_ubatch *ub) {

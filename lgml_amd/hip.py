@@ -34,7 +34,10 @@ SYMBOLS = (
     "lgmlh_moe_sum", "lgmlh_plan_ring", "lgmlh_geglu", "lgmlh_softcap",
     "lgmlh_mul_mat_noalloc_limit", "lgmlh_mul_mat_noalloc", "lgmlh_mul_mat_ggml",
     "lgmlh_mul_mat_id_ggml", "lgmlh_quantize_act", "lgmlh_forward_release",
+    "lgmlh_plan_tree", "lgmlh_paged_attention_q8", "lgmlh_kv_q8_layer_bytes", "lgmlh_kv_store_q8",
+    "lgmlh_kv_gather_q8", "lgmlh_kv_move", "lgmlh_log_probs_workspace", "lgmlh_log_probs",
 )
+PLAN_TREE, TREE_MAX = -1, 1024
 GATING_SOFTMAX, GATING_SIGMOID = 1, 2
 TRACE_ATTN, TRACE_GEMM, TRACE_EXPERTS = 1, 2, 4
 
@@ -186,6 +189,16 @@ def _declare(L):
         "lgmlh_mul_mat_id_ggml": ([i32, vp, i64, i64, i64, vp, i32, i64, vp, i64, i32, vp, vp, sz,
                                    vp], i32),
         "lgmlh_moe_sum": ([vp, vp, i64, i32, i64, vp, vp, vp], i32),
+        "lgmlh_plan_tree": ([i32, vp, vp, vp, vp, i32, i64, vp, i32, i32, i32, vp, sz,
+                             C.POINTER(PlanInfo)], i32),
+        "lgmlh_paged_attention_q8": ([vp, i32, i32, i32, C.c_float, vp, vp, C.POINTER(Ubatch), vp,
+                                      vp, sz, vp], i32),
+        "lgmlh_kv_q8_layer_bytes": ([i64, i32, i32], i64),
+        "lgmlh_kv_store_q8": ([vp, vp, i64, i32, i32, vp, vp, vp, vp, i64, vp], i32),
+        "lgmlh_kv_gather_q8": ([vp, i32, i64, i32, i32, vp, i64, vp, i32, vp], i32),
+        "lgmlh_kv_move": ([i32, vp, i32, i64, i32, i32, vp, vp, vp, vp, i64, vp], i32),
+        "lgmlh_log_probs_workspace": ([i64, i64, i32], sz),
+        "lgmlh_log_probs": ([vp, i64, i64, vp, i32, vp, vp, i32, vp, vp, vp, sz, vp], i32),
     }
     for name, (args, res) in sig.items():
         f = getattr(L, name)

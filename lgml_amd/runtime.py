@@ -124,11 +124,15 @@ class Plan:
     """A planned ubatch (lgmlh_plan), copied to the device. With ring_tab
     (n_seq, ring_blocks) and window, the plan of the sliding-window layers
     over the sequences' rings (lgmlh_plan_ring); pool_blocks is then the
-    ring pools' block count. .ring: the pass's ring plan, if any."""
+    ring pools' block count. With parents (one per token: the index within its
+    sequence's tokens of the token it follows, or -1), the plan of drafted
+    trees (lgmlh_plan_tree). .ring: the pass's ring plan, if any."""
 
     def __init__(self, seq_n, seq_npast, block_tab, ids, n_head, n_head_kv, pool_blocks,
-                 blocks_per_split=0, ring_tab=None, window=0):
+                 blocks_per_split=0, ring_tab=None, window=0, parents=None):
         L = hip.lib()
+        if ring_tab is not None and parents is not None:
+            raise ValueError("a tree plan has no sliding-window form")
         self.ring = None
         self.seq_n = np.ascontiguousarray(seq_n, np.int32)
         self.seq_npast = np.ascontiguousarray(seq_npast, np.int32)
@@ -139,7 +143,15 @@ class Plan:
         self.ids = np.ascontiguousarray(ids, np.int32)
         assert len(self.ids) == int(self.seq_n.sum())
         self.info = hip.PlanInfo()
-        if ring_tab is None:
+        if parents is not None:
+            self.parents = np.ascontiguousarray(parents, np.int32).reshape(-1)
+            if len(self.parents) != len(self.ids):
+                raise ValueError("%d parents for %d tokens" % (len(self.parents), len(self.ids)))
+            fn = L.lgmlh_plan_tree
+            args = (len(self.seq_n), ptr(self.seq_n), ptr(self.seq_npast), ptr(self.parents),
+                    ptr(bt), bt.shape[1], int(pool_blocks), ptr(self.ids), n_head, n_head_kv,
+                    blocks_per_split)
+        elif ring_tab is None:
             fn = L.lgmlh_plan
             args = (len(self.seq_n), ptr(self.seq_n), ptr(self.seq_npast), ptr(bt), bt.shape[1],
                     int(pool_blocks), ptr(self.ids), n_head, n_head_kv, blocks_per_split)
