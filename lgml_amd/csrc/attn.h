@@ -202,7 +202,14 @@ __device__ __forceinline__ void finish_item(const f32x4 (&o)[D / 16], float m, f
   }
 }
 
-// The rows that sequence tokens of a tree plan see, in the blocks that hold the
+// The chunks' places in the rows of K and V tiles in LDS (shared runs).
+template <int D>
+__device__ __forceinline__ int swk(int r) {  // distinct over the 16 rows of a tile (s_cell)
+  return D / 8 >= 16 ? (r & 3) | ((r >> 1) & 12) : ((r >> 1) & 1) | ((r >> 2) & 6);
+}
+__device__ __forceinline__ int swv(int r) { return (r >> 1) & 7; }
+
+// What sequence tokens of a tree plan see, in the blocks that hold the
 // pass's own tokens: bit c of word w of token t is cell c of block npast / 64 + w
 // (lgmlh_plan_tree). They stand behind the plan's last array.
 __host__ __device__ inline const uint64_t *plan_vis(const int32_t *order, int n_single) {

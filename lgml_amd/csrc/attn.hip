@@ -387,12 +387,6 @@ paged_attn_kernel(const float *__restrict__ q, int H, int Hkv, float scale_log2,
 // bank once.
 constexpr int SHARED_WAVES = ATTN_SHARED;
 
-template <int D>
-__device__ __forceinline__ int swk(int r) {  // distinct over the 16 rows of a tile (s_cell)
-  return D / 8 >= 16 ? (r & 3) | ((r >> 1) & 12) : ((r >> 1) & 1) | ((r >> 2) & 6);
-}
-__device__ __forceinline__ int swv(int r) { return (r >> 1) & 7; }
-
 template <int D, bool TREE = false>
 __global__ void __launch_bounds__(64 * SHARED_WAVES)
 paged_attn_shared_kernel(const float *__restrict__ q, int H, int Hkv, float scale_log2,

@@ -7,15 +7,24 @@
 // S^T. q rows are scaled by a power of two to just below 2^15, so that hi + lo
 // carries 22 bits of every element down to 2^-17 of the row's largest.
 // o_rd = sum_c (p_rc dv_cb) v8_cd, b = d / 32: dv goes into P, per block of 32
-// dims, P dv as f16 hi + lo scaled by the power of two that puts the row's
-// largest dv of the block at 2^14 to 2^15; the f32 result, scaled back, adds to
-// O^T. A cell that a row does not see has its p and dv as zeros, so that nothing
-// in it (a scale that is infinite or NaN) reaches the row.
+// dims, and P dv enters the MFMAs as f16 hi + lo, Q8_P times as large (O with it,
+// and l in the end). In a block whose cells every row sees and whose largest dv of
+// each 32 dims is in [2^-10, 4) (values of 0.12 to 500; or 0), P is split once
+// and multiplied by dv in packed f16, the product's rounding caught by an fma: hi
+// = P_hi dv, lo = P_lo dv + (P_hi dv - hi), 24 operations a lane instead of 88.
+// There hi + lo keep 22 bits of p dv down to 2^-16 of the row's largest, and below
+// are at most 2^-38 of it off. Else P dv is made in f32 and scaled by the power
+// of two that puts the row's largest dv at 2^14 to 2^15, the products scaled back
+// as they add to O^T; a cell that a row does not see has p and dv as zeros, so that
+// nothing in it (a scale that is infinite or NaN) reaches the row.
 #include <type_traits>
 
 #include "attn.h"
 
 namespace lgmlh {
+
+constexpr float Q8_P = 8192.0f;  // the scale of P
+constexpr int SHARED_MAX = ATTN_SHARED;  // the most items of a shared run
 
 __device__ __forceinline__ f32x4 mfma16q(f16x8 a, f16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
@@ -34,6 +43,9 @@ __device__ __forceinline__ f16x8 half8(uint32_t w0, uint32_t w1) {
   half4(w1, c, d);
   return f16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
+// The value is made here (else the compiler moves the sums of a block's products
+// behind its last one, and all of them wait in registers).
+__device__ __forceinline__ void here(f32x4 &v) { asm volatile("" : "+v"(v)); }
 __device__ __forceinline__ float pow2(int e) { return __builtin_amdgcn_ldexpf(1.0f, e); }
 
 template <int D>
@@ -111,19 +123,18 @@ __device__ __forceinline__ void softmax_q8(f32x4 (&st)[4], float rscale, bool ma
 }
 
 // P dv of one block of 32 dims as f16 hi + lo (cells 32 h + 8 quad + e), scaled;
-// the factor that undoes it. sc: the lane's cells' scales.
-__device__ __forceinline__ float weigh_p(const f32x4 (&st)[4], const u32x4 (&sc)[2], bool masked,
+// the factor that undoes it. s0, s1: the lane's cells' scales.
+__device__ __forceinline__ float weigh_p(const f32x4 (&st)[4], u32x4 s0, u32x4 s1, bool masked,
                                          uint64_t word, int quad, f16x8 (&ph)[2], f16x8 (&pl)[2]) {
-  f16x8 dv[2] = {__builtin_bit_cast(f16x8, sc[0]), __builtin_bit_cast(f16x8, sc[1])};
-  if (masked) {
+  if (masked) {  // wave-uniform
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-      const uint32_t bits = (uint32_t)(word >> (32 * h + 8 * quad)) & 0xff;
-#pragma unroll
-      for (int e = 0; e < 8; e++)
-        if (!(bits >> e & 1)) dv[h][e] = (f16)0.0f;
+    for (int i = 0; i < 4; i++) {
+      const uint32_t b0 = (uint32_t)(word >> (8 * quad + 2 * i)), b1 = (uint32_t)(word >> (32 + 8 * quad + 2 * i));
+      s0[i] &= (b0 & 1 ? 0xffffu : 0) | (b0 & 2 ? 0xffff0000u : 0);
+      s1[i] &= (b1 & 1 ? 0xffffu : 0) | (b1 & 2 ? 0xffff0000u : 0);
     }
   }
+  const f16x8 dv[2] = {__builtin_bit_cast(f16x8, s0), __builtin_bit_cast(f16x8, s1)};
   f16x8 big = __builtin_elementwise_max(dv[0], dv[1]);
   f16x4 b4 = __builtin_elementwise_max(f16x4{big[0], big[1], big[2], big[3]},
                                        f16x4{big[4], big[5], big[6], big[7]});
@@ -132,15 +143,95 @@ __device__ __forceinline__ float weigh_p(const f32x4 (&st)[4], const u32x4 (&sc)
   mx = fmaxf(mx, __shfl_xor(mx, 32));
   const int ex = __builtin_amdgcn_frexp_expf(mx);  // mx in [2^(ex - 1), 2^ex)
   const float up = pow2(15 - ex);
+  // hi by truncation, two at a time: lo takes up what it leaves
 #pragma unroll
   for (int h = 0; h < 2; h++)
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-      const float x = st[2 * h + (e >> 2)][e & 3] * up * (float)dv[h][e];
-      ph[h][e] = (f16)x;
-      pl[h][e] = (f16)(x - (float)ph[h][e]);
+    for (int e = 0; e < 8; e += 2) {
+      const float x0 = st[2 * h + (e >> 2)][e & 3] * up * (float)dv[h][e];
+      const float x1 = st[2 * h + (e >> 2)][(e & 3) + 1] * up * (float)dv[h][e + 1];
+      const f16x2 hi = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(x0, x1));
+      ph[h][e] = hi[0];
+      ph[h][e + 1] = hi[1];
+      pl[h][e] = (f16)fmaf((float)hi[0], -1.0f, x0);
+      pl[h][e + 1] = (f16)fmaf((float)hi[1], -1.0f, x1);
     }
   return pow2(ex - 15);
+}
+
+// Whether a lane's 8 scales of a group of 32 dims (the group's 64 in 8 aligned
+// lanes) leave the group to the packed products.
+__device__ __forceinline__ bool plain_scales(u32x4 sc) {
+  const f16x8 d = __builtin_bit_cast(f16x8, sc);
+  const f16x4 a = __builtin_elementwise_max(f16x4{d[0], d[1], d[2], d[3]}, f16x4{d[4], d[5], d[6], d[7]});
+  const float mx = group_max<8>(fmaxf(fmaxf((float)a[0], (float)a[1]), fmaxf((float)a[2], (float)a[3])));
+  return mx == 0.0f || (mx >= 0x1p-10f && mx < 4.0f);
+}
+
+// P (cells 32 h + 8 quad + e) as f16 hi + lo, Q8_P times as large.
+__device__ __forceinline__ void split_p(const f32x4 (&st)[4], f16x8 (&ph)[2], f16x8 (&pl)[2]) {
+#pragma unroll
+  for (int h = 0; h < 2; h++)
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+      const float x0 = st[2 * h + (e >> 2)][e & 3] * Q8_P, x1 = st[2 * h + (e >> 2)][(e & 3) + 1] * Q8_P;
+      const f16x2 hi = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(x0, x1));
+      ph[h][e] = hi[0];
+      ph[h][e + 1] = hi[1];
+      pl[h][e] = (f16)fmaf((float)hi[0], -1.0f, x0);
+      pl[h][e + 1] = (f16)fmaf((float)hi[1], -1.0f, x1);
+    }
+}
+
+// O^T += V^T (P dv)^T over a block. scale(b, h): the lane's cells' dv; frag(t, kc):
+// V's operand. plain: no masks, and plain_scales of all (the same for the wave).
+template <int D, typename S, typename V>
+__device__ __forceinline__ void values_q8(f32x4 (&o)[D / 16], const f32x4 (&st)[4], bool plain,
+                                          bool masked, uint64_t word, int quad, S scale, V frag) {
+  constexpr int NB = D / 32;
+  if (plain) {
+    f16x8 ph[2], pl[2];
+    split_p(st, ph, pl);
+#pragma unroll
+    for (int b = 0; b < NB; b++) {
+      f16x8 hi[2], lo[2];
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const f16x8 dv = __builtin_bit_cast(f16x8, scale(b, h));
+        hi[h] = ph[h] * dv;
+        lo[h] = __builtin_elementwise_fma(pl[h], dv, __builtin_elementwise_fma(ph[h], dv, -hi[h]));
+      }
+#pragma unroll
+      for (int t = 2 * b; t < 2 * b + 2; t++)
+#pragma unroll
+        for (int kc = 0; kc < 2; kc++) {
+          const f16x8 v = frag(t, kc);
+          o[t] = mfma16q(v, hi[kc], o[t]);
+          o[t] = mfma16q(v, lo[kc], o[t]);
+        }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    return;
+  }
+#pragma unroll
+  for (int b = 0; b < NB; b++) {
+    f16x8 ph[2], pl[2];
+    const float back = Q8_P * weigh_p(st, scale(b, 0), scale(b, 1), masked, word, quad, ph, pl);
+#pragma unroll
+    for (int t = 2 * b; t < 2 * b + 2; t++) {
+      f32x4 acc = {0, 0, 0, 0};
+#pragma unroll
+      for (int kc = 0; kc < 2; kc++) {
+        const f16x8 v = frag(t, kc);
+        acc = mfma16q(v, ph[kc], acc);
+        acc = mfma16q(v, pl[kc], acc);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; i++) o[t][i] = fmaf(acc[i], back, o[t][i]);
+      here(o[t]);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
 }
 
 // What a row (its last visible slot p_row, its token's mask words) sees of a
@@ -151,9 +242,18 @@ struct Sight {
   int b_tree;
   const uint64_t *vrow;
   bool rvalid;
-  __device__ __forceinline__ bool full(int blk) const {
-    if (ring < 0) return blk < b_tree;
-    return blk * 64 + 63 <= p_first && (ring == 0 || blk * 64 > p_last - window);
+  // Whether some row of the item does not see all of a block (the same for the
+  // wave, and for every plan that shows the rows the same cells), and the row's
+  // word then.
+  __device__ __forceinline__ bool masks(int blk, uint64_t &w) const {
+    if (ring < 0) {
+      if (blk < b_tree) return false;
+      w = word(blk);
+      return __builtin_amdgcn_ballot_w64(rvalid && ~w != 0) != 0;
+    }
+    if (blk * 64 + 63 <= p_first && (ring == 0 || blk * 64 > p_last - window)) return false;
+    w = word(blk);
+    return true;
   }
   __device__ __forceinline__ uint64_t word(int blk) const {
     if (!rvalid) return 0;
@@ -207,29 +307,41 @@ paged_attn_q8_kernel(const float *__restrict__ q, int H, int Hkv, float scale_lo
     const int64_t b = ring > 0 ? bt[blk % ring] : bt[blk];
     return pool + (b * Hkv + kvh) * (int64_t)F::TILE;
   };
-  u32x4 kq[4][J], ksc[NB][2], vq[DT], vsc[NB][2];
-  auto load_sc = [&](const uint8_t *t, u32x4(&sc)[NB][2]) {
-#pragma unroll
-    for (int b = 0; b < NB; b++)
-#pragma unroll
-      for (int h = 0; h < 2; h++)
-        sc[b][h] = *(const u32x4 *)(t + 64 * D + 2 * (b * 64 + 32 * h + 8 * quad));
-  };
+  // A block's values in registers, a lane's place in a tile being the same in
+  // all (the tile's own address stays scalar). Its scales come 16 bytes a lane and
+  // go through LDS: in registers they are 16 lanes' copies, as many as the values.
+  constexpr int SR = D > 128 ? 2 : 1;    // registers' worth: K's and V's, or K's then V's
+  constexpr int SL = D > 128 ? 64 : NB * 8;  // lanes of K's scales
+  u32x4 kq[4][J], vq[DT], sreg[SR];
+  const uint32_t koff = (8 * (row >> 2) + (row & 3)) * 64 + quad * 16, voff = row * 64 + quad * 16;
   auto load_k = [&](int blk) {
     const uint8_t *t = tile(kpool, blk);
 #pragma unroll
     for (int ct = 0; ct < 4; ct++)
 #pragma unroll
       for (int j = 0; j < J; j++)
-        kq[ct][j] = *(const u32x4 *)(t + ((j * 64 + s_cell(ct, row)) * 4 + quad) * 16);
-    load_sc(t, ksc);
+        kq[ct][j] = *(const u32x4 *)(t + (j * 4096 + s_cell(ct, 0) * 64) + koff);
   };
   auto load_v = [&](int blk) {
     const uint8_t *t = tile(vpool, blk);
 #pragma unroll
-    for (int dt = 0; dt < DT; dt++) vq[dt] = *(const u32x4 *)(t + (dt * 16 + row) * 64 + quad * 16);
-    load_sc(t, vsc);
+    for (int dt = 0; dt < DT; dt++) vq[dt] = *(const u32x4 *)(t + dt * 1024 + voff);
   };
+  auto load_s = [&](int blk) {
+    const uint8_t *k = tile(kpool, blk) + 64 * D, *v = tile(vpool, blk) + 64 * D;
+    if constexpr (SR == 2) {
+      sreg[0] = *(const u32x4 *)(k + lane * 16u);
+      sreg[1] = *(const u32x4 *)(v + lane * 16u);
+    } else {
+      sreg[0] = *(const u32x4 *)((lane < SL ? k : v) + lane % SL * 16u);
+    }
+  };
+  __shared__ __align__(16) u32x4 scl[SR * 64];  // K's scales, then V's
+  auto store_s = [&]() {
+#pragma unroll
+    for (int i = 0; i < SR; i++) scl[i * 64 + lane] = sreg[i];
+  };
+  auto scale_of = [&](int v, int b, int h) { return scl[v * SL + b * 8 + h * 4 + quad]; };
   float rscale;
   {
     const float *qr = q + ((int64_t)(tok0 + (rvalid ? rtok : ntok - 1)) * H + rhead) * D;
@@ -240,6 +352,7 @@ paged_attn_q8_kernel(const float *__restrict__ q, int H, int Hkv, float scale_lo
       qa[2 * b + 1] = *(const f32x4 *)(qr + 32 * b + 8 * quad + 4);
     }
     const int b_first = blo < bhi ? blo : 0;  // block 0 of a planned sequence is a pool block
+    load_s(b_first);
     load_k(b_first);
     load_v(b_first);
     f16x8 hi[NB], lo[NB];
@@ -259,49 +372,220 @@ paged_attn_q8_kernel(const float *__restrict__ q, int H, int Hkv, float scale_lo
     constexpr bool NEXT = decltype(next)::value;
     const int nxt = blk + 1 < bhi ? blk + 1 : blk;
     f32x4 st[4];
+    int ql_at = lane;
+    asm volatile("" : "+v"(ql_at));  // Q's operands are read anew: held, they spill others
+    // (the lanes of K's scales have no part in this)
+    const bool plain = !__builtin_amdgcn_ballot_w64(!plain_scales(sreg[SR - 1]) &&
+                                                    (SR == 2 || (lane >= SL && lane < 2 * SL)));
+    store_s();
+    if constexpr (NEXT) load_s(nxt);
 #pragma unroll
     for (int ct = 0; ct < 4; ct++) st[ct] = f32x4{0, 0, 0, 0};
 #pragma unroll
     for (int b = 0; b < NB; b++) {
-      const f16x8 qh = qsh[b * 64 + lane], ql = qsl[b * 64 + lane];
+      const f16x8 d2[2] = {__builtin_bit_cast(f16x8, scale_of(0, b, 0)),
+                           __builtin_bit_cast(f16x8, scale_of(0, b, 1))};
+      const f16x8 qh = qsh[b * 64 + ql_at], ql = qsl[b * 64 + ql_at];
 #pragma unroll
       for (int ct = 0; ct < 4; ct++) {
         const u32x4 w = kq[ct][b / 2];
         const f16x8 k = half8(w[2 * (b & 1)], w[2 * (b & 1) + 1]);
         f32x4 acc = mfma16q(k, qh, f32x4{0, 0, 0, 0});
         acc = mfma16q(k, ql, acc);
-        const f16x8 d = __builtin_bit_cast(f16x8, ksc[b][ct >> 1]);
 #pragma unroll
-        for (int i = 0; i < 4; i++) st[ct][i] = fmaf((float)d[4 * (ct & 1) + i], acc[i], st[ct][i]);
+        for (int i = 0; i < 4; i++)
+          st[ct][i] = fmaf((float)d2[ct >> 1][4 * (ct & 1) + i], acc[i], st[ct][i]);
+        here(st[ct]);
       }
+      __builtin_amdgcn_sched_barrier(0);
     }
     if constexpr (NEXT) load_k(nxt);
-    const bool masked = !see.full(blk);
-    const uint64_t word = masked ? see.word(blk) : ~(uint64_t)0;
+    uint64_t word = ~(uint64_t)0;
+    const bool masked = see.masks(blk, word);
     softmax_q8<DT>(st, rscale, masked, word, quad, m, l, o);
-#pragma unroll
-    for (int b = 0; b < NB; b++) {
-      f16x8 ph[2], pl[2];
-      const float back = weigh_p(st, vsc[b], masked, word, quad, ph, pl);
-#pragma unroll
-      for (int t = 0; t < 2; t++) {
-        const u32x4 w = vq[2 * b + t];
-        f32x4 acc = {0, 0, 0, 0};
-#pragma unroll
-        for (int kc = 0; kc < 2; kc++) {
-          const f16x8 v = half8(w[2 * kc], w[2 * kc + 1]);
-          acc = mfma16q(v, ph[kc], acc);
-          acc = mfma16q(v, pl[kc], acc);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; i++) o[2 * b + t][i] = fmaf(acc[i], back, o[2 * b + t][i]);
-      }
-    }
+    __builtin_amdgcn_sched_barrier(0);
+    values_q8<D>(o, st, plain && !masked, masked, word, quad,
+                 [&](int b, int h) { return scale_of(1, b, h); },
+                 [&](int t, int kc) { return half8(vq[t][2 * kc], vq[t][2 * kc + 1]); });
     if constexpr (NEXT) load_v(nxt);
   };
   for (int blk = blo; blk + 1 < bhi; blk++) block(blk, std::true_type{});
   if (blo < bhi) block(bhi - 1, std::false_type{});
-  finish_item<D>(o, m, l, mg, rvalid, tok0, rtok, rhead, ntok, G, row, quad, item, kvh, Hkv, H, out,
+  finish_item<D>(o, m, l * Q8_P, mg, rvalid, tok0, rtok, rhead, ntok, G, row, quad, item, kvh, Hkv, H, out,
+                 planes, npad, xf, part);
+}
+
+// Shared runs (a chunk's or a tree's query groups in sets): a workgroup of W waves
+// per (run, KV head), wave w on the run's item w of a half of the set (W = 4) or
+// of the whole (W = 8). Each block is loaded once, 16 bytes a lane, made f16 on its
+// way into LDS, and read from there by every wave, whose arithmetic is the
+// per-item kernel's: an item gives the same bits in either. The next block's
+// bytes are in flight while this one is used. Two buffers take one barrier a
+// block; where two workgroups of one buffer each share a CU (heads of 256, W =
+// 4) there are two. LDS slots of 16 B: K slot (cell, c) holds dims 8 (c ^ swk), V
+// slot (d, c) cells 8 (c ^ swv): a fragment's 16 rows touch every bank once.
+template <int D, int W>
+__global__ void __launch_bounds__(64 * W, 2)
+paged_attn_q8_shared_kernel(const float *__restrict__ q, int H, int Hkv, float scale_log2,
+                            const uint8_t *__restrict__ kpool, const uint8_t *__restrict__ vpool,
+                            const int32_t *__restrict__ items, const int32_t *__restrict__ shared,
+                            const int32_t *__restrict__ seq_off,
+                            const int32_t *__restrict__ seq_npast,
+                            const int32_t *__restrict__ block_tab, int max_blocks, int ring,
+                            int window, float *__restrict__ out, f16 *__restrict__ planes,
+                            int64_t npad, int xf, float *__restrict__ part,
+                            const uint64_t *__restrict__ vis) {
+  typedef Q8Frag<D> F;
+  constexpr int NB = F::NB, DT = F::DT, KC = D / 8;
+  constexpr int CH = D / (8 * W);           // 16-byte pieces a thread: K's 4 D, then V's
+  constexpr int BUFS = D == 256 && W == 4 ? 1 : 2;
+  constexpr int TILE = 64 * D;              // f16 of a tile
+  __shared__ __align__(16) f16 kb[BUFS][TILE], vb[BUFS][TILE];
+  __shared__ __align__(16) u32x4 scl[BUFS][2 * NB * 8];  // K's scales, then V's
+  __shared__ int odd_scales[BUFS];  // some of V's are not plain_scales
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int half = W < SHARED_MAX ? (int)blockIdx.z * W : 0;
+  const int first = shared[2 * blockIdx.x] + half, n = shared[2 * blockIdx.x + 1] - half;
+  if (n <= 0) return;  // a set of one half
+  const int kvh = blockIdx.y;
+  const int G = H / Hkv;
+  const bool active = wave < n;
+  const int item = first + (active ? wave : 0);
+  const int s = items[4 * first + 0];
+  const int blo = items[4 * first + 3] & 0xffff, bhi = (items[4 * first + 3] >> 16) & 0xffff;
+  const int tok0 = items[4 * item + 1];
+  const int ntok = items[4 * item + 2] & 31, mg = (items[4 * item + 2] >> 5) - 1;
+  const int row = lane & 15, quad = lane >> 4;
+  const int rtok = row / G, rhead = kvh * G + row % G;
+  const bool rvalid = rtok < ntok;
+  const int npast = seq_npast[s];
+  Sight see;
+  see.ring = ring;
+  see.window = window;
+  see.p_first = npast + (tok0 - seq_off[s]);
+  see.p_row = see.p_first + rtok;
+  see.p_last = see.p_first + ntok - 1;
+  see.b_tree = npast / KV_BLOCK;
+  see.vrow = ring < 0 ? vis + (int64_t)(tok0 + (rvalid ? rtok : 0)) * window : nullptr;
+  see.rvalid = rvalid;
+
+  const int32_t *bt = block_tab + (int64_t)s * max_blocks;
+  u32x4 raw[CH], sraw;
+  auto load = [&](int blk) {
+    const int64_t at = ((int64_t)bt[blk] * Hkv + kvh) * F::TILE;
+#pragma unroll
+    for (int i = 0; i < CH; i++) {
+      const int c = i * 64 * W + tid;  // a wave's pieces are K's or V's
+      raw[i] = i * 64 * W + 64 * wave < 4 * D ? *(const u32x4 *)(kpool + at + c * 16u)
+                                              : *(const u32x4 *)(vpool + at + (c - 4 * D) * 16u);
+    }
+    if (tid < NB * 16)
+      sraw = *(const u32x4 *)((tid < NB * 8 ? kpool : vpool) + at + 64 * D + tid % (NB * 8) * 16u);
+  };
+  auto store = [&](int buf) {
+#pragma unroll
+    for (int i = 0; i < CH; i++) {
+      const int c = i * 64 * W + tid;
+      const f16x8 lo = half8(raw[i][0], raw[i][1]), hi = half8(raw[i][2], raw[i][3]);
+      if (i * 64 * W + 64 * wave < 4 * D) {  // (j, cell, quad): dims of blocks 2 j and 2 j + 1
+        const int j = c >> 8, cell = c >> 2 & 63, qd = c & 3;
+        *(f16x8 *)(kb[buf] + (cell * KC + ((8 * j + qd) ^ swk<D>(cell))) * 8) = lo;
+        *(f16x8 *)(kb[buf] + (cell * KC + ((8 * j + 4 + qd) ^ swk<D>(cell))) * 8) = hi;
+      } else {  // (d, quad): cells 8 quad .. and 32 + 8 quad ..
+        const int d = (c - 4 * D) >> 2, qd = c & 3;
+        *(f16x8 *)(vb[buf] + (d * 8 + (qd ^ swv(d))) * 8) = lo;
+        *(f16x8 *)(vb[buf] + (d * 8 + ((4 + qd) ^ swv(d))) * 8) = hi;
+      }
+    }
+    if (tid < NB * 16) scl[buf][tid] = sraw;
+    // V's scales are in two waves at most (NB * 8 lanes from lane NB * 8 on)
+    if (wave == NB * 8 / 64) {
+      const bool odd = !plain_scales(sraw) && tid >= NB * 8 && tid < NB * 16;
+      const uint64_t any = __builtin_amdgcn_ballot_w64(odd);
+      if (lane == 0) odd_scales[buf] = any != 0;
+    }
+  };
+  if (blo < bhi) load(blo);
+  f16x8 qh[NB], ql[NB];
+  float rscale;
+  {
+    const float *qr = q + ((int64_t)(tok0 + (rvalid ? rtok : ntok - 1)) * H + rhead) * D;
+    f32x4 qa[2 * NB];
+#pragma unroll
+    for (int b = 0; b < NB; b++) {
+      qa[2 * b] = *(const f32x4 *)(qr + 32 * b + 8 * quad);
+      qa[2 * b + 1] = *(const f32x4 *)(qr + 32 * b + 8 * quad + 4);
+    }
+    rscale = split_q<NB>(qa, rvalid, scale_log2, qh, ql);
+  }
+  f32x4 o[DT];
+#pragma unroll
+  for (int i = 0; i < DT; i++) o[i] = f32x4{0, 0, 0, 0};
+  float m = -INFINITY, l = 0.0f;
+
+  // A lane's places in the tiles: the swizzles take from the cell and from d what
+  // only the lane's row decides, and from a block of dims its two low bits. The
+  // rest of an address is constant.
+  constexpr int KB = NB < 4 ? NB : 4;
+  int kat[KB], vat[2];
+  const int r0 = s_cell(0, row);
+#pragma unroll
+  for (int b = 0; b < KB; b++) kat[b] = (r0 * KC + ((b * 4 + quad) ^ swk<D>(r0))) * 8;
+#pragma unroll
+  for (int kc = 0; kc < 2; kc++) vat[kc] = (row * 8 + ((kc * 4 + quad) ^ swv(row))) * 8;
+
+  for (int blk = blo; blk < bhi; blk++) {
+    const int buf = BUFS == 2 ? (blk - blo) & 1 : 0;
+    if (BUFS == 1 && blk > blo) lds_sync();  // everyone is done with the buffer
+    store(buf);
+    if (blk + 1 < bhi) load(blk + 1);
+    lds_sync();
+    if (!active || blk * 64 > see.p_last) continue;
+    // places in this buffer, made here: otherwise every fragment's address is made
+    // ahead of the loop and takes a register
+    int ka[KB], va[2], sa = buf * (2 * NB * 8) + quad;
+#pragma unroll
+    for (int b = 0; b < KB; b++) {
+      ka[b] = buf * TILE + kat[b];
+      asm volatile("" : "+v"(ka[b]));
+    }
+#pragma unroll
+    for (int kc = 0; kc < 2; kc++) {
+      va[kc] = buf * TILE + vat[kc];
+      asm volatile("" : "+v"(va[kc]));
+    }
+    asm volatile("" : "+v"(sa));
+    const u32x4 *sc = scl[0] + sa;
+    f32x4 st[4];
+#pragma unroll
+    for (int ct = 0; ct < 4; ct++) st[ct] = f32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int b = 0; b < NB; b++) {
+      const f16x8 d2[2] = {__builtin_bit_cast(f16x8, sc[b * 8]), __builtin_bit_cast(f16x8, sc[b * 8 + 4])};
+#pragma unroll
+      for (int ct = 0; ct < 4; ct++) {
+        const f16x8 k = *(const f16x8 *)(kb[0] + ka[b % KB] + (s_cell(ct, 0) * KC + b / 4 * 16) * 8);
+        f32x4 acc = mfma16q(k, qh[b], f32x4{0, 0, 0, 0});
+        acc = mfma16q(k, ql[b], acc);
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+          st[ct][i] = fmaf((float)d2[ct >> 1][4 * (ct & 1) + i], acc[i], st[ct][i]);
+        here(st[ct]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    uint64_t word = ~(uint64_t)0;
+    const bool masked = see.masks(blk, word);
+    softmax_q8<DT>(st, rscale, masked, word, quad, m, l, o);
+    __builtin_amdgcn_sched_barrier(0);
+    values_q8<D>(o, st, odd_scales[buf] == 0 && !masked, masked, word, quad,
+                 [&](int b, int h) { return sc[NB * 8 + b * 8 + 4 * h]; },
+                 [&](int t, int kc) { return *(const f16x8 *)(vb[0] + va[kc] + t * 1024); });
+  }
+  if (!active) return;
+  finish_item<D>(o, m, l * Q8_P, mg, rvalid, tok0, rtok, rhead, ntok, G, row, quad, item, kvh, Hkv, H, out,
                  planes, npad, xf, part);
 }
 
@@ -311,10 +595,23 @@ static void launch_attn_q8(const float *q, int H, int Hkv, float scale_log2, con
                            int64_t npad, int xf, float *part, hipStream_t st) {
   const uint64_t *vis =
       ub->ring == LGMLH_PLAN_TREE ? plan_vis(ub->order, ub->n_single) : nullptr;
-  hipLaunchKernelGGL(paged_attn_q8_kernel<D>, dim3((uint32_t)ub->n_items * Hkv), dim3(64), 0, st, q,
-                     H, Hkv, scale_log2, (const uint8_t *)kp, (const uint8_t *)vp, ub->items,
-                     ub->seq_off, ub->seq_npast, ub->block_tab, ub->max_blocks, ub->ring, ub->window,
-                     out, planes, npad, xf, part, ub->order, ub->order ? ub->n_single : 0, vis);
+  if (ub->n_single > 0)
+    hipLaunchKernelGGL(paged_attn_q8_kernel<D>, dim3((uint32_t)ub->n_single * Hkv), dim3(64), 0, st,
+                       q, H, Hkv, scale_log2, (const uint8_t *)kp, (const uint8_t *)vp, ub->items,
+                       ub->seq_off, ub->seq_npast, ub->block_tab, ub->max_blocks, ub->ring,
+                       ub->window, out, planes, npad, xf, part, ub->order,
+                       ub->order ? ub->n_single : 0, vis);
+  if (ub->n_shared > 0) {
+    // sets of up to half a workgroup's waves on average: workgroups of half as many
+    const bool small = ub->n_items - ub->n_single <= SHARED_MAX / 2 * ub->n_shared;
+    const auto kern = small ? paged_attn_q8_shared_kernel<D, SHARED_MAX / 2>
+                            : paged_attn_q8_shared_kernel<D, SHARED_MAX>;
+    hipLaunchKernelGGL(kern, dim3(ub->n_shared, Hkv, small ? 2 : 1),
+                       dim3(64 * (small ? SHARED_MAX / 2 : SHARED_MAX)), 0, st, q, H, Hkv, scale_log2,
+                       (const uint8_t *)kp, (const uint8_t *)vp, ub->items, ub->shared, ub->seq_off,
+                       ub->seq_npast, ub->block_tab, ub->max_blocks, ub->ring, ub->window, out,
+                       planes, npad, xf, part, vis);
+  }
   merge_dev(D, ub, H, Hkv, part, out, planes, npad, xf, st);
 }
 

@@ -261,17 +261,17 @@ def test_move_takes_the_cells_as_they_were(L, q8, D, n):
 
 
 # ---- attention -------------------------------------------------------------------
-def check_attention(L, q8, H, kv, D, seq_n, npast, parents, bps, seed, q_gain=1.0, spoil=None, window=0, ring=0):
+def check_attention(L, q8, H, kv, D, seq_n, npast, parents, bps, seed, q_gain=1.0, v_gain=None, window=0, ring=0):
     rng = np.random.default_rng(seed)
     flat = None if parents is None else sum(parents, [])
     P = Pass(seq_n, npast, H, kv, flat, bps, seed, ring=ring, window=window)
     k = rng.standard_normal((P.n_cells, kv, D)).astype(np.float32)
     v = rng.standard_normal((P.n_cells, kv, D)).astype(np.float32)
     k[:, :, ::17] *= 6
+    if v_gain is not None:
+        v *= v_gain(rng, v.shape).astype(np.float32)
     q = (rng.standard_normal((sum(seq_n), H, D)) * q_gain).astype(np.float32)
     pools, kx, vx = fill(L, P, kv, D, k, v, q8)
-    if spoil is not None:
-        spoil(P, pools)
     scale = D ** -0.5
     got = run_attention(L, P, H, kv, D, scale, q, pools, q8)
     t, worst = 0, 0.0
@@ -361,6 +361,46 @@ def test_q8_attention_of_small_and_large_queries(L, gain):
             if x[h][order[-1]] - x[h][order[-2]] > 40 + np.abs(x[h]).max() * 2.0**-15:
                 want = vx[c[vis[order[-1]]], h // (H // kv)]
                 assert np.abs(got[j, h] - want).max() <= np.abs(want).max() * 2.0**-20
+
+
+GAINS = {
+    "tiny": lambda rng, s: np.full(s, 2e-5), "small": lambda rng, s: np.full(s, 2e-3),
+    "large": lambda rng, s: np.full(s, 1e3), "huge": lambda rng, s: np.full(s, 3e5),
+    "zero": lambda rng, s: np.zeros(s),
+    # some 32 dims of a head quiet, loud or 0 beside the others; some cells loud
+    "dims": lambda rng, s: np.repeat(rng.choice([0, 1e-4, 1, 1, 300], s[:2] + (s[2] // 32,)), 32, -1),
+    "cells": lambda rng, s: np.where(rng.random(s[:1] + (1, 1)) < 0.01, 1e4, 1.0) * np.ones(s),
+}
+
+
+@pytest.mark.parametrize("gain", list(GAINS))
+@pytest.mark.parametrize("H,kv,D", [(8, 2, 64), (8, 2, 128), (8, 4, 256)])
+def test_q8_attention_of_small_and_large_values(L, gain, H, kv, D):
+    """V's scales inside and outside the range of the packed products, in one
+    pass of decoding sequences, a chunk (shared runs) and long contexts. Quiet
+    dims are held to their own size: each 32 dims of a head by itself."""
+    seq_n, npast = [1, 40, 1], [500, 70, 64]
+    rng = np.random.default_rng(77)
+    P = Pass(seq_n, npast, H, kv, None, 3, 77)
+    k = rng.standard_normal((P.n_cells, kv, D)).astype(np.float32)
+    v = rng.standard_normal((P.n_cells, kv, D)).astype(np.float32)
+    v = (v * GAINS[gain](rng, v.shape)).astype(np.float32)
+    q = rng.standard_normal((sum(seq_n), H, D)).astype(np.float32)
+    pools, kx, vx = fill(L, P, kv, D, k, v, True)
+    got = run_attention(L, P, H, kv, D, D ** -0.5, q, pools, True)
+    t = 0
+    for s, (n, p0) in enumerate(zip(seq_n, npast)):
+        c = P.cells(s)
+        for j in range(n):
+            vis = list(range(p0 + j + 1))
+            qt = q[t].astype(np.float64)
+            want = attend(qt, kx[c], vx[c], D ** -0.5, vis)
+            for b in range(D // 32):
+                part = vx[c][vis][:, :, 32 * b:32 * b + 32]
+                tol = bound(qt, kx[c][vis], part, D ** -0.5, len(vis))
+                err = np.abs(got[t] - want)[:, 32 * b:32 * b + 32].max()
+                assert err <= tol, (s, j, b, err, tol)
+            t += 1
 
 
 def spoil_cells(q8, kv, D, which_cells):
