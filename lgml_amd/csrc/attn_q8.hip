@@ -183,6 +183,44 @@ __device__ __forceinline__ void split_p(const f32x4 (&st)[4], f16x8 (&ph)[2], f1
     }
 }
 
+// S^T of a block: read(b, p, k, d) gives the K operands of tiles 2 p and 2 p + 1
+// and the lane's cells' dk for block b of dims, query(b, hi, lo) the row's. A step
+// reads the next step's operands and issues this one's products, and adds the
+// last one's, scaled, while they run. (Two tiles a step: with four, heads of 256
+// spill, and each spill is waited for.)
+template <int NB, typename R, typename Q>
+__device__ __forceinline__ void scores_q8(f32x4 (&st)[4], R read, Q query) {
+  f16x8 k[2][2], d[2], hi, lo;
+  f32x4 acc[2][2];
+#pragma unroll
+  for (int ct = 0; ct < 4; ct++) st[ct] = f32x4{0, 0, 0, 0};
+  read(0, 0, k[0], d[0]);
+  auto add = [&](int p) {
+#pragma unroll
+    for (int t = 0; t < 2; t++) {
+      f32x4 &s = st[2 * p + t];
+#pragma unroll
+      for (int i = 0; i < 4; i++) s[i] = fmaf((float)d[p][4 * t + i], acc[p][t][i], s[i]);
+      here(s);
+    }
+  };
+#pragma unroll
+  for (int b = 0; b < NB; b++) {
+    query(b, hi, lo);
+#pragma unroll
+    for (int p = 0; p < 2; p++) {
+#pragma unroll
+      for (int t = 0; t < 2; t++) acc[p][t] = mfma16q(k[p][t], hi, f32x4{0, 0, 0, 0});
+#pragma unroll
+      for (int t = 0; t < 2; t++) acc[p][t] = mfma16q(k[p][t], lo, acc[p][t]);
+      if (b + p > 0) add(p ^ 1);
+      if (p == 0 || b + 1 < NB) read(b + p, p ^ 1, k[p ^ 1], d[p ^ 1]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+  add(1);
+}
+
 // O^T += V^T (P dv)^T over a block. scale(b, h): the lane's cells' dv; frag(t, kc):
 // V's operand. plain: no masks, and plain_scales of all (the same for the wave).
 template <int D, typename S, typename V>
@@ -190,25 +228,35 @@ __device__ __forceinline__ void values_q8(f32x4 (&o)[D / 16], const f32x4 (&st)[
                                           bool masked, uint64_t word, int quad, S scale, V frag) {
   constexpr int NB = D / 32;
   if (plain) {
-    f16x8 ph[2], pl[2];
+    // a step reads the next 16 dims' V (and makes the next block's P dv) while
+    // the products of this one run
+    f16x8 ph[2], pl[2], hi[2][2], lo[2][2], v[2][2];
     split_p(st, ph, pl);
+    auto fetch = [&](int t) {
 #pragma unroll
-    for (int b = 0; b < NB; b++) {
-      f16x8 hi[2], lo[2];
+      for (int kc = 0; kc < 2; kc++) v[t & 1][kc] = frag(t, kc);
+    };
+    auto weigh = [&](int b) {
 #pragma unroll
       for (int h = 0; h < 2; h++) {
         const f16x8 dv = __builtin_bit_cast(f16x8, scale(b, h));
-        hi[h] = ph[h] * dv;
-        lo[h] = __builtin_elementwise_fma(pl[h], dv, __builtin_elementwise_fma(ph[h], dv, -hi[h]));
+        f16x8 &x = hi[b & 1][h];
+        x = ph[h] * dv;
+        lo[b & 1][h] = __builtin_elementwise_fma(pl[h], dv, __builtin_elementwise_fma(ph[h], dv, -x));
       }
+    };
+    fetch(0);
+    weigh(0);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int t = 2 * b; t < 2 * b + 2; t++)
+    for (int t = 0; t < D / 16; t++) {
 #pragma unroll
-        for (int kc = 0; kc < 2; kc++) {
-          const f16x8 v = frag(t, kc);
-          o[t] = mfma16q(v, hi[kc], o[t]);
-          o[t] = mfma16q(v, lo[kc], o[t]);
-        }
+      for (int kc = 0; kc < 2; kc++) {
+        o[t] = mfma16q(v[t & 1][kc], hi[t >> 1 & 1][kc], o[t]);
+        o[t] = mfma16q(v[t & 1][kc], lo[t >> 1 & 1][kc], o[t]);
+      }
+      if (t + 1 < D / 16) fetch(t + 1);
+      if (t % 2 == 0 && t / 2 + 1 < NB) weigh(t / 2 + 1);
       __builtin_amdgcn_sched_barrier(0);
     }
     return;
@@ -379,26 +427,20 @@ paged_attn_q8_kernel(const float *__restrict__ q, int H, int Hkv, float scale_lo
                                                     (SR == 2 || (lane >= SL && lane < 2 * SL)));
     store_s();
     if constexpr (NEXT) load_s(nxt);
+    scores_q8<NB>(
+        st,
+        [&](int b, int p, f16x8(&k)[2], f16x8 &d) {
 #pragma unroll
-    for (int ct = 0; ct < 4; ct++) st[ct] = f32x4{0, 0, 0, 0};
-#pragma unroll
-    for (int b = 0; b < NB; b++) {
-      const f16x8 d2[2] = {__builtin_bit_cast(f16x8, scale_of(0, b, 0)),
-                           __builtin_bit_cast(f16x8, scale_of(0, b, 1))};
-      const f16x8 qh = qsh[b * 64 + ql_at], ql = qsl[b * 64 + ql_at];
-#pragma unroll
-      for (int ct = 0; ct < 4; ct++) {
-        const u32x4 w = kq[ct][b / 2];
-        const f16x8 k = half8(w[2 * (b & 1)], w[2 * (b & 1) + 1]);
-        f32x4 acc = mfma16q(k, qh, f32x4{0, 0, 0, 0});
-        acc = mfma16q(k, ql, acc);
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-          st[ct][i] = fmaf((float)d2[ct >> 1][4 * (ct & 1) + i], acc[i], st[ct][i]);
-        here(st[ct]);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-    }
+          for (int t = 0; t < 2; t++) {
+            const u32x4 w = kq[2 * p + t][b / 2];
+            k[t] = half8(w[2 * (b & 1)], w[2 * (b & 1) + 1]);
+          }
+          d = __builtin_bit_cast(f16x8, scale_of(0, b, p));
+        },
+        [&](int b, f16x8 &hi, f16x8 &lo) {
+          hi = qsh[b * 64 + ql_at];
+          lo = qsl[b * 64 + ql_at];
+        });
     if constexpr (NEXT) load_k(nxt);
     uint64_t word = ~(uint64_t)0;
     const bool masked = see.masks(blk, word);
@@ -559,23 +601,18 @@ paged_attn_q8_shared_kernel(const float *__restrict__ q, int H, int Hkv, float s
     asm volatile("" : "+v"(sa));
     const u32x4 *sc = scl[0] + sa;
     f32x4 st[4];
+    scores_q8<NB>(
+        st,
+        [&](int b, int p, f16x8(&k)[2], f16x8 &d) {
 #pragma unroll
-    for (int ct = 0; ct < 4; ct++) st[ct] = f32x4{0, 0, 0, 0};
-#pragma unroll
-    for (int b = 0; b < NB; b++) {
-      const f16x8 d2[2] = {__builtin_bit_cast(f16x8, sc[b * 8]), __builtin_bit_cast(f16x8, sc[b * 8 + 4])};
-#pragma unroll
-      for (int ct = 0; ct < 4; ct++) {
-        const f16x8 k = *(const f16x8 *)(kb[0] + ka[b % KB] + (s_cell(ct, 0) * KC + b / 4 * 16) * 8);
-        f32x4 acc = mfma16q(k, qh[b], f32x4{0, 0, 0, 0});
-        acc = mfma16q(k, ql[b], acc);
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-          st[ct][i] = fmaf((float)d2[ct >> 1][4 * (ct & 1) + i], acc[i], st[ct][i]);
-        here(st[ct]);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-    }
+          for (int t = 0; t < 2; t++)
+            k[t] = *(const f16x8 *)(kb[0] + ka[b % KB] + (s_cell(2 * p + t, 0) * KC + b / 4 * 16) * 8);
+          d = __builtin_bit_cast(f16x8, sc[b * 8 + 4 * p]);
+        },
+        [&](int b, f16x8 &hi, f16x8 &lo) {
+          hi = qh[b];
+          lo = ql[b];
+        });
     uint64_t word = ~(uint64_t)0;
     const bool masked = see.masks(blk, word);
     softmax_q8<DT>(st, rscale, masked, word, quad, m, l, o);
