@@ -377,7 +377,9 @@ paged_attn_kernel(const float *__restrict__ q, int H, int Hkv, float scale_log2,
 // first + w (w < n). Each K / V block of the run is loaded once into LDS
 // (global-to-LDS, the next block's loads in flight while this one is
 // used) and every wave reads its MFMA fragments from there: the context
-// of a chunk is read once per set instead of once per group. The
+// of a chunk is read once per set instead of once per group. (W waves: a tree
+// plan's sets of up to half as many items take workgroups of half as many
+// waves, two to a CU; a larger set then takes two.) The
 // arithmetic of a wave is the per-item kernel's (same fragments, same
 // order), so an item gives the same bits in either kernel. A block past a
 // wave's last position is skipped (it would add nothing).
@@ -387,8 +389,8 @@ paged_attn_kernel(const float *__restrict__ q, int H, int Hkv, float scale_log2,
 // bank once.
 constexpr int SHARED_WAVES = ATTN_SHARED;
 
-template <int D, bool TREE = false>
-__global__ void __launch_bounds__(64 * SHARED_WAVES)
+template <int D, bool TREE = false, int W = SHARED_WAVES>
+__global__ void __launch_bounds__(64 * W, 2)
 paged_attn_shared_kernel(const float *__restrict__ q, int H, int Hkv, float scale_log2,
                          const uint16_t *__restrict__ kpool, const uint16_t *__restrict__ vpool,
                          const int32_t *__restrict__ items, const int32_t *__restrict__ shared,
@@ -400,13 +402,15 @@ paged_attn_shared_kernel(const float *__restrict__ q, int H, int Hkv, float scal
   constexpr int KS = D / 32, DT = D / 16;
   constexpr int TILE = 64 * D;             // f16 of one K (or V) tile
   constexpr int KC = D / 8;                // 16-byte chunks per K row
-  constexpr int LOADS = TILE / 8 / (64 * SHARED_WAVES);  // per lane and tile
+  constexpr int LOADS = TILE / 8 / (64 * W);  // per lane and tile
   __shared__ __align__(16) uint16_t kb0[TILE], kb1[TILE], vb0[TILE], vb1[TILE];
   typedef __attribute__((address_space(3))) void lds_t;
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int first = shared[2 * blockIdx.x], n = shared[2 * blockIdx.x + 1];
+  const int half = W < SHARED_WAVES ? (int)blockIdx.z * W : 0;
+  const int first = shared[2 * blockIdx.x] + half, n = shared[2 * blockIdx.x + 1] - half;
+  if (W < SHARED_WAVES && n <= 0) return;  // a set of one half
   const int kvh = blockIdx.y;
   const int G = H / Hkv;
   const bool active = wave < n;
@@ -454,13 +458,13 @@ paged_attn_shared_kernel(const float *__restrict__ q, int H, int Hkv, float scal
 
   const int32_t *bt = block_tab + (int64_t)s * max_blocks;
   // Global-to-LDS loads of block blk into buffer buf: load j of this lane
-  // fills slot (j * SHARED_WAVES + wave) * 64 + lane of each tile.
+  // fills slot (j * W + wave) * 64 + lane of each tile.
   auto load = [&](int blk, int buf) {
     const int64_t base = ((int64_t)bt[blk] * Hkv + kvh) * TILE;
     uint16_t *kd = buf ? kb1 : kb0, *vd = buf ? vb1 : vb0;
 #pragma unroll
     for (int j = 0; j < LOADS; j++) {
-      const int slot0 = (j * SHARED_WAVES + wave) * 64, sl = slot0 + lane;
+      const int slot0 = (j * W + wave) * 64, sl = slot0 + lane;
       const int kr = sl / KC, kc = (sl % KC) ^ swk<D>(sl / KC);
       const int vr = sl / 8, vc = (sl % 8) ^ swv(sl / 8);
       __builtin_amdgcn_global_load_lds((const void *)(kpool + base + kr * D + kc * 8),
@@ -514,7 +518,9 @@ paged_attn_shared_kernel(const float *__restrict__ q, int H, int Hkv, float scal
         if (!full) {
           auto frag = [&](int dt, int kc) {
             const int r = dt * 16 + row;
-            return load_f16x8(vt + (r * 8 + ((kc * 4 + quad) ^ swv(r))) * 8);
+            int at = (r * 8 + ((kc * 4 + quad) ^ swv(r))) * 8;
+            asm volatile("" : "+v"(at));  // made here, not ahead of the loops
+            return load_f16x8(vt + at);
           };
           bool bad = false;
 #pragma unroll 1
@@ -567,13 +573,14 @@ paged_attn_shared_kernel(const float *__restrict__ q, int H, int Hkv, float scal
 // outputs with the m and l of the position's row, and finds the row's max
 // M, the split weights w = exp2(m - M) and L = sum l w itself (the threads
 // of a row agree), adding the outputs weighted, in split order. A merge of
-// up to SC splits is one round trip.
+// up to SC splits is one round trip; with 4 or fewer SC is 4, else 16 (the loads
+// past the last split repeat it).
 constexpr int MERGE_THREADS = 256;
-template <int D>
-__global__ void __launch_bounds__(MERGE_THREADS)
-merge_kernel(const int32_t *__restrict__ merge, int H, int Hkv, const float *__restrict__ part,
-             float *__restrict__ out, f16 *__restrict__ planes, int64_t npad, int xf) {
-  constexpr int SC = 16, MT = MERGE_THREADS;  // splits per load round
+template <int D, int SC>
+__device__ __forceinline__ void merge_group(const int32_t *__restrict__ merge, int H, int Hkv,
+                                            const float *__restrict__ part, float *__restrict__ out,
+                                            f16 *__restrict__ planes, int64_t npad, int xf) {
+  constexpr int MT = MERGE_THREADS;
   const int tid = threadIdx.x, lane = tid & 63, mg = blockIdx.x, kvh = blockIdx.y;
   const int first = merge[4 * mg + 0], ns = merge[4 * mg + 1];
   const int tok0 = merge[4 * mg + 2], ntok = merge[4 * mg + 3] & 0xff;
@@ -700,6 +707,16 @@ merge_kernel(const int32_t *__restrict__ merge, int H, int Hkv, const float *__r
   }
 }
 
+template <int D>
+__global__ void __launch_bounds__(MERGE_THREADS)
+merge_kernel(const int32_t *__restrict__ merge, int H, int Hkv, const float *__restrict__ part,
+             float *__restrict__ out, f16 *__restrict__ planes, int64_t npad, int xf) {
+  if (merge[4 * blockIdx.x + 1] <= 4)
+    merge_group<D, 4>(merge, H, Hkv, part, out, planes, npad, xf);
+  else
+    merge_group<D, 16>(merge, H, Hkv, part, out, planes, npad, xf);
+}
+
 }  // namespace lgmlh
 
 using namespace lgmlh;
@@ -753,11 +770,16 @@ static void launch_attn(const float *q, int H, int Hkv, float scale_log2, const 
   }
   if (ub->ring <= 0 && ub->n_shared > 0) {
     if constexpr (D <= 128 && D >= 64) {
-      const auto kern = tree ? paged_attn_shared_kernel<D, true> : paged_attn_shared_kernel<D, false>;
-      hipLaunchKernelGGL(kern, dim3(ub->n_shared, Hkv), dim3(64 * SHARED_WAVES), 0, st, q, H, Hkv,
-                         scale_log2, (const uint16_t *)kp, (const uint16_t *)vp, ub->items,
-                         ub->shared, ub->seq_off, ub->seq_npast, ub->block_tab, ub->max_blocks, out,
-                         planes, npad, xf, part, vis, ub->window);
+      constexpr int HALF = SHARED_WAVES / 2;
+      const bool small = tree && ub->n_items - ub->n_single <= HALF * ub->n_shared;
+      const auto kern = small  ? paged_attn_shared_kernel<D, true, HALF>
+                        : tree ? paged_attn_shared_kernel<D, true>
+                               : paged_attn_shared_kernel<D, false>;
+      hipLaunchKernelGGL(kern, dim3(ub->n_shared, Hkv, small ? 2 : 1),
+                         dim3(64 * (small ? HALF : SHARED_WAVES)), 0, st, q, H, Hkv, scale_log2,
+                         (const uint16_t *)kp, (const uint16_t *)vp, ub->items, ub->shared,
+                         ub->seq_off, ub->seq_npast, ub->block_tab, ub->max_blocks, out, planes,
+                         npad, xf, part, vis, ub->window);
     }
   }
   merge_dev(D, ub, H, Hkv, part, out, planes, npad, xf, st);
