@@ -200,57 +200,85 @@ kv_gather_q8_kernel(const uint8_t *__restrict__ pool, int which, int64_t n_cells
 }
 
 // Cells src -> dst of every pool tensor (K at even places, V at odd ones), each
-// dst as its src was before the call: a workgroup takes one slice of dims of
-// one head of one tensor, reads all the moves' values of it, then writes.
+// dst as its src was before the call: a workgroup takes rows of one head's tiles
+// of one tensor (16-byte pieces of K's cells, V's dims, Q8_0's scales), reads all
+// the moves' values of them into registers, then writes. It is bound by V, whose
+// cells are 2 (or 1) bytes of a line each.
 constexpr int MOVE_MAX = 1024, MOVE_THREADS = 256;
-// One slice's value i of a cell, as an index into the tile.
-template <bool Q8>
-__device__ __forceinline__ int move_at(int is_v, int cell, int d, int D) {
-  if (Q8)
-    return is_v ? d * 64 + cell % 32 / 8 * 16 + cell / 32 * 8 + cell % 8
-                : ((d / 64 * 64 + cell) * 4 + d % 32 / 8) * 16 + d % 64 / 32 * 8 + d % 8;
-  return is_v ? d * KV_BLOCK + cell : cell * D + d;
+
+// The values (row r, move m), m fastest or (CELLS) r fastest, at base + off[m] +
+// at(r): PER a thread, the rest of the index stepped without a division.
+template <typename T, int PER, bool CELLS, typename At>
+__device__ __forceinline__ void move_rows(uint8_t *base, const int64_t *from, const int64_t *to, int n,
+                                          int rows, At at) {
+  const int total = n * rows, inner = CELLS ? rows : n;
+  int lo[PER], hi[PER];
+  T v[PER];
+  int b = (int)threadIdx.x / inner, a = (int)threadIdx.x % inner;
+  const int db = MOVE_THREADS / inner, da = MOVE_THREADS % inner;
+#pragma unroll
+  for (int j = 0; j < PER; j++) {
+    lo[j] = CELLS ? b : a;  // the move
+    hi[j] = at(CELLS ? a : b);
+    a += da;
+    b += db;
+    if (a >= inner) {
+      a -= inner;
+      b++;
+    }
+    if (j * MOVE_THREADS + (int)threadIdx.x < total && from[lo[j]] >= 0)
+      v[j] = *(const T *)(base + from[lo[j]] + hi[j]);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < PER; j++)
+    if (j * MOVE_THREADS + (int)threadIdx.x < total && from[lo[j]] >= 0)
+      *(T *)(base + to[lo[j]] + hi[j]) = v[j];
 }
-template <bool Q8>
+
+// Rows of a workgroup: K's 16-byte pieces of a cell, V's dims.
+struct MoveShape {
+  int k_rows, v_rows;
+};
+template <bool Q8, int PER>
 __global__ void __launch_bounds__(MOVE_THREADS)
 kv_move_kernel(void *const *__restrict__ pools, int64_t n_cells, int Hkv, int D,
-               const int64_t *__restrict__ src, const int64_t *__restrict__ dst, int n) {
-  typedef typename std::conditional<Q8, uint8_t, uint16_t>::type T;
-  extern __shared__ __align__(16) uint8_t lds[];
-  constexpr int S = 32;  // dims of a slice (16 in heads of 16)
-  const int w = D < S ? D : S, slices = D / w;
+               const int64_t *__restrict__ src, const int64_t *__restrict__ dst, int n,
+               MoveShape shape) {
+  __shared__ int64_t from[MOVE_MAX], to[MOVE_MAX];
   const int p = blockIdx.y, is_v = p & 1;
-  const int h = blockIdx.x / slices, s = blockIdx.x % slices;
+  const int h = blockIdx.x % Hkv, s = blockIdx.x / Hkv;
+  const int all = is_v ? D : Q8 ? D / 16 : D / 8, rows = is_v ? shape.v_rows : shape.k_rows;
+  const bool scales = Q8 && s == (int)(gridDim.x / Hkv) - 1;
+  if (!scales && s * rows >= all) return;
   uint8_t *pool = (uint8_t *)pools[p];
-  const int64_t bytes = Q8 ? 68 * (int64_t)D : 128 * (int64_t)D;
-  T *vals = (T *)lds;
-  uint16_t *scales = (uint16_t *)(lds + ((int64_t)n * w * sizeof(T) + 15) / 16 * 16);
-  // K: a cell's dims are neighbours; V: a dim's cells are
-  auto each = [&](auto &&f) {
-    for (int i = threadIdx.x; i < n * w; i += MOVE_THREADS) {
-      const int m = is_v ? i % n : i / w, d = is_v ? i / n : i % w;
-      f(i, m, s * w + d);
-    }
+  const int64_t tile = Q8 ? 68 * (int64_t)D : 128 * (int64_t)D;
+  // a cell's place in its tile, without the row
+  auto place = [&](int64_t c) {
+    const int o = (int)(c % KV_BLOCK);
+    const int in = scales  ? 64 * D + 2 * o
+                   : !is_v ? (Q8 ? o * 64 : o * D * 2)
+                           : (Q8 ? o % 32 / 8 * 16 + o / 32 * 8 + o % 8 : 2 * o);
+    return ((c / KV_BLOCK) * Hkv + h) * tile + in;
   };
-  auto tile = [&](int64_t c) { return pool + ((c / KV_BLOCK) * Hkv + h) * bytes; };
-  auto good = [&](int m) { return (uint64_t)src[m] < (uint64_t)n_cells && (uint64_t)dst[m] < (uint64_t)n_cells; };
-  each([&](int i, int m, int d) {
-    const int64_t c = src[m];
-    if (good(m)) vals[i] = ((const T *)tile(c))[move_at<Q8>(is_v, (int)(c % KV_BLOCK), d, D)];
-  });
-  if (Q8)
-    for (int m = threadIdx.x; m < n; m += MOVE_THREADS)
-      if (good(m))
-        scales[m] = *(const uint16_t *)(tile(src[m]) + 64 * D + 2 * (s * 64 + src[m] % KV_BLOCK));
+  for (int m = threadIdx.x; m < n; m += MOVE_THREADS) {
+    const int64_t a = src[m], b = dst[m];
+    const bool good = (uint64_t)a < (uint64_t)n_cells && (uint64_t)b < (uint64_t)n_cells;
+    from[m] = good ? place(a) : -1;
+    to[m] = good ? place(b) : -1;
+  }
   __syncthreads();
-  each([&](int i, int m, int d) {
-    const int64_t c = dst[m];
-    if (good(m)) ((T *)tile(c))[move_at<Q8>(is_v, (int)(c % KV_BLOCK), d, D)] = vals[i];
-  });
-  if (Q8)
-    for (int m = threadIdx.x; m < n; m += MOVE_THREADS)
-      if (good(m))
-        *(uint16_t *)(tile(dst[m]) + 64 * D + 2 * (s * 64 + dst[m] % KV_BLOCK)) = scales[m];
+  const int r0 = s * rows, left = all - r0 < rows ? all - r0 : rows;
+  if (scales)
+    move_rows<uint16_t, PER, false>(pool, from, to, n, D / 32, [](int r) { return 128 * r; });
+  else if (!is_v)
+    move_rows<u32x4, PER, true>(pool, from, to, n, left, [&](int r) {
+      return Q8 ? (r0 + r) / 4 * 4096 + (r0 + r) % 4 * 16 : 16 * (r0 + r);
+    });
+  else if (Q8)
+    move_rows<uint8_t, PER, false>(pool, from, to, n, left, [&](int r) { return 64 * (r0 + r); });
+  else
+    move_rows<uint16_t, PER, false>(pool, from, to, n, left, [&](int r) { return 128 * (r0 + r); });
 }
 
 // Range and distinctness of cells that a call writes. Cells come in runs (c, c +
@@ -391,14 +419,27 @@ extern "C" int lgmlh_kv_move(int type, void *const *pools, int n_pools, int64_t 
     }
   LGMLH_TRY(check_write_cells(h_dst, n, n_cells, "kv_move"));
   if (n == 0) return LGMLH_OK;
-  const int w = head_dim < 32 ? head_dim : 32;
-  const size_t lds = ((size_t)n * w * (q8 ? 1 : 2) + 15) / 16 * 16 + (q8 ? 2 * (size_t)n : 0);
-  const dim3 grid((unsigned)(n_head_kv * (head_dim / w)), (unsigned)n_pools);
-  if (q8)
-    hipLaunchKernelGGL(kv_move_kernel<true>, grid, dim3(MOVE_THREADS), lds, as_stream(stream), pools,
-                       n_cells, n_head_kv, head_dim, src, dst, (int)n);
-  else
-    hipLaunchKernelGGL(kv_move_kernel<false>, grid, dim3(MOVE_THREADS), lds, as_stream(stream), pools,
-                       n_cells, n_head_kv, head_dim, src, dst, (int)n);
+  // as few values a thread (8, 16, 32) as leave a workgroup 8 rows, a cache line's
+  // of K; then as many rows as it holds
+  const int per = n <= MOVE_THREADS ? 8 : n <= 2 * MOVE_THREADS ? 16 : 32;
+  const int hold = per * MOVE_THREADS / (int)n;
+  auto fit = [&](int all) {
+    int r = all;
+    while (r > hold) r = (r + 1) / 2;
+    return r;
+  };
+  const int pieces = head_dim / (q8 ? 16 : 8);
+  const MoveShape shape = {fit(pieces), fit(head_dim)};
+  const int slices_k = (pieces + shape.k_rows - 1) / shape.k_rows,
+            slices_v = (head_dim + shape.v_rows - 1) / shape.v_rows;
+  const int slices = (slices_k > slices_v ? slices_k : slices_v) + (q8 ? 1 : 0);
+  const auto kern = q8 ? (per == 8    ? kv_move_kernel<true, 8>
+                          : per == 16 ? kv_move_kernel<true, 16>
+                                      : kv_move_kernel<true, 32>)
+                       : (per == 8    ? kv_move_kernel<false, 8>
+                          : per == 16 ? kv_move_kernel<false, 16>
+                                      : kv_move_kernel<false, 32>);
+  hipLaunchKernelGGL(kern, dim3((unsigned)(n_head_kv * slices), (unsigned)n_pools), dim3(MOVE_THREADS),
+                     0, as_stream(stream), pools, n_cells, n_head_kv, head_dim, src, dst, (int)n, shape);
   return hip_check(hipGetLastError(), "kv_move");
 }
