@@ -29,174 +29,244 @@ struct Q8Tile {
   __device__ static int scale_at(int b, int cell) { return scales + 2 * (b * 64 + cell); }
 };
 
-constexpr int Q8_TOKENS = 32, Q8_THREADS = 256;  // of a workgroup, for one head of K or V
+// A workgroup takes W consecutive tokens (64, or 16 of a call of few) of one head
+// of K or V, 4 values a thread and step. V turns in LDS: 8 tokens whose cells are
+// 8 in a row from a multiple of 8 on (a whole group) are 8 consecutive bytes of
+// each dim, and 8 lanes take a dim's 64 bytes. Runs of cells start anywhere, so a
+// group belongs to the workgroup that has its first token, which also takes the
+// up to 7 of it that lie past its own; tokens in no whole group go byte by byte.
+constexpr int Q8_THREADS = 256, Q8_GROUP = 8, Q8_HALO = 7;
+constexpr int64_t Q8_CELLS = (int64_t)1 << 36;  // a block's number has 31 bits
 
-// The tokens of a workgroup start at a multiple of 8 cells when the call's
-// tokens are one run of cells (a prompt chunk): then groups of 8 tokens are 8
-// consecutive bytes of V.
-__device__ __forceinline__ int64_t first_token(const int64_t *__restrict__ cells) {
-  return (int64_t)blockIdx.x * Q8_TOKENS - cells[0] % 8;
+// The tile of cell c (>= 0) of one head: head is the first block's.
+template <int D, typename P>
+__device__ __forceinline__ P *tile_of(P *head, int64_t c, int Hkv) {
+  return head + (uint64_t)(uint32_t)((uint64_t)c >> 6) * (uint32_t)(Hkv * Q8Tile<D>::bytes);
 }
-// Whether tokens j .. j + 7 are 8 cells from a multiple of 8 on (lds: the
-// workgroup's cells, -1 for none).
-__device__ __forceinline__ bool whole_group(const int64_t *cell) {
-  bool w = cell[0] >= 0 && cell[0] % 8 == 0;
+
+template <int W>
+struct Q8Window {
+  int64_t cells[W + 2 * Q8_HALO];  // of tokens j0 - 7 .. j0 + W + 6; -1: none
+  int lead[W / Q8_GROUP + 1];      // first tokens of the whole groups, 0 .. W - 1
+  int lone[W];                     // tokens in no whole group
+  int n_lead, n_lone;
+  __device__ __forceinline__ int64_t cell(int t) const { return cells[t + Q8_HALO]; }
+  __device__ __forceinline__ bool leads(int t) const {
+    bool w = cell(t) >= 0 && cell(t) % 8 == 0;
 #pragma unroll
-  for (int i = 1; i < 8; i++) w &= cell[i] == cell[0] + i;
-  return w;
-}
-__device__ __forceinline__ void load_cells(int64_t *lds, const int64_t *__restrict__ cells,
-                                           int64_t j0, int64_t n, int64_t n_cells) {
-  if (threadIdx.x < Q8_TOKENS) {
-    const int64_t j = j0 + threadIdx.x, c = j >= 0 && j < n ? cells[j] : -1;
-    lds[threadIdx.x] = c < n_cells ? c : -1;
+    for (int i = 1; i < 8; i++) w &= cell(t + i) == cell(t) + i;
+    return w;
   }
-}
+  // All threads; the lists are there for V only.
+  __device__ __forceinline__ void fill(const int64_t *__restrict__ src, int64_t j0, int64_t n,
+                                       int64_t n_cells, bool lists) {
+    const int tid = threadIdx.x;
+    if (tid < W + 2 * Q8_HALO) {
+      const int64_t j = j0 + tid - Q8_HALO, c = j >= 0 && j < n ? src[j] : -1;
+      cells[tid] = c < n_cells ? c : -1;
+    }
+    __syncthreads();
+    if (lists && tid < 64) {
+      const int t = tid < W ? tid : W - 1;
+      const int64_t c = cell(t);
+      const bool is_lead = tid < W && leads(t);
+      const int back = c >= 0 ? (int)(c % 8) : 0;
+      const bool is_lone = tid < W && c >= 0 && !leads(t - back);
+      const uint64_t ml = __builtin_amdgcn_ballot_w64(is_lead), mo = __builtin_amdgcn_ballot_w64(is_lone);
+      const uint64_t below = ((uint64_t)1 << tid) - 1;
+      if (is_lead) lead[__builtin_popcountll(ml & below)] = t;
+      if (is_lone) lone[__builtin_popcountll(mo & below)] = t;
+      if (tid == 0) {
+        n_lead = __builtin_popcountll(ml);
+        n_lone = __builtin_popcountll(mo);
+      }
+    }
+    if (lists) __syncthreads();
+  }
+};
 
-// x (n, Hkv D) f32 rows into their cells. Per 32 values, the steps of
+// x (n, Hkv D) f32 rows into their cells. Per 32 values (8 lanes), the steps of
 // quantize_row_q8_0: d = amax / 127, q = round(x (1 / d)) with halves away from
-// zero, d kept as f16. A thread has 8 values; K leaves as 8 bytes, V turns in
-// LDS so that 8 cells leave as 8 bytes.
-template <int D>
+// zero, d kept as f16.
+template <int D, int W>
 __global__ void __launch_bounds__(Q8_THREADS)
 kv_store_q8_kernel(uint8_t *__restrict__ kp, uint8_t *__restrict__ vp, int64_t n_cells,
                    const float *__restrict__ ks, const float *__restrict__ vs,
                    const int64_t *__restrict__ cells, int64_t n, int Hkv) {
   typedef Q8Tile<D> T;
-  constexpr int G8 = D / 8, STEP = Q8_THREADS / G8, PAD = D + 4;
-  __shared__ int64_t cell[Q8_TOKENS];
-  __shared__ __align__(8) int8_t turn[Q8_TOKENS * PAD];
-  const int tid = threadIdx.x, h = blockIdx.y, is_v = blockIdx.z;
-  const int64_t j0 = first_token(cells);
-  load_cells(cell, cells, j0, n, n_cells);
-  const int g8 = tid % G8, t0 = tid / G8;
-  const float *src = (is_v ? vs : ks) + (int64_t)h * D + 8 * g8;
+  constexpr int G4 = D / 4, STEP = Q8_THREADS / G4, PAD = D + 4;
+  constexpr int ROWS = W + Q8_HALO, IT = (ROWS + STEP - 1) / STEP;
+  __shared__ Q8Window<W> win;
+  __shared__ __align__(4) int8_t turn[ROWS * PAD];
+  __shared__ uint16_t scale[D / 32 * W];
+  const int tid = threadIdx.x, h = blockIdx.x % (uint32_t)Hkv, is_v = blockIdx.y;
+  const int64_t j0 = (int64_t)(blockIdx.x / (uint32_t)Hkv) * W;
+  const int g4 = tid % G4, t0 = tid / G4;
+  const float *src = (is_v ? vs : ks) + (j0 * Hkv + h) * D + 4 * g4;
   uint8_t *pool = (is_v ? vp : kp) + (int64_t)h * T::bytes;
-  f32x4 x[Q8_TOKENS / STEP][2];
+  const int64_t left = n - j0 < (is_v ? ROWS : W) ? n - j0 : is_v ? ROWS : W;
+  f32x4 x[IT];
 #pragma unroll
-  for (int i = 0; i < Q8_TOKENS / STEP; i++) {
-    const int64_t j = j0 + t0 + i * STEP;
-    const f32x4_u *p = (const f32x4_u *)(src + j * Hkv * D);
-    const bool in = j >= 0 && j < n;
-    x[i][0] = in ? p[0] : f32x4{0, 0, 0, 0};
-    x[i][1] = in ? p[1] : f32x4{0, 0, 0, 0};
+  for (int i = 0; i < IT; i++) {
+    const int t = t0 + i * STEP;
+    x[i] = t < left ? *(const f32x4_u *)(src + (int64_t)t * Hkv * D) : f32x4{0, 0, 0, 0};
+  }
+  win.fill(cells, j0, n, n_cells, is_v);
+#pragma unroll
+  for (int i = 0; i < IT; i++) {
+    const int t = t0 + i * STEP;
+    float amax = fmaxf(fmaxf(fabsf(x[i][0]), fabsf(x[i][1])), fmaxf(fabsf(x[i][2]), fabsf(x[i][3])));
+    amax = group_max<8>(amax);  // the 8 lanes of a block
+    const float d = amax / 127.0f, id = d != 0.0f ? 1.0f / d : 0.0f;
+    uint32_t q = 0;
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+      q |= (uint32_t)((int)__builtin_roundf(x[i][e] * id) & 0xff) << 8 * e;
+    if (t >= left) continue;  // whole blocks of lanes leave together
+    if (g4 % 8 == 0 && t < W) scale[g4 / 8 * W + t] = f2h(d);
+    if (is_v) {
+      *(uint32_t *)(turn + t * PAD + 4 * g4) = q;
+    } else if (const int64_t c = win.cell(t); c >= 0) {
+      *(uint32_t *)(tile_of<D>(pool, c, Hkv) + T::k_at((int)c & 63, g4 / 2) + 4 * (g4 & 1)) = q;
+    }
   }
   __syncthreads();
-#pragma unroll
-  for (int i = 0; i < Q8_TOKENS / STEP; i++) {
-    const int t = t0 + i * STEP;
-    float amax = 0.0f;
-#pragma unroll
-    for (int e = 0; e < 8; e++) amax = fmaxf(amax, fabsf(x[i][e >> 2][e & 3]));
-    amax = group_max<4>(amax);  // the 4 lanes of a block
-    const float d = amax / 127.0f, id = d != 0.0f ? 1.0f / d : 0.0f;
-    uint32_t q[2] = {0, 0};
-#pragma unroll
-    for (int e = 0; e < 8; e++) {
-      const int v = (int)__builtin_roundf(x[i][e >> 2][e & 3] * id);
-      q[e >> 2] |= (uint32_t)(v & 0xff) << 8 * (e & 3);
-    }
-    const int64_t c = cell[t];
-    if (is_v) {
-      uint32_t *dst = (uint32_t *)(turn + t * PAD + 8 * g8);
-      dst[0] = q[0];
-      dst[1] = q[1];
-    }
-    if (c < 0) continue;  // groups of 4 lanes leave together
-    uint8_t *tile = pool + (c / KV_BLOCK) * Hkv * T::bytes;
-    const int o = (int)(c % KV_BLOCK);
-    if (!is_v) *(u32x2 *)(tile + T::k_at(o, g8)) = u32x2{q[0], q[1]};
-    if (g8 % 4 == 0) *(uint16_t *)(tile + T::scale_at(g8 / 4, o)) = f2h(d);
+  // the scales with tokens along the lanes, as a tile has them
+  for (int i = tid; i < D / 32 * W; i += Q8_THREADS) {
+    const int64_t c = win.cell(i % W);
+    if (c >= 0) *(uint16_t *)(tile_of<D>(pool, c, Hkv) + T::scale_at(i / W, (int)c & 63)) = scale[i];
   }
   if (!is_v) return;
-  __syncthreads();
-  for (int i = tid; i < Q8_TOKENS / 8 * D; i += Q8_THREADS) {
-    const int g = i / D, d = i % D;
-    const int64_t *cg = cell + 8 * g;
-    const int8_t *src8 = turn + 8 * g * PAD + d;
-    if (whole_group(cg)) {  // the same for a wave's lanes
-      uint8_t *tile = pool + (cg[0] / KV_BLOCK) * Hkv * T::bytes;
-      uint32_t q[2] = {0, 0};
+  const int ng = win.n_lead, no = win.n_lone;
+  for (int i = tid; i < Q8_GROUP * D; i += Q8_THREADS) {
+    const int g = i % Q8_GROUP, d = i / Q8_GROUP;
+    if (g >= ng) continue;
+    const int t = win.lead[g];
+    const int64_t c = win.cell(t);
+    const int8_t *s8 = turn + t * PAD + d;
+    uint32_t q[2] = {0, 0};
 #pragma unroll
-      for (int e = 0; e < 8; e++) q[e >> 2] |= (uint32_t)(uint8_t)src8[e * PAD] << 8 * (e & 3);
-      *(u32x2 *)(tile + T::v_at(d, (int)(cg[0] % KV_BLOCK))) = u32x2{q[0], q[1]};
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; e++) {
-        const int64_t c = cg[e];
-        if (c < 0) continue;
-        uint8_t *tile = pool + (c / KV_BLOCK) * Hkv * T::bytes;
-        tile[T::v_at(d, (int)(c % KV_BLOCK))] = (uint8_t)src8[e * PAD];
-      }
-    }
+    for (int e = 0; e < 8; e++) q[e >> 2] |= (uint32_t)(uint8_t)s8[e * PAD] << 8 * (e & 3);
+    *(u32x2 *)(tile_of<D>(pool, c, Hkv) + T::v_at(d, (int)c & 63)) = u32x2{q[0], q[1]};
+  }
+  const int sh = no > 1 ? 32 - __builtin_clz(no - 1) : 0;  // lone tokens to a power of two
+  for (int i = tid; no > 0 && i < D << sh; i += Q8_THREADS) {
+    const int k = i & ((1 << sh) - 1), d = i >> sh;
+    if (k >= no) continue;
+    const int t = win.lone[k];
+    const int64_t c = win.cell(t);
+    tile_of<D>(pool, c, Hkv)[T::v_at(d, (int)c & 63)] = (uint8_t)turn[t * PAD + d];
   }
 }
 
-// Cells as rows (n, Hkv D) of f32 or f16: the same shape the other way round.
-template <int D, typename OutT>
+// A value's four of a row: f32 or f16 of d q.
+template <typename OutT>
+__device__ __forceinline__ void put4(OutT *out, uint32_t q, float d) {
+  typedef OutT o4 __attribute__((ext_vector_type(4), aligned(sizeof(OutT))));
+  o4 y;
+#pragma unroll
+  for (int e = 0; e < 4; e++) y[e] = (OutT)(d * (float)(int8_t)(q >> 8 * e));
+  *(o4 *)out = y;
+}
+
+// The scales of N tokens (cell(t), -1: none) into LDS, tokens along the lanes, as
+// a tile has them: 64 cells' of 32 dims are a line. (By the lanes that use them
+// they are 8 lines a wave and 64 tokens, twice the values'.)
+template <int D, int N, typename C>
+__device__ __forceinline__ void load_scales(uint16_t *lds, const uint8_t *head, int Hkv, C cell) {
+#pragma unroll
+  for (int k = 0; k < (D / 32 * N + Q8_THREADS - 1) / Q8_THREADS; k++) {
+    const int i = threadIdx.x + k * Q8_THREADS;
+    if (i >= D / 32 * N) break;
+    const int64_t c = cell(i % N);
+    lds[i] = c < 0 ? 0
+                   : *(const uint16_t *)(tile_of<D>(head, c, Hkv) + Q8Tile<D>::scale_at(i / N, (int)c & 63));
+  }
+}
+
+// Cells as rows (n, Hkv D) of f32 or f16, the store the other way round: the values
+// into LDS as rows (K's 16 bytes a lane are 8 dims of two blocks), the scales too,
+// then out 4 values a lane. (K's values straight from the tile, 4 bytes a lane,
+// need each token's address in each lane: 32768 tokens of 8 heads of 128 54 us.)
+template <int D, int W, bool IS_V, typename OutT>
 __global__ void __launch_bounds__(Q8_THREADS)
-kv_gather_q8_kernel(const uint8_t *__restrict__ pool, int which, int64_t n_cells,
+kv_gather_q8_kernel(const uint8_t *__restrict__ pool, int64_t n_cells,
                     const int64_t *__restrict__ cells, int64_t n, int Hkv,
                     OutT *__restrict__ out) {
   typedef Q8Tile<D> T;
-  constexpr int G8 = D / 8, STEP = Q8_THREADS / G8, PAD = D + 4;
-  __shared__ int64_t cell[Q8_TOKENS];
-  __shared__ __align__(8) int8_t turn[Q8_TOKENS * PAD];
-  const int tid = threadIdx.x, h = blockIdx.y;
-  const int64_t j0 = first_token(cells);
-  load_cells(cell, cells, j0, n, n_cells);
-  __syncthreads();
+  constexpr int G4 = D / 4, STEP = Q8_THREADS / G4, PAD = IS_V ? D + 4 : D + 8;
+  constexpr int ROWS = IS_V ? W + Q8_HALO : W, NS = IS_V ? W + 8 : W;
+  __shared__ Q8Window<W> win;
+  __shared__ __align__(8) int8_t turn[ROWS * PAD];
+  __shared__ uint8_t mine[ROWS];  // the rows of turn that are this workgroup's
+  __shared__ uint16_t scale[D / 32 * NS];
+  const int tid = threadIdx.x, h = blockIdx.x % (uint32_t)Hkv;
+  const int64_t j0 = (int64_t)(blockIdx.x / (uint32_t)Hkv) * W;
   const uint8_t *head = pool + (int64_t)h * T::bytes;
-  if (which) {
-    for (int i = tid; i < Q8_TOKENS / 8 * D; i += Q8_THREADS) {
-      const int g = i / D, d = i % D;
-      const int64_t *cg = cell + 8 * g;
-      int8_t *dst = turn + 8 * g * PAD + d;
-      if (whole_group(cg)) {
-        const uint8_t *tile = head + (cg[0] / KV_BLOCK) * Hkv * T::bytes;
-        const u32x2 q = *(const u32x2 *)(tile + T::v_at(d, (int)(cg[0] % KV_BLOCK)));
+  win.fill(cells, j0, n, n_cells, IS_V);
+  load_scales<D, NS>(scale, head, Hkv, [&](int t) { return t < ROWS ? win.cell(t) : -1; });
+  if constexpr (IS_V) {
+    const int ng = win.n_lead, no = win.n_lone;
+    if (tid < ROWS) mine[tid] = tid < W && win.cell(tid) < 0;  // a cell outside: zeros
+    constexpr int GI = Q8_GROUP * D / Q8_THREADS;
+    u32x2 q8[GI];
 #pragma unroll
-        for (int e = 0; e < 8; e++) dst[e * PAD] = (int8_t)(q[e >> 2] >> 8 * (e & 3));
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-          const int64_t c = cg[e];
-          const uint8_t *tile = head + (c / KV_BLOCK) * Hkv * T::bytes;
-          dst[e * PAD] = c < 0 ? (int8_t)0 : (int8_t)tile[T::v_at(d, (int)(c % KV_BLOCK))];
-        }
-      }
+    for (int i = 0; i < GI; i++) {
+      const int k = tid + i * Q8_THREADS, g = k % Q8_GROUP, d = k / Q8_GROUP;
+      if (g >= ng) continue;
+      const int64_t c = win.cell(win.lead[g]);
+      q8[i] = *(const u32x2 *)(tile_of<D>(head, c, Hkv) + T::v_at(d, (int)c & 63));
     }
     __syncthreads();
-  }
-  const int g8 = tid % G8, t0 = tid / G8;
+    if (tid < 8 * ng) mine[win.lead[tid >> 3] + (tid & 7)] = 1;
+    if (tid < no) mine[win.lone[tid]] = 1;
 #pragma unroll
-  for (int i = 0; i < Q8_TOKENS / STEP; i++) {
-    const int t = t0 + i * STEP;
-    const int64_t j = j0 + t, c = cell[t];
-    if (j < 0 || j >= n) continue;
-    u32x2 q = {0, 0};
-    float d = 0.0f;
-    if (c >= 0) {
-      const uint8_t *tile = head + (c / KV_BLOCK) * Hkv * T::bytes;
-      const int o = (int)(c % KV_BLOCK);
-      d = h2f(*(const uint16_t *)(tile + T::scale_at(g8 / 4, o)));
-      if (which) {
-        const uint32_t *s = (const uint32_t *)(turn + t * PAD + 8 * g8);
-        q = u32x2{s[0], s[1]};
-      } else {
-        q = *(const u32x2 *)(tile + T::k_at(o, g8));
+    for (int i = 0; i < GI; i++) {
+      const int k = tid + i * Q8_THREADS, g = k % Q8_GROUP, d = k / Q8_GROUP;
+      if (g >= ng) continue;
+      int8_t *s8 = turn + win.lead[g] * PAD + d;
+#pragma unroll
+      for (int e = 0; e < 8; e++) s8[e * PAD] = (int8_t)(q8[i][e >> 2] >> 8 * (e & 3));
+    }
+    const int sh = no > 1 ? 32 - __builtin_clz(no - 1) : 0;  // lone tokens to a power of two
+    if (no > 0)
+#pragma unroll 4
+      for (int i = tid; i < D << sh; i += Q8_THREADS) {
+        const int k = i & ((1 << sh) - 1), d = i >> sh;
+        if (k >= no) continue;
+        const int t = win.lone[k];
+        const int64_t c = win.cell(t);
+        turn[t * PAD + d] = (int8_t)tile_of<D>(head, c, Hkv)[T::v_at(d, (int)c & 63)];
       }
-    }
-    typedef OutT o4 __attribute__((ext_vector_type(4), aligned(sizeof(OutT))));
-    OutT *dst = out + (j * Hkv + h) * (int64_t)D + 8 * g8;
+  } else {
+    constexpr int PI = (W * D / 16 + Q8_THREADS - 1) / Q8_THREADS;
 #pragma unroll
-    for (int v = 0; v < 2; v++) {
-      o4 y;
-#pragma unroll
-      for (int e = 0; e < 4; e++) y[e] = (OutT)(d * (float)(int8_t)(q[v] >> 8 * e));
-      *(o4 *)(dst + 4 * v) = y;
+    for (int i = 0; i < PI; i++) {  // (token, j, quad), tokens of 4 quads in a row
+      const int k = tid + i * Q8_THREADS, t = k / 4 % W, j = k / (4 * W), quad = k % 4;
+      if (k >= W * D / 16) break;
+      const int64_t c = win.cell(t);
+      if (c < 0) continue;
+      const u32x4 q = *(const u32x4 *)(tile_of<D>(head, c, Hkv) + T::k_at((int)c & 63, 8 * j + quad));
+      *(u32x2 *)(turn + t * PAD + 64 * j + 8 * quad) = u32x2{q[0], q[1]};
+      *(u32x2 *)(turn + t * PAD + 64 * j + 32 + 8 * quad) = u32x2{q[2], q[3]};
     }
   }
+  __syncthreads();
+  const int g4 = tid % G4;
+  const int left = n - j0 < ROWS ? (int)(n - j0) : ROWS;
+#pragma unroll 8
+  for (int t = tid / G4; t < left; t += STEP) {
+    if (IS_V && !mine[t]) continue;
+    const uint32_t q = win.cell(t) < 0 ? 0 : *(const uint32_t *)(turn + t * PAD + 4 * g4);
+    put4(out + ((j0 + t) * Hkv + h) * (int64_t)D + 4 * g4, q, h2f(scale[g4 / 8 * NS + t]));
+  }
+}
+
+// Tokens of a workgroup: 64 (32 of heads of 256), but 16 where that makes fewer
+// than 256 workgroups.
+constexpr int q8_tokens(int D) { return D > 128 ? 32 : 64; }
+static bool q8_small(int64_t n, int n_head_kv, int kinds, int D) {
+  return (n + q8_tokens(D) - 1) / q8_tokens(D) * n_head_kv * kinds < 256;
 }
 
 // Cells src -> dst of every pool tensor (K at even places, V at odd ones), each
@@ -351,17 +421,20 @@ extern "C" int lgmlh_kv_store_q8(void *kpool, void *vpool, int64_t n_cells, int 
                                  const int64_t *cells, const int64_t *h_cells, int64_t n,
                                  void *stream) {
   if (!kpool || !vpool || !k_src || !v_src || !cells || n < 0 || n_cells <= 0 ||
-      n_cells % KV_BLOCK || n_head_kv <= 0 || n_head_kv > 65535 || !q8_head(head_dim)) {
+      n_cells > Q8_CELLS || n_cells % KV_BLOCK || n_head_kv <= 0 || n > INT32_MAX / n_head_kv || !q8_head(head_dim)) {
     set_error("kv_store_q8: bad arguments (heads of 64, 128 or 256)");
     return LGMLH_EINVAL;
   }
   LGMLH_TRY(check_write_cells(h_cells, n, n_cells, "kv_store_q8"));
   if (n == 0) return LGMLH_OK;
-  const dim3 grid((unsigned)((n + 7 + Q8_TOKENS - 1) / Q8_TOKENS), (unsigned)n_head_kv, 2);
+  const bool small = q8_small(n, n_head_kv, 2, head_dim);
+  const int w = small ? 16 : q8_tokens(head_dim);
+  // heads fastest: those of the same rows run together
+  const dim3 grid((unsigned)((n + w - 1) / w * n_head_kv), 2);
   hipStream_t st = as_stream(stream);
-  const auto kern = head_dim == 64    ? kv_store_q8_kernel<64>
-                    : head_dim == 128 ? kv_store_q8_kernel<128>
-                                      : kv_store_q8_kernel<256>;
+  const auto kern = head_dim == 64    ? (small ? kv_store_q8_kernel<64, 16> : kv_store_q8_kernel<64, 64>)
+                    : head_dim == 128 ? (small ? kv_store_q8_kernel<128, 16> : kv_store_q8_kernel<128, 64>)
+                                      : (small ? kv_store_q8_kernel<256, 16> : kv_store_q8_kernel<256, 32>);
   hipLaunchKernelGGL(kern, grid, dim3(Q8_THREADS), 0, st, (uint8_t *)kpool, (uint8_t *)vpool,
                      n_cells, k_src, v_src, cells, n, n_head_kv);
   return hip_check(hipGetLastError(), "kv_store_q8");
@@ -371,21 +444,35 @@ extern "C" int lgmlh_kv_gather_q8(const void *pool, int which, int64_t n_cells, 
                                   int head_dim, const int64_t *cells, int64_t n, void *out,
                                   int out_type, void *stream) {
   if (!pool || !cells || !out || n < 0 || (which != 0 && which != 1) || n_cells <= 0 ||
-      n_cells % KV_BLOCK || n_head_kv <= 0 || n_head_kv > 65535 || !q8_head(head_dim) ||
+      n_cells > Q8_CELLS || n_cells % KV_BLOCK || n_head_kv <= 0 || n > INT32_MAX / n_head_kv || !q8_head(head_dim) ||
       (out_type != LGMLH_F32 && out_type != LGMLH_F16)) {
     set_error("kv_gather_q8: bad arguments (heads of 64, 128 or 256; out f32 or f16)");
     return LGMLH_EINVAL;
   }
   if (n == 0) return LGMLH_OK;
-  const dim3 grid((unsigned)((n + 7 + Q8_TOKENS - 1) / Q8_TOKENS), (unsigned)n_head_kv);
+  const bool small = q8_small(n, n_head_kv, 1, head_dim);
+  const int w = small ? 16 : q8_tokens(head_dim);
+  const dim3 grid((unsigned)((n + w - 1) / w * n_head_kv));
   hipStream_t st = as_stream(stream);
   auto go = [&](auto out_t) {
-    typedef decltype(out_t) OutT;
-    const auto kern = head_dim == 64    ? kv_gather_q8_kernel<64, OutT>
-                      : head_dim == 128 ? kv_gather_q8_kernel<128, OutT>
-                                        : kv_gather_q8_kernel<256, OutT>;
-    hipLaunchKernelGGL(kern, grid, dim3(Q8_THREADS), 0, st, (const uint8_t *)pool, which, n_cells,
-                       cells, n, n_head_kv, (OutT *)out);
+    typedef decltype(out_t) T;
+    auto launch = [&](auto kern) {
+      hipLaunchKernelGGL(kern, grid, dim3(Q8_THREADS), 0, st, (const uint8_t *)pool, n_cells, cells, n,
+                         n_head_kv, (T *)out);
+    };
+    auto of = [&](auto d) {
+      constexpr int D = decltype(d)::value, big = q8_tokens(D);
+      if (which)
+        launch(small ? kv_gather_q8_kernel<D, 16, true, T> : kv_gather_q8_kernel<D, big, true, T>);
+      else
+        launch(small ? kv_gather_q8_kernel<D, 16, false, T> : kv_gather_q8_kernel<D, big, false, T>);
+    };
+    if (head_dim == 64)
+      of(std::integral_constant<int, 64>{});
+    else if (head_dim == 128)
+      of(std::integral_constant<int, 128>{});
+    else
+      of(std::integral_constant<int, 256>{});
   };
   if (out_type == LGMLH_F32)
     go(float{});
