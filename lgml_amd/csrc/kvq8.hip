@@ -47,7 +47,7 @@ __device__ __forceinline__ P *tile_of(P *head, int64_t c, int Hkv) {
 template <int W>
 struct Q8Window {
   int64_t cells[W + 2 * Q8_HALO];  // of tokens j0 - 7 .. j0 + W + 6; -1: none
-  int lead[W / Q8_GROUP + 1];      // first tokens of the whole groups, 0 .. W - 1
+  int lead[W / Q8_GROUP];          // first tokens of the whole groups, 0 .. W - 1
   int lone[W];                     // tokens in no whole group
   int n_lead, n_lone;
   __device__ __forceinline__ int64_t cell(int t) const { return cells[t + Q8_HALO]; }
@@ -85,6 +85,16 @@ struct Q8Window {
   }
 };
 
+// Threads for n lone tokens: the power of two that holds them, as bits.
+__device__ __forceinline__ int lone_bits(int n) { return n > 1 ? 32 - __builtin_clz(n - 1) : 0; }
+
+// To the nearest integer, halves away from zero, below 2^23: the largest number
+// under a half takes a half up to the next integer (its sum rounds there) and
+// nothing below it.
+__device__ __forceinline__ int round_away(float x) {
+  return (int)(x + __builtin_copysignf(0x1.fffffep-2f, x));
+}
+
 // x (n, Hkv D) f32 rows into their cells. Per 32 values (8 lanes), the steps of
 // quantize_row_q8_0: d = amax / 127, q = round(x (1 / d)) with halves away from
 // zero, d kept as f16.
@@ -95,7 +105,7 @@ kv_store_q8_kernel(uint8_t *__restrict__ kp, uint8_t *__restrict__ vp, int64_t n
                    const int64_t *__restrict__ cells, int64_t n, int Hkv) {
   typedef Q8Tile<D> T;
   constexpr int G4 = D / 4, STEP = Q8_THREADS / G4, PAD = D + 4;
-  constexpr int ROWS = W + Q8_HALO, IT = (ROWS + STEP - 1) / STEP;
+  constexpr int ROWS = W + Q8_HALO, IT = (ROWS + STEP - 1) / STEP, GROUPS = W / Q8_GROUP;
   __shared__ Q8Window<W> win;
   __shared__ __align__(4) int8_t turn[ROWS * PAD];
   __shared__ uint16_t scale[D / 32 * W];
@@ -120,8 +130,7 @@ kv_store_q8_kernel(uint8_t *__restrict__ kp, uint8_t *__restrict__ vp, int64_t n
     const float d = amax / 127.0f, id = d != 0.0f ? 1.0f / d : 0.0f;
     uint32_t q = 0;
 #pragma unroll
-    for (int e = 0; e < 4; e++)
-      q |= (uint32_t)((int)__builtin_roundf(x[i][e] * id) & 0xff) << 8 * e;
+    for (int e = 0; e < 4; e++) q |= (uint32_t)(round_away(x[i][e] * id) & 0xff) << 8 * e;
     if (t >= left) continue;  // whole blocks of lanes leave together
     if (g4 % 8 == 0 && t < W) scale[g4 / 8 * W + t] = f2h(d);
     if (is_v) {
@@ -137,25 +146,27 @@ kv_store_q8_kernel(uint8_t *__restrict__ kp, uint8_t *__restrict__ vp, int64_t n
     if (c >= 0) *(uint16_t *)(tile_of<D>(pool, c, Hkv) + T::scale_at(i / W, (int)c & 63)) = scale[i];
   }
   if (!is_v) return;
-  const int ng = win.n_lead, no = win.n_lone;
-  for (int i = tid; i < Q8_GROUP * D; i += Q8_THREADS) {
-    const int g = i % Q8_GROUP, d = i / Q8_GROUP;
-    if (g >= ng) continue;
+  // a thread's group or lone token is the same in every step
+  if (const int g = tid % GROUPS; g < win.n_lead) {
     const int t = win.lead[g];
     const int64_t c = win.cell(t);
-    const int8_t *s8 = turn + t * PAD + d;
-    uint32_t q[2] = {0, 0};
+    uint8_t *tile = tile_of<D>(pool, c, Hkv) + T::v_at(0, (int)c & 63);
+#pragma unroll 4
+    for (int d = tid / GROUPS; d < D; d += Q8_THREADS / GROUPS) {
+      const int8_t *s8 = turn + t * PAD + d;
+      uint32_t q[2] = {0, 0};
 #pragma unroll
-    for (int e = 0; e < 8; e++) q[e >> 2] |= (uint32_t)(uint8_t)s8[e * PAD] << 8 * (e & 3);
-    *(u32x2 *)(tile_of<D>(pool, c, Hkv) + T::v_at(d, (int)c & 63)) = u32x2{q[0], q[1]};
+      for (int e = 0; e < 8; e++) q[e >> 2] |= (uint32_t)(uint8_t)s8[e * PAD] << 8 * (e & 3);
+      *(u32x2 *)(tile + 64 * d) = u32x2{q[0], q[1]};
+    }
   }
-  const int sh = no > 1 ? 32 - __builtin_clz(no - 1) : 0;  // lone tokens to a power of two
-  for (int i = tid; no > 0 && i < D << sh; i += Q8_THREADS) {
-    const int k = i & ((1 << sh) - 1), d = i >> sh;
-    if (k >= no) continue;
+  const int no = win.n_lone, sh = lone_bits(no);
+  if (const int k = tid & ((1 << sh) - 1); k < no) {
     const int t = win.lone[k];
     const int64_t c = win.cell(t);
-    tile_of<D>(pool, c, Hkv)[T::v_at(d, (int)c & 63)] = (uint8_t)turn[t * PAD + d];
+    uint8_t *tile = tile_of<D>(pool, c, Hkv) + T::v_at(0, (int)c & 63);
+#pragma unroll 8
+    for (int d = tid >> sh; d < D; d += Q8_THREADS >> sh) tile[64 * d] = (uint8_t)turn[t * PAD + d];
   }
 }
 
@@ -195,7 +206,7 @@ kv_gather_q8_kernel(const uint8_t *__restrict__ pool, int64_t n_cells,
                     OutT *__restrict__ out) {
   typedef Q8Tile<D> T;
   constexpr int G4 = D / 4, STEP = Q8_THREADS / G4, PAD = IS_V ? D + 4 : D + 8;
-  constexpr int ROWS = IS_V ? W + Q8_HALO : W, NS = IS_V ? W + 8 : W;
+  constexpr int ROWS = IS_V ? W + Q8_HALO : W, NS = IS_V ? W + 8 : W, GROUPS = W / Q8_GROUP;
   __shared__ Q8Window<W> win;
   __shared__ __align__(8) int8_t turn[ROWS * PAD];
   __shared__ uint8_t mine[ROWS];  // the rows of turn that are this workgroup's
@@ -208,36 +219,39 @@ kv_gather_q8_kernel(const uint8_t *__restrict__ pool, int64_t n_cells,
   if constexpr (IS_V) {
     const int ng = win.n_lead, no = win.n_lone;
     if (tid < ROWS) mine[tid] = tid < W && win.cell(tid) < 0;  // a cell outside: zeros
-    constexpr int GI = Q8_GROUP * D / Q8_THREADS;
+    constexpr int GI = (GROUPS * D + Q8_THREADS - 1) / Q8_THREADS;
+    const int g = tid % GROUPS, lead = g < ng ? win.lead[g] : -1;
     u32x2 q8[GI];
+    if (lead >= 0) {
+      const int64_t c = win.cell(lead);
+      const uint8_t *tile = tile_of<D>(head, c, Hkv) + T::v_at(0, (int)c & 63);
 #pragma unroll
-    for (int i = 0; i < GI; i++) {
-      const int k = tid + i * Q8_THREADS, g = k % Q8_GROUP, d = k / Q8_GROUP;
-      if (g >= ng) continue;
-      const int64_t c = win.cell(win.lead[g]);
-      q8[i] = *(const u32x2 *)(tile_of<D>(head, c, Hkv) + T::v_at(d, (int)c & 63));
+      for (int i = 0; i < GI; i++) {
+        const int d = tid / GROUPS + i * (Q8_THREADS / GROUPS);
+        if (d < D) q8[i] = *(const u32x2 *)(tile + 64 * d);
+      }
     }
     __syncthreads();
     if (tid < 8 * ng) mine[win.lead[tid >> 3] + (tid & 7)] = 1;
     if (tid < no) mine[win.lone[tid]] = 1;
+    if (lead >= 0) {
 #pragma unroll
-    for (int i = 0; i < GI; i++) {
-      const int k = tid + i * Q8_THREADS, g = k % Q8_GROUP, d = k / Q8_GROUP;
-      if (g >= ng) continue;
-      int8_t *s8 = turn + win.lead[g] * PAD + d;
+      for (int i = 0; i < GI; i++) {
+        const int d = tid / GROUPS + i * (Q8_THREADS / GROUPS);
+        int8_t *s8 = turn + lead * PAD + d;
+        if (d < D)
 #pragma unroll
-      for (int e = 0; e < 8; e++) s8[e * PAD] = (int8_t)(q8[i][e >> 2] >> 8 * (e & 3));
-    }
-    const int sh = no > 1 ? 32 - __builtin_clz(no - 1) : 0;  // lone tokens to a power of two
-    if (no > 0)
-#pragma unroll 4
-      for (int i = tid; i < D << sh; i += Q8_THREADS) {
-        const int k = i & ((1 << sh) - 1), d = i >> sh;
-        if (k >= no) continue;
-        const int t = win.lone[k];
-        const int64_t c = win.cell(t);
-        turn[t * PAD + d] = (int8_t)tile_of<D>(head, c, Hkv)[T::v_at(d, (int)c & 63)];
+          for (int e = 0; e < 8; e++) s8[e * PAD] = (int8_t)(q8[i][e >> 2] >> 8 * (e & 3));
       }
+    }
+    const int sh = lone_bits(no);
+    if (const int k = tid & ((1 << sh) - 1); k < no) {
+      const int t = win.lone[k];
+      const int64_t c = win.cell(t);
+      const uint8_t *tile = tile_of<D>(head, c, Hkv) + T::v_at(0, (int)c & 63);
+#pragma unroll 8
+      for (int d = tid >> sh; d < D; d += Q8_THREADS >> sh) turn[t * PAD + d] = (int8_t)tile[64 * d];
+    }
   } else {
     constexpr int PI = (W * D / 16 + Q8_THREADS - 1) / Q8_THREADS;
 #pragma unroll
