@@ -36,6 +36,9 @@ __device__ __forceinline__ uint32_t order_of(float x) {
   const uint32_t u = __builtin_bit_cast(uint32_t, x);
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
+__device__ __forceinline__ float value_of(uint32_t order) {
+  return __builtin_bit_cast(float, order & 0x80000000u ? order ^ 0x80000000u : ~order);
+}
 // e^d for d <= 0 or NaN
 __device__ __forceinline__ float exp_of(float d) { return __builtin_amdgcn_exp2f(d * LP_LOG2E); }
 
@@ -82,18 +85,19 @@ lp_slice_kernel(const float *__restrict__ x, int64_t n, int slices, Slice *__res
 #pragma unroll
   for (int w = 0; w < LP_THREADS / 64; w++) m = fmaxf(m, red[0][w]);
   __syncthreads();
-  float c = 0.0f, s = 0.0f, t = 0.0f;
+  float s = 0.0f, t = 0.0f;
+  int nc = 0;
 #pragma unroll
   for (int i = 0; i < LOADS; i++)
 #pragma unroll
     for (int e = 0; e < 4; e++) {
       const bool top = v[i][e] == m;
-      const float d = v[i][e] - m, p = exp_of(d);
-      c += top ? 1.0f : 0.0f;
-      s += top ? 0.0f : p;
-      t += top ? 0.0f : p * fmaxf(d, -200.0f);  // (0 x -inf; p is 0 long before)
+      nc += __builtin_popcountll(__builtin_amdgcn_ballot_w64(top));  // the wave's
+      const float d = v[i][e] - m, p = top ? 0.0f : exp_of(d);
+      s += p;
+      t += p * fmaxf(d, -200.0f);  // (0 x -inf, 0 x NaN of inf - inf; p is 0 long before)
     }
-  c = wave_sum(c);
+  float c = (float)nc;
   s = wave_sum(s);
   t = wave_sum(t);
   if ((tid & 63) == 0) {
@@ -125,56 +129,72 @@ __device__ __forceinline__ Slice join(Slice a, Slice b) {
   return Slice{a.m, a.c, a.s + w * (b.c + b.s), a.t + w * (b.t + d * (b.c + b.s))};
 }
 
+constexpr int LP_HELD = 16;  // groups' values a thread holds (rows of up to 262144)
 constexpr int LP_LIST = LP_TOP * LP_GROUP;  // the most candidates
-// The k largest of n keys in list (LDS), all different and none 0, to out[0 ..
-// min(k, n)) in no order; n and k <= 256 the same for all threads. While there are
-// more than 256, a thread takes every 256th, and what is below the k-th largest
-// of the threads' maxima goes.
-struct Select {
-  uint64_t tmax[LP_THREADS];
-  uint64_t cut;
-  int count;
-};
-// The k-th largest of the threads' keys (0: a thread without one, and the
-// answer if fewer than k have one).
-__device__ __forceinline__ uint64_t kth_of_threads(Select &sh, uint64_t key, int k) {
-  const int tid = threadIdx.x;
-  if (tid == 0) sh.cut = 0;
-  sh.tmax[tid] = key;
-  __syncthreads();
-  int above = 0;
-#pragma unroll 8
-  for (int j = 0; j < LP_THREADS; j++) above += sh.tmax[j] > key;
-  if (key && above == k - 1) sh.cut = key;
-  __syncthreads();
-  const uint64_t cut = sh.cut;
-  __syncthreads();
+
+// The k largest of keys (value, then ~index: all different, none 0) are found by
+// cuts: a thread takes every 256th key, and where at least k threads' maxima are at
+// or above a cut, so are the k largest keys. The cut grows bit by bit from the top;
+// each wave holds all 256 maxima, 4 a lane, and counts by ballots, so the waves
+// agree without a barrier. It stops at the first cut that k to `most` maxima reach
+// (most >= k; with all 64 bits set exactly k do). 0 where fewer than k threads have
+// a key.
+__device__ __forceinline__ uint64_t cut_of(const uint64_t *tmax, int k, int most) {
+  const int lane = threadIdx.x & 63;
+  uint64_t key[LP_THREADS / 64];
+#pragma unroll
+  for (int i = 0; i < LP_THREADS / 64; i++) key[i] = tmax[64 * i + lane];
+  uint64_t cut = 0;
+  for (int bit = 63; bit >= 0; bit--) {
+    const uint64_t c = cut | (uint64_t)1 << bit;
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < LP_THREADS / 64; i++)
+      n += __builtin_popcountll(__builtin_amdgcn_ballot_w64(key[i] >= c));
+    if (n < k) continue;
+    cut = c;
+    if (n <= most) break;
+  }
   return cut;
 }
 
+struct Select {
+  uint64_t tmax[LP_THREADS];
+  int count;
+};
+// The number of list's n keys left, at most 256, the k largest among them.
 __device__ __forceinline__ int narrow(Select &sh, uint64_t *list, int n, int k) {
   const int tid = threadIdx.x;
-  while (n > LP_THREADS) {
-    uint64_t best = 0;
-    for (int i = tid; i < n; i += LP_THREADS) best = list[i] > best ? list[i] : best;
-    const uint64_t cut = kth_of_threads(sh, best, k);
-    // a thread's keys (16 at most) wait in registers for the list to be free
-    if (tid == 0) sh.count = 0;
-    uint64_t kept[LP_LIST / LP_THREADS];
+  while (n > LP_THREADS) {  // n falls: at most k threads' keys stay, of 4 k or more
+    uint64_t kept[LP_LIST / LP_THREADS], best = 0;  // a thread's keys
 #pragma unroll
     for (int j = 0; j < LP_LIST / LP_THREADS; j++) {
       const int i = tid + j * LP_THREADS;
-      kept[j] = i < n && list[i] >= cut ? list[i] : 0;
+      kept[j] = i < n ? list[i] : 0;
+      best = kept[j] > best ? kept[j] : best;
     }
+    sh.tmax[tid] = best;
+    if (tid == 0) sh.count = 0;
     __syncthreads();
+    const uint64_t cut = cut_of(sh.tmax, k, k);
 #pragma unroll
     for (int j = 0; j < LP_LIST / LP_THREADS; j++)
-      if (kept[j]) list[atomicAdd(&sh.count, 1)] = kept[j];
+      if (kept[j] && kept[j] >= cut) list[atomicAdd(&sh.count, 1)] = kept[j];
     __syncthreads();
     n = sh.count;
     __syncthreads();
   }
   return n;
+}
+
+// How many of list's m keys (m <= 256) are above a thread's own; the keys after
+// the last are zeros up to a multiple of 8, so that 8 reads are in flight.
+__device__ __forceinline__ int rank_of(const uint64_t *list, int m, uint64_t key) {
+  int above = 0;
+  for (int j = 0; j < m; j += 8)
+#pragma unroll
+    for (int i = 0; i < 8; i++) above += list[j + i] > key;
+  return above;
 }
 
 // One workgroup per row.
@@ -185,43 +205,71 @@ lp_row_kernel(const float *__restrict__ x, int64_t n, int slices, const Slice *_
               int32_t *__restrict__ top_ids, float *__restrict__ top_lp) {
   __shared__ Slice red[LP_THREADS / 64];
   __shared__ Select sh;
-  __shared__ uint64_t list[LP_LIST];
+  __shared__ uint64_t list[LP_LIST + 8];
   __shared__ int chosen[LP_TOP];
+  __shared__ uint32_t last;  // the least of the chosen groups' values
   const int tid = threadIdx.x;
   const int64_t r = blockIdx.x;
   const float *row = x + r * n;
+  // the groups' keys: (largest value, first)
+  const float *grow = groups ? groups + r * n_groups : nullptr;
+  if (k == 0) n_groups = 0;
+  auto key_of = [](float v, uint32_t i) { return (uint64_t)order_of(v) << 32 | (uint32_t)~i; };
+  if (tid == 0) sh.count = 0;
+  // a thread's values stay in registers (all their loads at once) up to 16
+  float held[LP_HELD];
+#pragma unroll
+  for (int j = 0; j < LP_HELD; j++) {
+    const int i = tid + j * LP_THREADS;
+    held[j] = i < n_groups ? grow[i] : 0.0f;
+  }
+  // a given token's logit, on its way meanwhile
+  const int32_t id = tid < n_ids ? ids[r * n_ids + tid] : -1;
+  const float given = id >= 0 && id < n ? row[id] : -INFINITY;
+  // the parts of the row join while the values come
   Slice a = {-INFINITY, 0.0f, 0.0f, 0.0f};
   for (int i = tid; i < slices; i += LP_THREADS) a = join(a, part[r * slices + i]);
   for (int o = 1; o < 64; o <<= 1)
     a = join(a, Slice{__shfl_xor(a.m, o), __shfl_xor(a.c, o), __shfl_xor(a.s, o), __shfl_xor(a.t, o)});
   if ((tid & 63) == 0) red[tid >> 6] = a;
+  uint64_t best = 0;
+#pragma unroll
+  for (int j = 0; j < LP_HELD; j++) {
+    if (j * LP_THREADS >= n_groups) break;
+    const int i = tid + j * LP_THREADS;
+    const uint64_t key = i < n_groups ? key_of(held[j], i) : 0;
+    best = key > best ? key : best;
+  }
+  for (int i = tid + LP_HELD * LP_THREADS; i < n_groups; i += LP_THREADS) {
+    const uint64_t key = key_of(grow[i], i);
+    best = key > best ? key : best;
+  }
+  sh.tmax[tid] = best;
   __syncthreads();
   a = red[0];
   for (int w = 1; w < LP_THREADS / 64; w++) a = join(a, red[w]);
   // a row of -inf alone has no distribution: log p is -inf, H 0
   const bool none = a.m == -INFINITY && a.s == a.s;
-  const float log_z = logf(a.c) + log1pf(a.s / a.c);
+  const float log_z = a.c == 1.0f ? log1pf(a.s) : logf(a.c) + log1pf(a.s / a.c);
   auto log_p = [&](float v) {
     if (none) return -INFINITY;
-    return v == a.m ? -log_z : (v - a.m) - log_z;
+    return v == a.m ? -log_z : (v - a.m) - log_z;  // (+inf, or equal: no inf - inf)
   };
   if (entropy && tid == 0) entropy[r] = none ? 0.0f : log_z - a.t / (a.c + a.s);
-  if (tid < n_ids) {
-    const int32_t id = ids[r * n_ids + tid];
-    id_lp[r * n_ids + tid] = id >= 0 && id < n ? log_p(row[id]) : -INFINITY;
-  }
+  if (tid < n_ids) id_lp[r * n_ids + tid] = id >= 0 && id < n ? log_p(given) : -INFINITY;
   if (k == 0) return;
-  // the groups: keys (largest value, first), those at or above the cut
-  const float *grow = groups + r * n_groups;
-  auto key_of = [](float v, uint32_t i) { return (uint64_t)order_of(v) << 32 | (uint32_t)~i; };
-  if (tid == 0) sh.count = 0;
-  uint64_t best = 0;
-  for (int i = tid; i < n_groups; i += LP_THREADS) {
-    const uint64_t key = key_of(grow[i], i);
-    best = key > best ? key : best;
+  // the groups at or above the cut; a few more than k may stay, as many as the
+  // list holds
+  const int per = (n_groups + LP_THREADS - 1) / LP_THREADS, hold = LP_LIST / per;
+  const uint64_t cut = cut_of(sh.tmax, k, 2 * k < hold ? 2 * k : hold);
+#pragma unroll
+  for (int j = 0; j < LP_HELD; j++) {
+    if (j * LP_THREADS >= n_groups) break;
+    const int i = tid + j * LP_THREADS;
+    const uint64_t key = i < n_groups ? key_of(held[j], i) : 0;
+    if (key && key >= cut) list[atomicAdd(&sh.count, 1)] = key;
   }
-  uint64_t cut = kth_of_threads(sh, best, k);
-  for (int i = tid; i < n_groups; i += LP_THREADS) {
+  for (int i = tid + LP_HELD * LP_THREADS; i < n_groups; i += LP_THREADS) {
     const uint64_t key = key_of(grow[i], i);
     if (key >= cut) list[atomicAdd(&sh.count, 1)] = key;
   }
@@ -230,35 +278,48 @@ lp_row_kernel(const float *__restrict__ x, int64_t n, int slices, const Slice *_
   __syncthreads();
   m = narrow(sh, list, m, k);
   const int kg = k < n_groups ? k : n_groups;
+  if (tid < 8) list[m + tid] = 0;
+  __syncthreads();
   if (tid < m) {
     const uint64_t key = list[tid];
-    int above = 0;
-    for (int j = 0; j < m; j++) above += list[j] > key;
+    const int above = rank_of(list, m, key);
     if (above < kg) chosen[above] = (int)~(uint32_t)key;
-    if (above == kg - 1) sh.cut = key;
+    if (above == kg - 1) last = (uint32_t)(key >> 32);
   }
   if (tid == 0) sh.count = 0;
   __syncthreads();
   // their tokens: at or above the last chosen group's largest value
-  const uint32_t floor_v = (uint32_t)(sh.cut >> 32);
-  for (int i = tid; i < kg * LP_GROUP; i += LP_THREADS) {
-    const int64_t c = (int64_t)chosen[i / LP_GROUP] * LP_GROUP + i % LP_GROUP;
-    if (c >= n) continue;
-    const uint64_t key = key_of(row[c], (uint32_t)c);
-    if ((uint32_t)(key >> 32) >= floor_v || kg < k) list[atomicAdd(&sh.count, 1)] = key;
+  const uint32_t floor_v = last;
+  constexpr int IT = LP_LIST / LP_THREADS;
+  float x_of[IT];
+#pragma unroll
+  for (int j = 0; j < IT; j++) {
+    const int i = tid + j * LP_THREADS;
+    const int64_t c = i < kg * LP_GROUP ? (int64_t)chosen[i / LP_GROUP] * LP_GROUP + i % LP_GROUP : n;
+    x_of[j] = c < n ? row[c] : 0.0f;
+  }
+#pragma unroll
+  for (int j = 0; j < IT; j++) {
+    if (j * LP_THREADS >= kg * LP_GROUP) break;
+    const int i = tid + j * LP_THREADS;
+    const int64_t c = i < kg * LP_GROUP ? (int64_t)chosen[i / LP_GROUP] * LP_GROUP + i % LP_GROUP : n;
+    const uint64_t key = key_of(x_of[j], (uint32_t)c);
+    if (c < n && ((uint32_t)(key >> 32) >= floor_v || kg < k)) list[atomicAdd(&sh.count, 1)] = key;
   }
   __syncthreads();
   m = sh.count;
   __syncthreads();
   m = narrow(sh, list, m, k);
+  if (tid < 8) list[m + tid] = 0;
+  __syncthreads();
   if (tid < m) {
     const uint64_t key = list[tid];
-    int above = 0;
-    for (int j = 0; j < m; j++) above += list[j] > key;
+    const int above = rank_of(list, m, key);
     if (above < k) {
       const uint32_t id = ~(uint32_t)key;
       if (top_ids) top_ids[r * k + above] = (int32_t)id;
-      if (top_lp) top_lp[r * k + above] = log_p(row[id]);
+      // (a NaN is back as -inf, but then log Z is NaN)
+      if (top_lp) top_lp[r * k + above] = log_p(value_of((uint32_t)(key >> 32)));
     }
   }
 }
