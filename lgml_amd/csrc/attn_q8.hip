@@ -53,6 +53,18 @@ struct Q8Frag {
   static constexpr int TILE = 68 * D, NB = D / 32, J = D / 64, DT = D / 16;
 };
 
+// The largest v of a row's four quads: lanes 16, then 32 apart change places on
+// the vector ALU (a shuffle goes through the LDS unit, which the shared kernel's
+// operands fill).
+__device__ __forceinline__ float quads_max(float v) {
+  const uint32_t a = __builtin_bit_cast(uint32_t, v);
+  const auto p = __builtin_amdgcn_permlane16_swap(a, a, false, false);
+  v = fmaxf(__builtin_bit_cast(float, (uint32_t)p[0]), __builtin_bit_cast(float, (uint32_t)p[1]));
+  const uint32_t b = __builtin_bit_cast(uint32_t, v);
+  const auto q = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+  return fmaxf(__builtin_bit_cast(float, (uint32_t)q[0]), __builtin_bit_cast(float, (uint32_t)q[1]));
+}
+
 // q row pieces -> B operands, hi and lo, of the row scaled by 2^(15 - e); the
 // factor of the scores that undoes it.
 template <int NB>
@@ -63,8 +75,7 @@ __device__ __forceinline__ float split_q(const f32x4 (&qa)[2 * NB], bool rvalid,
   for (int i = 0; i < 2 * NB; i++)
 #pragma unroll
     for (int j = 0; j < 4; j++) mx = fmaxf(mx, fabsf(qa[i][j]));
-  mx = fmaxf(mx, __shfl_xor(mx, 16));
-  mx = fmaxf(mx, __shfl_xor(mx, 32));
+  mx = quads_max(mx);
   int e = __builtin_amdgcn_frexp_expf(mx);
   e = e < -110 ? -110 : e;
   const float up = rvalid ? pow2(15 - e) : 0.0f;
@@ -80,7 +91,8 @@ __device__ __forceinline__ float split_q(const f32x4 (&qa)[2 * NB], bool rvalid,
 }
 
 // Scores (scaled, in units of log2) -> P in place, the running maximum and sum,
-// the rescale of O^T. masked: cells without a bit in word are dropped.
+// the rescale of O^T. masked: cells without a bit in word are dropped. l is of the
+// lane's own cells; the quads' add up at the end.
 template <int DT>
 __device__ __forceinline__ void softmax_q8(f32x4 (&st)[4], float rscale, bool masked, uint64_t word,
                                            int quad, float &m, float &l, f32x4 (&o)[DT]) {
@@ -98,8 +110,7 @@ __device__ __forceinline__ void softmax_q8(f32x4 (&st)[4], float rscale, bool ma
   for (int ct = 0; ct < 4; ct++)
 #pragma unroll
     for (int i = 0; i < 4; i++) mx = fmaxf(mx, st[ct][i]);
-  mx = fmaxf(mx, __shfl_xor(mx, 16));
-  mx = fmaxf(mx, __shfl_xor(mx, 32));
+  mx = quads_max(mx);
   const float m_new = fmaxf(m, mx);
   const float m_use = m_new == -INFINITY ? 0.0f : m_new;
   float rs = 0.0f;
@@ -110,8 +121,6 @@ __device__ __forceinline__ void softmax_q8(f32x4 (&st)[4], float rscale, bool ma
       st[ct][i] = __builtin_amdgcn_exp2f(st[ct][i] - m_use);  // exp2(-inf) = 0
       rs += st[ct][i];
     }
-  rs += __shfl_xor(rs, 16);
-  rs += __shfl_xor(rs, 32);
   if (__builtin_amdgcn_ballot_w64(m_new != m)) {
     const float alpha = __builtin_amdgcn_exp2f(m - m_use);
     l *= alpha;
@@ -139,8 +148,7 @@ __device__ __forceinline__ float weigh_p(const f32x4 (&st)[4], u32x4 s0, u32x4 s
   f16x4 b4 = __builtin_elementwise_max(f16x4{big[0], big[1], big[2], big[3]},
                                        f16x4{big[4], big[5], big[6], big[7]});
   float mx = fmaxf(fmaxf((float)b4[0], (float)b4[1]), fmaxf((float)b4[2], (float)b4[3]));
-  mx = fmaxf(mx, __shfl_xor(mx, 16));
-  mx = fmaxf(mx, __shfl_xor(mx, 32));
+  mx = quads_max(mx);
   const int ex = __builtin_amdgcn_frexp_expf(mx);  // mx in [2^(ex - 1), 2^ex)
   const float up = pow2(15 - ex);
   // hi by truncation, two at a time: lo takes up what it leaves
@@ -230,7 +238,7 @@ __device__ __forceinline__ void values_q8(f32x4 (&o)[D / 16], const f32x4 (&st)[
   if (plain) {
     // a step reads the next 16 dims' V (and makes the next block's P dv) while
     // the products of this one run
-    f16x8 ph[2], pl[2], hi[2][2], lo[2][2], v[2][2];
+    f16x8 ph[2], pl[2], hi[2], lo[2], v[2][2];
     split_p(st, ph, pl);
     auto fetch = [&](int t) {
 #pragma unroll
@@ -240,9 +248,8 @@ __device__ __forceinline__ void values_q8(f32x4 (&o)[D / 16], const f32x4 (&st)[
 #pragma unroll
       for (int h = 0; h < 2; h++) {
         const f16x8 dv = __builtin_bit_cast(f16x8, scale(b, h));
-        f16x8 &x = hi[b & 1][h];
-        x = ph[h] * dv;
-        lo[b & 1][h] = __builtin_elementwise_fma(pl[h], dv, __builtin_elementwise_fma(ph[h], dv, -x));
+        hi[h] = ph[h] * dv;
+        lo[h] = __builtin_elementwise_fma(pl[h], dv, __builtin_elementwise_fma(ph[h], dv, -hi[h]));
       }
     };
     fetch(0);
@@ -252,11 +259,11 @@ __device__ __forceinline__ void values_q8(f32x4 (&o)[D / 16], const f32x4 (&st)[
     for (int t = 0; t < D / 16; t++) {
 #pragma unroll
       for (int kc = 0; kc < 2; kc++) {
-        o[t] = mfma16q(v[t & 1][kc], hi[t >> 1 & 1][kc], o[t]);
-        o[t] = mfma16q(v[t & 1][kc], lo[t >> 1 & 1][kc], o[t]);
+        o[t] = mfma16q(v[t & 1][kc], hi[kc], o[t]);
+        o[t] = mfma16q(v[t & 1][kc], lo[kc], o[t]);
       }
       if (t + 1 < D / 16) fetch(t + 1);
-      if (t % 2 == 0 && t / 2 + 1 < NB) weigh(t / 2 + 1);
+      if (t % 2 == 1 && t / 2 + 1 < NB) weigh(t / 2 + 1);
       __builtin_amdgcn_sched_barrier(0);
     }
     return;
@@ -453,6 +460,8 @@ paged_attn_q8_kernel(const float *__restrict__ q, int H, int Hkv, float scale_lo
   };
   for (int blk = blo; blk + 1 < bhi; blk++) block(blk, std::true_type{});
   if (blo < bhi) block(bhi - 1, std::false_type{});
+  l += __shfl_xor(l, 16);
+  l += __shfl_xor(l, 32);
   finish_item<D>(o, m, l * Q8_P, mg, rvalid, tok0, rtok, rhead, ntok, G, row, quad, item, kvh, Hkv, H, out,
                  planes, npad, xf, part);
 }
@@ -515,7 +524,11 @@ paged_attn_q8_shared_kernel(const float *__restrict__ q, int H, int Hkv, float s
 
   const int32_t *bt = block_tab + (int64_t)s * max_blocks;
   u32x4 raw[CH], sraw;
+  // (a thread's places are made anew each block, from an opaque copy of its number:
+  // held over the loop they are a dozen registers, and heads of 256 have none)
   auto load = [&](int blk) {
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));
     const int64_t at = ((int64_t)bt[blk] * Hkv + kvh) * F::TILE;
 #pragma unroll
     for (int i = 0; i < CH; i++) {
@@ -527,6 +540,8 @@ paged_attn_q8_shared_kernel(const float *__restrict__ q, int H, int Hkv, float s
       sraw = *(const u32x4 *)((tid < NB * 8 ? kpool : vpool) + at + 64 * D + tid % (NB * 8) * 16u);
   };
   auto store = [&](int buf) {
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));
 #pragma unroll
     for (int i = 0; i < CH; i++) {
       const int c = i * 64 * W + tid;
@@ -622,6 +637,8 @@ paged_attn_q8_shared_kernel(const float *__restrict__ q, int H, int Hkv, float s
                  [&](int t, int kc) { return *(const f16x8 *)(vb[0] + va[kc] + t * 1024); });
   }
   if (!active) return;
+  l += __shfl_xor(l, 16);
+  l += __shfl_xor(l, 32);
   finish_item<D>(o, m, l * Q8_P, mg, rvalid, tok0, rtok, rhead, ntok, G, row, quad, item, kvh, Hkv, H, out,
                  planes, npad, xf, part);
 }
