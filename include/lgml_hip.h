@@ -110,8 +110,9 @@ int lgmlh_set_rows_f16(uint16_t *dst, int64_t dst_rows, int64_t row, const float
  * (cache types q8_0, lua/lgml/kv.lua:14-20, without its rotation of the
  * rows), 17/32 of the f16 pool's bytes. The same blocks, cell ids, plans and
  * bookkeeping; head sizes 64, 128 and 256. A block of one layer's K (or V) is
- * 68 * Hkv * D bytes, blocks one after the other, so whole blocks are copied,
- * spilled and grown as bytes. Within a (block, KV head) tile of 68 * D bytes:
+ * 68 * Hkv * D bytes, blocks one after the other: lgmlh_kv_block_bytes,
+ * lgmlh_kv_block_host and lgmlh_kv_grow, which copy whole blocks, take such a
+ * pool as one of f16 heads of 17 D / 32. Within a (block, KV head) tile of 68 * D bytes:
  * 64 * D int8 values, then f16 scales [D / 32][64 cells]; values of K
  * [D / 64][cell][4][2][8] with dim 64 j + 32 b + 8 q + e at (j, cell, q, b,
  * e), of V [D][4][2][8] with cell 32 b + 8 q + e at (d, q, b, e).
@@ -471,6 +472,13 @@ int lgmlh_qkv_rope_store(float *qkv, int64_t n, int n_head, int n_head_kv, int h
     int n_rot, int neox, float freq_base, const float *freq_factors, const float *q_norm,
     const float *k_norm, float eps, const int32_t *pos, void *kpool, void *vpool,
     int64_t n_cells, const int64_t *cells, float *q_out, void *stream);
+/* lgmlh_qkv_rope_store into Q8_0 pools (the values and bytes of
+ * lgmlh_kv_store_q8 on the normed and roped rows); cells of one call are
+ * distinct (device data here, not checked). */
+int lgmlh_qkv_rope_store_q8(float *qkv, int64_t n, int n_head, int n_head_kv, int head_dim,
+    int n_rot, int neox, float freq_base, const float *freq_factors, const float *q_norm,
+    const float *k_norm, float eps, const int32_t *pos, void *kpool, void *vpool,
+    int64_t n_cells, const int64_t *cells, float *q_out, void *stream);
 /* silu(g) * u (transformer.lua:2048) for gu = (n, 2F) rows [g | u]; out f32 or f16. */
 int lgmlh_swiglu(const float *gu, int64_t n, int64_t F, void *out, int out_type, void *stream);
 /* gelu(g) * u, the gemma FFN (graph:geglu_split, src/ops_nn.c:165-172;
@@ -604,6 +612,12 @@ typedef struct {
  * products queue behind the other's. If creating them fails, or a fifth
  * caller stream asks, the pass runs on the caller's stream alone. */
 int lgmlh_forward(const lgmlh_model *m, const lgmlh_ubatch *ub, const lgmlh_ubatch *ub_ring,
+    const int32_t *out_rows, int n_out, float *logits, void *workspace, size_t ws_bytes,
+    lgmlh_trace *trace, void *stream);
+/* lgmlh_forward of a model whose K / V pools (and ring pools) are in Q8_0
+ * (lgmlh_kv_q8_layer_bytes; the layers' kpool / vpool): same plans, workspace
+ * and logit rows. Head sizes 64, 128 and 256. */
+int lgmlh_forward_q8(const lgmlh_model *m, const lgmlh_ubatch *ub, const lgmlh_ubatch *ub_ring,
     const int32_t *out_rows, int n_out, float *logits, void *workspace, size_t ws_bytes,
     lgmlh_trace *trace, void *stream);
 /* Destroy the side streams and events that lgmlh_forward made for the

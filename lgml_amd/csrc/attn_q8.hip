@@ -16,7 +16,8 @@
 // are at most 2^-38 of it off. Else P dv is made in f32 and scaled by the power
 // of two that puts the row's largest dv at 2^14 to 2^15, the products scaled back
 // as they add to O^T; a cell that a row does not see has p and dv as zeros, so that
-// nothing in it (a scale that is infinite or NaN) reaches the row.
+// nothing in it (a scale that is infinite or NaN) reaches the row. Which of the two
+// a row takes in a block that it does not see all of goes by the cells it does see.
 #include <type_traits>
 
 #include "attn.h"
@@ -131,10 +132,10 @@ __device__ __forceinline__ void softmax_q8(f32x4 (&st)[4], float rscale, bool ma
   m = m_new;
 }
 
-// P dv of one block of 32 dims as f16 hi + lo (cells 32 h + 8 quad + e), scaled;
-// the factor that undoes it. s0, s1: the lane's cells' scales.
-__device__ __forceinline__ float weigh_p(const f32x4 (&st)[4], u32x4 s0, u32x4 s1, bool masked,
-                                         uint64_t word, int quad, f16x8 (&ph)[2], f16x8 (&pl)[2]) {
+// The scales of a lane's cells (32 h + 8 quad + e) of one block of 32 dims, those
+// of cells that word leaves out as zeros, and the row's largest.
+__device__ __forceinline__ float row_scales(u32x4 s0, u32x4 s1, bool masked, uint64_t word, int quad,
+                                            f16x8 (&dv)[2]) {
   if (masked) {  // wave-uniform
 #pragma unroll
     for (int i = 0; i < 4; i++) {
@@ -143,12 +144,18 @@ __device__ __forceinline__ float weigh_p(const f32x4 (&st)[4], u32x4 s0, u32x4 s
       s1[i] &= (b1 & 1 ? 0xffffu : 0) | (b1 & 2 ? 0xffff0000u : 0);
     }
   }
-  const f16x8 dv[2] = {__builtin_bit_cast(f16x8, s0), __builtin_bit_cast(f16x8, s1)};
-  f16x8 big = __builtin_elementwise_max(dv[0], dv[1]);
-  f16x4 b4 = __builtin_elementwise_max(f16x4{big[0], big[1], big[2], big[3]},
-                                       f16x4{big[4], big[5], big[6], big[7]});
-  float mx = fmaxf(fmaxf((float)b4[0], (float)b4[1]), fmaxf((float)b4[2], (float)b4[3]));
-  mx = quads_max(mx);
+  dv[0] = __builtin_bit_cast(f16x8, s0);
+  dv[1] = __builtin_bit_cast(f16x8, s1);
+  const f16x8 big = __builtin_elementwise_max(dv[0], dv[1]);
+  const f16x4 b4 = __builtin_elementwise_max(f16x4{big[0], big[1], big[2], big[3]},
+                                             f16x4{big[4], big[5], big[6], big[7]});
+  return quads_max(fmaxf(fmaxf((float)b4[0], (float)b4[1]), fmaxf((float)b4[2], (float)b4[3])));
+}
+
+// P dv of one block of 32 dims as f16 hi + lo, scaled by the row's largest dv; the
+// factor that undoes it.
+__device__ __forceinline__ float weigh_p(const f32x4 (&st)[4], const f16x8 (&dv)[2], float mx,
+                                         f16x8 (&ph)[2], f16x8 (&pl)[2]) {
   const int ex = __builtin_amdgcn_frexp_expf(mx);  // mx in [2^(ex - 1), 2^ex)
   const float up = pow2(15 - ex);
   // hi by truncation, two at a time: lo takes up what it leaves
@@ -167,13 +174,17 @@ __device__ __forceinline__ float weigh_p(const f32x4 (&st)[4], u32x4 s0, u32x4 s
   return pow2(ex - 15);
 }
 
+// Whether a block of dims whose largest scale is mx goes by the packed products.
+__device__ __forceinline__ bool plain_scale(float mx) {
+  return mx == 0.0f || (mx >= 0x1p-10f && mx < 4.0f);
+}
 // Whether a lane's 8 scales of a group of 32 dims (the group's 64 in 8 aligned
 // lanes) leave the group to the packed products.
 __device__ __forceinline__ bool plain_scales(u32x4 sc) {
   const f16x8 d = __builtin_bit_cast(f16x8, sc);
   const f16x4 a = __builtin_elementwise_max(f16x4{d[0], d[1], d[2], d[3]}, f16x4{d[4], d[5], d[6], d[7]});
-  const float mx = group_max<8>(fmaxf(fmaxf((float)a[0], (float)a[1]), fmaxf((float)a[2], (float)a[3])));
-  return mx == 0.0f || (mx >= 0x1p-10f && mx < 4.0f);
+  return plain_scale(
+      group_max<8>(fmaxf(fmaxf((float)a[0], (float)a[1]), fmaxf((float)a[2], (float)a[3]))));
 }
 
 // P (cells 32 h + 8 quad + e) as f16 hi + lo, Q8_P times as large.
@@ -268,21 +279,60 @@ __device__ __forceinline__ void values_q8(f32x4 (&o)[D / 16], const f32x4 (&st)[
     }
     return;
   }
+  if (!masked) {
+#pragma unroll
+    for (int b = 0; b < NB; b++) {
+      f16x8 dv[2], ph[2], pl[2];
+      const float mx = row_scales(scale(b, 0), scale(b, 1), false, 0, quad, dv);
+      const float back = Q8_P * weigh_p(st, dv, mx, ph, pl);
+#pragma unroll
+      for (int t = 2 * b; t < 2 * b + 2; t++) {
+        f32x4 acc = {0, 0, 0, 0};
+#pragma unroll
+        for (int kc = 0; kc < 2; kc++) {
+          const f16x8 v = frag(t, kc);
+          acc = mfma16q(v, ph[kc], acc);
+          acc = mfma16q(v, pl[kc], acc);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) o[t][i] = fmaf(acc[i], back, o[t][i]);
+        here(o[t]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    return;
+  }
+  // Some rows do not see all of the block. Both ways, and each row takes the one
+  // that the scales of the cells it sees ask for: that depends on nothing else, so
+  // a row has the same bits in any group of rows.
+  bool row_plain = true;
+#pragma unroll 1
+  for (int b = 0; b < NB; b++) {
+    f16x8 dv[2];
+    row_plain &= plain_scale(row_scales(scale(b, 0), scale(b, 1), true, word, quad, dv));
+  }
+  f16x8 fh[2], fl[2];
+  split_p(st, fh, fl);
 #pragma unroll
   for (int b = 0; b < NB; b++) {
-    f16x8 ph[2], pl[2];
-    const float back = Q8_P * weigh_p(st, scale(b, 0), scale(b, 1), masked, word, quad, ph, pl);
+    f16x8 dv[2], ph[2], pl[2];
+    const float mx = row_scales(scale(b, 0), scale(b, 1), true, word, quad, dv);
+    const float back = Q8_P * weigh_p(st, dv, mx, ph, pl);
 #pragma unroll
     for (int t = 2 * b; t < 2 * b + 2; t++) {
-      f32x4 acc = {0, 0, 0, 0};
+      f32x4 acc = {0, 0, 0, 0}, fast = o[t];
 #pragma unroll
       for (int kc = 0; kc < 2; kc++) {
         const f16x8 v = frag(t, kc);
         acc = mfma16q(v, ph[kc], acc);
         acc = mfma16q(v, pl[kc], acc);
+        const f16x8 hi = fh[kc] * dv[kc];
+        const f16x8 lo = __builtin_elementwise_fma(fl[kc], dv[kc], __builtin_elementwise_fma(fh[kc], dv[kc], -hi));
+        fast = mfma16q(v, hi, fast);
+        fast = mfma16q(v, lo, fast);
       }
 #pragma unroll
-      for (int i = 0; i < 4; i++) o[t][i] = fmaf(acc[i], back, o[t][i]);
+      for (int i = 0; i < 4; i++) o[t][i] = row_plain ? fast[i] : fmaf(acc[i], back, o[t][i]);
       here(o[t]);
     }
     __builtin_amdgcn_sched_barrier(0);

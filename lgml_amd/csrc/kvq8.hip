@@ -1,32 +1,19 @@
 // The KV pool in Q8_0 (8-bit values, an f16 scale per 32), and moves of cells
 // within a pool of either type (gfx950).
-//
-// A (block, KV head) tile of K or V is 68 D bytes: 64 D int8 values, then the
-// f16 scales [D / 32][64 cells]. Values are placed so that one 16-byte load a
-// lane gives its part of two of the attention's 16x16x32 operands:
-//   K: [D / 64][cell][4][2][8], dim 64 j + 32 b + 8 q + e at (j, cell, q, b, e)
-//   V: [D][4][2][8], cell 32 b + 8 q + e at (d, q, b, e)
-// The scales' order is the one in which a lane has 8 cells of a block of 32
-// dims in 16 bytes.
 #include <type_traits>
 
-#include "common.h"
+#include "kvq8.h"
 
 namespace lgmlh {
 
+// The places (kvq8.h) for a head size: K's dims 8 g8 .. + 7 are 8 bytes, V's cells 8 c
+// .. + 7 of a dim too.
 template <int D>
 struct Q8Tile {
-  static constexpr int bytes = 68 * D, scales = 64 * D;
-  // byte of K's dims 8 g8 .. + 7 of a cell
-  __device__ static int k_at(int cell, int g8) {
-    return ((g8 / 8 * 64 + cell) * 4 + g8 % 4) * 16 + g8 % 8 / 4 * 8;
-  }
-  // byte of V's (d, cell); cells 8 c .. 8 c + 7 are consecutive
-  __device__ static int v_at(int d, int cell) {
-    return d * 64 + cell % 32 / 8 * 16 + cell / 32 * 8 + cell % 8;
-  }
-  // byte of the scale of dims 32 b .. + 31
-  __device__ static int scale_at(int b, int cell) { return scales + 2 * (b * 64 + cell); }
+  static constexpr int bytes = q8_tile_bytes(D);
+  __device__ static int k_at(int cell, int g8) { return q8_k_at(cell, 8 * g8); }
+  __device__ static int v_at(int d, int cell) { return q8_v_at(d, cell); }
+  __device__ static int scale_at(int b, int cell) { return q8_scale_at(D, b, cell); }
 };
 
 // A workgroup takes W consecutive tokens (64, or 16 of a call of few) of one head
@@ -87,13 +74,6 @@ struct Q8Window {
 
 // Threads for n lone tokens: the power of two that holds them, as bits.
 __device__ __forceinline__ int lone_bits(int n) { return n > 1 ? 32 - __builtin_clz(n - 1) : 0; }
-
-// To the nearest integer, halves away from zero, below 2^23: the largest number
-// under a half takes a half up to the next integer (its sum rounds there) and
-// nothing below it.
-__device__ __forceinline__ int round_away(float x) {
-  return (int)(x + __builtin_copysignf(0x1.fffffep-2f, x));
-}
 
 // x (n, Hkv D) f32 rows into their cells. Per 32 values (8 lanes), the steps of
 // quantize_row_q8_0: d = amax / 127, q = round(x (1 / d)) with halves away from

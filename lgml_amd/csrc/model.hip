@@ -29,7 +29,12 @@ int qkv_rope_store_dev(float *qkv, int64_t n, int n_head, int n_head_kv, int hea
                        int neox, float freq_base, const float *freq_factors, const float *q_norm,
                        const float *k_norm, float eps, const int32_t *pos, void *kpool,
                        void *vpool, int64_t n_cells, const int64_t *cells, float *q_out,
-                       void *stream, Pending pa, Pending pb, int vmode, const float *table);
+                       void *stream, Pending pa, Pending pb, int vmode, const float *table,
+                       bool q8);
+int paged_attention_q8_dev(const float *q, int n_head, int n_head_kv, int head_dim, float scale,
+                           const void *kpool, const void *vpool, const lgmlh_ubatch *ub, float *out,
+                           f16 *planes, int64_t npad, void *workspace, size_t workspace_bytes,
+                           hipStream_t st, int xf);
 int rope_table_dev(const int32_t *pos, int64_t n, int n_rot, float freq_base,
                    const float *freq_factors, float *table, hipStream_t st);
 size_t partial_bytes(int type, int64_t M, int64_t K, int64_t N);
@@ -320,10 +325,10 @@ extern "C" int lgmlh_forward_release(void) {
   return LGMLH_OK;
 }
 
-extern "C" int lgmlh_forward(const lgmlh_model *m, const lgmlh_ubatch *ub,
-                             const lgmlh_ubatch *ub_ring, const int32_t *out_rows, int n_out,
-                             float *logits, void *workspace, size_t ws_bytes, lgmlh_trace *trace,
-                             void *stream) {
+// The pass of lgmlh_forward (q8: over Q8_0 pools).
+static int forward_impl(const lgmlh_model *m, const lgmlh_ubatch *ub, const lgmlh_ubatch *ub_ring,
+                        const int32_t *out_rows, int n_out, float *logits, void *workspace,
+                        size_t ws_bytes, lgmlh_trace *trace, void *stream, bool q8) {
   if (!m || !ub || !logits || !workspace || !m->layers || m->n_layer <= 0) {
     set_error("forward: bad arguments");
     return LGMLH_EINVAL;
@@ -495,7 +500,7 @@ extern "C" int lgmlh_forward(const lgmlh_model *m, const lgmlh_ubatch *ub,
     LGMLH_TRY(qkv_rope_store_dev(qkv, z.N, (int)z.H, d.Hkv, d.D, d.n_rot, m->rope_neox, rk.base,
                                  rk.ff, L.q_norm, L.k_norm, m->eps, ub->pos, L.kpool, L.vpool,
                                  L.swa ? m->ring_cells : m->n_cells, lub->cells, q, st, p_qk, p_v,
-                                 vmode, tab));
+                                 vmode, tab, q8));
     // a quantized output product takes its X (split planes, ggml's Q8_0
     // blocks, or its Q8_K blocks when a block's heads are of one KV head's
     // group) from the attention (and merge) kernels themselves; heads too
@@ -505,9 +510,9 @@ extern "C" int lgmlh_forward(const lgmlh_model *m, const lgmlh_ubatch *ub,
                o_split = oq && (xo == XF_Q8K ? attn_q8k_fits(d.D, (int)z.H / d.Hkv) : d.D >= 32);
     {
       Span sp(trace, LGMLH_TRACE_ATTN, st);
-      LGMLH_TRY(paged_attention_dev(q, (int)z.H, d.Hkv, d.D, scale, L.kpool, L.vpool,
-                                    lub, o_split ? nullptr : att, o_split ? xs : nullptr,
-                                    split_npad(z.N), aws, z.attn_ws, st, xo));
+      LGMLH_TRY((q8 ? paged_attention_q8_dev : paged_attention_dev)(
+          q, (int)z.H, d.Hkv, d.D, scale, L.kpool, L.vpool, lub, o_split ? nullptr : att,
+          o_split ? xs : nullptr, split_npad(z.N), aws, z.attn_ws, st, xo));
     }
     if (oq && !o_split)
       LGMLH_TRY(split_x(att, LGMLH_F32, z.N, z.H * d.D, xs, st, xfo(L.wo_type)));
@@ -574,4 +579,28 @@ extern "C" int lgmlh_forward(const lgmlh_model *m, const lgmlh_ubatch *ub,
     if (m->softcap > 0) LGMLH_TRY(softcap_dev(logits, (int64_t)n_out * z.V, m->softcap, st));
   }
   return LGMLH_OK;
+}
+
+extern "C" int lgmlh_forward(const lgmlh_model *m, const lgmlh_ubatch *ub,
+                             const lgmlh_ubatch *ub_ring, const int32_t *out_rows, int n_out,
+                             float *logits, void *workspace, size_t ws_bytes, lgmlh_trace *trace,
+                             void *stream) {
+  return forward_impl(m, ub, ub_ring, out_rows, n_out, logits, workspace, ws_bytes, trace, stream,
+                      false);
+}
+
+extern "C" int lgmlh_forward_q8(const lgmlh_model *m, const lgmlh_ubatch *ub,
+                                const lgmlh_ubatch *ub_ring, const int32_t *out_rows, int n_out,
+                                float *logits, void *workspace, size_t ws_bytes,
+                                lgmlh_trace *trace, void *stream) {
+  if (m && m->layers)
+    for (int il = 0; il < m->n_layer; il++) {
+      const int D = dims_of(m, m->layers[il]).D;
+      if (D != 64 && D != 128 && D != 256) {
+        set_error("forward_q8: layer %d has heads of %d (64, 128, 256)", il, D);
+        return LGMLH_EINVAL;
+      }
+    }
+  return forward_impl(m, ub, ub_ring, out_rows, n_out, logits, workspace, ws_bytes, trace, stream,
+                      true);
 }

@@ -4,6 +4,7 @@
 #include <stdio.h>
 
 #include "common.h"
+#include "kvq8.h"
 #include "quant.h"
 #include "split.h"
 
@@ -229,7 +230,9 @@ __global__ void rope_table_kernel(const int32_t *__restrict__ pos, int n_rot, fl
 // (q_norm / k_norm; on gemma the V norm without a weight, :1782-1784),
 // rope for q and k heads, and the store: q to q_out, k and v to their pool
 // cell. With QKV_V_FROM_K a V head is the raw K head (transformer.lua:1779).
+// Q8: the pool is in Q8_0 (kvq8.h); a block of 32 values is half a wave's.
 constexpr int QKV_HEADS = 8;
+template <bool Q8>
 __global__ void __launch_bounds__(64 * QKV_HEADS)
 qkv_rope_store_kernel(const float *__restrict__ qkv, int H, int Hkv, int D, int n_rot, int neox,
                       float theta_scale, const float *__restrict__ ff,
@@ -310,6 +313,17 @@ qkv_rope_store_kernel(const float *__restrict__ qkv, int H, int Hkv, int D, int 
   const int64_t cell = cells[t];
   if (cell < 0 || cell >= n_cells) return;  // a cell outside the pool is never written
   const int64_t b = cell / KV_BLOCK, o = cell % KV_BLOCK;
+  if constexpr (Q8) {
+    const int hh = is_k ? h - H : h - H - Hkv;
+    uint8_t *tile = (uint8_t *)(is_k ? kp : vp) + (b * Hkv + hh) * (int64_t)q8_tile_bytes(D);
+    for (int d = lane; d < D; d += 64) {  // D is a multiple of 64
+      const float x = v[d];
+      const float dd = group_max<32>(fabsf(x)) / 127.0f, id = dd != 0.0f ? 1.0f / dd : 0.0f;
+      tile[is_k ? q8_k_at((int)o, d) : q8_v_at(d, (int)o)] = (uint8_t)round_away(x * id);
+      if (lane % 32 == 0) *(uint16_t *)(tile + q8_scale_at(D, d / 32, (int)o)) = f2h(dd);
+    }
+    return;
+  }
   if (is_k) {
     const int hk = h - H;
     for (int d = lane; d < D; d += 64) kp[((b * Hkv + hk) * KV_BLOCK + o) * D + d] = f2h(v[d]);
@@ -615,20 +629,21 @@ int qkv_rope_store_dev(float *qkv, int64_t n, int n_head, int n_head_kv,
                                     const float *k_norm, float eps, const int32_t *pos,
                                     void *kpool, void *vpool, int64_t n_cells,
                                     const int64_t *cells, float *q_out, void *stream, Pending pa,
-                       Pending pb, int vmode, const float *table) {
+                       Pending pb, int vmode, const float *table, bool q8) {
   if (!qkv || !pos || !kpool || !vpool || !cells || !q_out || n < 0 || n_head <= 0 ||
       n_head_kv <= 0 || head_dim <= 0 || head_dim % 8 || head_dim > 1024 || n_rot <= 0 ||
       n_rot > head_dim ||
-      n_rot % 2 || n_cells % KV_BLOCK || pa.cols % 8 || pb.cols % 8) {
-    set_error("qkv_rope_store: bad arguments");
+      n_rot % 2 || n_cells % KV_BLOCK || pa.cols % 8 || pb.cols % 8 ||
+      (q8 && head_dim != 64 && head_dim != 128 && head_dim != 256)) {
+    set_error("qkv_rope_store%s: bad arguments", q8 ? "_q8" : "");
     return LGMLH_EINVAL;
   }
   if (n == 0) return LGMLH_OK;
   const float theta_scale = rope_theta_scale(freq_base, n_rot);
   const size_t lds = ((size_t)QKV_HEADS * head_dim + n_rot) * sizeof(float);
   const int groups = (n_head + 2 * n_head_kv + QKV_HEADS - 1) / QKV_HEADS;
-  hipLaunchKernelGGL(qkv_rope_store_kernel, dim3((unsigned)n, (unsigned)groups),
-                     dim3(64 * QKV_HEADS), lds,
+  hipLaunchKernelGGL(q8 ? qkv_rope_store_kernel<true> : qkv_rope_store_kernel<false>,
+                     dim3((unsigned)n, (unsigned)groups), dim3(64 * QKV_HEADS), lds,
                      as_stream(stream), qkv, n_head, n_head_kv, head_dim, n_rot, neox,
                      theta_scale, freq_factors, q_norm, k_norm, eps, pos, (uint16_t *)kpool,
                      (uint16_t *)vpool, cells, n_cells, q_out, pa, pb, vmode, table);
@@ -652,7 +667,18 @@ extern "C" int lgmlh_qkv_rope_store(float *qkv, int64_t n, int n_head, int n_hea
                                     const int64_t *cells, float *q_out, void *stream) {
   return qkv_rope_store_dev(qkv, n, n_head, n_head_kv, head_dim, n_rot, neox, freq_base,
                             freq_factors, q_norm, k_norm, eps, pos, kpool, vpool, n_cells, cells,
-                            q_out, stream, Pending{}, Pending{}, 0, nullptr);
+                            q_out, stream, Pending{}, Pending{}, 0, nullptr, false);
+}
+
+extern "C" int lgmlh_qkv_rope_store_q8(float *qkv, int64_t n, int n_head, int n_head_kv,
+                                       int head_dim, int n_rot, int neox, float freq_base,
+                                       const float *freq_factors, const float *q_norm,
+                                       const float *k_norm, float eps, const int32_t *pos,
+                                       void *kpool, void *vpool, int64_t n_cells,
+                                       const int64_t *cells, float *q_out, void *stream) {
+  return qkv_rope_store_dev(qkv, n, n_head, n_head_kv, head_dim, n_rot, neox, freq_base,
+                            freq_factors, q_norm, k_norm, eps, pos, kpool, vpool, n_cells, cells,
+                            q_out, stream, Pending{}, Pending{}, 0, nullptr, true);
 }
 
 extern "C" int lgmlh_swiglu(const float *gu, int64_t n, int64_t F, void *out, int out_type,

@@ -144,6 +144,10 @@ class PoolSeqs:
     def copy_block(self, src, dst, n):
         """M.copy_block (transformer.lua:989-1007) on the device, every layer."""
         m = self.model
+        if getattr(m, "kv_type", hip.F16) == hip.Q8_0:
+            cells = np.arange(n, dtype=np.int64)
+            m.move_cells(src * BLOCK + cells, dst * BLOCK + cells)
+            return
         D, Hkv = getattr(m, "paged_dims", (m.hp["head_dim"], m.hp["n_head_kv"]))
         for il, (kp, vp) in enumerate(zip(m.kpools, m.vpools)):
             if getattr(m, "swa", None) and m.swa[il]:
@@ -390,7 +394,8 @@ class Engine:
     def block_host(self, b, buf, out):
         m = self.model
         check(hip.lib().lgmlh_kv_block_host(m.pools_dev.data_ptr(), m.n_pools, m.n_cells,
-                                            m.paged_dims[1], m.paged_dims[0], b, buf.data_ptr(),
+                                            m.paged_dims[1], m.block_dim(m.paged_dims[0]), b,
+                                            buf.data_ptr(),
                                             1 if out else 0, stream()))
 
     def spill_block(self, b, key, prio):
@@ -548,7 +553,7 @@ class Engine:
         """The bytes of slot's ring blocks in every sliding layer's K and V
         ring pools (device uint8 views, in layer order)."""
         m, R = self.model, self.ring_blocks
-        bb = hip.lib().lgmlh_kv_block_bytes(m.ring_dims[1], m.ring_dims[0])
+        bb = hip.lib().lgmlh_kv_block_bytes(m.ring_dims[1], m.block_dim(m.ring_dims[0]))
         views = []
         for il, swa in enumerate(m.swa):
             if swa:

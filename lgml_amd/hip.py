@@ -36,6 +36,7 @@ SYMBOLS = (
     "lgmlh_mul_mat_id_ggml", "lgmlh_quantize_act", "lgmlh_forward_release",
     "lgmlh_plan_tree", "lgmlh_paged_attention_q8", "lgmlh_kv_q8_layer_bytes", "lgmlh_kv_store_q8",
     "lgmlh_kv_gather_q8", "lgmlh_kv_move", "lgmlh_log_probs_workspace", "lgmlh_log_probs",
+    "lgmlh_qkv_rope_store_q8", "lgmlh_forward_q8",
 )
 PLAN_TREE, TREE_MAX = -1, 1024
 GATING_SOFTMAX, GATING_SIGMOID = 1, 2
@@ -200,6 +201,8 @@ def _declare(L):
         "lgmlh_log_probs_workspace": ([i64, i64, i32], sz),
         "lgmlh_log_probs": ([vp, i64, i64, vp, i32, vp, vp, i32, vp, vp, vp, sz, vp], i32),
     }
+    sig["lgmlh_qkv_rope_store_q8"] = sig["lgmlh_qkv_rope_store"]
+    sig["lgmlh_forward_q8"] = sig["lgmlh_forward"]
     for name, (args, res) in sig.items():
         f = getattr(L, name)
         f.argtypes = args

@@ -120,6 +120,36 @@ def load_gguf(path, n_cells, ring_cells=0):
     return DeviceModel(hp, w, n_cells, ring_cells)
 
 
+def log_probs(logits, ids=None, top=0):
+    """lgmlh_log_probs of rows of logits (n, vocab) f32 on the device: a dict
+    with entropy (n); of given ids (n, m) int32, lp (n, m); and with top > 0
+    the most likely tokens, top_ids and top_lp (n, top)."""
+    L = hip.lib()
+    if logits.dim() != 2 or logits.dtype != torch.float32 or not logits.is_contiguous():
+        raise ValueError("logits: contiguous f32 rows")
+    n, v = logits.shape
+    m = 0
+    if ids is not None:
+        ids = torch.as_tensor(ids, dtype=torch.int32).to(DEV).contiguous()
+        if ids.dim() != 2 or ids.shape[0] != n:
+            raise ValueError("ids: (%d, m)" % n)
+        m = ids.shape[1]
+
+    def new(*shape, dtype=torch.float32):
+        return torch.empty(shape, dtype=dtype, device=DEV)
+
+    out = {"entropy": new(n)}
+    if m:
+        out["lp"] = new(n, m)
+    if top:
+        out["top_ids"], out["top_lp"] = new(n, top, dtype=torch.int32), new(n, top)
+    ws = _empty(max(L.lgmlh_log_probs_workspace(n, v, top), 16))
+    check(L.lgmlh_log_probs(logits.data_ptr(), n, v, ptr(ids) if m else None, m, ptr(out.get("lp")),
+                            out["entropy"].data_ptr(), top, ptr(out.get("top_ids")),
+                            ptr(out.get("top_lp")), ws.data_ptr(), ws.numel(), stream()))
+    return out
+
+
 class Plan:
     """A planned ubatch (lgmlh_plan), copied to the device. With ring_tab
     (n_seq, ring_blocks) and window, the plan of the sliding-window layers
@@ -218,7 +248,7 @@ class DeviceModel:
     """A llama / qwen3 / qwen3moe / gemma model on the device with its paged
     KV pool (and, for sliding-window layers, ring pools)."""
 
-    def __init__(self, hp, w, n_cells, ring_cells=0, kv_initial=0):
+    def __init__(self, hp, w, n_cells, ring_cells=0, kv_initial=0, kv_type=hip.F16):
         """w: a weights dict of numpy arrays, or a callable source
         w(name, layer, rows, cols) -> (device tensor, type, rows) such as
         generated_weights() (gemma layers then follow workload.gemma_layer).
@@ -226,7 +256,9 @@ class DeviceModel:
         64; the sequences' ring tables index its blocks). kv_initial: the
         paged pool starts at this many cells and grows (grow_pool) up to
         n_cells, as the reference's pool starts at KV_INITIAL and doubles
-        (engine.lua:49, transformer.lua:831-908); 0: n_cells from the start."""
+        (engine.lua:49, transformer.lua:831-908); 0: n_cells from the start.
+        kv_type: hip.F16, or hip.Q8_0 for pools (and rings) of 8-bit values
+        with a scale per 32 (heads of 64, 128 and 256; 17/32 of the bytes)."""
         from . import workload
         L = hip.lib()
         self.hp = hp
@@ -235,6 +267,9 @@ class DeviceModel:
         self.max_cells = int(n_cells)
         self.n_cells = int(kv_initial) if kv_initial else self.max_cells
         self.ring_cells = int(ring_cells)
+        if kv_type not in (hip.F16, hip.Q8_0):
+            raise ValueError("kv_type %r: hip.F16 or hip.Q8_0" % (kv_type,))
+        self.kv_type = kv_type
         assert self.n_cells % 64 == 0 and self.ring_cells % 64 == 0
         assert self.max_cells % 64 == 0 and self.n_cells <= self.max_cells
         self._keep = []
@@ -342,7 +377,11 @@ class DeviceModel:
                 t, ty, _ = repack_concat([mat("down", il, E, F)], F)
                 Ly.wdown, Ly.wdown_type = keep(t).data_ptr(), ty
             # the pool tensors live in kpools / vpools (grow_pool replaces them)
-            kvb_l = L.lgmlh_kv_layer_bytes(self.ring_cells if Ly.swa else self.n_cells, Hl, Dl)
+            nc = self.ring_cells if Ly.swa else self.n_cells
+            kvb_l = (L.lgmlh_kv_q8_layer_bytes if kv_type == hip.Q8_0 else
+                     L.lgmlh_kv_layer_bytes)(nc, Hl, Dl)
+            if kvb_l < 0:
+                raise ValueError("a Q8_0 pool takes heads of 64, 128 or 256, not %d" % Dl)
             kp = _zeros(kvb_l)
             vp = _zeros(kvb_l)
             self.kpools.append(kp)
@@ -408,8 +447,14 @@ class DeviceModel:
                 ptrs += [self.kpools[il].data_ptr(), self.vpools[il].data_ptr()]
         self.n_pools = len(ptrs)
         self.pools_dev = torch.tensor(ptrs or [0], dtype=torch.int64, device=DEV)
-        self.block_bytes_all = self.n_pools * L.lgmlh_kv_block_bytes(self.paged_dims[1],
-                                                                     self.paged_dims[0])
+        self.block_bytes_all = self.n_pools * L.lgmlh_kv_block_bytes(
+            self.paged_dims[1], self.block_dim(self.paged_dims[0]))
+
+    def block_dim(self, head_dim):
+        """The f16 head size whose blocks have the bytes of the pools' blocks,
+        for the entry points that copy whole blocks: a Q8_0 block is 17/32 of
+        an f16 one."""
+        return head_dim * 17 // 32 if self.kv_type == hip.Q8_0 else head_dim
 
     @property
     def pool_blocks(self):
@@ -429,7 +474,7 @@ class DeviceModel:
         if cells <= self.n_cells:
             return self.n_cells
         L, hp = hip.lib(), self.hp
-        D, Hkv = self.paged_dims
+        Hkv, D = self.paged_dims[1], self.block_dim(self.paged_dims[0])
         nb = L.lgmlh_kv_layer_bytes(cells, Hkv, D)
         for il in range(hp["n_layer"]):
             if self.swa[il]:
@@ -454,8 +499,10 @@ class DeviceModel:
 
     ring_blocks_per_split = 0  # the ring plans' run length (0: as blocks_per_split; 12 for heads of 256)
 
-    def plan(self, seq_n, seq_npast, block_tab, ids, blocks_per_split=0, ring_tab=None):
-        """The pass's plan; with sliding layers also its ring plan (.ring)
+    def plan(self, seq_n, seq_npast, block_tab, ids, blocks_per_split=0, ring_tab=None,
+             parents=None):
+        """The pass's plan; with parents the plan of drafted trees (Plan);
+        with sliding layers also its ring plan (.ring)
         over ring_tab (n_seq, ring blocks), the sequences' rings.
         blocks_per_split 0: for heads of 256 (their kernel holds one wave per
         SIMD), runs of 28 KV blocks over the paged pool (fewer, longer items
@@ -477,8 +524,10 @@ class DeviceModel:
         if len(ids) and (ids.min() < 0 or ids.max() >= self.hp["n_vocab"]):
             raise ValueError("token id out of range [0, %d)" % self.hp["n_vocab"])
         p = Plan(seq_n, seq_npast, block_tab, ids, self.hp["n_head"], self.paged_dims[1],
-                 self.pool_blocks, blocks_per_split)
+                 self.pool_blocks, blocks_per_split, parents=parents)
         if any(self.swa):
+            if parents is not None:
+                raise ValueError("a tree of drafted tokens needs a model without sliding layers")
             if ring_tab is None:
                 raise ValueError("the model has sliding-window layers: pass ring_tab")
             p.ring = Plan(seq_n, seq_npast, ring_tab, ids, self.hp["n_head"],
@@ -515,12 +564,28 @@ class DeviceModel:
         ws, ws_bytes = self.workspace(plan, n_out, slot)
         if logits is None:
             logits = torch.empty((n_out, self.hp["n_vocab"]), dtype=torch.float32, device=DEV)
-        check(hip.lib().lgmlh_forward(C.byref(self.m), C.byref(plan.ub),
-                                      C.byref(plan.ring.ub) if plan.ring is not None else None,
-                                      ptr(rows), n_out, logits.data_ptr(), ws.data_ptr(),
-                                      ws_bytes,
-                                      C.byref(trace.c) if trace is not None else None, stream()))
+        fn = hip.lib().lgmlh_forward_q8 if self.kv_type == hip.Q8_0 else hip.lib().lgmlh_forward
+        check(fn(C.byref(self.m), C.byref(plan.ub),
+                 C.byref(plan.ring.ub) if plan.ring is not None else None, ptr(rows), n_out,
+                 logits.data_ptr(), ws.data_ptr(), ws_bytes,
+                 C.byref(trace.c) if trace is not None else None, stream()))
         return logits
+
+    def move_cells(self, src, dst):
+        """Cells src to dst in every paged layer's K and V, each dst as its
+        src was before (lgmlh_kv_move): the accepted tokens of a verified tree
+        to the slots behind the context, or a block's first cells to another.
+        Up to 1024 cells."""
+        src, dst = (np.ascontiguousarray(a, np.int64).reshape(-1) for a in (src, dst))
+        if len(src) != len(dst):
+            raise ValueError("%d cells to %d places" % (len(src), len(dst)))
+        if not len(src) or not self.n_pools:
+            return
+        ds, dd = _dev(src), _dev(dst)
+        D, Hkv = self.paged_dims
+        check(hip.lib().lgmlh_kv_move(self.kv_type, self.pools_dev.data_ptr(), self.n_pools,
+                                      self.n_cells, Hkv, D, ds.data_ptr(), dd.data_ptr(), ptr(src),
+                                      ptr(dst), len(src), stream()))
 
     def gather_kv(self, layer, cells, which=0):
         """Cells of a layer's K (0) or V (1) as (n, Hkv*D) f16 bits (uint16)
@@ -531,6 +596,10 @@ class DeviceModel:
         out = torch.empty((len(cells), Hkv * D), dtype=torch.int16, device=DEV)
         pool = (self.kpools if which == 0 else self.vpools)[layer]
         n = self.ring_cells if self.swa[layer] else self.n_cells
+        if self.kv_type == hip.Q8_0:  # the f16 of the values held
+            check(hip.lib().lgmlh_kv_gather_q8(pool.data_ptr(), which, n, Hkv, D, dc.data_ptr(),
+                                               len(cells), out.data_ptr(), hip.F16, stream()))
+            return out.cpu().numpy().view(np.uint16)
         check(hip.lib().lgmlh_kv_gather(pool.data_ptr(), which, n, Hkv, D,
                                         dc.data_ptr(), len(cells), out.data_ptr(), stream()))
         return out.cpu().numpy().view(np.uint16)
