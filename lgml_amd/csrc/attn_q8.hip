@@ -246,6 +246,19 @@ template <int D, typename S, typename V>
 __device__ __forceinline__ void values_q8(f32x4 (&o)[D / 16], const f32x4 (&st)[4], bool plain,
                                           bool masked, uint64_t word, int quad, S scale, V frag) {
   constexpr int NB = D / 32;
+  // Which way a row's part is made goes by the scales of the cells it sees, and by
+  // nothing else, so that a row has the same bits in any group of rows.
+  bool row_plain = plain;
+  if (masked) {  // wave-uniform: some row does not see all of the block
+    row_plain = true;
+#pragma unroll 1
+    for (int b = 0; b < NB; b++) {
+      f16x8 dv[2];
+      row_plain &= plain_scale(row_scales(scale(b, 0), scale(b, 1), true, word, quad, dv));
+    }
+    // a cell that a row does not see has p of 0 there, and a finite scale here
+    plain &= __builtin_amdgcn_ballot_w64(!row_plain) == 0;
+  }
   if (plain) {
     // a step reads the next 16 dims' V (and makes the next block's P dv) while
     // the products of this one run
@@ -302,15 +315,8 @@ __device__ __forceinline__ void values_q8(f32x4 (&o)[D / 16], const f32x4 (&st)[
     }
     return;
   }
-  // Some rows do not see all of the block. Both ways, and each row takes the one
-  // that the scales of the cells it sees ask for: that depends on nothing else, so
-  // a row has the same bits in any group of rows.
-  bool row_plain = true;
-#pragma unroll 1
-  for (int b = 0; b < NB; b++) {
-    f16x8 dv[2];
-    row_plain &= plain_scale(row_scales(scale(b, 0), scale(b, 1), true, word, quad, dv));
-  }
+  // Some rows do not see all of the block, and not all of them go the same way:
+  // both are made, and each row takes its own.
   f16x8 fh[2], fl[2];
   split_p(st, fh, fl);
 #pragma unroll
@@ -503,7 +509,7 @@ paged_attn_q8_kernel(const float *__restrict__ q, int H, int Hkv, float scale_lo
     const bool masked = see.masks(blk, word);
     softmax_q8<DT>(st, rscale, masked, word, quad, m, l, o);
     __builtin_amdgcn_sched_barrier(0);
-    values_q8<D>(o, st, plain && !masked, masked, word, quad,
+    values_q8<D>(o, st, plain, masked, word, quad,
                  [&](int b, int h) { return scale_of(1, b, h); },
                  [&](int t, int kc) { return half8(vq[t][2 * kc], vq[t][2 * kc + 1]); });
     if constexpr (NEXT) load_v(nxt);
@@ -682,7 +688,7 @@ paged_attn_q8_shared_kernel(const float *__restrict__ q, int H, int Hkv, float s
     const bool masked = see.masks(blk, word);
     softmax_q8<DT>(st, rscale, masked, word, quad, m, l, o);
     __builtin_amdgcn_sched_barrier(0);
-    values_q8<D>(o, st, odd_scales[buf] == 0 && !masked, masked, word, quad,
+    values_q8<D>(o, st, odd_scales[buf] == 0, masked, word, quad,
                  [&](int b, int h) { return sc[NB * 8 + b * 8 + 4 * h]; },
                  [&](int t, int kc) { return *(const f16x8 *)(vb[0] + va[kc] + t * 1024); });
   }

@@ -403,6 +403,30 @@ def test_q8_attention_of_small_and_large_values(L, gain, H, kv, D):
             t += 1
 
 
+@pytest.mark.parametrize("gain", [None, "dims", "cells", "small"])
+@pytest.mark.parametrize("H,kv,D", [(8, 2, 64), (16, 2, 128), (8, 4, 256)])
+@pytest.mark.parametrize("bps", [2, 40])
+def test_a_row_over_q8_has_its_bits_in_any_group_of_rows(L, gain, H, kv, D, bps):
+    """A chunk's tokens together, and each by itself with the later cells of its
+    block as the chunk left them (quieter and louder ones among them)."""
+    from lgml_amd import runtime
+    n, past = 70, 45
+    rng = np.random.default_rng(5)
+    P = Pass([n], [past], H, kv, None, bps, 5)
+    k = rng.standard_normal((P.n_cells, kv, D)).astype(np.float32)
+    v = rng.standard_normal((P.n_cells, kv, D)).astype(np.float32)
+    if gain:
+        v = (v * GAINS[gain](rng, v.shape)).astype(np.float32)
+    q = rng.standard_normal((n, H, D)).astype(np.float32)
+    pools, _, _ = fill(L, P, kv, D, k, v, True)
+    got = run_attention(L, P, H, kv, D, D ** -0.5, q, pools, True)
+    for j in range(n):
+        P.plan = runtime.Plan([1], [past + j], P.tab, np.zeros(1, np.int32), H, kv, P.blocks, bps)
+        P.info, P.ub = P.plan.info, P.plan.ub
+        one = run_attention(L, P, H, kv, D, D ** -0.5, q[j:j + 1], pools, True)
+        assert np.array_equal(one[0], got[j]), j
+
+
 def spoil_cells(q8, kv, D, which_cells):
     """Infinite and NaN contents for some cells: f16 values, or Q8_0 scales."""
     def spoil(P, pools):
