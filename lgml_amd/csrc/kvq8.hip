@@ -267,8 +267,13 @@ static bool q8_small(int64_t n, int n_head_kv, int kinds, int D) {
 // dst as its src was before the call: a workgroup takes rows of one head's tiles
 // of one tensor (16-byte pieces of K's cells, V's dims, Q8_0's scales), reads all
 // the moves' values of them into registers, then writes. It is bound by V, whose
-// cells are 2 (or 1) bytes of a line each.
-constexpr int MOVE_MAX = 1024, MOVE_THREADS = 256;
+// cells are 2 (or 1) bytes of a line each: 320 moves of 32 layers of 8 heads of
+// 128 in f16 are 84 MB of values, but 172 MB fetched and 97 MB written, in 91 us
+// (K's part 14; reads alone 52, writes alone 33). Stores past the caches take 95
+// us there and others 109, reads past them 144; 512 threads of 8 values 91 and 256
+// of 16 95; a head's slices in turn over the dies 129, as its dies' L2 then share
+// no tile.
+constexpr int MOVE_MAX = 1024, MOVE_THREADS = 512;
 
 // The values (row r, move m), m fastest or (CELLS) r fastest, at base + off[m] +
 // at(r): PER a thread, the rest of the index stepped without a division.
@@ -297,7 +302,7 @@ __device__ __forceinline__ void move_rows(uint8_t *base, const int64_t *from, co
 #pragma unroll
   for (int j = 0; j < PER; j++)
     if (j * MOVE_THREADS + (int)threadIdx.x < total && from[lo[j]] >= 0)
-      *(T *)(base + to[lo[j]] + hi[j]) = v[j];
+      __builtin_nontemporal_store(v[j], (T *)(base + to[lo[j]] + hi[j]));
 }
 
 // Rows of a workgroup: K's 16-byte pieces of a cell, V's dims.
@@ -500,9 +505,9 @@ extern "C" int lgmlh_kv_move(int type, void *const *pools, int n_pools, int64_t 
     }
   LGMLH_TRY(check_write_cells(h_dst, n, n_cells, "kv_move"));
   if (n == 0) return LGMLH_OK;
-  // as few values a thread (8, 16, 32) as leave a workgroup 8 rows, a cache line's
-  // of K; then as many rows as it holds
-  const int per = n <= MOVE_THREADS ? 8 : n <= 2 * MOVE_THREADS ? 16 : 32;
+  // as few values a thread as leave a workgroup 8 rows, a cache line's of K; then
+  // as many rows as it holds
+  const int per = n <= MOVE_THREADS ? 8 : 16;
   const int hold = per * MOVE_THREADS / (int)n;
   auto fit = [&](int all) {
     int r = all;
@@ -514,12 +519,8 @@ extern "C" int lgmlh_kv_move(int type, void *const *pools, int n_pools, int64_t 
   const int slices_k = (pieces + shape.k_rows - 1) / shape.k_rows,
             slices_v = (head_dim + shape.v_rows - 1) / shape.v_rows;
   const int slices = (slices_k > slices_v ? slices_k : slices_v) + (q8 ? 1 : 0);
-  const auto kern = q8 ? (per == 8    ? kv_move_kernel<true, 8>
-                          : per == 16 ? kv_move_kernel<true, 16>
-                                      : kv_move_kernel<true, 32>)
-                       : (per == 8    ? kv_move_kernel<false, 8>
-                          : per == 16 ? kv_move_kernel<false, 16>
-                                      : kv_move_kernel<false, 32>);
+  const auto kern = q8 ? (per == 8 ? kv_move_kernel<true, 8> : kv_move_kernel<true, 16>)
+                       : (per == 8 ? kv_move_kernel<false, 8> : kv_move_kernel<false, 16>);
   hipLaunchKernelGGL(kern, dim3((unsigned)(n_head_kv * slices), (unsigned)n_pools), dim3(MOVE_THREADS),
                      0, as_stream(stream), pools, n_cells, n_head_kv, head_dim, src, dst, (int)n, shape);
   return hip_check(hipGetLastError(), "kv_move");
