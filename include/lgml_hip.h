@@ -119,9 +119,9 @@ int lgmlh_set_rows_f16(uint16_t *dst, int64_t dst_rows, int64_t row, const float
  * ===================================================================== */
 /* Bytes of one layer's K (or V); -1 for an unsupported shape. */
 int64_t lgmlh_kv_q8_layer_bytes(int64_t n_cells, int n_head_kv, int head_dim);
-/* lgmlh_kv_store into Q8_0 pools, the rows quantized as ggml's
- * quantize_row_q8_0 does: per 32 values d = max|x| / 127, q = x (1 / d)
- * rounded with halves away from zero, d kept as f16. Rows are finite and below
+/* lgmlh_kv_store into Q8_0 pools, the rows quantized in the format's steps
+ * (f32): per 32 values d = max|x| / 127, q = x (1 / d) rounded with halves away
+ * from zero, d kept as f16. Rows are finite and below
  * 127 * 65504 (d is f16; above it reads back as infinite). Cells of one call
  * are distinct: a cell twice, which would mix two rows, is LGMLH_EINVAL. */
 int lgmlh_kv_store_q8(void *kpool, void *vpool, int64_t n_cells, int n_head_kv, int head_dim,
@@ -280,7 +280,8 @@ int lgmlh_plan_ring(int n_seq, const int32_t *seq_n, const int32_t *seq_npast,
  * last tokens, so pass the wanted rows as out_rows. After a verification the
  * accepted tokens' cells go to the slots behind the context with
  * lgmlh_kv_move. info->ring is LGMLH_PLAN_TREE, info->window the 64-bit words
- * of a token's mask (the masks stand last in the buffer).
+ * of a token's mask (the masks stand last in the buffer and are found from
+ * items, so a bound plan keeps its items and counts).
  * Errors: as lgmlh_plan; LGMLH_ERANGE for a parent that is no earlier token. */
 enum { LGMLH_PLAN_TREE = -1, LGMLH_TREE_MAX = 1024 };
 int lgmlh_plan_tree(int n_seq, const int32_t *seq_n, const int32_t *seq_npast,
@@ -300,7 +301,7 @@ int lgmlh_plan_bind(const lgmlh_plan_info *info, const void *dev, lgmlh_ubatch *
  * q: (n_tokens, H, D) f32; out: (n_tokens, H, D) f32 written in place in
  * pass order (the concat chain of :2413 is not needed). K/V from the pool
  * layout above. scale: 1/sqrt(D) for llama (transformer.lua:1845).
- * D in {64, 128, 256}; H a multiple of Hkv with H/Hkv in {1, 2, 4, 8, 16}.
+ * D in {16, 32, 64, 128, 256}; H a multiple of Hkv with H/Hkv in {1, 2, 4, 8, 16}.
  * ===================================================================== */
 size_t lgmlh_attention_workspace(const lgmlh_plan_info *info, int head_dim);
 int lgmlh_paged_attention(const float *q, int n_head, int n_head_kv, int head_dim, float scale,
@@ -498,8 +499,9 @@ int lgmlh_argmax(const float *x, int64_t n_rows, int64_t n_cols, int32_t *out, v
  * likely tokens and their log p, largest first, ties to the smaller id (either
  * may be NULL). A -inf logit is a token of probability 0; a row of nothing else
  * gives -inf, entropy 0 and the first ids. A NaN makes the row's log p and
- * entropy NaN and ranks as -inf. The workspace (16-byte aligned) needs no
- * initialisation. */
+ * entropy NaN and ranks as -inf. A row's last bits may differ between calls of
+ * different n_rows, which picks how a row is cut; calls of the same shape repeat
+ * them. The workspace (16-byte aligned) needs no initialisation. */
 size_t lgmlh_log_probs_workspace(int64_t n_rows, int64_t n_cols, int n_top);
 int lgmlh_log_probs(const float *logits, int64_t n_rows, int64_t n_cols, const int32_t *ids,
     int n_ids, float *id_lp, float *entropy, int n_top, int32_t *top_ids, float *top_lp,

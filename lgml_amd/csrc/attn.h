@@ -209,11 +209,15 @@ __device__ __forceinline__ int swk(int r) {  // distinct over the 16 rows of a t
 }
 __device__ __forceinline__ int swv(int r) { return (r >> 1) & 7; }
 
-// What sequence tokens of a tree plan see, in the blocks that hold the
-// pass's own tokens: bit c of word w of token t is cell c of block npast / 64 + w
-// (lgmlh_plan_tree). They stand behind the plan's last array.
-__host__ __device__ inline const uint64_t *plan_vis(const int32_t *order, int n_single) {
-  return (const uint64_t *)((const char *)order + ((4 * (int64_t)n_single + 15) & ~int64_t(15)));
+// What the tokens of a tree plan see, in the blocks that hold the pass's own
+// tokens: bit c of word w of token t is cell c of block npast / 64 + w
+// (lgmlh_plan_tree). They stand behind the plan's last arrays (items, merge,
+// shared, order; `order` itself may be another or NULL).
+inline const uint64_t *plan_vis(const lgmlh_ubatch *ub) {
+  auto align16 = [](int64_t x) { return (x + 15) & ~int64_t(15); };
+  return (const uint64_t *)((const char *)ub->items + 16 * (int64_t)ub->n_items +
+                            16 * (int64_t)ub->n_merge + align16(8 * (int64_t)ub->n_shared) +
+                            align16(4 * (int64_t)ub->n_single));
 }
 
 // The fixed-order merge of a plan's split groups (attn.hip), for the kernels

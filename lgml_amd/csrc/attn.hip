@@ -750,7 +750,7 @@ static void launch_attn(const float *q, int H, int Hkv, float scale_log2, const 
                         const void *vp, const lgmlh_ubatch *ub, float *out, f16 *planes,
                         int64_t npad, int xf, float *part, hipStream_t st) {
   const bool tree = ub->ring == LGMLH_PLAN_TREE;
-  const uint64_t *vis = tree ? plan_vis(ub->order, ub->n_single) : nullptr;
+  const uint64_t *vis = tree ? plan_vis(ub) : nullptr;
   // one workgroup per (item, KV head), the items on their own in the
   // plan's order
   if (ub->ring > 0)

@@ -8,16 +8,22 @@
 // carries 22 bits of every element down to 2^-17 of the row's largest.
 // o_rd = sum_c (p_rc dv_cb) v8_cd, b = d / 32: dv goes into P, per block of 32
 // dims, and P dv enters the MFMAs as f16 hi + lo, Q8_P times as large (O with it,
-// and l in the end). In a block whose cells every row sees and whose largest dv of
-// each 32 dims is in [2^-10, 4) (values of 0.12 to 500; or 0), P is split once
-// and multiplied by dv in packed f16, the product's rounding caught by an fma: hi
-// = P_hi dv, lo = P_lo dv + (P_hi dv - hi), 24 operations a lane instead of 88.
+// and l in the end). Where the largest dv that a row sees of each 32 dims of the
+// block is in [2^-10, 4) (values of 0.12 to 500; or 0), P is split once and
+// multiplied by dv in packed f16, the product's rounding caught by an fma: hi =
+// P_hi dv, lo = P_lo dv + (P_hi dv - hi), 24 operations a lane instead of 88.
 // There hi + lo keep 22 bits of p dv down to 2^-16 of the row's largest, and below
 // are at most 2^-38 of it off. Else P dv is made in f32 and scaled by the power
 // of two that puts the row's largest dv at 2^14 to 2^15, the products scaled back
-// as they add to O^T; a cell that a row does not see has p and dv as zeros, so that
-// nothing in it (a scale that is infinite or NaN) reaches the row. Which of the two
-// a row takes in a block that it does not see all of goes by the cells it does see.
+// as they add to O^T; a cell that a row does not see has p and dv as zeros there,
+// so that nothing in it (a scale that is infinite or NaN) reaches the row.
+//
+// Bounds. One token of 64 sequences at 128 to 4096 cells, 32 / 8 heads of 128, is
+// 67 + 6 us from HBM: 296 MB at 4.4 TB/s in the first (54 with the cells in the
+// memory-side cache). Trees of 61 tokens of 8
+// sequences at 1024 to 16384 cells, 8 / 4 heads of 256, are 151 + 10 us: 35 GFLOP
+// (16-bit halves of q and P make them 70) in 176 workgroups of 256 CUs, whose waves
+// wait in turn for LDS (48 reads of 16 bytes a block and product) and the vector ALU.
 #include <type_traits>
 
 #include "attn.h"
@@ -241,7 +247,7 @@ __device__ __forceinline__ void scores_q8(f32x4 (&st)[4], R read, Q query) {
 }
 
 // O^T += V^T (P dv)^T over a block. scale(b, h): the lane's cells' dv; frag(t, kc):
-// V's operand. plain: no masks, and plain_scales of all (the same for the wave).
+// V's operand. plain: plain_scales of all cells (the same for the wave).
 template <int D, typename S, typename V>
 __device__ __forceinline__ void values_q8(f32x4 (&o)[D / 16], const f32x4 (&st)[4], bool plain,
                                           bool masked, uint64_t word, int quad, S scale, V frag) {
@@ -704,7 +710,7 @@ static void launch_attn_q8(const float *q, int H, int Hkv, float scale_log2, con
                            const void *vp, const lgmlh_ubatch *ub, float *out, f16 *planes,
                            int64_t npad, int xf, float *part, hipStream_t st) {
   const uint64_t *vis =
-      ub->ring == LGMLH_PLAN_TREE ? plan_vis(ub->order, ub->n_single) : nullptr;
+      ub->ring == LGMLH_PLAN_TREE ? plan_vis(ub) : nullptr;
   if (ub->n_single > 0)
     hipLaunchKernelGGL(paged_attn_q8_kernel<D>, dim3((uint32_t)ub->n_single * Hkv), dim3(64), 0, st,
                        q, H, Hkv, scale_log2, (const uint8_t *)kp, (const uint8_t *)vp, ub->items,

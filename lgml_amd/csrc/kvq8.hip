@@ -22,6 +22,10 @@ struct Q8Tile {
 // each dim, and 8 lanes take a dim's 64 bytes. Runs of cells start anywhere, so a
 // group belongs to the workgroup that has its first token, which also takes the
 // up to 7 of it that lie past its own; tokens in no whole group go byte by byte.
+// 8192 tokens of 8 heads of 128, K and V: 67 MB of rows read, 18 MB written, 23 us
+// with the rows in the memory-side cache (3.7 TB/s; with V's bytes one by one 39),
+// 31 from HBM; 64 tokens of them 5.7 us, the time of one workgroup's reads, turn and
+// writes after another.
 constexpr int Q8_THREADS = 256, Q8_GROUP = 8, Q8_HALO = 7;
 constexpr int64_t Q8_CELLS = (int64_t)1 << 36;  // a block's number has 31 bits
 
@@ -75,8 +79,8 @@ struct Q8Window {
 // Threads for n lone tokens: the power of two that holds them, as bits.
 __device__ __forceinline__ int lone_bits(int n) { return n > 1 ? 32 - __builtin_clz(n - 1) : 0; }
 
-// x (n, Hkv D) f32 rows into their cells. Per 32 values (8 lanes), the steps of
-// quantize_row_q8_0: d = amax / 127, q = round(x (1 / d)) with halves away from
+// x (n, Hkv D) f32 rows into their cells. Per 32 values (8 lanes), the format's
+// steps in f32: d = amax / 127, q = round(x (1 / d)) with halves away from
 // zero, d kept as f16.
 template <int D, int W>
 __global__ void __launch_bounds__(Q8_THREADS)
@@ -179,6 +183,8 @@ __device__ __forceinline__ void load_scales(uint16_t *lds, const uint8_t *head, 
 // into LDS as rows (K's 16 bytes a lane are 8 dims of two blocks), the scales too,
 // then out 4 values a lane. (K's values straight from the tile, 4 bytes a lane,
 // need each token's address in each lane: 32768 tokens of 8 heads of 128 54 us.)
+// Bound by HBM's writes: those tokens' K are 35 MB read and 134 MB of f32 written
+// in 36 us (4.7 TB/s), V as many in 39.
 template <int D, int W, bool IS_V, typename OutT>
 __global__ void __launch_bounds__(Q8_THREADS)
 kv_gather_q8_kernel(const uint8_t *__restrict__ pool, int64_t n_cells,
@@ -268,11 +274,12 @@ static bool q8_small(int64_t n, int n_head_kv, int kinds, int D) {
 // of one tensor (16-byte pieces of K's cells, V's dims, Q8_0's scales), reads all
 // the moves' values of them into registers, then writes. It is bound by V, whose
 // cells are 2 (or 1) bytes of a line each: 320 moves of 32 layers of 8 heads of
-// 128 in f16 are 84 MB of values, but 172 MB fetched and 97 MB written, in 91 us
-// (K's part 14; reads alone 52, writes alone 33). Stores past the caches take 95
-// us there and others 109, reads past them 144; 512 threads of 8 values 91 and 256
-// of 16 95; a head's slices in turn over the dies 129, as its dies' L2 then share
-// no tile.
+// 128 in f16 are 84 MB of values, but 2.1 million lines of V, 134 us with the pool
+// in HBM (reads alone 58, writes alone, whose lines are fetched to be merged into,
+// 106: 128 bytes each way are 540 MB at 4 to 5 TB/s; K's part 13) and 91 with its
+// lines in the memory-side cache. Stores past the caches take those 91 where
+// others take 104, reads past them 140; 512 threads of 8 values 91 and 256 of 16
+// 95; a head's slices on all dies at once 129 (149 from HBM).
 constexpr int MOVE_MAX = 1024, MOVE_THREADS = 512;
 
 // The values (row r, move m), m fastest or (CELLS) r fastest, at base + off[m] +
@@ -404,6 +411,10 @@ static int check_write_cells(const int64_t *h, int64_t n, int64_t n_cells, const
   return LGMLH_OK;
 }
 
+// Heads of cells in one call: a launch has fewer than 2^32 threads, 256 for 32 or
+// more of them.
+constexpr int64_t Q8_ROWS = int64_t(1) << 29;
+
 static bool q8_head(int D) { return D == 64 || D == 128 || D == 256; }
 
 }  // namespace lgmlh
@@ -420,7 +431,7 @@ extern "C" int lgmlh_kv_store_q8(void *kpool, void *vpool, int64_t n_cells, int 
                                  const int64_t *cells, const int64_t *h_cells, int64_t n,
                                  void *stream) {
   if (!kpool || !vpool || !k_src || !v_src || !cells || n < 0 || n_cells <= 0 ||
-      n_cells > Q8_CELLS || n_cells % KV_BLOCK || n_head_kv <= 0 || n > INT32_MAX / n_head_kv || !q8_head(head_dim)) {
+      n_cells > Q8_CELLS || n_cells % KV_BLOCK || n_head_kv <= 0 || n >= Q8_ROWS / n_head_kv || !q8_head(head_dim)) {
     set_error("kv_store_q8: bad arguments (heads of 64, 128 or 256)");
     return LGMLH_EINVAL;
   }
@@ -443,7 +454,7 @@ extern "C" int lgmlh_kv_gather_q8(const void *pool, int which, int64_t n_cells, 
                                   int head_dim, const int64_t *cells, int64_t n, void *out,
                                   int out_type, void *stream) {
   if (!pool || !cells || !out || n < 0 || (which != 0 && which != 1) || n_cells <= 0 ||
-      n_cells > Q8_CELLS || n_cells % KV_BLOCK || n_head_kv <= 0 || n > INT32_MAX / n_head_kv || !q8_head(head_dim) ||
+      n_cells > Q8_CELLS || n_cells % KV_BLOCK || n_head_kv <= 0 || n >= Q8_ROWS / n_head_kv || !q8_head(head_dim) ||
       (out_type != LGMLH_F32 && out_type != LGMLH_F16)) {
     set_error("kv_gather_q8: bad arguments (heads of 64, 128 or 256; out f32 or f16)");
     return LGMLH_EINVAL;
@@ -485,7 +496,7 @@ extern "C" int lgmlh_kv_move(int type, void *const *pools, int n_pools, int64_t 
                              const int64_t *h_src, const int64_t *h_dst, int64_t n, void *stream) {
   const bool q8 = type == LGMLH_Q8_0;
   if ((!q8 && type != LGMLH_F16) || !pools || !src || !dst || n_pools <= 0 || n_pools > 65535 ||
-      n_pools % 2 || n_cells <= 0 || n_cells % KV_BLOCK || n_head_kv <= 0 || n < 0 ||
+      n_pools % 2 || n_cells <= 0 || n_cells % KV_BLOCK || n_head_kv <= 0 || n_head_kv > 65535 || n < 0 ||
       (q8 ? !q8_head(head_dim) : head_dim != 16 && (head_dim <= 0 || head_dim % 32))) {
     set_error("kv_move: bad arguments (K and V tensors in turn, of f16 or Q8_0)");
     return LGMLH_EINVAL;

@@ -13,6 +13,11 @@
 // first index) keys: a token of another group is behind k tokens, one of each
 // of those. So a second launch, a workgroup per row, joins the slices, selects k
 // of the groups' maxima and then k of those groups' 64 k values.
+//
+// 1000 rows of 151936 and their 20 first: the slices take 119 us, 608 MB at 5.1
+// TB/s, a large read's rate being 6.2; the rows 19. One row of 128256 takes 3.2 +
+// 7.8 us: two launches' reads one after another, in the second one the maxima,
+// then the chosen groups.
 #include <math.h>
 
 #include "common.h"
@@ -23,7 +28,7 @@ constexpr int LP_THREADS = 256, LP_GROUP = 64, LP_TOP = 64, LP_IDS = 64;
 constexpr int64_t LP_COLS = 1 << 20;  // the largest row: 64 groups a thread, 64 x 64 candidates
 constexpr float LP_LOG2E = 1.4426950408889634f;
 // Vectors of 4 a thread holds: a slice of 8192, or of 2048 where the larger ones
-// make few workgroups.
+// make few workgroups (one row of 128256: 16 of them, and 63 of the smaller).
 constexpr int LP_WIDE = 8, LP_SLIM = 2;
 
 struct Slice {
@@ -367,7 +372,7 @@ extern "C" int lgmlh_log_probs(const float *logits, int64_t n_rows, int64_t n_co
   const int n_groups = (int)((n_cols + LP_GROUP - 1) / LP_GROUP);
   Slice *part = (Slice *)workspace;
   float *groups = n_top ? (float *)(part + n_rows * slices) : nullptr;
-  if (n_rows * slices > INT32_MAX) {
+  if (n_rows * slices >= (int64_t)1 << 24) {  // a launch has fewer than 2^32 threads
     set_error("log_probs: %lld rows of %lld in one call", (long long)n_rows, (long long)n_cols);
     return LGMLH_EINVAL;
   }

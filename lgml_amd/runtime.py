@@ -127,6 +127,8 @@ def log_probs(logits, ids=None, top=0):
     L = hip.lib()
     if logits.dim() != 2 or logits.dtype != torch.float32 or not logits.is_contiguous():
         raise ValueError("logits: contiguous f32 rows")
+    if not logits.is_cuda or logits.device.index != torch.cuda.current_device():
+        raise ValueError("logits: on %s, not the current device" % logits.device)
     n, v = logits.shape
     m = 0
     if ids is not None:
@@ -143,6 +145,8 @@ def log_probs(logits, ids=None, top=0):
         out["lp"] = new(n, m)
     if top:
         out["top_ids"], out["top_lp"] = new(n, top, dtype=torch.int32), new(n, top)
+    if not n:
+        return out
     ws = _empty(max(L.lgmlh_log_probs_workspace(n, v, top), 16))
     check(L.lgmlh_log_probs(logits.data_ptr(), n, v, ptr(ids) if m else None, m, ptr(out.get("lp")),
                             out["entropy"].data_ptr(), top, ptr(out.get("top_ids")),

@@ -334,6 +334,22 @@ def test_a_line_of_tokens_is_the_causal_plan(L, q8):
     assert np.array_equal(a, b)
 
 
+@pytest.mark.parametrize("q8", [False, True])
+def test_a_tree_plan_in_another_dispatch_order(L, q8):
+    """order, which picks only who runs an item, may be NULL or the caller's own."""
+    H, kv, D, seq_n, npast = 16, 2, 64, [1, 2, 40, 1], [700, 64, 100, 5]
+    rng = np.random.default_rng(21)
+    P = Pass(seq_n, npast, H, kv, sum([tree(rng, n) for n in seq_n], []), 2, 21)
+    k, v = (rng.standard_normal((P.n_cells, kv, D)).astype(np.float32) for _ in range(2))
+    q = rng.standard_normal((sum(seq_n), H, D)).astype(np.float32)
+    pools, _, _ = fill(L, P, kv, D, k, v, q8)
+    want = run_attention(L, P, H, kv, D, D ** -0.5, q, pools, q8)
+    own = dev(np.arange(P.info.n_single, dtype=np.int32)[::-1])
+    for order in (own.data_ptr(), None):
+        P.ub.order = order
+        assert np.array_equal(run_attention(L, P, H, kv, D, D ** -0.5, q, pools, q8), want)
+
+
 @pytest.mark.parametrize("gain", [1e-30, 1e-6, 3e3, 1e7])
 def test_q8_attention_of_small_and_large_queries(L, gain):
     """q keeps its bits at any size (f16 parts of scaled rows); large scores leave
@@ -619,3 +635,81 @@ def test_log_probs_parts_alone(L):
         hip.check(L.lgmlh_log_probs(xd.data_ptr(), 2, 777, None, 0, None, None, 9, hip.ptr(i), hip.ptr(l),
                                     ws.data_ptr(), ws.numel(), st()))
     assert np.array_equal(ti.cpu().numpy(), b[2]) and np.array_equal(tl.cpu().numpy(), b[3])
+
+
+@pytest.mark.parametrize("q8", [False, True])
+def test_cells_behind_4_gib(L, q8):
+    """The last blocks of a pool whose tensors pass 4 GiB: stored, moved, read
+    back and attended to as in a small pool (the same bits)."""
+    from lgml_amd import hip, runtime
+    H, kv, D, n, past = 16, 8, 256, 40, 70
+    per = (68 if q8 else 128) * D * kv
+    big = (1 << 32) // per + 12
+    rng = np.random.default_rng(8)
+    k, v = (rng.standard_normal((past + n, kv, D)).astype(np.float32) for _ in range(2))
+    q = rng.standard_normal((n, H, D)).astype(np.float32)
+    parents = np.array(tree(rng, n), np.int32)
+    src, dst = np.array([past + 3, past + 9, past + 20]), np.array([past, past + 1, past + 2])
+    results = []
+    for blocks in (8, big):
+        tab = blocks - 1 - np.array([[3, 0]], np.int32)
+
+        def cell(p):
+            return tab[0][p // 64].astype(np.int64) * 64 + p % 64
+
+        pools = [torch.empty(blocks * per, dtype=torch.uint8, device="cuda") for _ in range(2)]
+        cells = cell(np.arange(past + n))
+        dc, kd, vd = dev(cells), dev(k), dev(v)
+        hip.check((L.lgmlh_kv_store_q8 if q8 else L.lgmlh_kv_store)(
+            pools[0].data_ptr(), pools[1].data_ptr(), 64 * blocks, kv, D, kd.data_ptr(), vd.data_ptr(),
+            dc.data_ptr(), cells.ctypes.data, len(cells), st()))
+
+        class P:
+            plan = runtime.Plan([n], [past], tab, np.zeros(n, np.int32), H, kv, blocks, 2, parents=parents)
+
+        P.info, P.ub = P.plan.info, P.plan.ub
+        got = [run_attention(L, P, H, kv, D, D ** -0.5, q, pools, q8)]
+        one = runtime.Plan([1], [past], tab, np.zeros(1, np.int32), H, kv, blocks, 2)
+        P.info, P.ub = one.info, one.ub
+        got.append(run_attention(L, P, H, kv, D, D ** -0.5, q[:1], pools, q8))
+        addr = torch.tensor([p.data_ptr() for p in pools], dtype=torch.int64, device="cuda")
+        a, b = cell(src), cell(dst)
+        da, db = dev(a), dev(b)
+        hip.check(L.lgmlh_kv_move(hip.Q8_0 if q8 else hip.F16, addr.data_ptr(), 2, 64 * blocks, kv, D,
+                                  da.data_ptr(), db.data_ptr(), a.ctypes.data, b.ctypes.data, 3, st()))
+        for w in range(2):
+            out = torch.empty((len(cells), kv, D), dtype=torch.float16, device="cuda")
+            if q8:
+                hip.check(L.lgmlh_kv_gather_q8(pools[w].data_ptr(), w, 64 * blocks, kv, D, dc.data_ptr(),
+                                               len(cells), out.data_ptr(), hip.F16, st()))
+            else:
+                hip.check(L.lgmlh_kv_gather(pools[w].data_ptr(), w, 64 * blocks, kv, D, dc.data_ptr(),
+                                            len(cells), out.data_ptr(), st()))
+            got.append(out.cpu().numpy())
+        results.append(got)
+        want = (values(k) if q8 else k).astype(np.float16)
+        want[dst] = want[src]
+        assert np.array_equal(got[2], want)
+    for a, b in zip(*results):
+        assert np.array_equal(a, b)
+
+
+def test_log_probs_behind_the_32_bit_element(L):
+    """The last row of more than 2^31 logits."""
+    v = 1 << 20
+    rows = (1 << 31) // v + 2
+    x = torch.zeros((rows, v), dtype=torch.float32, device="cuda")
+    last = np.random.default_rng(4).standard_normal(v).astype(np.float32)
+    x[-1] = dev(last)
+    from lgml_amd import runtime
+    ids = torch.full((rows, 1), 77, dtype=torch.int32)
+    got = runtime.log_probs(x, ids, 3)
+    y = last.astype(np.float64)
+    lz = np.log(np.exp(y).sum())
+    order = np.lexsort((np.arange(v), -y))[:3]
+    assert list(got["top_ids"][-1].cpu().numpy()) == list(order)
+    # |x| up to 6 and log Z near 14.4, each a rounding or two; the sum's 2^-18 at most
+    tol = 32 * 2.0**-23 + 2.0**-18
+    assert np.abs(got["top_lp"][-1].cpu().numpy() - (y[order] - lz)).max() <= tol
+    assert abs(got["lp"][-1, 0].item() - (y[77] - lz)) <= tol
+    assert abs(got["lp"][0, 0].item() + np.log(v)) <= tol

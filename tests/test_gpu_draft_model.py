@@ -372,3 +372,12 @@ def test_two_steps_on_two_streams_at_once():
     for step, ref in ((one, ref1), (two, ref2)):
         for x, y in zip(step.results(), ref.results()):
             assert torch.equal(x, y)
+
+
+def test_log_probs_of_no_rows_and_of_host_rows():
+    from lgml_amd import runtime
+    none = runtime.log_probs(torch.empty((0, 100), device="cuda"), torch.empty((0, 2)), 4)
+    assert none["lp"].shape == (0, 2) and none["top_ids"].shape == (0, 4)
+    for bad in (torch.zeros(2, 8), torch.zeros(8, 2, device="cuda").t(), torch.zeros(2, 8, device="cuda").half()):
+        with pytest.raises(ValueError):
+            runtime.log_probs(bad, None, 1)

@@ -210,3 +210,13 @@ def test_forward_refuses_a_tree_through_sliding_layers(hip):
     assert L.lgmlh_forward(C.byref(m), C.byref(ub), C.byref(ub), None, 0, d, d, 1 << 30, None,
                            None) == hip.EINVAL
     assert "tree" in hip.last_error()
+
+
+def test_refusals_of_more_than_a_launch_holds(hip):
+    """Before anything of the arguments is read."""
+    L, d = hip.lib(), C.c_void_p(256)
+    n = (1 << 29) // 8
+    assert L.lgmlh_kv_store_q8(d, d, 128, 8, 128, d, d, d, d, n, None) == hip.EINVAL
+    assert L.lgmlh_kv_gather_q8(d, 0, 128, 8, 128, d, n, d, hip.F32, None) == hip.EINVAL
+    assert L.lgmlh_kv_move(hip.F16, d, 2, 128, 1 << 16, 64, d, d, d, d, 1, None) == hip.EINVAL
+    assert L.lgmlh_log_probs(d, 1 << 24, 1, None, 0, None, d, 0, None, None, d, 1 << 40, None) == hip.EINVAL
