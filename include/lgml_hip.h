@@ -301,6 +301,10 @@ int lgmlh_plan_bind(const lgmlh_plan_info *info, const void *dev, lgmlh_ubatch *
  * q: (n_tokens, H, D) f32; out: (n_tokens, H, D) f32 written in place in
  * pass order (the concat chain of :2413 is not needed). K/V from the pool
  * layout above. scale: 1/sqrt(D) for llama (transformer.lua:1845).
+ * The V of the cells behind a row's position in its own last block is multiplied
+ * by 0 in causal and ring plans, so it has to be finite (pools start zeroed, as
+ * lgmlh_kv_grow's do); in tree plans, and over Q8_0 pools in all plans, such cells
+ * may hold anything.
  * D in {16, 32, 64, 128, 256}; H a multiple of Hkv with H/Hkv in {1, 2, 4, 8, 16}.
  * ===================================================================== */
 size_t lgmlh_attention_workspace(const lgmlh_plan_info *info, int head_dim);

@@ -138,8 +138,20 @@ __device__ __forceinline__ void softmax_q8(f32x4 (&st)[4], float rscale, bool ma
   m = m_new;
 }
 
+// The largest |scale| of 8 or more as the f16's bits: in them NaN is above the
+// infinity, where a maximum of numbers would pass it by. A float of the number
+// goes through the lanes' maxima.
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ u16x2 scale_bits(u32x4 s) {
+  u16x2 w[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) w[i] = __builtin_bit_cast(u16x2, s[i] & 0x7fff7fffu);
+  return __builtin_elementwise_max(__builtin_elementwise_max(w[0], w[1]), __builtin_elementwise_max(w[2], w[3]));
+}
+__device__ __forceinline__ float larger(u16x2 b) { return (float)(b[0] > b[1] ? b[0] : b[1]); }
+
 // The scales of a lane's cells (32 h + 8 quad + e) of one block of 32 dims, those
-// of cells that word leaves out as zeros, and the row's largest.
+// of cells that word leaves out as zeros, and the bits of the row's largest.
 __device__ __forceinline__ float row_scales(u32x4 s0, u32x4 s1, bool masked, uint64_t word, int quad,
                                             f16x8 (&dv)[2]) {
   if (masked) {  // wave-uniform
@@ -152,16 +164,14 @@ __device__ __forceinline__ float row_scales(u32x4 s0, u32x4 s1, bool masked, uin
   }
   dv[0] = __builtin_bit_cast(f16x8, s0);
   dv[1] = __builtin_bit_cast(f16x8, s1);
-  const f16x8 big = __builtin_elementwise_max(dv[0], dv[1]);
-  const f16x4 b4 = __builtin_elementwise_max(f16x4{big[0], big[1], big[2], big[3]},
-                                             f16x4{big[4], big[5], big[6], big[7]});
-  return quads_max(fmaxf(fmaxf((float)b4[0], (float)b4[1]), fmaxf((float)b4[2], (float)b4[3])));
+  return quads_max(larger(__builtin_elementwise_max(scale_bits(s0), scale_bits(s1))));
 }
 
-// P dv of one block of 32 dims as f16 hi + lo, scaled by the row's largest dv; the
-// factor that undoes it.
-__device__ __forceinline__ float weigh_p(const f32x4 (&st)[4], const f16x8 (&dv)[2], float mx,
+// P dv of one block of 32 dims as f16 hi + lo, scaled by the row's largest dv (its
+// bits); the factor that undoes it.
+__device__ __forceinline__ float weigh_p(const f32x4 (&st)[4], const f16x8 (&dv)[2], float bits,
                                          f16x8 (&ph)[2], f16x8 (&pl)[2]) {
+  const float mx = (float)__builtin_bit_cast(f16, (unsigned short)bits);
   const int ex = __builtin_amdgcn_frexp_expf(mx);  // mx in [2^(ex - 1), 2^ex)
   const float up = pow2(15 - ex);
   // hi by truncation, two at a time: lo takes up what it leaves
@@ -180,17 +190,15 @@ __device__ __forceinline__ float weigh_p(const f32x4 (&st)[4], const f16x8 (&dv)
   return pow2(ex - 15);
 }
 
-// Whether a block of dims whose largest scale is mx goes by the packed products.
-__device__ __forceinline__ bool plain_scale(float mx) {
-  return mx == 0.0f || (mx >= 0x1p-10f && mx < 4.0f);
+// Whether a block of dims goes by the packed products: its largest scale (bits) is
+// 0 or in [2^-10, 4).
+__device__ __forceinline__ bool plain_scale(float bits) {
+  return bits == 0.0f || (bits >= (float)0x1400 && bits < (float)0x4400);
 }
 // Whether a lane's 8 scales of a group of 32 dims (the group's 64 in 8 aligned
 // lanes) leave the group to the packed products.
 __device__ __forceinline__ bool plain_scales(u32x4 sc) {
-  const f16x8 d = __builtin_bit_cast(f16x8, sc);
-  const f16x4 a = __builtin_elementwise_max(f16x4{d[0], d[1], d[2], d[3]}, f16x4{d[4], d[5], d[6], d[7]});
-  return plain_scale(
-      group_max<8>(fmaxf(fmaxf((float)a[0], (float)a[1]), fmaxf((float)a[2], (float)a[3]))));
+  return plain_scale(group_max<8>(larger(scale_bits(sc))));
 }
 
 // P (cells 32 h + 8 quad + e) as f16 hi + lo, Q8_P times as large.

@@ -501,6 +501,30 @@ def test_cells_a_row_does_not_see_change_nothing(L, q8, H, kv, D):
     assert checked > 20
 
 
+@pytest.mark.parametrize("bits", [0x7e00, 0xffff, 0x7c00, 0xfc00, 0xbc00, 0x7bff, 0x0001])
+@pytest.mark.parametrize("lone", [False, True])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("is_tree", [False, True])
+def test_unseen_q8_cells_of_any_scale(L, bits, lone, D, is_tree):
+    """The cells past each sequence, or the last one alone, with scales of NaN,
+    infinity, either sign, the largest and the smallest."""
+    H, kv, seq_n, npast = 8, 2, [1, 40, 9], [70, 131, 3]
+    rng = np.random.default_rng(19)
+    parents = sum([tree(rng, n) for n in seq_n], []) if is_tree else None
+    P = Pass(seq_n, npast, H, kv, parents, 2, 19)
+    k, v = (rng.standard_normal((P.n_cells, kv, D)).astype(np.float32) for _ in range(2))
+    q = rng.standard_normal((sum(seq_n), H, D)).astype(np.float32)
+    pools, _, _ = fill(L, P, kv, D, k, v, True)
+    want = run_attention(L, P, H, kv, D, D ** -0.5, q, pools, True)
+    for s in range(len(seq_n)):
+        last = int(P.cells(s)[-1])
+        for w in range(2):
+            scales = pools[w].view(-1, kv, 68 * D)[last // 64, :, 64 * D:].view(torch.int16).view(kv, D // 32, 64)
+            scales[:, :, 63 if lone else slice(last % 64 + 1, 64)] = bits - (bits >> 15 << 16)
+    assert np.isfinite(want).all()
+    assert np.array_equal(run_attention(L, P, H, kv, D, D ** -0.5, q, pools, True), want)
+
+
 # ---- log probabilities -----------------------------------------------------------
 def log_probs(L, x, ids=None, top=0, entropy=True, lead=0):
     from lgml_amd import hip
@@ -657,7 +681,12 @@ def test_cells_behind_4_gib(L, q8):
         def cell(p):
             return tab[0][p // 64].astype(np.int64) * 64 + p % 64
 
-        pools = [torch.empty(blocks * per, dtype=torch.uint8, device="cuda") for _ in range(2)]
+        # Memory never written is no input: a causal f16 plan takes 0 times the V of
+        # unseen cells of a row's own blocks, and 0 x NaN is NaN. So the rest of the
+        # pools is of defined bytes: finite f16, and NaN scales in Q8_0, where a row
+        # holds whatever unseen cells hold.
+        pools = [torch.full((blocks * per,), 0xFF if q8 else 0xA5, dtype=torch.uint8, device="cuda")
+                 for _ in range(2)]
         cells = cell(np.arange(past + n))
         dc, kd, vd = dev(cells), dev(k), dev(v)
         hip.check((L.lgmlh_kv_store_q8 if q8 else L.lgmlh_kv_store)(
