@@ -305,6 +305,19 @@ def test_tree_attention(L, q8, H, kv, D, case, bps):
     check_attention(L, q8, H, kv, D, seq_n, npast, [tree(rng, n) for n in seq_n], bps, 3 + case)
 
 
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("H,kv,D", [(4, 2, 64), (16, 2, 128), (8, 4, 256)])
+@pytest.mark.parametrize("bps", [1, 0])
+def test_tree_rows_that_see_nothing_of_whole_runs(L, q8, H, kv, D, bps):
+    """Wide trees without a context, up to the largest: most of a sequence's blocks
+    hold nothing that a token sees."""
+    seq_n, npast = [200, 1024, 3], [0, 37, 0]
+    rng = np.random.default_rng(29)
+    parents = [[-1 if j == 0 or rng.random() < 0.5 else int(rng.integers(max(0, j - 200), j)) for j in range(n)]
+               for n in seq_n]
+    check_attention(L, q8, H, kv, D, seq_n, npast, parents, bps, 29)
+
+
 @pytest.mark.parametrize("D", [16, 32])
 def test_tree_attention_small_heads(L, D):
     rng = np.random.default_rng(D)
