@@ -115,7 +115,8 @@ int lgmlh_set_rows_f16(uint16_t *dst, int64_t dst_rows, int64_t row, const float
  * pool as one of f16 heads of 17 D / 32. Within a (block, KV head) tile of 68 * D bytes:
  * 64 * D int8 values, then f16 scales [D / 32][64 cells]; values of K
  * [D / 64][cell][4][2][8] with dim 64 j + 32 b + 8 q + e at (j, cell, q, b,
- * e), of V [D][4][2][8] with cell 32 b + 8 q + e at (d, q, b, e).
+ * e), of V [D][4][2][8] with cell 32 b + 8 q + e at (d, q, b, e). Tensors are
+ * 16-byte aligned.
  * ===================================================================== */
 /* Bytes of one layer's K (or V); -1 for an unsupported shape. */
 int64_t lgmlh_kv_q8_layer_bytes(int64_t n_cells, int n_head_kv, int head_dim);

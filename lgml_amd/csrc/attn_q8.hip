@@ -748,6 +748,10 @@ int paged_attention_q8_dev(const float *q, int n_head, int n_head_kv, int head_d
     set_error("paged_attention_q8: head_dim %d not supported (64, 128, 256)", head_dim);
     return LGMLH_EINVAL;
   }
+  if (((uintptr_t)kpool | (uintptr_t)vpool) & 15) {
+    set_error("paged_attention_q8: pools are 16-byte aligned");
+    return LGMLH_EINVAL;
+  }
   int run = 0;
   LGMLH_TRY(attn_check("paged_attention_q8", q, n_head, n_head_kv, head_dim, kpool, vpool, ub, out,
                        planes, xf, workspace, workspace_bytes, &run));

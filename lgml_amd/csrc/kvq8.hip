@@ -431,8 +431,13 @@ extern "C" int lgmlh_kv_store_q8(void *kpool, void *vpool, int64_t n_cells, int 
                                  const int64_t *cells, const int64_t *h_cells, int64_t n,
                                  void *stream) {
   if (!kpool || !vpool || !k_src || !v_src || !cells || n < 0 || n_cells <= 0 ||
-      n_cells > Q8_CELLS || n_cells % KV_BLOCK || n_head_kv <= 0 || n >= Q8_ROWS / n_head_kv || !q8_head(head_dim)) {
+      n_cells > Q8_CELLS || n_cells % KV_BLOCK || n_head_kv <= 0 ||
+      n >= Q8_ROWS / n_head_kv || !q8_head(head_dim)) {
     set_error("kv_store_q8: bad arguments (heads of 64, 128 or 256)");
+    return LGMLH_EINVAL;
+  }
+  if (((uintptr_t)kpool | (uintptr_t)vpool) & 15) {
+    set_error("kv_store_q8: pools are 16-byte aligned");
     return LGMLH_EINVAL;
   }
   LGMLH_TRY(check_write_cells(h_cells, n, n_cells, "kv_store_q8"));
@@ -454,9 +459,14 @@ extern "C" int lgmlh_kv_gather_q8(const void *pool, int which, int64_t n_cells, 
                                   int head_dim, const int64_t *cells, int64_t n, void *out,
                                   int out_type, void *stream) {
   if (!pool || !cells || !out || n < 0 || (which != 0 && which != 1) || n_cells <= 0 ||
-      n_cells > Q8_CELLS || n_cells % KV_BLOCK || n_head_kv <= 0 || n >= Q8_ROWS / n_head_kv || !q8_head(head_dim) ||
+      n_cells > Q8_CELLS || n_cells % KV_BLOCK || n_head_kv <= 0 ||
+      n >= Q8_ROWS / n_head_kv || !q8_head(head_dim) ||
       (out_type != LGMLH_F32 && out_type != LGMLH_F16)) {
     set_error("kv_gather_q8: bad arguments (heads of 64, 128 or 256; out f32 or f16)");
+    return LGMLH_EINVAL;
+  }
+  if ((uintptr_t)pool & 15) {
+    set_error("kv_gather_q8: pools are 16-byte aligned");
     return LGMLH_EINVAL;
   }
   if (n == 0) return LGMLH_OK;

@@ -638,7 +638,8 @@ int qkv_rope_store_dev(float *qkv, int64_t n, int n_head, int n_head_kv,
       n_head_kv <= 0 || head_dim <= 0 || head_dim % 8 || head_dim > 1024 || n_rot <= 0 ||
       n_rot > head_dim ||
       n_rot % 2 || n_cells % KV_BLOCK || pa.cols % 8 || pb.cols % 8 ||
-      (q8 && head_dim != 64 && head_dim != 128 && head_dim != 256)) {
+      (q8 && ((head_dim != 64 && head_dim != 128 && head_dim != 256) ||
+              (((uintptr_t)kpool | (uintptr_t)vpool) & 15)))) {
     set_error("qkv_rope_store%s: bad arguments", q8 ? "_q8" : "");
     return LGMLH_EINVAL;
   }

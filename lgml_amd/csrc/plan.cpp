@@ -45,7 +45,8 @@ using namespace lgmlh;
 static int plan_impl(int n_seq, const int32_t *seq_n, const int32_t *seq_npast,
                      const int32_t *block_tab, int max_blocks, int64_t pool_blocks,
                      const int32_t *ids, int n_head, int n_head_kv, int blocks_per_split,
-                     int window, int plan_ring, const int32_t *parents, void *buf, size_t buf_bytes, lgmlh_plan_info *info) {
+                     int window, int plan_ring, const int32_t *parents, void *buf,
+                     size_t buf_bytes, lgmlh_plan_info *info) {
   if (n_seq < 0 || !seq_n || !seq_npast || !block_tab || max_blocks <= 0 || !info ||
       n_head_kv <= 0 || n_head <= 0 || n_head % n_head_kv || n_head / n_head_kv > 16 ||
       16 % (n_head / n_head_kv) || blocks_per_split < 0 || (plan_ring > 0 && window < 1)) {

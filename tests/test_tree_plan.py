@@ -220,3 +220,18 @@ def test_refusals_of_more_than_a_launch_holds(hip):
     assert L.lgmlh_kv_gather_q8(d, 0, 128, 8, 128, d, n, d, hip.F32, None) == hip.EINVAL
     assert L.lgmlh_kv_move(hip.F16, d, 2, 128, 1 << 16, 64, d, d, d, d, 1, None) == hip.EINVAL
     assert L.lgmlh_log_probs(d, 1 << 24, 1, None, 0, None, d, 0, None, None, d, 1 << 40, None) == hip.EINVAL
+
+
+def test_q8_pools_off_their_alignment_are_refused(hip):
+    L, d, odd = hip.lib(), C.c_void_p(256), C.c_void_p(264)
+    c = np.array([3], np.int64)
+    h = c.ctypes.data
+    assert L.lgmlh_kv_store_q8(odd, d, 128, 8, 128, d, d, d, h, 1, None) == hip.EINVAL
+    assert L.lgmlh_kv_store_q8(d, odd, 128, 8, 128, d, d, d, h, 1, None) == hip.EINVAL
+    assert L.lgmlh_kv_gather_q8(odd, 0, 128, 8, 128, d, 1, d, hip.F32, None) == hip.EINVAL
+    assert L.lgmlh_qkv_rope_store_q8(d, 1, 4, 2, 64, 64, 0, 1e4, None, None, None, 1e-5, d, d, odd, 128, d, d,
+                                     None) == hip.EINVAL
+    rc, info, buf = plan_tree(hip, [3], [10], [-1, 0, 0], np.array([[0, 1]], np.int32), 4, 2, 2)
+    ub = hip.Ubatch()
+    assert L.lgmlh_plan_bind(C.byref(info), buf.ctypes.data, C.byref(ub)) == 0
+    assert L.lgmlh_paged_attention_q8(d, 4, 2, 64, 1.0, d, odd, C.byref(ub), d, d, 1 << 20, None) == hip.EINVAL
