@@ -24,11 +24,15 @@ __device__ __forceinline__ int q8_scale_at(int D, int b, int cell) {
   return 64 * D + 2 * (b * 64 + cell);
 }
 
-// To the nearest integer, halves away from zero, below 2^23: the largest number
-// under a half takes a half up to the next integer (its sum rounds there) and
-// nothing below it.
-__device__ __forceinline__ int round_away(float x) {
-  return (int)(x + __builtin_copysignf(0x1.fffffep-2f, x));
+// The f32 product x y to the nearest integer, halves away from zero, below 2^23:
+// the largest number under a half takes a half up to the next integer (its sum
+// rounds there) and nothing below it. The product is rounded by itself first, as
+// the format defines it: in an fma with the sum, a product just below a half that
+// rounds to it goes down (6 of 1.3e8 normal values).
+__device__ __forceinline__ int round_away(float x, float y) {
+#pragma clang fp contract(off)
+  const float p = x * y;
+  return (int)(p + __builtin_copysignf(0x1.fffffep-2f, p));
 }
 
 }  // namespace lgmlh

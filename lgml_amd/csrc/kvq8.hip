@@ -114,7 +114,7 @@ kv_store_q8_kernel(uint8_t *__restrict__ kp, uint8_t *__restrict__ vp, int64_t n
     const float d = amax / 127.0f, id = d != 0.0f ? 1.0f / d : 0.0f;
     uint32_t q = 0;
 #pragma unroll
-    for (int e = 0; e < 4; e++) q |= (uint32_t)(round_away(x[i][e] * id) & 0xff) << 8 * e;
+    for (int e = 0; e < 4; e++) q |= (uint32_t)(round_away(x[i][e], id) & 0xff) << 8 * e;
     if (t >= left) continue;  // whole blocks of lanes leave together
     if (g4 % 8 == 0 && t < W) scale[g4 / 8 * W + t] = f2h(d);
     if (is_v) {

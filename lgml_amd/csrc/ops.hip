@@ -323,7 +323,7 @@ qkv_rope_store_kernel(const float *__restrict__ qkv, int H, int Hkv, int D, int 
     for (int d = lane; d < D; d += 64) {  // D is a multiple of 64
       const float x = v[d];
       const float dd = group_max<32>(fabsf(x)) / 127.0f, id = dd != 0.0f ? 1.0f / dd : 0.0f;
-      tile[is_k ? q8_k_at((int)o, d) : q8_v_at(d, (int)o)] = (uint8_t)round_away(x * id);
+      tile[is_k ? q8_k_at((int)o, d) : q8_v_at(d, (int)o)] = (uint8_t)round_away(x, id);
       if (lane % 32 == 0) *(uint16_t *)(tile + q8_scale_at(D, d / 32, (int)o)) = f2h(dd);
     }
     return;

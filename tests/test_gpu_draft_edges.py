@@ -1,0 +1,102 @@
+"""Calls around drafted tokens and the Q8_0 pool at their edges, on the GPU:
+products that end on a half of a step."""
+import numpy as np
+import pytest
+
+from tests.test_gpu_draft import dev, k_tile, quants, st, v_tile
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+
+@pytest.fixture(scope="module")
+def L():
+    from lgml_amd import hip
+    assert torch.cuda.is_available(), "GPU tests need a GPU"
+    return hip.lib()
+
+
+# ---- the rounding of the Q8_0 stores -----------------------------------------------
+def half_block(rng):
+    """32 f32 values of a block whose products with 1 / d end on k + 1/2 in f32, most
+    of them with an exact product below it; the block's largest is the first."""
+    a = np.float32(rng.uniform(0.3, 4.0))
+    inv = np.float32(1) / (a / np.float32(127))
+    y = (np.arange(126) + 0.5).astype(np.float32)
+    x = (y / inv).astype(np.float32)
+    near = np.stack([np.nextafter(x, np.float32(0)), x, np.nextafter(x, np.float32(9))])
+    exact = near.astype(np.float64) * np.float64(inv)  # 48 bits at most
+    tie = (near * inv).astype(np.float32) == y
+    below, any_ = near[tie & (exact < y)], near[tie]
+    take = rng.permutation(below)[:27]
+    take = np.concatenate([take, rng.permutation(any_)[:31 - len(take)]])
+    take = np.concatenate([take, np.full(31 - len(take), y[0] / inv, np.float32)])
+    block = np.concatenate([[a], take * rng.choice([-1, 1], 31)]).astype(np.float32)
+    return block
+
+
+def halves(n, kv, D, seed):
+    """Rows (n, kv, D) of such blocks; in every fourth d is 1 and the values are
+    k + 1/2 and the numbers next to it."""
+    rng = np.random.default_rng(seed)
+    out = np.zeros((n * kv * D // 32, 32), np.float32)
+    for i in range(len(out)):
+        if i % 4:
+            out[i] = half_block(rng)
+        else:
+            h = (rng.integers(0, 127, 31) + 0.5).astype(np.float32) * rng.choice([-1, 1], 31).astype(np.float32)
+            to = rng.choice([-1000, 0, 1000], 31).astype(np.float32)
+            h = np.where(to == 0, h, np.nextafter(h, to)).astype(np.float32)
+            out[i] = np.concatenate([[127], h])
+    out[0, 1:3] = 13.5, -13.5
+    # a block of largest 0x1.62fe6p+1 takes -0x1.2de266p-2 to -13.5
+    out[1, 0], out[1, 1] = float.fromhex("0x1.62fe6p+1"), float.fromhex("-0x1.2de266p-2")
+    out[1, 2:] = 0
+    rows = out.reshape(n, kv, D)
+    g = rows.reshape(-1, 32)
+    inv = np.float32(1) / (np.abs(g).max(1) / np.float32(127))
+    y = np.abs((g * inv[:, None]).astype(np.float32))
+    on_half = y % 1 == 0.5
+    low = on_half & (np.abs(g.astype(np.float64) * inv[:, None].astype(np.float64)) < y)
+    assert on_half.mean() > 0.4 and low.mean() > 0.1, (on_half.mean(), low.mean())
+    return rows
+
+
+def tiles_of(x, cells, blocks, D, make):
+    """The pool bytes (blocks, kv, 68 D) of rows x in cells, zeros elsewhere."""
+    q, d = quants(x)
+    kv = x.shape[1]
+    out = np.zeros((blocks, kv, 68 * D), np.uint8)
+    for b in range(blocks):
+        for h in range(kv):
+            tq, td = np.zeros((64, D), np.int8), np.zeros((64, D // 32), np.float16)
+            for j in np.flatnonzero(cells // 64 == b):
+                tq[cells[j] % 64], td[cells[j] % 64] = q[j, h], d[j, h]
+            out[b, h] = make(tq, td, D)
+    return out
+
+
+@pytest.mark.parametrize("D,kv", [(64, 2), (128, 1), (256, 2)])
+def test_stores_round_the_f32_product(L, D, kv):
+    """q is the f32 product x (1 / d) rounded with halves away from zero, in the plain
+    store and in the fused one (at position 0, where the rope keeps K's rows)."""
+    from lgml_amd import hip
+    n, blocks, H = 40, 2, kv
+    k, v = halves(n, kv, D, D), halves(n, kv, D, D + 1)
+    cells = np.arange(70, 70 + n, dtype=np.int64)
+    want = [tiles_of(k, cells, blocks, D, k_tile), tiles_of(v, cells, blocks, D, v_tile)]
+    dc, kd, vd = dev(cells), dev(k), dev(v)
+    pools = [torch.zeros(want[0].size, dtype=torch.uint8, device="cuda") for _ in range(4)]
+    hip.check(L.lgmlh_kv_store_q8(pools[0].data_ptr(), pools[1].data_ptr(), 64 * blocks, kv, D, kd.data_ptr(),
+                                  vd.data_ptr(), dc.data_ptr(), cells.ctypes.data, n, st()))
+    qkv = dev(np.concatenate([k, k, v], 1).reshape(n, -1))
+    pos = torch.zeros(n, dtype=torch.int32, device="cuda")
+    q = torch.empty(n, H * D, device="cuda")
+    hip.check(L.lgmlh_qkv_rope_store_q8(qkv.data_ptr(), n, H, kv, D, D, 0, 1e4, None, None, None, 1e-5,
+                                        pos.data_ptr(), pools[2].data_ptr(), pools[3].data_ptr(), 64 * blocks,
+                                        dc.data_ptr(), q.data_ptr(), st()))
+    assert torch.equal(q.view(n, kv, D), kd)
+    for i, p in enumerate(pools):
+        got = p.cpu().numpy().reshape(want[0].shape)
+        assert np.array_equal(got, want[i % 2]), (i, int((got != want[i % 2]).sum()))
