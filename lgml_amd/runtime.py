@@ -30,6 +30,15 @@ def _dev(arr):
     return t.to(DEV)
 
 
+def _dev_behind(arr):
+    """Copy a numpy array to a new device tensor behind the work of the current
+    stream, which the host does not wait for (by way of pinned memory)."""
+    a = np.ascontiguousarray(arr)
+    t = torch.empty(a.shape, dtype=torch.from_numpy(a[:0]).dtype, pin_memory=True)
+    t.numpy()[...] = a
+    return t.to(DEV, non_blocking=True)
+
+
 def _empty(nbytes):
     return torch.empty(max(int(nbytes), 1), dtype=torch.uint8, device=DEV)
 
@@ -579,17 +588,20 @@ class DeviceModel:
         """Cells src to dst in every paged layer's K and V, each dst as its
         src was before (lgmlh_kv_move): the accepted tokens of a verified tree
         to the slots behind the context, or a block's first cells to another.
-        Up to 1024 cells."""
+        Up to 1024 cells. The move is queued on the current stream and waits for
+        nothing on the host; a captured stream is refused."""
         src, dst = (np.ascontiguousarray(a, np.int64).reshape(-1) for a in (src, dst))
         if len(src) != len(dst):
             raise ValueError("%d cells to %d places" % (len(src), len(dst)))
         if not len(src) or not self.n_pools:
             return
-        ds, dd = _dev(src), _dev(dst)
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("move_cells takes its cells from the host: capture lgmlh_kv_move instead")
+        both = _dev_behind(np.stack([src, dst]))
         D, Hkv = self.paged_dims
         check(hip.lib().lgmlh_kv_move(self.kv_type, self.pools_dev.data_ptr(), self.n_pools,
-                                      self.n_cells, Hkv, D, ds.data_ptr(), dd.data_ptr(), ptr(src),
-                                      ptr(dst), len(src), stream()))
+                                      self.n_cells, Hkv, D, both[0].data_ptr(), both[1].data_ptr(),
+                                      ptr(src), ptr(dst), len(src), stream()))
 
     def gather_kv(self, layer, cells, which=0):
         """Cells of a layer's K (0) or V (1) as (n, Hkv*D) f16 bits (uint16)

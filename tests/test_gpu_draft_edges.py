@@ -1,5 +1,6 @@
 """Calls around drafted tokens and the Q8_0 pool at their edges, on the GPU:
-products that end on a half of a step."""
+products that end on a half of a step, moves and copies of cells behind a busy
+stream."""
 import numpy as np
 import pytest
 
@@ -100,3 +101,62 @@ def test_stores_round_the_f32_product(L, D, kv):
     for i, p in enumerate(pools):
         got = p.cpu().numpy().reshape(want[0].shape)
         assert np.array_equal(got, want[i % 2]), (i, int((got != want[i % 2]).sum()))
+
+
+# ---- moves of cells wait for nothing --------------------------------------------------
+@pytest.mark.parametrize("kind", ["F16", "Q8_0"])
+def test_moves_are_queued_behind_a_busy_stream(kind):
+    """move_cells, and the engine's copy of a partial block, return while earlier
+    work of the stream still runs, as lgmlh_kv_copy_block does, and move the cells
+    that they were given then."""
+    from lgml_amd import engine, hip, runtime
+    from oracle import models
+    hp, w = models.build("c1", seed=7)
+    m = runtime.DeviceModel(hp, w, 1024, kv_type=getattr(hip, kind))
+    seqs = engine.PoolSeqs(m)
+    rng = np.random.default_rng(2)
+    for pool in m.kpools + m.vpools:
+        pool.copy_(dev(rng.integers(0, 60, pool.numel()).astype(np.uint8)))
+    before = [m.gather_kv(1, np.arange(1024), which) for which in (0, 1)]
+    seqs.copy_block(9, 10, 5)
+    m.move_cells([900], [901])  # first uses
+    a = torch.randn(8192, 8192, device="cuda")
+    torch.mm(a, a)
+    torch.cuda.synchronize()
+    for _ in range(20):  # some 100 ms
+        torch.mm(a, a)
+    done = torch.cuda.Event()
+    done.record()
+    src, dst = np.array([70, 71, 3]), np.array([64, 65, 66])
+    m.move_cells(src, dst)
+    src[:], dst[:] = 0, 0
+    seqs.copy_block(2, 5, 17)
+    early = not done.query()
+    for i in range(40):  # (their host memory is not used again too early)
+        m.move_cells([200 + i], [300 + i])
+    torch.cuda.synchronize()
+    assert early
+    frm = np.arange(1024)
+    frm[64 * 10:64 * 10 + 5] = 64 * 9 + np.arange(5)
+    frm[901] = 900
+    frm[[64, 65, 66]] = [70, 71, 3]
+    frm[64 * 5:64 * 5 + 17] = 64 * 2 + np.arange(17)
+    frm[300:340] = np.arange(200, 240)
+    for which in (0, 1):
+        assert np.array_equal(m.gather_kv(1, np.arange(1024), which), before[which][frm])
+
+
+def test_move_cells_of_a_captured_stream_is_refused():
+    from lgml_amd import runtime
+    from oracle import models
+    hp, w = models.build("c1", seed=7)
+    m = runtime.DeviceModel(hp, w, 256)
+    x = torch.zeros(8, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        x += 1
+        with pytest.raises(RuntimeError, match="lgmlh_kv_move"):
+            m.move_cells([1], [2])
+    graph.replay()
+    torch.cuda.synchronize()
+    assert bool((x == 1).all())
