@@ -131,8 +131,8 @@ def load_gguf(path, n_cells, ring_cells=0):
 
 def log_probs(logits, ids=None, top=0):
     """lgmlh_log_probs of rows of logits (n, vocab) f32 on the device: a dict
-    with entropy (n); of given ids (n, m) int32, lp (n, m); and with top > 0
-    the most likely tokens, top_ids and top_lp (n, top)."""
+    with entropy (n); of given ids (n, m), lp (n, m), -inf for an id outside the
+    row; and with top > 0 the most likely tokens, top_ids and top_lp (n, top)."""
     L = hip.lib()
     if logits.dim() != 2 or logits.dtype != torch.float32 or not logits.is_contiguous():
         raise ValueError("logits: contiguous f32 rows")
@@ -141,7 +141,11 @@ def log_probs(logits, ids=None, top=0):
     n, v = logits.shape
     m = 0
     if ids is not None:
-        ids = torch.as_tensor(ids, dtype=torch.int32).to(DEV).contiguous()
+        ids = torch.as_tensor(ids).to(DEV)
+        if ids.dtype != torch.int32:  # a wider id of no row stays one
+            ids = ids.to(torch.int64)
+            ids = torch.where((ids >= 0) & (ids < v), ids, -1).to(torch.int32)
+        ids = ids.contiguous()
         if ids.dim() != 2 or ids.shape[0] != n:
             raise ValueError("ids: (%d, m)" % n)
         m = ids.shape[1]

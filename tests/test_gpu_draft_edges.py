@@ -1,6 +1,6 @@
 """Calls around drafted tokens and the Q8_0 pool at their edges, on the GPU:
 products that end on a half of a step, moves and copies of cells behind a busy
-stream."""
+stream, ids that no row holds."""
 import numpy as np
 import pytest
 
@@ -160,3 +160,21 @@ def test_move_cells_of_a_captured_stream_is_refused():
     graph.replay()
     torch.cuda.synchronize()
     assert bool((x == 1).all())
+
+
+# ---- given ids of any integer type -----------------------------------------------------
+def test_log_probs_of_ids_that_no_row_holds():
+    """-inf for an id outside the row, of any width: none is taken for another."""
+    from lgml_amd import runtime
+    x = torch.randn(2, 300, generator=torch.Generator("cuda").manual_seed(3), device="cuda")
+    ids = np.array([[7, 2**32 + 7, -1, 300], [2**33 + 5, -2**32 + 9, 5, 2**31 + 5]], np.int64)
+    want = torch.log_softmax(x.double().cpu(), 1).numpy()
+    for given in (ids, ids.tolist(), torch.from_numpy(ids), torch.from_numpy(ids).cuda()):
+        lp = runtime.log_probs(x, given)["lp"].cpu().numpy()
+        assert abs(lp[0, 0] - want[0, 7]) < 1e-5 and abs(lp[1, 2] - want[1, 5]) < 1e-5
+        assert np.isneginf(lp).tolist() == [[False, True, True, True], [True, True, False, True]]
+    small = runtime.log_probs(x, torch.tensor([[255], [5]], dtype=torch.uint8))["lp"].cpu().numpy()
+    assert abs(small[0, 0] - want[0, 255]) < 1e-5 and abs(small[1, 0] - want[1, 5]) < 1e-5
+    x = x[:, :200].contiguous()
+    small = runtime.log_probs(x, torch.tensor([[255], [5]], dtype=torch.uint8))["lp"].cpu().numpy()
+    assert np.isneginf(small).tolist() == [[True], [False]]
