@@ -124,7 +124,8 @@ int64_t lgmlh_kv_q8_layer_bytes(int64_t n_cells, int n_head_kv, int head_dim);
  * (f32): per 32 values d = max|x| / 127, q = x (1 / d) rounded with halves away
  * from zero, d kept as f16. Rows are finite and below
  * 127 * 65504 (d is f16; above it reads back as infinite). Cells of one call
- * are distinct: a cell twice, which would mix two rows, is LGMLH_EINVAL. */
+ * are distinct: a cell twice, which would mix two rows, is LGMLH_EINVAL. Up to
+ * 65535 KV heads, here and in the read back. */
 int lgmlh_kv_store_q8(void *kpool, void *vpool, int64_t n_cells, int n_head_kv, int head_dim,
     const float *k_src, const float *v_src, const int64_t *cells, const int64_t *h_cells,
     int64_t n, void *stream);

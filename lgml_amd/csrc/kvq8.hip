@@ -419,8 +419,11 @@ static int check_write_cells(const int64_t *h, int64_t n, int64_t n_cells, const
 }
 
 // Heads of cells in one call: a launch has fewer than 2^32 threads, 256 for 32 or
-// more of them.
+// more of them. KV heads: the bytes of a block, 68 D for each, are counted in 31
+// bits (tile_of).
 constexpr int64_t Q8_ROWS = int64_t(1) << 29;
+constexpr int Q8_HEADS = 65535;
+static_assert((int64_t)Q8_HEADS * q8_tile_bytes(256) < INT32_MAX, "tile_of");
 
 static bool q8_head(int D) { return D == 64 || D == 128 || D == 256; }
 
@@ -438,7 +441,7 @@ extern "C" int lgmlh_kv_store_q8(void *kpool, void *vpool, int64_t n_cells, int 
                                  const int64_t *cells, const int64_t *h_cells, int64_t n,
                                  void *stream) {
   if (!kpool || !vpool || !k_src || !v_src || !cells || n < 0 || n_cells <= 0 ||
-      n_cells > Q8_CELLS || n_cells % KV_BLOCK || n_head_kv <= 0 ||
+      n_cells > Q8_CELLS || n_cells % KV_BLOCK || n_head_kv <= 0 || n_head_kv > Q8_HEADS ||
       n >= Q8_ROWS / n_head_kv || !q8_head(head_dim)) {
     set_error("kv_store_q8: bad arguments (heads of 64, 128 or 256)");
     return LGMLH_EINVAL;
@@ -466,7 +469,7 @@ extern "C" int lgmlh_kv_gather_q8(const void *pool, int which, int64_t n_cells, 
                                   int head_dim, const int64_t *cells, int64_t n, void *out,
                                   int out_type, void *stream) {
   if (!pool || !cells || !out || n < 0 || (which != 0 && which != 1) || n_cells <= 0 ||
-      n_cells > Q8_CELLS || n_cells % KV_BLOCK || n_head_kv <= 0 ||
+      n_cells > Q8_CELLS || n_cells % KV_BLOCK || n_head_kv <= 0 || n_head_kv > Q8_HEADS ||
       n >= Q8_ROWS / n_head_kv || !q8_head(head_dim) ||
       (out_type != LGMLH_F32 && out_type != LGMLH_F16)) {
     set_error("kv_gather_q8: bad arguments (heads of 64, 128 or 256; out f32 or f16)");

@@ -38,3 +38,12 @@ def test_a_cell_twice_is_found_among_any_cells(hip, blocks):
     for at in (0, len(cells) // 2, len(cells) - 1):
         assert store(hip, np.append(rng.permutation(cells), cells[at]), top) == hip.EINVAL
         assert "block %d is written twice" % (cells[at] // 64) in hip.last_error()
+
+
+@pytest.mark.parametrize("kv", [65536, 130000, 1 << 28])
+def test_pools_of_more_kv_heads_than_a_launch_takes_are_refused(hip, kv):
+    """(The bytes of a block past 2^31 would not be counted right.)"""
+    L, d, c = hip.lib(), C.c_void_p(256), np.zeros(1, np.int64)
+    assert L.lgmlh_kv_store_q8(d, d, 64, kv, 256, d, d, d, c.ctypes.data, 1, None) == hip.EINVAL
+    assert L.lgmlh_kv_gather_q8(d, 0, 64, kv, 256, d, 1, d, hip.F32, None) == hip.EINVAL
+    assert L.lgmlh_kv_gather_q8(d, 1, 64, kv, 256, d, 0, d, hip.F32, None) == hip.EINVAL
