@@ -397,7 +397,7 @@ class DeviceModel:
             nc = self.ring_cells if Ly.swa else self.n_cells
             kvb_l = (L.lgmlh_kv_q8_layer_bytes if kv_type == hip.Q8_0 else
                      L.lgmlh_kv_layer_bytes)(nc, Hl, Dl)
-            if kvb_l < 0:
+            if kvb_l < 0 and kv_type == hip.Q8_0 and nc:
                 raise ValueError("a Q8_0 pool takes heads of 64, 128 or 256, not %d" % Dl)
             kp = _zeros(kvb_l)
             vp = _zeros(kvb_l)

@@ -1,6 +1,6 @@
 """Calls around drafted tokens and the Q8_0 pool at their edges, on the GPU:
 products that end on a half of a step, moves and copies of cells behind a busy
-stream, ids that no row holds."""
+stream, ids that no row holds, models without cells."""
 import numpy as np
 import pytest
 
@@ -178,3 +178,26 @@ def test_log_probs_of_ids_that_no_row_holds():
     x = x[:, :200].contiguous()
     small = runtime.log_probs(x, torch.tensor([[255], [5]], dtype=torch.uint8))["lp"].cpu().numpy()
     assert np.isneginf(small).tolist() == [[True], [False]]
+
+
+# ---- models -----------------------------------------------------------------------------
+@pytest.mark.parametrize("kind", ["F16", "Q8_0"])
+def test_a_model_without_cells_is_built(kind):
+    """And refuses tokens, not the heads of its pool."""
+    from lgml_amd import hip, runtime
+    from oracle import models
+    hp, w = models.build("c1", seed=7)
+    m = runtime.DeviceModel(hp, w, 0, kv_type=getattr(hip, kind))
+    with pytest.raises(hip.LgmlhError):
+        m.plan([1], [0], np.zeros((1, 1), np.int32), [1])
+
+
+def test_q8_pools_of_other_heads_are_refused():
+    from lgml_amd import hip, runtime
+    from oracle import models
+    hp, w = models.build("c1", seed=7)
+    hp = dict(hp, head_dim=hp["head_dim"] // 2, n_head=2 * hp["n_head"], n_head_kv=2 * hp["n_head_kv"],
+              n_rot=hp["head_dim"] // 2)
+    runtime.DeviceModel(hp, w, 128)
+    with pytest.raises(ValueError, match="heads of 64, 128 or 256, not %d" % hp["head_dim"]):
+        runtime.DeviceModel(hp, w, 128, kv_type=hip.Q8_0)
