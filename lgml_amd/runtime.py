@@ -120,13 +120,14 @@ def generated_weights(hp, seed, policy):
     return get
 
 
-def load_gguf(path, n_cells, ring_cells=0):
+def load_gguf(path, n_cells, ring_cells=0, kv_type=hip.F16):
     """A DeviceModel from a gguf file (lgml_amd.gguf.load: llama, qwen3,
     qwen3moe, gemma4; a gemma4 model's sliding and global layers keep their
-    own head sizes and KV head counts)."""
+    own head sizes and KV head counts). kv_type: of its KV pools, hip.F16 or
+    hip.Q8_0."""
     from . import gguf
     hp, w = gguf.load(path)
-    return DeviceModel(hp, w, n_cells, ring_cells)
+    return DeviceModel(hp, w, n_cells, ring_cells, kv_type=kv_type)
 
 
 def log_probs(logits, ids=None, top=0):

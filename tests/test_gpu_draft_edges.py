@@ -201,3 +201,17 @@ def test_q8_pools_of_other_heads_are_refused():
     runtime.DeviceModel(hp, w, 128)
     with pytest.raises(ValueError, match="heads of 64, 128 or 256, not %d" % hp["head_dim"]):
         runtime.DeviceModel(hp, w, 128, kv_type=hip.Q8_0)
+
+
+def test_a_gguf_model_takes_a_q8_cache(tmp_path):
+    from lgml_amd import hip, runtime
+    from tests.gpu_util import lcg_ints
+    from tests.test_gpu_gguf import c2_like_gguf
+    path = str(tmp_path / "m.gguf")
+    hp, w = c2_like_gguf(path)
+    a = runtime.DeviceModel(hp, w, 256, kv_type=hip.Q8_0)
+    b = runtime.load_gguf(path, 256, kv_type=hip.Q8_0)
+    assert b.kpools[0].numel() == a.kpools[0].numel()
+    ids, bt = np.array(lcg_ints(11, 37, 0, hp["n_vocab"]), np.int32), np.array([[0, 1]], np.int32)
+    la, lb = (m.forward(m.plan([37], [0], bt, ids)).cpu().numpy() for m in (a, b))
+    assert np.array_equal(la.view(np.uint32), lb.view(np.uint32))
