@@ -193,6 +193,8 @@ class Plan:
         self.info = hip.PlanInfo()
         if parents is not None:
             self.parents = np.ascontiguousarray(parents, np.int32).reshape(-1)
+            if (self.parents != np.reshape(parents, -1)).any():
+                raise ValueError("parents: whole numbers of 32 bits")
             if len(self.parents) != len(self.ids):
                 raise ValueError("%d parents for %d tokens" % (len(self.parents), len(self.ids)))
             fn = L.lgmlh_plan_tree

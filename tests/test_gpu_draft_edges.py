@@ -215,3 +215,14 @@ def test_a_gguf_model_takes_a_q8_cache(tmp_path):
     ids, bt = np.array(lcg_ints(11, 37, 0, hp["n_vocab"]), np.int32), np.array([[0, 1]], np.int32)
     la, lb = (m.forward(m.plan([37], [0], bt, ids)).cpu().numpy() for m in (a, b))
     assert np.array_equal(la.view(np.uint32), lb.view(np.uint32))
+
+
+# ---- parents of any integer type ---------------------------------------------------------
+@pytest.mark.parametrize("bad", [[-1, 2**32, 0], [-1, -2**32, 0], [-1.0, 0.5, 0.0]])
+def test_parents_past_32_bits_are_no_parents(bad):
+    from lgml_amd import runtime
+    tab, ids = np.array([[0, 1]], np.int32), np.zeros(3, np.int32)
+    for good in ([-1, 0, 0], np.array([-1, 0, 0], np.int64), np.array([[-1, 0, 0]])):
+        assert list(runtime.Plan([3], [10], tab, ids, 4, 2, 2, parents=good).parents) == [-1, 0, 0]
+    with pytest.raises(ValueError):
+        runtime.Plan([3], [10], tab, ids, 4, 2, 2, parents=np.array(bad))
