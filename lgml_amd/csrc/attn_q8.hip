@@ -7,16 +7,20 @@
 // S^T. q rows are scaled by a power of two to just below 2^15, so that hi + lo
 // carries 22 bits of every element down to 2^-17 of the row's largest.
 // o_rd = sum_c (p_rc dv_cb) v8_cd, b = d / 32: dv goes into P, per block of 32
-// dims, and P dv enters the MFMAs as f16 hi + lo, Q8_P times as large (O with it,
-// and l in the end). Where the largest dv that a row sees of each 32 dims of the
-// block is in [2^-10, 4) (values of 0.12 to 500; or 0), P is split once and
-// multiplied by dv in packed f16, the product's rounding caught by an fma: hi =
-// P_hi dv, lo = P_lo dv + (P_hi dv - hi), 24 operations a lane instead of 88.
-// There hi + lo keep 22 bits of p dv down to 2^-16 of the row's largest, and below
-// are at most 2^-38 of it off. Else P dv is made in f32 and scaled by the power
-// of two that puts the row's largest dv at 2^14 to 2^15, the products scaled back
-// as they add to O^T; a cell that a row does not see has p and dv as zeros there,
-// so that nothing in it (a scale that is infinite or NaN) reaches the row.
+// dims, and P dv enters the MFMAs as f16 hi + lo; O and l are Q8_O times as large.
+// Where each dv that a row sees of the block is 0 or in [2^-12, 2^-2) (largest
+// values of 0.03 to 31), P is split once and multiplied by Q8_DV dv in packed f16,
+// the product's rounding caught by an fma: hi = P_hi dv, lo = P_lo dv + (P_hi dv -
+// hi), 24 operations a lane. hi + lo keep 22 bits of a p dv of 2^-19 or more there,
+// and are at most 2^-42 off below: the dv of a cell of weight 1 keeps its bits. Else
+// P dv is made in f32 and scaled by the power of two that puts the row's largest of
+// the 32 dims at 2^14 to 2^15 (22 bits down to 2^-16 of it, at most 2^-39 of it off
+// below), the products scaled back as they add to O^T, some 200 operations; a cell
+// that a row does not see has p and dv as zeros there, so that nothing in it (a
+// scale that is infinite or NaN) reaches the row. Scaled by the largest dv instead,
+// a row that attends to one quiet cell among loud ones had the loud ones' step: V
+// 1e-4 of the others' was 5e-5 of itself off. The second way takes the decode of 64
+// sequences below 80 us where the first takes 58 (cells in the memory-side cache).
 //
 // Bounds. One token of 64 sequences at 128 to 4096 cells, 32 / 8 heads of 128, is
 // 67 + 6 us from HBM: 296 MB at 4.4 TB/s in the first (54 with the cells in the
@@ -30,7 +34,9 @@
 
 namespace lgmlh {
 
-constexpr float Q8_P = 8192.0f;  // the scale of P
+constexpr float Q8_P = 8192.0f;       // the scale of P in its halves
+constexpr float Q8_DV = 16.0f;        // of V's scales in the packed products
+constexpr float Q8_O = Q8_P * Q8_DV;  // of O^T and l
 constexpr int SHARED_MAX = ATTN_SHARED;  // the most items of a shared run
 
 __device__ __forceinline__ f32x4 mfma16q(f16x8 a, f16x8 b, f32x4 c) {
@@ -97,20 +103,34 @@ __device__ __forceinline__ float split_q(const f32x4 (&qa)[2 * NB], bool rvalid,
   return scale_log2 * pow2(e - 15);
 }
 
+// The lane, of which what follows is made anew where it is used: held over a loop, it
+// takes registers that heads of 256 do not have.
+__device__ __forceinline__ int lane_anew() {
+  int lane = threadIdx.x;
+  asm volatile("" : "+v"(lane));
+  return lane & 63;
+}
+
+// A block's word from the lane's first cell, 8 quad, on.
+__device__ __forceinline__ uint64_t lane_cells(uint64_t word) { return word >> (lane_anew() >> 1 & 24); }
+
 // Scores (scaled, in units of log2) -> P in place, the running maximum and sum,
 // the rescale of O^T. masked: cells without a bit in word are dropped. l is of the
 // lane's own cells; the quads' add up at the end.
 template <int DT>
 __device__ __forceinline__ void softmax_q8(f32x4 (&st)[4], float rscale, bool masked, uint64_t word,
-                                           int quad, float &m, float &l, f32x4 (&o)[DT]) {
+                                           float &m, float &l, f32x4 (&o)[DT]) {
 #pragma unroll
-  for (int ct = 0; ct < 4; ct++) st[ct] *= rscale;
+  for (int ct = 0; ct < 4; ct++)
+#pragma unroll
+    for (int i = 0; i < 4; i++) st[ct][i] *= rscale;  // (of vectors: the factor would be held four times)
   if (masked) {  // wave-uniform
+    word = lane_cells(word);  // s_cell(ct, 4 quad + i) = 8 quad + s_cell(ct, i)
 #pragma unroll
     for (int ct = 0; ct < 4; ct++)
 #pragma unroll
       for (int i = 0; i < 4; i++)
-        if (!(word >> s_cell(ct, 4 * quad + i) & 1)) st[ct][i] = -INFINITY;
+        if (!(word >> s_cell(ct, i) & 1)) st[ct][i] = -INFINITY;
   }
   float mx = -INFINITY;
 #pragma unroll
@@ -138,82 +158,107 @@ __device__ __forceinline__ void softmax_q8(f32x4 (&st)[4], float rscale, bool ma
   m = m_new;
 }
 
-// The largest |scale| of 8 or more as the f16's bits: in them NaN is above the
-// infinity, where a maximum of numbers would pass it by. A float of the number
-// goes through the lanes' maxima.
+// |scale| as the f16's bits, where NaN is above the infinity: the largest of 8,
+// and the least but for zeros, less 1 (none: 0xffff). Floats of the numbers go
+// through the lanes' maxima.
 typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
-__device__ __forceinline__ u16x2 scale_bits(u32x4 s) {
+__device__ __forceinline__ float high_bits(u32x4 s) {
   u16x2 w[4];
 #pragma unroll
   for (int i = 0; i < 4; i++) w[i] = __builtin_bit_cast(u16x2, s[i] & 0x7fff7fffu);
-  return __builtin_elementwise_max(__builtin_elementwise_max(w[0], w[1]), __builtin_elementwise_max(w[2], w[3]));
+  const u16x2 m = __builtin_elementwise_max(__builtin_elementwise_max(w[0], w[1]), __builtin_elementwise_max(w[2], w[3]));
+  return (float)(m[0] > m[1] ? m[0] : m[1]);
 }
-__device__ __forceinline__ float larger(u16x2 b) { return (float)(b[0] > b[1] ? b[0] : b[1]); }
-
-// The scales of a lane's cells (32 h + 8 quad + e) of one block of 32 dims, those
-// of cells that word leaves out as zeros, and the bits of the row's largest.
-__device__ __forceinline__ float row_scales(u32x4 s0, u32x4 s1, bool masked, uint64_t word, int quad,
-                                            f16x8 (&dv)[2]) {
-  if (masked) {  // wave-uniform
+__device__ __forceinline__ float low_bits(u32x4 s) {
+  u16x2 w[4];
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const uint32_t b0 = (uint32_t)(word >> (8 * quad + 2 * i)), b1 = (uint32_t)(word >> (32 + 8 * quad + 2 * i));
-      s0[i] &= (b0 & 1 ? 0xffffu : 0) | (b0 & 2 ? 0xffff0000u : 0);
-      s1[i] &= (b1 & 1 ? 0xffffu : 0) | (b1 & 2 ? 0xffff0000u : 0);
-    }
-  }
-  dv[0] = __builtin_bit_cast(f16x8, s0);
-  dv[1] = __builtin_bit_cast(f16x8, s1);
-  return quads_max(larger(__builtin_elementwise_max(scale_bits(s0), scale_bits(s1))));
+  for (int i = 0; i < 4; i++) w[i] = __builtin_bit_cast(u16x2, s[i] & 0x7fff7fffu) - u16x2{1, 1};
+  const u16x2 m = __builtin_elementwise_min(__builtin_elementwise_min(w[0], w[1]), __builtin_elementwise_min(w[2], w[3]));
+  return (float)(m[0] < m[1] ? m[0] : m[1]);
 }
-
-// P dv of one block of 32 dims as f16 hi + lo, scaled by the row's largest dv (its
-// bits); the factor that undoes it.
-__device__ __forceinline__ float weigh_p(const f32x4 (&st)[4], const f16x8 (&dv)[2], float bits,
-                                         f16x8 (&ph)[2], f16x8 (&pl)[2]) {
-  const float mx = (float)__builtin_bit_cast(f16, (unsigned short)bits);
-  const int ex = __builtin_amdgcn_frexp_expf(mx);  // mx in [2^(ex - 1), 2^ex)
-  const float up = pow2(15 - ex);
-  // hi by truncation, two at a time: lo takes up what it leaves
-#pragma unroll
-  for (int h = 0; h < 2; h++)
-#pragma unroll
-    for (int e = 0; e < 8; e += 2) {
-      const float x0 = st[2 * h + (e >> 2)][e & 3] * up * (float)dv[h][e];
-      const float x1 = st[2 * h + (e >> 2)][(e & 3) + 1] * up * (float)dv[h][e + 1];
-      const f16x2 hi = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(x0, x1));
-      ph[h][e] = hi[0];
-      ph[h][e + 1] = hi[1];
-      pl[h][e] = (f16)fmaf((float)hi[0], -1.0f, x0);
-      pl[h][e + 1] = (f16)fmaf((float)hi[1], -1.0f, x1);
-    }
-  return pow2(ex - 15);
-}
-
-// Whether a block of dims goes by the packed products: its largest scale (bits) is
-// 0 or in [2^-10, 4).
-__device__ __forceinline__ bool plain_scale(float bits) {
-  return bits == 0.0f || (bits >= (float)0x1400 && bits < (float)0x4400);
+// Whether scales go by the packed products: each is 0 or in [2^-12, 2^-2). (Up to
+// 2^15 with P's and its own factor; from 2^-12 on a p of 1 keeps 22 bits.)
+__device__ __forceinline__ bool plain_range(float low, float high) {
+  return high < (float)0x3400 && low >= (float)(0x0c00 - 1);
 }
 // Whether a lane's 8 scales of a group of 32 dims (the group's 64 in 8 aligned
 // lanes) leave the group to the packed products.
 __device__ __forceinline__ bool plain_scales(u32x4 sc) {
-  return plain_scale(group_max<8>(larger(scale_bits(sc))));
+  return plain_range(-group_max<8>(-low_bits(sc)), group_max<8>(high_bits(sc)));
 }
 
-// P (cells 32 h + 8 quad + e) as f16 hi + lo, Q8_P times as large.
-__device__ __forceinline__ void split_p(const f32x4 (&st)[4], f16x8 (&ph)[2], f16x8 (&pl)[2]) {
+// The scales of a lane's cells (32 h + 8 quad + e) of one block of 32 dims, those
+// of cells that word leaves out as zeros.
+__device__ __forceinline__ void seen_scales(u32x4 &s0, u32x4 &s1, uint64_t word) {
+  word = lane_cells(word);
+  const uint32_t w0 = (uint32_t)word, w1 = (uint32_t)(word >> 32);
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    s0[i] &= (w0 >> 2 * i & 1 ? 0xffffu : 0) | (w0 >> 2 * i & 2 ? 0xffff0000u : 0);
+    s1[i] &= (w1 >> 2 * i & 1 ? 0xffffu : 0) | (w1 >> 2 * i & 2 ? 0xffff0000u : 0);
+  }
+}
+
+// The exponent of the row's largest P dv of one block of 32 dims (the least of use).
+__device__ __forceinline__ int largest_pdv(const f32x4 (&st)[4], const f16x8 (&dv)[2]) {
+  float mx = 0.0f;
 #pragma unroll
   for (int h = 0; h < 2; h++)
 #pragma unroll
-    for (int e = 0; e < 8; e += 2) {
-      const float x0 = st[2 * h + (e >> 2)][e & 3] * Q8_P, x1 = st[2 * h + (e >> 2)][(e & 3) + 1] * Q8_P;
-      const f16x2 hi = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(x0, x1));
-      ph[h][e] = hi[0];
-      ph[h][e + 1] = hi[1];
-      pl[h][e] = (f16)fmaf((float)hi[0], -1.0f, x0);
-      pl[h][e + 1] = (f16)fmaf((float)hi[1], -1.0f, x1);
+    for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(st[2 * h + (e >> 2)][e & 3] * (float)dv[h][e]));
+  const int ex = __builtin_amdgcn_frexp_expf(quads_max(mx));  // it is in [2^(ex - 1), 2^ex)
+  return ex < -100 ? -100 : ex;
+}
+
+// x0 and x1 as f16 hi + lo: hi by truncation, lo takes up what it leaves.
+__device__ __forceinline__ void split2(float x0, float x1, f16x2 &hi, f16x2 &lo) {
+  hi = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(x0, x1));
+  lo = f16x2{(f16)fmaf((float)hi[0], -1.0f, x0), (f16)fmaf((float)hi[1], -1.0f, x1)};
+}
+// P dv from P's halves in packed f16, the rounding of hi caught in lo.
+template <typename H>
+__device__ __forceinline__ void packed_pdv(H ph, H pl, H dv, H &hi, H &lo) {
+  hi = ph * dv;
+  lo = __builtin_elementwise_fma(pl, dv, __builtin_elementwise_fma(ph, dv, -hi));
+}
+// P of the cells 32 h + 8 quad + e, Q8_P times as large.
+__device__ __forceinline__ void split_p(const f32x4 (&st)[4], int h, f16x8 &hi, f16x8 &lo) {
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) {
+    const f32x4 &s = st[2 * h + (e >> 2)];
+    f16x2 a, b;
+    split2(s[e & 3] * Q8_P, s[(e & 3) + 1] * Q8_P, a, b);
+    hi[e] = a[0];
+    hi[e + 1] = a[1];
+    lo[e] = b[0];
+    lo[e + 1] = b[1];
+  }
+}
+// P dv of those cells times up, or (MASKED) of a plain row as the packed products
+// make it. (What other calls make alike is not held for this one: the copies are
+// opaque.)
+template <bool MASKED>
+__device__ __forceinline__ void weigh_p(const f32x4 (&st)[4], int h, f16x8 dv, bool plain, float up, f16x8 &hi,
+                                        f16x8 &lo) {
+  float q8_p = Q8_P;
+  asm volatile("" : "+s"(q8_p), "+v"(dv));
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) {
+    const float p0 = st[2 * h + (e >> 2)][e & 3], p1 = st[2 * h + (e >> 2)][(e & 3) + 1];
+    f16x2 a, b;
+    split2(p0 * (float)dv[e] * up, p1 * (float)dv[e + 1] * up, a, b);
+    if constexpr (MASKED) {
+      f16x2 c, d, ph, pl;
+      split2(p0 * q8_p, p1 * q8_p, ph, pl);
+      packed_pdv(ph, pl, f16x2{dv[e], dv[e + 1]} * (f16)Q8_DV, c, d);
+      a = plain ? c : a;
+      b = plain ? d : b;
     }
+    hi[e] = a[0];
+    hi[e + 1] = a[1];
+    lo[e] = b[0];
+    lo[e + 1] = b[1];
+  }
 }
 
 // S^T of a block: read(b, p, k, d) gives the K operands of tiles 2 p and 2 p + 1
@@ -254,41 +299,35 @@ __device__ __forceinline__ void scores_q8(f32x4 (&st)[4], R read, Q query) {
   add(1);
 }
 
+// V's scales as the packed products take them.
+__device__ __forceinline__ u32x4 times_dv(u32x4 s) {
+  f16x8 v = __builtin_bit_cast(f16x8, s);
+  v *= (f16)Q8_DV;
+  return __builtin_bit_cast(u32x4, v);
+}
+
 // O^T += V^T (P dv)^T over a block. scale(b, h): the lane's cells' dv; frag(t, kc):
-// V's operand. plain: plain_scales of all cells (the same for the wave).
+// V's operand. plain (the same for the wave): plain_scales of all the block's cells,
+// whose scales are Q8_DV times as large here. Which way a row's part is made goes
+// by the scales of the cells it sees, and by nothing else, so that a row has the
+// same bits in any group of rows: in a plain block all its rows' cells are plain.
 template <int D, typename S, typename V>
 __device__ __forceinline__ void values_q8(f32x4 (&o)[D / 16], const f32x4 (&st)[4], bool plain,
-                                          bool masked, uint64_t word, int quad, S scale, V frag) {
+                                          bool masked, uint64_t word, S scale, V frag) {
   constexpr int NB = D / 32;
-  // Which way a row's part is made goes by the scales of the cells it sees, and by
-  // nothing else, so that a row has the same bits in any group of rows.
-  bool row_plain = plain;
-  if (masked) {  // wave-uniform: some row does not see all of the block
-    row_plain = true;
-#pragma unroll 1
-    for (int b = 0; b < NB; b++) {
-      f16x8 dv[2];
-      row_plain &= plain_scale(row_scales(scale(b, 0), scale(b, 1), true, word, quad, dv));
-    }
-    // a cell that a row does not see has p of 0 there, and a finite scale here
-    plain &= __builtin_amdgcn_ballot_w64(!row_plain) == 0;
-  }
   if (plain) {
     // a step reads the next 16 dims' V (and makes the next block's P dv) while
     // the products of this one run
     f16x8 ph[2], pl[2], hi[2], lo[2], v[2][2];
-    split_p(st, ph, pl);
+    split_p(st, 0, ph[0], pl[0]);
+    split_p(st, 1, ph[1], pl[1]);
     auto fetch = [&](int t) {
 #pragma unroll
       for (int kc = 0; kc < 2; kc++) v[t & 1][kc] = frag(t, kc);
     };
     auto weigh = [&](int b) {
 #pragma unroll
-      for (int h = 0; h < 2; h++) {
-        const f16x8 dv = __builtin_bit_cast(f16x8, scale(b, h));
-        hi[h] = ph[h] * dv;
-        lo[h] = __builtin_elementwise_fma(pl[h], dv, __builtin_elementwise_fma(ph[h], dv, -hi[h]));
-      }
+      for (int h = 0; h < 2; h++) packed_pdv(ph[h], pl[h], __builtin_bit_cast(f16x8, scale(b, h)), hi[h], lo[h]);
     };
     fetch(0);
     weigh(0);
@@ -306,83 +345,85 @@ __device__ __forceinline__ void values_q8(f32x4 (&o)[D / 16], const f32x4 (&st)[
     }
     return;
   }
-  if (!masked) {
+  auto weighed = [&](auto some_hidden, bool row_plain) __attribute__((always_inline)) {
+    constexpr bool MASKED = decltype(some_hidden)::value;
 #pragma unroll
     for (int b = 0; b < NB; b++) {
-      f16x8 dv[2], ph[2], pl[2];
-      const float mx = row_scales(scale(b, 0), scale(b, 1), false, 0, quad, dv);
-      const float back = Q8_P * weigh_p(st, dv, mx, ph, pl);
+      u32x4 s0 = scale(b, 0), s1 = scale(b, 1);
+      if constexpr (MASKED) seen_scales(s0, s1, word);
+      const f16x8 dv[2] = {__builtin_bit_cast(f16x8, s0), __builtin_bit_cast(f16x8, s1)};
+      const int ex = largest_pdv(st, dv);
+      const float up = pow2(15 - ex), back = Q8_O * pow2(ex - 15);
+      f32x4 acc[2];
 #pragma unroll
-      for (int t = 2 * b; t < 2 * b + 2; t++) {
-        f32x4 acc = {0, 0, 0, 0};
+      for (int t = 0; t < 2; t++)
 #pragma unroll
-        for (int kc = 0; kc < 2; kc++) {
-          const f16x8 v = frag(t, kc);
-          acc = mfma16q(v, ph[kc], acc);
-          acc = mfma16q(v, pl[kc], acc);
+        for (int i = 0; i < 4; i++) acc[t][i] = row_plain ? o[2 * b + t][i] : 0.0f;
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        f16x8 hi, lo;
+        weigh_p<MASKED>(st, h, dv[h], row_plain, up, hi, lo);
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+          const f16x8 v = frag(2 * b + t, h);
+          acc[t] = mfma16q(v, hi, acc[t]);
+          acc[t] = mfma16q(v, lo, acc[t]);
         }
+      }
 #pragma unroll
-        for (int i = 0; i < 4; i++) o[t][i] = fmaf(acc[i], back, o[t][i]);
-        here(o[t]);
+      for (int t = 0; t < 2; t++) {
+        f32x4 &ot = o[2 * b + t];
+#pragma unroll
+        for (int i = 0; i < 4; i++) ot[i] = row_plain ? acc[t][i] : fmaf(acc[t][i], back, ot[i]);
+        here(ot);
       }
       __builtin_amdgcn_sched_barrier(0);
     }
+  };
+  if (!masked) {  // wave-uniform: all rows see all of the block, none is plain
+    weighed(std::false_type{}, false);
     return;
   }
-  // Some rows do not see all of the block, and not all of them go the same way:
-  // both are made, and each row takes its own.
-  f16x8 fh[2], fl[2];
-  split_p(st, fh, fl);
-#pragma unroll
+  // each row takes its own way
+  float low = 65535.0f, high = 0.0f;
+#pragma unroll 1
   for (int b = 0; b < NB; b++) {
-    f16x8 dv[2], ph[2], pl[2];
-    const float mx = row_scales(scale(b, 0), scale(b, 1), true, word, quad, dv);
-    const float back = Q8_P * weigh_p(st, dv, mx, ph, pl);
-#pragma unroll
-    for (int t = 2 * b; t < 2 * b + 2; t++) {
-      f32x4 acc = {0, 0, 0, 0}, fast = o[t];
-#pragma unroll
-      for (int kc = 0; kc < 2; kc++) {
-        const f16x8 v = frag(t, kc);
-        acc = mfma16q(v, ph[kc], acc);
-        acc = mfma16q(v, pl[kc], acc);
-        const f16x8 hi = fh[kc] * dv[kc];
-        const f16x8 lo = __builtin_elementwise_fma(fl[kc], dv[kc], __builtin_elementwise_fma(fh[kc], dv[kc], -hi));
-        fast = mfma16q(v, hi, fast);
-        fast = mfma16q(v, lo, fast);
-      }
-#pragma unroll
-      for (int i = 0; i < 4; i++) o[t][i] = row_plain ? fast[i] : fmaf(acc[i], back, o[t][i]);
-      here(o[t]);
-    }
-    __builtin_amdgcn_sched_barrier(0);
+    u32x4 s0 = scale(b, 0), s1 = scale(b, 1);
+    seen_scales(s0, s1, word);
+    low = fminf(low, fminf(low_bits(s0), low_bits(s1)));
+    high = fmaxf(high, fmaxf(high_bits(s0), high_bits(s1)));
   }
+  weighed(std::true_type{}, plain_range(-quads_max(-low), quads_max(high)));
 }
 
-// What a row (its last visible slot p_row, its token's mask words) sees of a
-// block of a causal, ring or tree plan.
+// A lane's row of an item: its token of the item, its head among the G (1, 2, 4, 8
+// or 16) of the KV head, and whether the item has it.
+struct RowOf {
+  int row, quad, rtok, head;
+  bool valid;
+  __device__ __forceinline__ RowOf(int lane, int G, int ntok)
+      : row(lane & 15), quad(lane >> 4), rtok(row >> __builtin_ctz(G)), head(row & (G - 1)), valid(rtok < ntok) {}
+};
+
+// What the rows of an item see of a block of a causal, ring or tree plan.
 struct Sight {
-  int ring, window;        // of the plan; ring LGMLH_PLAN_TREE: a tree
-  int p_first, p_row, p_last;  // the item's first slot, the row's own, the item's last
+  int ring, window;     // of the plan; ring LGMLH_PLAN_TREE: a tree
+  int p_first, p_last;  // the item's first and last slots
   int b_tree;
-  const uint64_t *vrow;
-  bool rvalid;
+  int G, ntok;
+  const uint64_t *vis;  // the mask words of the item's first token
   // Whether some row of the item does not see all of a block (the same for the
-  // wave, and for every plan that shows the rows the same cells), and the row's
-  // word then.
+  // wave, and for every plan that shows the rows the same cells), and the lane's
+  // row's word then (0 of a row that the item does not have).
   __device__ __forceinline__ bool masks(int blk, uint64_t &w) const {
-    if (ring < 0) {
-      if (blk < b_tree) return false;
-      w = word(blk);
-      return __builtin_amdgcn_ballot_w64(rvalid && ~w != 0) != 0;
-    }
-    if (blk * 64 + 63 <= p_first && (ring == 0 || blk * 64 > p_last - window)) return false;
-    w = word(blk);
-    return true;
+    if (ring < 0 ? blk < b_tree : blk * 64 + 63 <= p_first && (ring == 0 || blk * 64 > p_last - window)) return false;
+    const RowOf r(lane_anew(), G, ntok);
+    w = r.valid ? word(blk, r.rtok) : 0;
+    return ring >= 0 || __builtin_amdgcn_ballot_w64(r.valid && ~w != 0) != 0;
   }
-  __device__ __forceinline__ uint64_t word(int blk) const {
-    if (!rvalid) return 0;
-    if (ring < 0) return vrow[blk - b_tree];
+  __device__ __forceinline__ uint64_t word(int blk, int rtok) const {
+    if (ring < 0) return vis[rtok * window + blk - b_tree];
+    const int p_row = p_first + rtok;  // the row's last visible slot
     const int hi = p_row - blk * 64, lo = ring > 0 ? p_row - window + 1 - blk * 64 : 0;
     uint64_t w = hi >= 63 ? ~(uint64_t)0 : hi < 0 ? 0 : ((uint64_t)2 << hi) - 1;
     if (lo >= 64)
@@ -413,19 +454,16 @@ paged_attn_q8_kernel(const float *__restrict__ q, int H, int Hkv, float scale_lo
   const int s = items[4 * item + 0], tok0 = items[4 * item + 1];
   const int ntok = items[4 * item + 2] & 31, mg = (items[4 * item + 2] >> 5) - 1;
   const int blo = items[4 * item + 3] & 0xffff, bhi = (items[4 * item + 3] >> 16) & 0xffff;
-  const int row = lane & 15, quad = lane >> 4;
-  const int rtok = row / G, rhead = kvh * G + row % G;
-  const bool rvalid = rtok < ntok;
   const int npast = seq_npast[s];
   Sight see;
   see.ring = ring;
   see.window = window;
   see.p_first = npast + (tok0 - seq_off[s]);
-  see.p_row = see.p_first + rtok;
   see.p_last = see.p_first + ntok - 1;
   see.b_tree = npast / KV_BLOCK;
-  see.vrow = ring < 0 ? vis + (int64_t)(tok0 + (rvalid ? rtok : 0)) * window : nullptr;
-  see.rvalid = rvalid;
+  see.G = G;
+  see.ntok = ntok;
+  see.vis = ring < 0 ? vis + (int64_t)tok0 * window : nullptr;
 
   const int32_t *bt = block_tab + (int64_t)s * max_blocks;
   auto tile = [&](const uint8_t *pool, int blk) {
@@ -438,6 +476,7 @@ paged_attn_q8_kernel(const float *__restrict__ q, int H, int Hkv, float scale_lo
   constexpr int SR = D > 128 ? 2 : 1;    // registers' worth: K's and V's, or K's then V's
   constexpr int SL = D > 128 ? 64 : NB * 8;  // lanes of K's scales
   u32x4 kq[4][J], vq[DT], sreg[SR];
+  const int row = lane & 15, quad = lane >> 4;
   const uint32_t koff = (8 * (row >> 2) + (row & 3)) * 64 + quad * 16, voff = row * 64 + quad * 16;
   auto load_k = [&](int blk) {
     const uint8_t *t = tile(kpool, blk);
@@ -462,26 +501,29 @@ paged_attn_q8_kernel(const float *__restrict__ q, int H, int Hkv, float scale_lo
     }
   };
   __shared__ __align__(16) u32x4 scl[SR * 64];  // K's scales, then V's
-  auto store_s = [&]() {
-#pragma unroll
-    for (int i = 0; i < SR; i++) scl[i * 64 + lane] = sreg[i];
+  auto store_s = [&](bool plain) {
+    if (SR == 2) scl[lane] = sreg[0];
+    u32x4 v = sreg[SR - 1];
+    if (plain && (SR == 2 || lane >= SL)) v = times_dv(v);
+    scl[(SR - 1) * 64 + lane] = v;
   };
   auto scale_of = [&](int v, int b, int h) { return scl[v * SL + b * 8 + h * 4 + quad]; };
   float rscale;
   {
-    const float *qr = q + ((int64_t)(tok0 + (rvalid ? rtok : ntok - 1)) * H + rhead) * D;
+    const RowOf r(lane, G, ntok);
+    const float *qr = q + ((int64_t)(tok0 + (r.valid ? r.rtok : ntok - 1)) * H + kvh * G + r.head) * D;
     f32x4 qa[2 * NB];
 #pragma unroll
     for (int b = 0; b < NB; b++) {
-      qa[2 * b] = *(const f32x4 *)(qr + 32 * b + 8 * quad);
-      qa[2 * b + 1] = *(const f32x4 *)(qr + 32 * b + 8 * quad + 4);
+      qa[2 * b] = *(const f32x4 *)(qr + 32 * b + 8 * r.quad);
+      qa[2 * b + 1] = *(const f32x4 *)(qr + 32 * b + 8 * r.quad + 4);
     }
     const int b_first = blo < bhi ? blo : 0;  // block 0 of a planned sequence is a pool block
     load_s(b_first);
     load_k(b_first);
     load_v(b_first);
     f16x8 hi[NB], lo[NB];
-    rscale = split_q<NB>(qa, rvalid, scale_log2, hi, lo);
+    rscale = split_q<NB>(qa, r.valid, scale_log2, hi, lo);
 #pragma unroll
     for (int b = 0; b < NB; b++) {
       qsh[b * 64 + lane] = hi[b];
@@ -502,7 +544,7 @@ paged_attn_q8_kernel(const float *__restrict__ q, int H, int Hkv, float scale_lo
     // (the lanes of K's scales have no part in this)
     const bool plain = !__builtin_amdgcn_ballot_w64(!plain_scales(sreg[SR - 1]) &&
                                                     (SR == 2 || (lane >= SL && lane < 2 * SL)));
-    store_s();
+    store_s(plain);
     if constexpr (NEXT) load_s(nxt);
     scores_q8<NB>(
         st,
@@ -521,9 +563,9 @@ paged_attn_q8_kernel(const float *__restrict__ q, int H, int Hkv, float scale_lo
     if constexpr (NEXT) load_k(nxt);
     uint64_t word = ~(uint64_t)0;
     const bool masked = see.masks(blk, word);
-    softmax_q8<DT>(st, rscale, masked, word, quad, m, l, o);
+    softmax_q8<DT>(st, rscale, masked, word, m, l, o);
     __builtin_amdgcn_sched_barrier(0);
-    values_q8<D>(o, st, plain, masked, word, quad,
+    values_q8<D>(o, st, plain, masked, word,
                  [&](int b, int h) { return scale_of(1, b, h); },
                  [&](int t, int kc) { return half8(vq[t][2 * kc], vq[t][2 * kc + 1]); });
     if constexpr (NEXT) load_v(nxt);
@@ -532,8 +574,9 @@ paged_attn_q8_kernel(const float *__restrict__ q, int H, int Hkv, float scale_lo
   if (blo < bhi) block(bhi - 1, std::false_type{});
   l += __shfl_xor(l, 16);
   l += __shfl_xor(l, 32);
-  finish_item<D>(o, m, l * Q8_P, mg, rvalid, tok0, rtok, rhead, ntok, G, row, quad, item, kvh, Hkv, H, out,
-                 planes, npad, xf, part);
+  const RowOf r(lane_anew(), G, ntok);
+  finish_item<D>(o, m, l * Q8_O, mg, r.valid, tok0, r.rtok, kvh * G + r.head, ntok, G, r.row, r.quad, item, kvh, Hkv,
+                 H, out, planes, npad, xf, part);
 }
 
 // Shared runs (a chunk's or a tree's query groups in sets): a workgroup of W waves
@@ -578,19 +621,16 @@ paged_attn_q8_shared_kernel(const float *__restrict__ q, int H, int Hkv, float s
   const int blo = items[4 * first + 3] & 0xffff, bhi = (items[4 * first + 3] >> 16) & 0xffff;
   const int tok0 = items[4 * item + 1];
   const int ntok = items[4 * item + 2] & 31, mg = (items[4 * item + 2] >> 5) - 1;
-  const int row = lane & 15, quad = lane >> 4;
-  const int rtok = row / G, rhead = kvh * G + row % G;
-  const bool rvalid = rtok < ntok;
   const int npast = seq_npast[s];
   Sight see;
   see.ring = ring;
   see.window = window;
   see.p_first = npast + (tok0 - seq_off[s]);
-  see.p_row = see.p_first + rtok;
   see.p_last = see.p_first + ntok - 1;
   see.b_tree = npast / KV_BLOCK;
-  see.vrow = ring < 0 ? vis + (int64_t)(tok0 + (rvalid ? rtok : 0)) * window : nullptr;
-  see.rvalid = rvalid;
+  see.G = G;
+  see.ntok = ntok;
+  see.vis = ring < 0 ? vis + (int64_t)tok0 * window : nullptr;
 
   const int32_t *bt = block_tab + (int64_t)s * max_blocks;
   u32x4 raw[CH], sraw;
@@ -626,26 +666,35 @@ paged_attn_q8_shared_kernel(const float *__restrict__ q, int H, int Hkv, float s
         *(f16x8 *)(vb[buf] + (d * 8 + ((4 + qd) ^ swv(d))) * 8) = hi;
       }
     }
-    if (tid < NB * 16) scl[buf][tid] = sraw;
-    // V's scales are in two waves at most (NB * 8 lanes from lane NB * 8 on)
+    // V's scales are in one wave (NB * 8 lanes from lane NB * 8 on)
+    bool plain = false;
     if (wave == NB * 8 / 64) {
       const bool odd = !plain_scales(sraw) && tid >= NB * 8 && tid < NB * 16;
-      const uint64_t any = __builtin_amdgcn_ballot_w64(odd);
-      if (lane == 0) odd_scales[buf] = any != 0;
+      plain = __builtin_amdgcn_ballot_w64(odd) == 0;
+      if (lane == 0) odd_scales[buf] = !plain;
     }
+    if (tid < NB * 16) scl[buf][tid] = plain && tid >= NB * 8 ? times_dv(sraw) : sraw;
   };
   if (blo < bhi) load(blo);
+  // Q's operands in registers, but for the last block of dims of heads of 256 (LDS)
+  constexpr int QR = D == 256 ? NB - 1 : NB;
+  __shared__ f16x8 q_last[D == 256 ? 2 * 64 * W : 1];
   f16x8 qh[NB], ql[NB];
   float rscale;
   {
-    const float *qr = q + ((int64_t)(tok0 + (rvalid ? rtok : ntok - 1)) * H + rhead) * D;
+    const RowOf r(lane, G, ntok);
+    const float *qr = q + ((int64_t)(tok0 + (r.valid ? r.rtok : ntok - 1)) * H + kvh * G + r.head) * D;
     f32x4 qa[2 * NB];
 #pragma unroll
     for (int b = 0; b < NB; b++) {
-      qa[2 * b] = *(const f32x4 *)(qr + 32 * b + 8 * quad);
-      qa[2 * b + 1] = *(const f32x4 *)(qr + 32 * b + 8 * quad + 4);
+      qa[2 * b] = *(const f32x4 *)(qr + 32 * b + 8 * r.quad);
+      qa[2 * b + 1] = *(const f32x4 *)(qr + 32 * b + 8 * r.quad + 4);
     }
-    rscale = split_q<NB>(qa, rvalid, scale_log2, qh, ql);
+    rscale = split_q<NB>(qa, r.valid, scale_log2, qh, ql);
+    if constexpr (QR < NB) {  // read by the lane that writes it
+      q_last[tid] = qh[QR];
+      q_last[64 * W + tid] = ql[QR];
+    }
   }
   f32x4 o[DT];
 #pragma unroll
@@ -656,12 +705,6 @@ paged_attn_q8_shared_kernel(const float *__restrict__ q, int H, int Hkv, float s
   // only the lane's row decides, and from a block of dims its two low bits. The
   // rest of an address is constant.
   constexpr int KB = NB < 4 ? NB : 4;
-  int kat[KB], vat[2];
-  const int r0 = s_cell(0, row);
-#pragma unroll
-  for (int b = 0; b < KB; b++) kat[b] = (r0 * KC + ((b * 4 + quad) ^ swk<D>(r0))) * 8;
-#pragma unroll
-  for (int kc = 0; kc < 2; kc++) vat[kc] = (row * 8 + ((kc * 4 + quad) ^ swv(row))) * 8;
 
   for (int blk = blo; blk < bhi; blk++) {
     const int buf = BUFS == 2 ? (blk - blo) & 1 : 0;
@@ -670,17 +713,20 @@ paged_attn_q8_shared_kernel(const float *__restrict__ q, int H, int Hkv, float s
     if (blk + 1 < bhi) load(blk + 1);
     lds_sync();
     if (!active || blk * 64 > see.p_last) continue;
-    // places in this buffer, made here: otherwise every fragment's address is made
-    // ahead of the loop and takes a register
-    int ka[KB], va[2], sa = buf * (2 * NB * 8) + quad;
+    // places in this buffer, made here from an opaque copy of the lane: otherwise every
+    // fragment's address is made ahead of the loop and takes a register
+    int at = lane;
+    asm volatile("" : "+v"(at));
+    const int arow = at & 15, aquad = at >> 4, r0 = s_cell(0, arow);
+    int ka[KB], va[2], sa = buf * (2 * NB * 8) + aquad;
 #pragma unroll
     for (int b = 0; b < KB; b++) {
-      ka[b] = buf * TILE + kat[b];
+      ka[b] = buf * TILE + (r0 * KC + ((b * 4 + aquad) ^ swk<D>(r0))) * 8;
       asm volatile("" : "+v"(ka[b]));
     }
 #pragma unroll
     for (int kc = 0; kc < 2; kc++) {
-      va[kc] = buf * TILE + vat[kc];
+      va[kc] = buf * TILE + (arow * 8 + ((kc * 4 + aquad) ^ swv(arow))) * 8;
       asm volatile("" : "+v"(va[kc]));
     }
     asm volatile("" : "+v"(sa));
@@ -695,22 +741,23 @@ paged_attn_q8_shared_kernel(const float *__restrict__ q, int H, int Hkv, float s
           d = __builtin_bit_cast(f16x8, sc[b * 8 + 4 * p]);
         },
         [&](int b, f16x8 &hi, f16x8 &lo) {
-          hi = qh[b];
-          lo = ql[b];
+          hi = b < QR ? qh[b] : q_last[64 * wave + at];
+          lo = b < QR ? ql[b] : q_last[64 * (W + wave) + at];
         });
     uint64_t word = ~(uint64_t)0;
     const bool masked = see.masks(blk, word);
-    softmax_q8<DT>(st, rscale, masked, word, quad, m, l, o);
+    softmax_q8<DT>(st, rscale, masked, word, m, l, o);
     __builtin_amdgcn_sched_barrier(0);
-    values_q8<D>(o, st, odd_scales[buf] == 0, masked, word, quad,
+    values_q8<D>(o, st, odd_scales[buf] == 0, masked, word,
                  [&](int b, int h) { return sc[NB * 8 + b * 8 + 4 * h]; },
                  [&](int t, int kc) { return *(const f16x8 *)(vb[0] + va[kc] + t * 1024); });
   }
   if (!active) return;
   l += __shfl_xor(l, 16);
   l += __shfl_xor(l, 32);
-  finish_item<D>(o, m, l * Q8_P, mg, rvalid, tok0, rtok, rhead, ntok, G, row, quad, item, kvh, Hkv, H, out,
-                 planes, npad, xf, part);
+  const RowOf r(lane_anew(), G, ntok);
+  finish_item<D>(o, m, l * Q8_O, mg, r.valid, tok0, r.rtok, kvh * G + r.head, ntok, G, r.row, r.quad, item, kvh, Hkv,
+                 H, out, planes, npad, xf, part);
 }
 
 template <int D>

@@ -1,10 +1,11 @@
 """Calls around drafted tokens and the Q8_0 pool at their edges, on the GPU:
 products that end on a half of a step, moves and copies of cells behind a busy
-stream, ids that no row holds, models without cells."""
+stream, ids that no row holds, models without cells, rows that attend to a cell
+much quieter than the others."""
 import numpy as np
 import pytest
 
-from tests.test_gpu_draft import dev, k_tile, quants, st, v_tile
+from tests.test_gpu_draft import Pass, dev, fill, k_tile, quants, run_attention, st, v_tile
 
 pytestmark = pytest.mark.gpu
 
@@ -226,3 +227,58 @@ def test_parents_past_32_bits_are_no_parents(bad):
         assert list(runtime.Plan([3], [10], tab, ids, 4, 2, 2, parents=good).parents) == [-1, 0, 0]
     with pytest.raises(ValueError):
         runtime.Plan([3], [10], tab, ids, 4, 2, 2, parents=np.array(bad))
+
+
+# ---- rows whose weight is on quiet cells -----------------------------------------------
+def bounds(q, k, v, scale):
+    """(the output (H, D) in 64 bits, how far it may be off (H, D)): q (H, D), k and v
+    (cells, kv, D) f64. A score is off by ds, as in the tests of attention; that
+    turns p_i v_i by p_i |v_i - o| ds, and 2^-21 and the sum's n / 16 + 64 roundings
+    come on sum p |v|; twice that for the terms of higher order. The f16 halves of
+    P dv hold 22 bits (within the 2^-21) down to a place that is fixed, half of
+    whose step each cell may be off: 2^-39 of the largest p dv of the cell's block,
+    which is no more than the largest of the row, whose 127 steps are in the 32
+    dims; or, where scales go by the packed products, 2^-42 times a value of up to
+    127. Signs of n cells' roundings are as good as independent: 7.5 sqrt(n) of the
+    latter (Hoeffding's bound for 1e-6 in all the values of these tests)."""
+    (H, D), (n, kv, _) = q.shape, k.shape
+    g = H // kv
+    qs, ks, vs = q.reshape(kv, g, D), k.transpose(1, 2, 0), v.transpose(1, 0, 2)
+    x = np.matmul(qs, ks) * scale
+    ds = np.matmul(np.abs(qs), np.abs(ks)).max() * scale * ((D + 40) * 2.0**-24 + 2.0**-21)
+    p = np.exp(x - x.max(-1, keepdims=True))
+    p /= p.sum(-1, keepdims=True)
+    o = np.matmul(p, vs)
+    turn = np.stack([np.einsum("gc,gcd->gd", p[h], np.abs(vs[h][None] - o[h][:, None])) for h in range(kv)])
+    size = np.matmul(p, np.abs(vs))
+    big = size.reshape(kv, g, D // 32, 32).max(-1, keepdims=True)
+    off = turn * ds + size * (2.0**-21 + (n / 16 + 64) * 2.0**-24)
+    off = 2 * off.reshape(kv, g, D // 32, 32) + big * n * 2.0**-39 + 127 * 2.0**-42 * 7.5 * n ** 0.5
+    return o.reshape(H, D), off.reshape(H, D)
+
+
+@pytest.mark.parametrize("loud", [0.2, 1, 30, 600])
+@pytest.mark.parametrize("quiet", [1e-2, 1e-4, 1e-5])
+@pytest.mark.parametrize("H,kv,D", [(8, 2, 64), (8, 2, 128), (8, 4, 256)])
+@pytest.mark.parametrize("n,past", [(1, 500), (40, 201)])
+def test_q8_attention_keeps_the_bits_of_quiet_cells(L, loud, quiet, H, kv, D, n, past):
+    """All but e^-12 to e^-20 of a row's weight on one cell whose V is far below the
+    others': the row has the bits of that V, whatever the scales beside it."""
+    rng = np.random.default_rng(int(loud) + D)
+    P = Pass([n], [past], H, kv, None, 8, 3)
+    k, v = (rng.standard_normal((P.n_cells, kv, D)).astype(np.float32) for _ in range(2))
+    q = rng.standard_normal((n, H, D)).astype(np.float32)
+    c = P.cells(0)
+    way = rng.standard_normal((kv, D)).astype(np.float32)
+    v *= np.float32(loud)
+    k[c[3]], v[c[3]] = 2 * way, v[c[3]] * np.float32(quiet / loud)
+    ahead = rng.choice([12, 20], (n, H, 1))
+    w = np.repeat(2 * way, H // kv, 0)
+    q = (q + ahead * w * (D ** 0.5 / (w * w).sum(1, keepdims=True))).astype(np.float32)
+    pools, kx, vx = fill(L, P, kv, D, k, v, True)
+    got = run_attention(L, P, H, kv, D, D ** -0.5, q, pools, True)
+    for j in range(n):
+        vis = c[:past + j + 1]
+        want, tol = bounds(q[j].astype(np.float64), kx[vis], vx[vis], D ** -0.5)
+        err = np.abs(got[j] - want)
+        assert (err <= tol).all(), (j, (err / tol).max())
