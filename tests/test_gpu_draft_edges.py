@@ -1,11 +1,11 @@
 """Calls around drafted tokens and the Q8_0 pool at their edges, on the GPU:
 products that end on a half of a step, moves and copies of cells behind a busy
 stream, ids that no row holds, models without cells, rows that attend to a cell
-much quieter than the others."""
+much quieter than the others, lines of drafted tokens at every head size."""
 import numpy as np
 import pytest
 
-from tests.test_gpu_draft import Pass, dev, fill, k_tile, quants, run_attention, st, v_tile
+from tests.test_gpu_draft import Pass, check_attention, dev, fill, k_tile, quants, run_attention, st, v_tile
 
 pytestmark = pytest.mark.gpu
 
@@ -282,3 +282,23 @@ def test_q8_attention_keeps_the_bits_of_quiet_cells(L, loud, quiet, H, kv, D, n,
         want, tol = bounds(q[j].astype(np.float64), kx[vis], vx[vis], D ** -0.5)
         err = np.abs(got[j] - want)
         assert (err <= tol).all(), (j, (err / tol).max())
+
+
+# ---- a line of drafted tokens --------------------------------------------------------
+LINES = {
+    "few": ([9, 64, 1], [100, 3, 64]),            # sets of a few query groups
+    "many": ([300, 128, 257], [70, 640, 0]),      # sets of eight
+    "edges": ([1, 2, 63, 65], [63, 62, 1, 191]),  # blocks that end with a token
+}
+
+
+@pytest.mark.parametrize("case", list(LINES))
+@pytest.mark.parametrize("q8,H,kv,D", [(False, 4, 2, 16), (False, 4, 2, 32), (False, 8, 2, 64), (False, 32, 8, 128),
+                                       (False, 8, 4, 256), (True, 8, 2, 64), (True, 32, 8, 128), (True, 8, 4, 256)])
+@pytest.mark.parametrize("bps", [0, 2])
+def test_a_line_of_tokens_is_the_causal_plan_at_every_head_size(L, case, q8, H, kv, D, bps):
+    seq_n, npast = LINES[case]
+    line = [[j - 1 for j in range(n)] for n in seq_n]
+    a = check_attention(L, q8, H, kv, D, seq_n, npast, line, bps, 23)
+    b = check_attention(L, q8, H, kv, D, seq_n, npast, None, bps, 23)
+    assert np.array_equal(a, b), np.argwhere(a != b)[:4]
