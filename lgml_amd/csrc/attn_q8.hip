@@ -23,11 +23,12 @@
 // sequences below 80 us where the first takes 58 (cells in the memory-side cache).
 //
 // Bounds. One token of 64 sequences at 128 to 4096 cells, 32 / 8 heads of 128, is
-// 67 + 6 us from HBM: 296 MB at 4.4 TB/s in the first (54 with the cells in the
-// memory-side cache). Trees of 61 tokens of 8
-// sequences at 1024 to 16384 cells, 8 / 4 heads of 256, are 151 + 10 us: 35 GFLOP
-// (16-bit halves of q and P make them 70) in 176 workgroups of 256 CUs, whose waves
-// wait in turn for LDS (48 reads of 16 bytes a block and product) and the vector ALU.
+// 63 + 5 us from HBM: 296 MB at 4.7 TB/s in the first (54 with the cells in the
+// memory-side cache). Trees of 61 tokens of 8 sequences at 1024 to 16384 cells, 8
+// / 4 heads of 256, are 144 + 10 us: 35 GFLOP (16-bit halves of q and P make them
+// 70) in 176 workgroups of 256 CUs, whose waves wait in turn for LDS: 98 reads of 1
+// KB a wave and block, 6300 cycles of a CU's at 128 bytes, where the products of
+// a SIMD's two waves fill 4096.
 #include <type_traits>
 
 #include "attn.h"
