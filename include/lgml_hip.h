@@ -36,7 +36,8 @@ enum {
 };
 
 /* Weight / element types, numbered as ggml's type ids. */
-enum { LGMLH_F32 = 0, LGMLH_F16 = 1, LGMLH_Q8_0 = 8, LGMLH_Q4_K = 12, LGMLH_Q6_K = 14 };
+enum { LGMLH_F32 = 0, LGMLH_F16 = 1, LGMLH_Q4_0 = 2, LGMLH_Q8_0 = 8, LGMLH_Q4_K = 12, LGMLH_Q6_K = 14 };
+/* (Q4_0 is a type of KV pools only.) */
 
 /* Text of the last error on this thread (never NULL). */
 const char *lgmlh_last_error(void);
@@ -137,13 +138,54 @@ int lgmlh_kv_gather_q8(const void *pool, int which, int64_t n_cells, int n_head_
 /* Move cells in every pool tensor at once: dst[j] takes what src[j] held
  * before the call, for all j (a cell may be a source and a target). For the
  * accepted tokens of a verified tree (lgmlh_plan_tree), which go to the slots
- * behind the context. type LGMLH_F16 or LGMLH_Q8_0; pools a DEVICE array of
+ * behind the context. type LGMLH_F16, LGMLH_Q8_0 or LGMLH_Q4_0; pools a DEVICE array of
  * n_pools tensor addresses, K and V of each layer in turn
  * (lgmlh_kv_block_host's). n up to 1024; h_src and h_dst are host copies for
  * the checks (LGMLH_ERANGE; a target twice is LGMLH_EINVAL). */
 int lgmlh_kv_move(int type, void *const *pools, int n_pools, int64_t n_cells, int n_head_kv,
     int head_dim, const int64_t *src, const int64_t *dst, const int64_t *h_src,
     const int64_t *h_dst, int64_t n, void *stream);
+
+/* ===================================================================== *
+ * The KV pool in Q4_0: 4 bits a value and an f16 scale per 32 values of a head,
+ * 9/32 of the f16 pool's bytes (the reference's cache types, lua/lgml/kv.lua:14-20,
+ * go down to 8 bits). The same blocks, cell ids, plans and bookkeeping; head sizes
+ * 64, 128 and 256; the entry points that copy whole blocks take such a pool as one
+ * of f16 heads of 9 D / 32. A (block, KV head) tile of 36 * D bytes: 32 * D bytes
+ * of values n of 0 .. 15, which stand for (n - 8) d, then f16 scales d [D / 32][64
+ * cells]. Values of K [D / (32 U)][cell][4][U][4], U = min(4, D / 32): dim 32 (U j
+ * + u) + 8 q + e of a cell are the four bits from 4 (e / 2) + 16 (e % 2) on of the
+ * 32-bit word (j, cell, q, u). Values of V [D / 32][16][4][2][8]: of the byte (j, r,
+ * q, b, p(e)), p = 0 2 1 3 4 6 5 7, cell 32 b + 8 q + e has dim 32 j + r in the low
+ * half, 32 j + 16 + r in the high one. Tensors are 16-byte aligned.
+ * ===================================================================== */
+/* Bytes of one layer's K (or V); -1 for an unsupported shape. */
+int64_t lgmlh_kv_q4_layer_bytes(int64_t n_cells, int n_head_kv, int head_dim);
+/* lgmlh_kv_store into Q4_0 pools, the rows quantized in the format's steps (f32): per
+ * 32 values m the one of largest size (the first of them), d = m / -8, n = min(15,
+ * trunc(x (1 / d) + 8.5)), d kept as f16. Rows are finite and below 8 * 65504. Cells
+ * of one call are distinct: a cell twice is LGMLH_EINVAL. Up to 65535 KV heads, here
+ * and in the read back. */
+int lgmlh_kv_store_q4(void *kpool, void *vpool, int64_t n_cells, int n_head_kv, int head_dim,
+    const float *k_src, const float *v_src, const int64_t *cells, const int64_t *h_cells,
+    int64_t n, void *stream);
+/* Read cells back as (n, Hkv*D) rows of the values (n - 8) d they stand for, as
+ * lgmlh_kv_gather_q8 does. */
+int lgmlh_kv_gather_q4(const void *pool, int which, int64_t n_cells, int n_head_kv, int head_dim,
+    const int64_t *cells, int64_t n, void *out, int out_type, void *stream);
+
+/* ===================================================================== *
+ * Copies of blocks in every layer at once: forks of a sequence, copy-on-write,
+ * compaction, cleared blocks. copies (n, 3) i32: {src, dst, cells}, the first
+ * `cells` (0 .. 64) cells of block dst become those of block src, or zeros where
+ * src is -1; the others of dst stay. A source may serve several targets; a target
+ * twice, or one that is a source of the call, is LGMLH_EINVAL (a block outside the
+ * pool LGMLH_ERANGE). type LGMLH_F16 (heads of a multiple of 8 up to 1024),
+ * LGMLH_Q8_0 or LGMLH_Q4_0; pools as in lgmlh_kv_move, their tensors 16-byte
+ * aligned; h_copies is the host copy for the checks.
+ * ===================================================================== */
+int lgmlh_kv_copy_blocks(int type, void *const *pools, int n_pools, int64_t n_cells, int n_head_kv,
+    int head_dim, const int32_t *copies, const int32_t *h_copies, int64_t n, void *stream);
 
 /* ===================================================================== *
  * Pool bookkeeping (host): lua/lgml/kvpool.lua in C. All state lives in
@@ -184,6 +226,11 @@ int32_t lgmlh_kvpool_lookup(void *pool, const char *key);
  * the shared token count in *shared. */
 int32_t lgmlh_kvpool_longest_kid(void *pool, const char *parent, const int32_t *tokens,
     int32_t max, int32_t *shared);
+/* Block src becomes block dst, a free one: its references, priority, key, tokens and
+ * age go along, src is free. For compaction, after the owner of the tensors copied
+ * the cells (lgmlh_kv_copy_blocks) and with the block tables that name src put
+ * right. It has no counterpart in the reference, whose blocks stay where they are. */
+int lgmlh_kvpool_relocate(void *pool, int32_t src, int32_t dst);
 /* P:set_cap (kvpool.lua:289-293). */
 int lgmlh_kvpool_set_cap(void *pool, int32_t cap);
 /* out[8]: n, size, cap, used, low, cached, tick, evicted. */
@@ -277,7 +324,7 @@ int lgmlh_plan_ring(int n_seq, const int32_t *seq_n, const int32_t *seq_npast,
  * seq_npast[s] + its depth (pos; rope). It sees the seq_npast[s] cached
  * cells, the tokens it follows and itself. A line of tokens (parents[t] = j -
  * 1) sees what lgmlh_plan's tokens see. Up to LGMLH_TREE_MAX tokens a sequence.
- * lgmlh_paged_attention, lgmlh_paged_attention_q8 and lgmlh_forward (of models
+ * lgmlh_paged_attention, its forms over quantised pools and lgmlh_forward (of models
  * without sliding layers) take the bound plan as any other; logit_rows are the
  * last tokens, so pass the wanted rows as out_rows. After a verification the
  * accepted tokens' cells go to the slots behind the context with
@@ -305,8 +352,8 @@ int lgmlh_plan_bind(const lgmlh_plan_info *info, const void *dev, lgmlh_ubatch *
  * layout above. scale: 1/sqrt(D) for llama (transformer.lua:1845).
  * The V of the cells behind a row's position in its own last block is multiplied
  * by 0 in causal and ring plans, so it has to be finite (pools start zeroed, as
- * lgmlh_kv_grow's do); in tree plans, and over Q8_0 pools in all plans, such cells
- * may hold anything.
+ * lgmlh_kv_grow's do); in tree plans, and over quantised pools in all plans, such
+ * cells may hold anything.
  * D in {16, 32, 64, 128, 256}; H a multiple of Hkv with H/Hkv in {1, 2, 4, 8, 16}.
  * ===================================================================== */
 size_t lgmlh_attention_workspace(const lgmlh_plan_info *info, int head_dim);
@@ -319,6 +366,10 @@ int lgmlh_paged_attention(const float *q, int n_head, int n_head_kv, int head_di
  * quantized). Head sizes 64, 128 and 256. Cells that a row does not see
  * change nothing in it, whatever their bytes. */
 int lgmlh_paged_attention_q8(const float *q, int n_head, int n_head_kv, int head_dim, float scale,
+    const void *kpool, const void *vpool, const lgmlh_ubatch *ub, float *out, void *workspace,
+    size_t workspace_bytes, void *stream);
+/* The same over Q4_0 pools (lgmlh_kv_store_q4). */
+int lgmlh_paged_attention_q4(const float *q, int n_head, int n_head_kv, int head_dim, float scale,
     const void *kpool, const void *vpool, const lgmlh_ubatch *ub, float *out, void *workspace,
     size_t workspace_bytes, void *stream);
 
@@ -486,6 +537,29 @@ int lgmlh_qkv_rope_store_q8(float *qkv, int64_t n, int n_head, int n_head_kv, in
     int n_rot, int neox, float freq_base, const float *freq_factors, const float *q_norm,
     const float *k_norm, float eps, const int32_t *pos, void *kpool, void *vpool,
     int64_t n_cells, const int64_t *cells, float *q_out, void *stream);
+/* The same into Q4_0 pools (lgmlh_kv_store_q4). */
+int lgmlh_qkv_rope_store_q4(float *qkv, int64_t n, int n_head, int n_head_kv, int head_dim,
+    int n_rot, int neox, float freq_base, const float *freq_factors, const float *q_norm,
+    const float *k_norm, float eps, const int32_t *pos, void *kpool, void *vpool,
+    int64_t n_cells, const int64_t *cells, float *q_out, void *stream);
+/* lgmlh_qkv_rope_store with positions of up to four axes (time, height, width and
+ * one more: tokens of images and video; graph:rope's several positions a token,
+ * src/lgml.c:2075-2079). pos (4, n) i32. Dims i and i + n_rot / 2 of a q or k head turn
+ * by pos[a][t] freq_base^(-2 i / n_rot) / freq_factors[i], a the axis of pair i:
+ * sections[4] (host) pairs of each axis, n_rot / 2 in all, one section after the
+ * other; interleaved: pairs in turn, of three axes (sections[3] = 0), pair i goes by
+ * axis a = i % 3 where i < 3 sections[a], else by axis 0. An axis without pairs is
+ * not read. Angles are made in 64 bits (those of lgmlh_qkv_rope_store are a running
+ * f32 product: a text token, whose positions are alike, has here what it has there but
+ * for that). K and V go to pools of kv_type LGMLH_F16, LGMLH_Q8_0 or LGMLH_Q4_0, 16-byte
+ * aligned, at distinct cells (a cell outside [0, n_cells) is not written), q to q_out
+ * (n, H, D), which shares nothing with qkv. Head sizes 64, 128 and 256; n_rot a
+ * multiple of 8. */
+int lgmlh_qkv_rope_store_axes(int kv_type, const float *qkv, int64_t n, int n_head, int n_head_kv,
+    int head_dim, int n_rot, const int32_t *sections, int interleaved, float freq_base,
+    const float *freq_factors, const float *q_norm, const float *k_norm, float eps,
+    const int32_t *pos, void *kpool, void *vpool, int64_t n_cells, const int64_t *cells,
+    float *q_out, void *stream);
 /* silu(g) * u (transformer.lua:2048) for gu = (n, 2F) rows [g | u]; out f32 or f16. */
 int lgmlh_swiglu(const float *gu, int64_t n, int64_t F, void *out, int out_type, void *stream);
 /* gelu(g) * u, the gemma FFN (graph:geglu_split, src/ops_nn.c:165-172;
@@ -626,6 +700,10 @@ int lgmlh_forward(const lgmlh_model *m, const lgmlh_ubatch *ub, const lgmlh_ubat
  * (lgmlh_kv_q8_layer_bytes; the layers' kpool / vpool): same plans, workspace
  * and logit rows. Head sizes 64, 128 and 256. */
 int lgmlh_forward_q8(const lgmlh_model *m, const lgmlh_ubatch *ub, const lgmlh_ubatch *ub_ring,
+    const int32_t *out_rows, int n_out, float *logits, void *workspace, size_t ws_bytes,
+    lgmlh_trace *trace, void *stream);
+/* The same over Q4_0 pools (lgmlh_kv_q4_layer_bytes). */
+int lgmlh_forward_q4(const lgmlh_model *m, const lgmlh_ubatch *ub, const lgmlh_ubatch *ub_ring,
     const int32_t *out_rows, int n_out, float *logits, void *workspace, size_t ws_bytes,
     lgmlh_trace *trace, void *stream);
 /* Destroy the side streams and events that lgmlh_forward made for the

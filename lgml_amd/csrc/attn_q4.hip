@@ -1,0 +1,452 @@
+// Paged GQA attention over Q4_0 KV blocks (gfx950): the work items, rows and
+// merge of attn.hip over the tiles of kvq4.hip, by the arithmetic of attnq.h.
+#include "attnq.h"
+#include "kvq4.h"
+
+namespace lgmlh {
+
+// n - 8 of a word's 4-bit values, as f16: bits 0 .. 3 and 16 .. 19 on the mantissa of
+// 1024 are 1024 + n, bits 4 .. 7 and 20 .. 23 on that of 64 are 64 + n, the differences
+// are exact.
+__device__ __forceinline__ f16x2 low_pair(uint32_t w) {
+  return __builtin_bit_cast(f16x2, (w & 0x000f000fu) | 0x64006400u) - f16x2{(f16)1032.0f, (f16)1032.0f};
+}
+__device__ __forceinline__ f16x2 high_pair(uint32_t w) {
+  return __builtin_bit_cast(f16x2, (w & 0x00f000f0u) | 0x54005400u) - f16x2{(f16)72.0f, (f16)72.0f};
+}
+__device__ __forceinline__ f16x8 join(f16x2 a, f16x2 b, f16x2 c, f16x2 d) {
+  return f16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+// K's word: 8 dims of a cell.
+__device__ __forceinline__ f16x8 k_half8(uint32_t w) {
+  return join(low_pair(w), high_pair(w), low_pair(w >> 8), high_pair(w >> 8));
+}
+// V's two words: 8 cells of a dim r (their low halves) or r + 16.
+__device__ __forceinline__ f16x8 v_half8(uint32_t w0, uint32_t w1, bool upper) {
+  return upper ? join(high_pair(w0), high_pair(w0 >> 8), high_pair(w1), high_pair(w1 >> 8))
+               : join(low_pair(w0), low_pair(w0 >> 8), low_pair(w1), low_pair(w1 >> 8));
+}
+
+template <int HEAD>
+struct Q4Frag {
+  static constexpr int D = HEAD, SCALES = 32 * D, TILE = q4_tile_bytes(D);
+  static constexpr int DV = 1;  // V's scales of 2^-8 to 2^2 (largest values of 0.03 to 31) go packed
+  static constexpr int U = q4_k_words(D);
+  typedef uint32_t KUnit __attribute__((ext_vector_type(U)));  // a cell's dims 32 (U j + u) + 8 quad ..
+  static constexpr int KJ = D / (32 * U), VJ = D / 32;
+  __device__ __forceinline__ static f16x8 k_frag(const KUnit (&k)[KJ], int b) { return k_half8(k[b / U][b % U]); }
+  __device__ __forceinline__ static f16x8 v_frag(const u32x4 (&v)[VJ], int t, int kc) {
+    return v_half8(v[t / 2][2 * kc], v[t / 2][2 * kc + 1], t & 1);
+  }
+  template <typename P>
+  __device__ __forceinline__ static void put_k(int c, u32x4 w, P put) {  // words (j, cell, quad, u) from 4 c on
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int q = U == 4 ? c & 3 : 2 * (c & 1) + i / 2;
+      const int cell = U == 4 ? c >> 2 & 63 : c >> 1, j = U == 4 ? c >> 8 : 0;
+      put(cell, 4 * (U * j + i % U) + q, k_half8(w[i]));
+    }
+  }
+  template <typename P>
+  __device__ __forceinline__ static void put_v(int c, u32x4 w, P put) {  // (j, r, quad)
+    const int d = (c >> 6) * 32 + (c >> 2 & 15), q = c & 3;
+#pragma unroll
+    for (int i = 0; i < 4; i++) put(d + 16 * (i & 1), 4 * (i >> 1) + q, v_half8(w[2 * (i >> 1)], w[2 * (i >> 1) + 1], i & 1));
+  }
+};
+
+template <int D>
+__global__ void __launch_bounds__(64, D <= 128 ? 2 : 1)
+paged_attn_q4_kernel(const float *__restrict__ q, int H, int Hkv, float scale_log2,
+                     const uint8_t *__restrict__ kpool, const uint8_t *__restrict__ vpool,
+                     const int32_t *__restrict__ items, const int32_t *__restrict__ seq_off,
+                     const int32_t *__restrict__ seq_npast, const int32_t *__restrict__ block_tab,
+                     int max_blocks, int ring, int window, float *__restrict__ out,
+                     f16 *__restrict__ planes, int64_t npad, int xf, float *__restrict__ part,
+                     const int32_t *__restrict__ order, int n_order,
+                     const uint64_t *__restrict__ vis) {
+  typedef Q4Frag<D> F;
+  constexpr int NB = D / 32, DT = D / 16;
+  __shared__ __align__(16) f16x8 qsh[NB * 64], qsl[NB * 64];
+  const int lane = threadIdx.x;
+  const int slot = (int)(blockIdx.x / (uint32_t)Hkv), kvh = (int)(blockIdx.x % (uint32_t)Hkv);
+  const int item = slot < n_order ? order[slot] : slot;
+  const int G = H / Hkv;
+  const int s = items[4 * item + 0], tok0 = items[4 * item + 1];
+  const int ntok = items[4 * item + 2] & 31, mg = (items[4 * item + 2] >> 5) - 1;
+  const int blo = items[4 * item + 3] & 0xffff, bhi = (items[4 * item + 3] >> 16) & 0xffff;
+  const int npast = seq_npast[s];
+  Sight see;
+  see.ring = ring;
+  see.window = window;
+  see.p_first = npast + (tok0 - seq_off[s]);
+  see.p_last = see.p_first + ntok - 1;
+  see.b_tree = npast / KV_BLOCK;
+  see.G = G;
+  see.ntok = ntok;
+  see.vis = ring < 0 ? vis + (int64_t)tok0 * window : nullptr;
+
+  const int32_t *bt = block_tab + (int64_t)s * max_blocks;
+  auto tile = [&](const uint8_t *pool, int blk) {
+    const int64_t b = ring > 0 ? bt[blk % ring] : bt[blk];
+    return pool + (b * Hkv + kvh) * (int64_t)F::TILE;
+  };
+  // A block's values in registers, a lane's place in a tile being the same in
+  // all (the tile's own address stays scalar). Its scales come 16 bytes a lane and
+  // go through LDS: in registers they are 16 lanes' copies, as many as the values.
+  constexpr int SR = D > 128 ? 2 : 1;    // registers' worth: K's and V's, or K's then V's
+  constexpr int SL = D > 128 ? 64 : NB * 8;  // lanes of K's scales
+  typename F::KUnit kq[4][F::KJ];
+  u32x4 vq[F::VJ], sreg[SR];
+  const int row = lane & 15, quad = lane >> 4;
+  constexpr int KC = 4 * sizeof(typename F::KUnit);  // bytes of a cell's units
+  const uint32_t koff = (8 * (row >> 2) + (row & 3)) * KC + quad * (KC / 4), voff = row * 64 + quad * 16;
+  auto load_k = [&](int blk) {
+    const uint8_t *t = tile(kpool, blk);
+#pragma unroll
+    for (int ct = 0; ct < 4; ct++)
+#pragma unroll
+      for (int j = 0; j < F::KJ; j++)
+        kq[ct][j] = *(const typename F::KUnit *)(t + (j * 4096 + s_cell(ct, 0) * KC) + koff);
+  };
+  auto load_v = [&](int blk) {
+    const uint8_t *t = tile(vpool, blk);
+#pragma unroll
+    for (int j = 0; j < F::VJ; j++) vq[j] = *(const u32x4 *)(t + j * 1024 + voff);
+  };
+  auto load_s = [&](int blk) {
+    const uint8_t *k = tile(kpool, blk) + F::SCALES, *v = tile(vpool, blk) + F::SCALES;
+    if constexpr (SR == 2) {
+      sreg[0] = *(const u32x4 *)(k + lane * 16u);
+      sreg[1] = *(const u32x4 *)(v + lane * 16u);
+    } else {
+      sreg[0] = *(const u32x4 *)((lane < SL ? k : v) + lane % SL * 16u);
+    }
+  };
+  __shared__ __align__(16) u32x4 scl[SR * 64];  // K's scales, then V's
+  auto store_s = [&](bool plain) {
+    if (SR == 2) scl[lane] = sreg[0];
+    u32x4 v = sreg[SR - 1];
+    if (plain && (SR == 2 || lane >= SL)) v = times_dv<F>(v);
+    scl[(SR - 1) * 64 + lane] = v;
+  };
+  auto scale_of = [&](int v, int b, int h) { return scl[v * SL + b * 8 + h * 4 + quad]; };
+  float rscale;
+  {
+    const RowOf r(lane, G, ntok);
+    const float *qr = q + ((int64_t)(tok0 + (r.valid ? r.rtok : ntok - 1)) * H + kvh * G + r.head) * D;
+    f32x4 qa[2 * NB];
+#pragma unroll
+    for (int b = 0; b < NB; b++) {
+      qa[2 * b] = *(const f32x4 *)(qr + 32 * b + 8 * r.quad);
+      qa[2 * b + 1] = *(const f32x4 *)(qr + 32 * b + 8 * r.quad + 4);
+    }
+    const int b_first = blo < bhi ? blo : 0;  // block 0 of a planned sequence is a pool block
+    load_s(b_first);
+    load_k(b_first);
+    load_v(b_first);
+    f16x8 hi[NB], lo[NB];
+    rscale = split_q<NB>(qa, r.valid, scale_log2, hi, lo);
+#pragma unroll
+    for (int b = 0; b < NB; b++) {
+      qsh[b * 64 + lane] = hi[b];
+      qsl[b * 64 + lane] = lo[b];
+    }
+  }
+  f32x4 o[DT];
+#pragma unroll
+  for (int i = 0; i < DT; i++) o[i] = f32x4{0, 0, 0, 0};
+  float m = -INFINITY, l = 0.0f;
+
+  auto block = [&](int blk, auto next) __attribute__((always_inline)) {
+    constexpr bool NEXT = decltype(next)::value;
+    const int nxt = blk + 1 < bhi ? blk + 1 : blk;
+    f32x4 st[4];
+    int ql_at = lane;
+    asm volatile("" : "+v"(ql_at));  // Q's operands are read anew: held, they spill others
+    // (the lanes of K's scales have no part in this)
+    const bool plain = !__builtin_amdgcn_ballot_w64(!plain_scales<F>(sreg[SR - 1]) &&
+                                                    (SR == 2 || (lane >= SL && lane < 2 * SL)));
+    store_s(plain);
+    if constexpr (NEXT) load_s(nxt);
+    scores_q<NB>(
+        st,
+        [&](int b, int p, f16x8(&k)[2], f16x8 &d) {
+#pragma unroll
+          for (int t = 0; t < 2; t++) k[t] = F::k_frag(kq[2 * p + t], b);
+          d = __builtin_bit_cast(f16x8, scale_of(0, b, p));
+        },
+        [&](int b, f16x8 &hi, f16x8 &lo) {
+          hi = qsh[b * 64 + ql_at];
+          lo = qsl[b * 64 + ql_at];
+        });
+    if constexpr (NEXT) load_k(nxt);
+    uint64_t word = ~(uint64_t)0;
+    const bool masked = see.masks(blk, word);
+    softmax_q<DT>(st, rscale, masked, word, m, l, o);
+    __builtin_amdgcn_sched_barrier(0);
+    values_q<F>(o, st, plain, masked, word,
+                 [&](int b, int h) { return scale_of(1, b, h); },
+                 [&](int t, int kc) { return F::v_frag(vq, t, kc); });
+    if constexpr (NEXT) load_v(nxt);
+  };
+  for (int blk = blo; blk + 1 < bhi; blk++) block(blk, std::true_type{});
+  if (blo < bhi) block(bhi - 1, std::false_type{});
+  l += __shfl_xor(l, 16);
+  l += __shfl_xor(l, 32);
+  const RowOf r(lane_anew(), G, ntok);
+  finish_item<D>(o, m, l * (QP * F::DV), mg, r.valid, tok0, r.rtok, kvh * G + r.head, ntok, G, r.row, r.quad, item, kvh, Hkv,
+                 H, out, planes, npad, xf, part);
+}
+
+// Shared runs (a chunk's or a tree's query groups in sets): a workgroup of W waves
+// per (run, KV head), wave w on the run's item w of a half of the set (W = 4) or
+// of the whole (W = 8). Each block is loaded once, 16 bytes a lane, made f16 on its
+// way into LDS, and read from there by every wave, whose arithmetic is the
+// per-item kernel's: an item gives the same bits in either. The next block's
+// bytes are in flight while this one is used. Two buffers take one barrier a
+// block; where two workgroups of one buffer each share a CU (heads of 256, W =
+// 4) there are two. LDS slots of 16 B: K slot (cell, c) holds dims 8 (c ^ swk), V
+// slot (d, c) cells 8 (c ^ swv): a fragment's 16 rows touch every bank once.
+template <int D, int W>
+__global__ void __launch_bounds__(64 * W, 2)
+paged_attn_q4_shared_kernel(const float *__restrict__ q, int H, int Hkv, float scale_log2,
+                            const uint8_t *__restrict__ kpool, const uint8_t *__restrict__ vpool,
+                            const int32_t *__restrict__ items, const int32_t *__restrict__ shared,
+                            const int32_t *__restrict__ seq_off,
+                            const int32_t *__restrict__ seq_npast,
+                            const int32_t *__restrict__ block_tab, int max_blocks, int ring,
+                            int window, float *__restrict__ out, f16 *__restrict__ planes,
+                            int64_t npad, int xf, float *__restrict__ part,
+                            const uint64_t *__restrict__ vis) {
+  typedef Q4Frag<D> F;
+  constexpr int NB = D / 32, DT = D / 16, KC = D / 8;
+  constexpr int PIECES = F::SCALES / 16;    // 16 bytes each, K's, then V's as many
+  constexpr int CH = (2 * PIECES + 64 * W - 1) / (64 * W);  // of a thread
+  constexpr int BUFS = D == 256 && W == 4 ? 1 : 2;
+  constexpr int TILE = 64 * D;              // f16 of a tile
+  __shared__ __align__(16) f16 kb[BUFS][TILE], vb[BUFS][TILE];
+  __shared__ __align__(16) u32x4 scl[BUFS][2 * NB * 8];  // K's scales, then V's
+  __shared__ int odd_scales[BUFS];  // some of V's are not plain_scales
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int half = W < SHARED_MAX ? (int)blockIdx.z * W : 0;
+  const int first = shared[2 * blockIdx.x] + half, n = shared[2 * blockIdx.x + 1] - half;
+  if (n <= 0) return;  // a set of one half
+  const int kvh = blockIdx.y;
+  const int G = H / Hkv;
+  const bool active = wave < n;
+  const int item = first + (active ? wave : 0);
+  const int s = items[4 * first + 0];
+  const int blo = items[4 * first + 3] & 0xffff, bhi = (items[4 * first + 3] >> 16) & 0xffff;
+  const int tok0 = items[4 * item + 1];
+  const int ntok = items[4 * item + 2] & 31, mg = (items[4 * item + 2] >> 5) - 1;
+  const int npast = seq_npast[s];
+  Sight see;
+  see.ring = ring;
+  see.window = window;
+  see.p_first = npast + (tok0 - seq_off[s]);
+  see.p_last = see.p_first + ntok - 1;
+  see.b_tree = npast / KV_BLOCK;
+  see.G = G;
+  see.ntok = ntok;
+  see.vis = ring < 0 ? vis + (int64_t)tok0 * window : nullptr;
+
+  const int32_t *bt = block_tab + (int64_t)s * max_blocks;
+  u32x4 raw[CH], sraw;
+  // (a thread's places are made anew each block, from an opaque copy of its number:
+  // held over the loop they are a dozen registers, and heads of 256 have none)
+  auto load = [&](int blk) {
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));
+    const int64_t at = ((int64_t)bt[blk] * Hkv + kvh) * F::TILE;
+#pragma unroll
+    for (int i = 0; i < CH; i++) {
+      const int c = i * 64 * W + tid;  // a wave's pieces are K's or V's
+      if (2 * PIECES % (64 * W) && i * 64 * W + 64 * wave >= 2 * PIECES) break;
+      raw[i] = i * 64 * W + 64 * wave < PIECES ? *(const u32x4 *)(kpool + at + c * 16u)
+                           : *(const u32x4 *)(vpool + at + (c - PIECES) * 16u);
+    }
+    if (tid < NB * 16)
+      sraw = *(const u32x4 *)((tid < NB * 8 ? kpool : vpool) + at + F::SCALES + tid % (NB * 8) * 16u);
+  };
+  auto store = [&](int buf) {
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));
+#pragma unroll
+    for (int i = 0; i < CH; i++) {
+      const int c = i * 64 * W + tid;
+      if (2 * PIECES % (64 * W) && i * 64 * W + 64 * wave >= 2 * PIECES) break;
+      const u32x4 w = raw[i];
+      if (i * 64 * W + 64 * wave < PIECES)
+        F::put_k(c, w, [&](int cell, int g8, f16x8 v) {
+          *(f16x8 *)(kb[buf] + (cell * KC + (g8 ^ swk<D>(cell))) * 8) = v;
+        });
+      else
+        F::put_v(c - PIECES, w, [&](int d, int c8, f16x8 v) {
+          *(f16x8 *)(vb[buf] + (d * 8 + (c8 ^ swv(d))) * 8) = v;
+        });
+    }
+    // V's scales are in one wave (NB * 8 lanes from lane NB * 8 on)
+    bool plain = false;
+    if (wave == NB * 8 / 64) {
+      const bool odd = !plain_scales<F>(sraw) && tid >= NB * 8 && tid < NB * 16;
+      plain = __builtin_amdgcn_ballot_w64(odd) == 0;
+      if (lane == 0) odd_scales[buf] = !plain;
+    }
+    if (tid < NB * 16) scl[buf][tid] = plain && tid >= NB * 8 ? times_dv<F>(sraw) : sraw;
+  };
+  if (blo < bhi) load(blo);
+  // Q's operands in registers, but for the last block of dims of heads of 256 (LDS)
+  constexpr int QR = D == 256 ? NB - 1 : NB;
+  __shared__ f16x8 q_last[D == 256 ? 2 * 64 * W : 1];
+  f16x8 qh[NB], ql[NB];
+  float rscale;
+  {
+    const RowOf r(lane, G, ntok);
+    const float *qr = q + ((int64_t)(tok0 + (r.valid ? r.rtok : ntok - 1)) * H + kvh * G + r.head) * D;
+    f32x4 qa[2 * NB];
+#pragma unroll
+    for (int b = 0; b < NB; b++) {
+      qa[2 * b] = *(const f32x4 *)(qr + 32 * b + 8 * r.quad);
+      qa[2 * b + 1] = *(const f32x4 *)(qr + 32 * b + 8 * r.quad + 4);
+    }
+    rscale = split_q<NB>(qa, r.valid, scale_log2, qh, ql);
+    if constexpr (QR < NB) {  // read by the lane that writes it
+      q_last[tid] = qh[QR];
+      q_last[64 * W + tid] = ql[QR];
+    }
+  }
+  f32x4 o[DT];
+#pragma unroll
+  for (int i = 0; i < DT; i++) o[i] = f32x4{0, 0, 0, 0};
+  float m = -INFINITY, l = 0.0f;
+
+  // A lane's places in the tiles: the swizzles take from the cell and from d what
+  // only the lane's row decides, and from a block of dims its two low bits. The
+  // rest of an address is constant.
+  constexpr int KB = NB < 4 ? NB : 4;
+
+  for (int blk = blo; blk < bhi; blk++) {
+    const int buf = BUFS == 2 ? (blk - blo) & 1 : 0;
+    if (BUFS == 1 && blk > blo) lds_sync();  // everyone is done with the buffer
+    store(buf);
+    if (blk + 1 < bhi) load(blk + 1);
+    lds_sync();
+    if (!active || blk * 64 > see.p_last) continue;
+    // places in this buffer, made here from an opaque copy of the lane: otherwise every
+    // fragment's address is made ahead of the loop and takes a register
+    int at = lane;
+    asm volatile("" : "+v"(at));
+    const int arow = at & 15, aquad = at >> 4, r0 = s_cell(0, arow);
+    int ka[KB], va[2], sa = buf * (2 * NB * 8) + aquad;
+#pragma unroll
+    for (int b = 0; b < KB; b++) {
+      ka[b] = buf * TILE + (r0 * KC + ((b * 4 + aquad) ^ swk<D>(r0))) * 8;
+      asm volatile("" : "+v"(ka[b]));
+    }
+#pragma unroll
+    for (int kc = 0; kc < 2; kc++) {
+      va[kc] = buf * TILE + (arow * 8 + ((kc * 4 + aquad) ^ swv(arow))) * 8;
+      asm volatile("" : "+v"(va[kc]));
+    }
+    asm volatile("" : "+v"(sa));
+    const u32x4 *sc = scl[0] + sa;
+    f32x4 st[4];
+    scores_q<NB>(
+        st,
+        [&](int b, int p, f16x8(&k)[2], f16x8 &d) {
+#pragma unroll
+          for (int t = 0; t < 2; t++)
+            k[t] = *(const f16x8 *)(kb[0] + ka[b % KB] + (s_cell(2 * p + t, 0) * KC + b / 4 * 16) * 8);
+          d = __builtin_bit_cast(f16x8, sc[b * 8 + 4 * p]);
+        },
+        [&](int b, f16x8 &hi, f16x8 &lo) {
+          hi = b < QR ? qh[b] : q_last[64 * wave + at];
+          lo = b < QR ? ql[b] : q_last[64 * (W + wave) + at];
+        });
+    uint64_t word = ~(uint64_t)0;
+    const bool masked = see.masks(blk, word);
+    softmax_q<DT>(st, rscale, masked, word, m, l, o);
+    __builtin_amdgcn_sched_barrier(0);
+    values_q<F>(o, st, odd_scales[buf] == 0, masked, word,
+                 [&](int b, int h) { return sc[NB * 8 + b * 8 + 4 * h]; },
+                 [&](int t, int kc) { return *(const f16x8 *)(vb[0] + va[kc] + t * 1024); });
+  }
+  if (!active) return;
+  l += __shfl_xor(l, 16);
+  l += __shfl_xor(l, 32);
+  const RowOf r(lane_anew(), G, ntok);
+  finish_item<D>(o, m, l * (QP * F::DV), mg, r.valid, tok0, r.rtok, kvh * G + r.head, ntok, G, r.row, r.quad, item, kvh, Hkv,
+                 H, out, planes, npad, xf, part);
+
+}
+
+template <int D>
+static void launch_attn_q4(const float *q, int H, int Hkv, float scale_log2, const void *kp,
+                           const void *vp, const lgmlh_ubatch *ub, float *out, f16 *planes,
+                           int64_t npad, int xf, float *part, hipStream_t st) {
+  const uint64_t *vis = ub->ring == LGMLH_PLAN_TREE ? plan_vis(ub) : nullptr;
+  if (ub->n_single > 0)
+    hipLaunchKernelGGL(paged_attn_q4_kernel<D>, dim3((uint32_t)ub->n_single * Hkv), dim3(64), 0, st,
+                       q, H, Hkv, scale_log2, (const uint8_t *)kp, (const uint8_t *)vp, ub->items,
+                       ub->seq_off, ub->seq_npast, ub->block_tab, ub->max_blocks, ub->ring,
+                       ub->window, out, planes, npad, xf, part, ub->order,
+                       ub->order ? ub->n_single : 0, vis);
+  if (ub->n_shared > 0) {
+    // sets of up to half a workgroup's waves on average: workgroups of half as many
+    const bool small = ub->n_items - ub->n_single <= SHARED_MAX / 2 * ub->n_shared;
+    const auto kern = small ? paged_attn_q4_shared_kernel<D, SHARED_MAX / 2>
+                            : paged_attn_q4_shared_kernel<D, SHARED_MAX>;
+    hipLaunchKernelGGL(kern, dim3(ub->n_shared, Hkv, small ? 2 : 1),
+                       dim3(64 * (small ? SHARED_MAX / 2 : SHARED_MAX)), 0, st, q, H, Hkv, scale_log2,
+                       (const uint8_t *)kp, (const uint8_t *)vp, ub->items, ub->shared, ub->seq_off,
+                       ub->seq_npast, ub->block_tab, ub->max_blocks, ub->ring, ub->window, out,
+                       planes, npad, xf, part, vis);
+  }
+  merge_dev(D, ub, H, Hkv, part, out, planes, npad, xf, st);
+}
+
+// paged_attention_dev over Q4_0 pools.
+int paged_attention_q4_dev(const float *q, int n_head, int n_head_kv, int head_dim, float scale,
+                           const void *kpool, const void *vpool, const lgmlh_ubatch *ub, float *out,
+                           f16 *planes, int64_t npad, void *workspace, size_t workspace_bytes,
+                           hipStream_t st, int xf) {
+  if (head_dim != 64 && head_dim != 128 && head_dim != 256) {
+    set_error("paged_attention_q4: head_dim %d not supported (64, 128, 256)", head_dim);
+    return LGMLH_EINVAL;
+  }
+  if (((uintptr_t)kpool | (uintptr_t)vpool) & 15) {
+    set_error("paged_attention_q4: pools are 16-byte aligned");
+    return LGMLH_EINVAL;
+  }
+  int run = 0;
+  LGMLH_TRY(attn_check("paged_attention_q4", q, n_head, n_head_kv, head_dim, kpool, vpool, ub, out,
+                       planes, xf, workspace, workspace_bytes, &run));
+  if (!run) return LGMLH_OK;
+  const float sl = scale * LOG2E;
+  float *part = (float *)workspace;
+  switch (head_dim) {
+    case 64: launch_attn_q4<64>(q, n_head, n_head_kv, sl, kpool, vpool, ub, out, planes, npad, xf, part, st); break;
+    case 128: launch_attn_q4<128>(q, n_head, n_head_kv, sl, kpool, vpool, ub, out, planes, npad, xf, part, st); break;
+    default: launch_attn_q4<256>(q, n_head, n_head_kv, sl, kpool, vpool, ub, out, planes, npad, xf, part, st); break;
+  }
+  return hip_check(hipGetLastError(), "paged_attention_q4");
+}
+
+}  // namespace lgmlh
+
+using namespace lgmlh;
+
+extern "C" int lgmlh_paged_attention_q4(const float *q, int n_head, int n_head_kv, int head_dim,
+                                        float scale, const void *kpool, const void *vpool,
+                                        const lgmlh_ubatch *ub, float *out, void *workspace,
+                                        size_t workspace_bytes, void *stream) {
+  if (!out) {
+    set_error("paged_attention_q4: bad arguments");
+    return LGMLH_EINVAL;
+  }
+  return paged_attention_q4_dev(q, n_head, n_head_kv, head_dim, scale, kpool, vpool, ub, out,
+                                nullptr, 0, workspace, workspace_bytes, as_stream(stream), XF_SPLIT);
+}

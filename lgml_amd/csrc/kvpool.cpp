@@ -374,6 +374,26 @@ extern "C" int32_t lgmlh_kvpool_longest_kid(void *pool, const char *parent, cons
   return best;
 }
 
+// Block src's record becomes the free block dst's.
+extern "C" int lgmlh_kvpool_relocate(void *pool, int32_t src, int32_t dst) {
+  View v;
+  if (!view_of(pool, v) || src < 0 || src >= v.h->n || dst < 0 || dst >= v.h->n || is_free(v, src) ||
+      !is_free(v, dst)) {
+    set_error("kvpool_relocate: block %d to %d: from a block in use or kept to a free one", src, dst);
+    return LGMLH_EINVAL;
+  }
+  Block *k = v.blk(src);
+  if (k->flags & F_KEY) {
+    const int32_t s = tab_find(v, k->key);
+    if (s >= 0 && v.tab[s] == src) v.tab[s] = dst;
+  }
+  memcpy(v.blk(dst), k, block_bytes(v.h->size));
+  k->refs = 0;
+  k->flags = 0;
+  if (src < v.h->low) v.h->low = src;
+  return LGMLH_OK;
+}
+
 // kvpool.lua:289-293
 extern "C" int lgmlh_kvpool_set_cap(void *pool, int32_t cap) {
   View v;

@@ -6,7 +6,9 @@
 #include <memory>
 #include <type_traits>
 
+#include "kvq4.h"
 #include "kvq8.h"
+#include "kvwindow.h"
 
 namespace lgmlh {
 
@@ -30,58 +32,13 @@ struct Q8Tile {
 // with the rows in the memory-side cache (3.7 TB/s; with V's bytes one by one 39),
 // 31 from HBM; 64 tokens of them 5.7 us, the time of one workgroup's reads, turn and
 // writes after another.
-constexpr int Q8_THREADS = 256, Q8_GROUP = 8, Q8_HALO = 7;
-constexpr int64_t Q8_CELLS = (int64_t)1 << 36;  // a block's number has 31 bits
+constexpr int Q8_THREADS = 256, Q8_GROUP = CELL_GROUP, Q8_HALO = CELL_HALO;
 
 // The tile of cell c (>= 0) of one head: head is the first block's.
 template <int D, typename P>
 __device__ __forceinline__ P *tile_of(P *head, int64_t c, int Hkv) {
   return head + (uint64_t)(uint32_t)((uint64_t)c >> 6) * (uint32_t)(Hkv * Q8Tile<D>::bytes);
 }
-
-template <int W>
-struct Q8Window {
-  int64_t cells[W + 2 * Q8_HALO];  // of tokens j0 - 7 .. j0 + W + 6; -1: none
-  int lead[W / Q8_GROUP];          // first tokens of the whole groups, 0 .. W - 1
-  int lone[W];                     // tokens in no whole group
-  int n_lead, n_lone;
-  __device__ __forceinline__ int64_t cell(int t) const { return cells[t + Q8_HALO]; }
-  __device__ __forceinline__ bool leads(int t) const {
-    bool w = cell(t) >= 0 && cell(t) % 8 == 0;
-#pragma unroll
-    for (int i = 1; i < 8; i++) w &= cell(t + i) == cell(t) + i;
-    return w;
-  }
-  // All threads; the lists are there for V only.
-  __device__ __forceinline__ void fill(const int64_t *__restrict__ src, int64_t j0, int64_t n,
-                                       int64_t n_cells, bool lists) {
-    const int tid = threadIdx.x;
-    if (tid < W + 2 * Q8_HALO) {
-      const int64_t j = j0 + tid - Q8_HALO, c = j >= 0 && j < n ? src[j] : -1;
-      cells[tid] = c < n_cells ? c : -1;
-    }
-    __syncthreads();
-    if (lists && tid < 64) {
-      const int t = tid < W ? tid : W - 1;
-      const int64_t c = cell(t);
-      const bool is_lead = tid < W && leads(t);
-      const int back = c >= 0 ? (int)(c % 8) : 0;
-      const bool is_lone = tid < W && c >= 0 && !leads(t - back);
-      const uint64_t ml = __builtin_amdgcn_ballot_w64(is_lead), mo = __builtin_amdgcn_ballot_w64(is_lone);
-      const uint64_t below = ((uint64_t)1 << tid) - 1;
-      if (is_lead) lead[__builtin_popcountll(ml & below)] = t;
-      if (is_lone) lone[__builtin_popcountll(mo & below)] = t;
-      if (tid == 0) {
-        n_lead = __builtin_popcountll(ml);
-        n_lone = __builtin_popcountll(mo);
-      }
-    }
-    if (lists) __syncthreads();
-  }
-};
-
-// Threads for n lone tokens: the power of two that holds them, as bits.
-__device__ __forceinline__ int lone_bits(int n) { return n > 1 ? 32 - __builtin_clz(n - 1) : 0; }
 
 // x (n, Hkv D) f32 rows into their cells. Per 32 values (8 lanes), the format's
 // steps in f32: d = amax / 127, q = round(x (1 / d)) with halves away from
@@ -94,7 +51,7 @@ kv_store_q8_kernel(uint8_t *__restrict__ kp, uint8_t *__restrict__ vp, int64_t n
   typedef Q8Tile<D> T;
   constexpr int G4 = D / 4, STEP = Q8_THREADS / G4, PAD = D + 4;
   constexpr int ROWS = W + Q8_HALO, IT = (ROWS + STEP - 1) / STEP, GROUPS = W / Q8_GROUP;
-  __shared__ Q8Window<W> win;
+  __shared__ CellWindow<W> win;
   __shared__ __align__(4) int8_t turn[ROWS * PAD];
   __shared__ uint16_t scale[D / 32 * W];
   const int tid = threadIdx.x, h = blockIdx.x % (uint32_t)Hkv, is_v = blockIdx.y;
@@ -197,7 +154,7 @@ kv_gather_q8_kernel(const uint8_t *__restrict__ pool, int64_t n_cells,
   typedef Q8Tile<D> T;
   constexpr int G4 = D / 4, STEP = Q8_THREADS / G4, PAD = IS_V ? D + 4 : D + 8;
   constexpr int ROWS = IS_V ? W + Q8_HALO : W, NS = IS_V ? W + 8 : W, GROUPS = W / Q8_GROUP;
-  __shared__ Q8Window<W> win;
+  __shared__ CellWindow<W> win;
   __shared__ __align__(8) int8_t turn[ROWS * PAD];
   __shared__ uint8_t mine[ROWS];  // the rows of turn that are this workgroup's
   __shared__ uint16_t scale[D / 32 * NS];
@@ -316,29 +273,35 @@ __device__ __forceinline__ void move_rows(uint8_t *base, const int64_t *from, co
       __builtin_nontemporal_store(v[j], (T *)(base + to[lo[j]] + hi[j]));
 }
 
-// Rows of a workgroup: K's 16-byte pieces of a cell, V's dims.
+// Rows of a tile: K's 16-byte pieces of a cell; V's dims (of Q4_0: pairs of dims).
+__host__ __device__ constexpr int move_k_rows(int type, int D) {
+  return type == LGMLH_Q8_0 ? D / 16 : type == LGMLH_Q4_0 ? D / 32 : D / 8;
+}
+__host__ __device__ constexpr int move_v_rows(int type, int D) { return type == LGMLH_Q4_0 ? D / 2 : D; }
+// Rows of a workgroup.
 struct MoveShape {
   int k_rows, v_rows;
 };
-template <bool Q8, int PER>
+template <int TYPE, int PER>
 __global__ void __launch_bounds__(MOVE_THREADS)
 kv_move_kernel(void *const *__restrict__ pools, int64_t n_cells, int Hkv, int D,
                const int64_t *__restrict__ src, const int64_t *__restrict__ dst, int n,
                MoveShape shape) {
+  constexpr bool Q8 = TYPE == LGMLH_Q8_0, Q4 = TYPE == LGMLH_Q4_0;
   __shared__ int64_t from[MOVE_MAX], to[MOVE_MAX];
   const int p = blockIdx.y, is_v = p & 1;
   const int h = blockIdx.x % Hkv, s = blockIdx.x / Hkv;
-  const int all = is_v ? D : Q8 ? D / 16 : D / 8, rows = is_v ? shape.v_rows : shape.k_rows;
-  const bool scales = Q8 && s == (int)(gridDim.x / Hkv) - 1;
+  const int all = is_v ? move_v_rows(TYPE, D) : move_k_rows(TYPE, D), rows = is_v ? shape.v_rows : shape.k_rows;
+  const bool scales = (Q8 || Q4) && s == (int)(gridDim.x / Hkv) - 1;
   if (!scales && s * rows >= all) return;
   uint8_t *pool = (uint8_t *)pools[p];
-  const int64_t tile = Q8 ? 68 * (int64_t)D : 128 * (int64_t)D;
+  const int64_t tile = (Q8 ? 68 : Q4 ? 36 : 128) * (int64_t)D;
   // a cell's place in its tile, without the row
   auto place = [&](int64_t c) {
     const int o = (int)(c % KV_BLOCK);
-    const int in = scales  ? 64 * D + 2 * o
-                   : !is_v ? (Q8 ? o * 64 : o * D * 2)
-                           : (Q8 ? o % 32 / 8 * 16 + o / 32 * 8 + o % 8 : 2 * o);
+    const int in = scales  ? (Q8 ? 64 : 32) * D + 2 * o
+                   : !is_v ? (Q8 ? o * 64 : Q4 ? q4_k_at(D, o, 0) : o * D * 2)
+                           : (Q8 ? q8_v_at(0, o) : Q4 ? q4_v_at(0, o) : 2 * o);
     return ((c / KV_BLOCK) * Hkv + h) * tile + in;
   };
   for (int m = threadIdx.x; m < n; m += MOVE_THREADS) {
@@ -353,9 +316,9 @@ kv_move_kernel(void *const *__restrict__ pools, int64_t n_cells, int Hkv, int D,
     move_rows<uint16_t, PER, false>(pool, from, to, n, D / 32, [](int r) { return 128 * r; });
   else if (!is_v)
     move_rows<u32x4, PER, true>(pool, from, to, n, left, [&](int r) {
-      return Q8 ? (r0 + r) / 4 * 4096 + (r0 + r) % 4 * 16 : 16 * (r0 + r);
+      return Q8 || Q4 ? (r0 + r) / 4 * 4096 + (r0 + r) % 4 * 16 : 16 * (r0 + r);
     });
-  else if (Q8)
+  else if (Q8 || Q4)
     move_rows<uint8_t, PER, false>(pool, from, to, n, left, [&](int r) { return 64 * (r0 + r); });
   else
     move_rows<uint16_t, PER, false>(pool, from, to, n, left, [&](int r) { return 128 * (r0 + r); });
@@ -366,7 +329,7 @@ kv_move_kernel(void *const *__restrict__ pools, int64_t n_cells, int Hkv, int D,
 // piece, and is twice as long (on the stack up to 512 pieces). 65536 cells in
 // a run take 0.1 ms of the host, each in a block of its own 0.6, 262144 of those
 // 2.5.
-static int check_write_cells(const int64_t *h, int64_t n, int64_t n_cells, const char *what) {
+int check_write_cells(const int64_t *h, int64_t n, int64_t n_cells, const char *what) {
   if (!h) {
     set_error("%s: the host copy of the cells is required for the checks", what);
     return LGMLH_EINVAL;
@@ -418,10 +381,7 @@ static int check_write_cells(const int64_t *h, int64_t n, int64_t n_cells, const
   return LGMLH_OK;
 }
 
-// Heads of cells in one call: a launch has fewer than 2^32 threads, 256 for 32 or
-// more of them. KV heads: the bytes of a block, 68 D for each, are counted in 31
-// bits (tile_of).
-constexpr int64_t Q8_ROWS = int64_t(1) << 29;
+// KV heads: the bytes of a block, 68 D for each, are counted in 31 bits (tile_of).
 constexpr int Q8_HEADS = 65535;
 static_assert((int64_t)Q8_HEADS * q8_tile_bytes(256) < INT32_MAX, "tile_of");
 
@@ -441,8 +401,8 @@ extern "C" int lgmlh_kv_store_q8(void *kpool, void *vpool, int64_t n_cells, int 
                                  const int64_t *cells, const int64_t *h_cells, int64_t n,
                                  void *stream) {
   if (!kpool || !vpool || !k_src || !v_src || !cells || n < 0 || n_cells <= 0 ||
-      n_cells > Q8_CELLS || n_cells % KV_BLOCK || n_head_kv <= 0 || n_head_kv > Q8_HEADS ||
-      n >= Q8_ROWS / n_head_kv || !q8_head(head_dim)) {
+      n_cells > CELLS_MAX || n_cells % KV_BLOCK || n_head_kv <= 0 || n_head_kv > Q8_HEADS ||
+      n >= CELL_ROWS / n_head_kv || !q8_head(head_dim)) {
     set_error("kv_store_q8: bad arguments (heads of 64, 128 or 256)");
     return LGMLH_EINVAL;
   }
@@ -469,8 +429,8 @@ extern "C" int lgmlh_kv_gather_q8(const void *pool, int which, int64_t n_cells, 
                                   int head_dim, const int64_t *cells, int64_t n, void *out,
                                   int out_type, void *stream) {
   if (!pool || !cells || !out || n < 0 || (which != 0 && which != 1) || n_cells <= 0 ||
-      n_cells > Q8_CELLS || n_cells % KV_BLOCK || n_head_kv <= 0 || n_head_kv > Q8_HEADS ||
-      n >= Q8_ROWS / n_head_kv || !q8_head(head_dim) ||
+      n_cells > CELLS_MAX || n_cells % KV_BLOCK || n_head_kv <= 0 || n_head_kv > Q8_HEADS ||
+      n >= CELL_ROWS / n_head_kv || !q8_head(head_dim) ||
       (out_type != LGMLH_F32 && out_type != LGMLH_F16)) {
     set_error("kv_gather_q8: bad arguments (heads of 64, 128 or 256; out f32 or f16)");
     return LGMLH_EINVAL;
@@ -514,11 +474,11 @@ extern "C" int lgmlh_kv_gather_q8(const void *pool, int which, int64_t n_cells, 
 extern "C" int lgmlh_kv_move(int type, void *const *pools, int n_pools, int64_t n_cells,
                              int n_head_kv, int head_dim, const int64_t *src, const int64_t *dst,
                              const int64_t *h_src, const int64_t *h_dst, int64_t n, void *stream) {
-  const bool q8 = type == LGMLH_Q8_0;
+  const bool q8 = type == LGMLH_Q8_0 || type == LGMLH_Q4_0;  // with scales
   if ((!q8 && type != LGMLH_F16) || !pools || !src || !dst || n_pools <= 0 || n_pools > 65535 ||
       n_pools % 2 || n_cells <= 0 || n_cells % KV_BLOCK || n_head_kv <= 0 || n_head_kv > 65535 || n < 0 ||
       (q8 ? !q8_head(head_dim) : head_dim != 16 && (head_dim <= 0 || head_dim % 32))) {
-    set_error("kv_move: bad arguments (K and V tensors in turn, of f16 or Q8_0)");
+    set_error("kv_move: bad arguments (K and V tensors in turn, of f16, Q8_0 or Q4_0)");
     return LGMLH_EINVAL;
   }
   if (n > MOVE_MAX) {
@@ -545,13 +505,15 @@ extern "C" int lgmlh_kv_move(int type, void *const *pools, int n_pools, int64_t 
     while (r > hold) r = (r + 1) / 2;
     return r;
   };
-  const int pieces = head_dim / (q8 ? 16 : 8);
-  const MoveShape shape = {fit(pieces), fit(head_dim)};
+  const int pieces = move_k_rows(type, head_dim), dims = move_v_rows(type, head_dim);
+  const MoveShape shape = {fit(pieces), fit(dims)};
   const int slices_k = (pieces + shape.k_rows - 1) / shape.k_rows,
-            slices_v = (head_dim + shape.v_rows - 1) / shape.v_rows;
+            slices_v = (dims + shape.v_rows - 1) / shape.v_rows;
   const int slices = (slices_k > slices_v ? slices_k : slices_v) + (q8 ? 1 : 0);
-  const auto kern = q8 ? (per == 8 ? kv_move_kernel<true, 8> : kv_move_kernel<true, 16>)
-                       : (per == 8 ? kv_move_kernel<false, 8> : kv_move_kernel<false, 16>);
+  auto of = [&](auto eight, auto sixteen) { return per == 8 ? eight : sixteen; };
+  const auto kern = type == LGMLH_Q8_0   ? of(kv_move_kernel<LGMLH_Q8_0, 8>, kv_move_kernel<LGMLH_Q8_0, 16>)
+                    : type == LGMLH_Q4_0 ? of(kv_move_kernel<LGMLH_Q4_0, 8>, kv_move_kernel<LGMLH_Q4_0, 16>)
+                                         : of(kv_move_kernel<LGMLH_F16, 8>, kv_move_kernel<LGMLH_F16, 16>);
   hipLaunchKernelGGL(kern, dim3((unsigned)(n_head_kv * slices), (unsigned)n_pools), dim3(MOVE_THREADS),
                      0, as_stream(stream), pools, n_cells, n_head_kv, head_dim, src, dst, (int)n, shape);
   return hip_check(hipGetLastError(), "kv_move");

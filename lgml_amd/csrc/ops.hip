@@ -4,6 +4,7 @@
 #include <stdio.h>
 
 #include "common.h"
+#include "kvq4.h"
 #include "kvq8.h"
 #include "quant.h"
 #include "split.h"
@@ -234,12 +235,12 @@ __global__ void rope_table_kernel(const int32_t *__restrict__ pos, int n_rot, fl
 // (q_norm / k_norm; on gemma the V norm without a weight, :1782-1784),
 // rope for q and k heads, and the store: q to q_out, k and v to their pool
 // cell. With QKV_V_FROM_K a V head is the raw K head (transformer.lua:1779).
-// Q8: the pool is in Q8_0 (kvq8.h); a block of 32 values is half a wave's. 64, 512
+// TYPE Q8_0 or Q4_0: the pool is quantised (kvq8.h, kvq4.h); a block of 32 values is half a wave's. 64, 512
 // and 2048 tokens of 32 / 8 heads of 128 take 6.6, 20 and 65 us, 6.3, 19.5 and 63
 // over f16 (18 and 59 of the 20 and 65 with V left out): the rows, angles and q
 // bound it, not V's single bytes.
 constexpr int QKV_HEADS = 8;
-template <bool Q8>
+template <int TYPE>
 __global__ void __launch_bounds__(64 * QKV_HEADS)
 qkv_rope_store_kernel(const float *__restrict__ qkv, int H, int Hkv, int D, int n_rot, int neox,
                       float theta_scale, const float *__restrict__ ff,
@@ -320,7 +321,24 @@ qkv_rope_store_kernel(const float *__restrict__ qkv, int H, int Hkv, int D, int 
   const int64_t cell = cells[t];
   if (cell < 0 || cell >= n_cells) return;  // a cell outside the pool is never written
   const int64_t b = cell / KV_BLOCK, o = cell % KV_BLOCK;
-  if constexpr (Q8) {
+  if constexpr (TYPE == LGMLH_Q4_0) {
+    const int hh = is_k ? h - H : h - H - Hkv;
+    uint8_t *tile = (uint8_t *)(is_k ? kp : vp) + (b * Hkv + hh) * (int64_t)q4_tile_bytes(D);
+    for (int d = lane; d < D; d += 64) {  // D is a multiple of 64
+      const float x[1] = {v[d]};
+      const float dd = group_first_abs<32>(x, group_max<32>(fabsf(x[0]))) * -0.125f;
+      const int n = (int)q4_round(x[0], dd != 0.0f ? 1.0f / dd : 0.0f);
+      // a byte holds K's dims e and e + 2 of 8, V's dims r and r + 16 of 32
+      const int byte = n | __shfl_xor(n, is_k ? 2 : 16) << 4;
+      const int e = d % 8;
+      if (is_k ? (e & 2) == 0 : d % 32 < 16)
+        tile[is_k ? q4_k_at(D, (int)o, d - e) + 2 * (e & 1) + e / 4 : q4_v_at(d / 32 * 16 + d % 16, (int)o)] =
+            (uint8_t)byte;
+      if (lane % 32 == 0) *(uint16_t *)(tile + q4_scale_at(D, d / 32, (int)o)) = f2h(dd);
+    }
+    return;
+  }
+  if constexpr (TYPE == LGMLH_Q8_0) {
     const int hh = is_k ? h - H : h - H - Hkv;
     uint8_t *tile = (uint8_t *)(is_k ? kp : vp) + (b * Hkv + hh) * (int64_t)q8_tile_bytes(D);
     for (int d = lane; d < D; d += 64) {  // D is a multiple of 64
@@ -636,21 +654,24 @@ int qkv_rope_store_dev(float *qkv, int64_t n, int n_head, int n_head_kv,
                                     const float *k_norm, float eps, const int32_t *pos,
                                     void *kpool, void *vpool, int64_t n_cells,
                                     const int64_t *cells, float *q_out, void *stream, Pending pa,
-                       Pending pb, int vmode, const float *table, bool q8) {
+                       Pending pb, int vmode, const float *table, int type) {
   if (!qkv || !pos || !kpool || !vpool || !cells || !q_out || n < 0 || n_head <= 0 ||
       n_head_kv <= 0 || head_dim <= 0 || head_dim % 8 || head_dim > 1024 || n_rot <= 0 ||
       n_rot > head_dim ||
       n_rot % 2 || n_cells % KV_BLOCK || pa.cols % 8 || pb.cols % 8 ||
-      (q8 && ((head_dim != 64 && head_dim != 128 && head_dim != 256) ||
-              (((uintptr_t)kpool | (uintptr_t)vpool) & 15)))) {
-    set_error("qkv_rope_store%s: bad arguments", q8 ? "_q8" : "");
+      (type != LGMLH_F16 && ((head_dim != 64 && head_dim != 128 && head_dim != 256) ||
+                              (((uintptr_t)kpool | (uintptr_t)vpool) & 15)))) {
+    set_error("qkv_rope_store%s: bad arguments", type == LGMLH_Q8_0 ? "_q8" : type == LGMLH_Q4_0 ? "_q4" : "");
     return LGMLH_EINVAL;
   }
   if (n == 0) return LGMLH_OK;
   const float theta_scale = rope_theta_scale(freq_base, n_rot);
   const size_t lds = ((size_t)QKV_HEADS * head_dim + n_rot) * sizeof(float);
   const int groups = (n_head + 2 * n_head_kv + QKV_HEADS - 1) / QKV_HEADS;
-  hipLaunchKernelGGL(q8 ? qkv_rope_store_kernel<true> : qkv_rope_store_kernel<false>,
+  const auto kern = type == LGMLH_Q8_0   ? qkv_rope_store_kernel<LGMLH_Q8_0>
+                    : type == LGMLH_Q4_0 ? qkv_rope_store_kernel<LGMLH_Q4_0>
+                                         : qkv_rope_store_kernel<LGMLH_F16>;
+  hipLaunchKernelGGL(kern,
                      dim3((unsigned)n, (unsigned)groups), dim3(64 * QKV_HEADS), lds,
                      as_stream(stream), qkv, n_head, n_head_kv, head_dim, n_rot, neox,
                      theta_scale, freq_factors, q_norm, k_norm, eps, pos, (uint16_t *)kpool,
@@ -675,7 +696,7 @@ extern "C" int lgmlh_qkv_rope_store(float *qkv, int64_t n, int n_head, int n_hea
                                     const int64_t *cells, float *q_out, void *stream) {
   return qkv_rope_store_dev(qkv, n, n_head, n_head_kv, head_dim, n_rot, neox, freq_base,
                             freq_factors, q_norm, k_norm, eps, pos, kpool, vpool, n_cells, cells,
-                            q_out, stream, Pending{}, Pending{}, 0, nullptr, false);
+                            q_out, stream, Pending{}, Pending{}, 0, nullptr, LGMLH_F16);
 }
 
 extern "C" int lgmlh_qkv_rope_store_q8(float *qkv, int64_t n, int n_head, int n_head_kv,
@@ -686,7 +707,18 @@ extern "C" int lgmlh_qkv_rope_store_q8(float *qkv, int64_t n, int n_head, int n_
                                        const int64_t *cells, float *q_out, void *stream) {
   return qkv_rope_store_dev(qkv, n, n_head, n_head_kv, head_dim, n_rot, neox, freq_base,
                             freq_factors, q_norm, k_norm, eps, pos, kpool, vpool, n_cells, cells,
-                            q_out, stream, Pending{}, Pending{}, 0, nullptr, true);
+                            q_out, stream, Pending{}, Pending{}, 0, nullptr, LGMLH_Q8_0);
+}
+
+extern "C" int lgmlh_qkv_rope_store_q4(float *qkv, int64_t n, int n_head, int n_head_kv,
+                                       int head_dim, int n_rot, int neox, float freq_base,
+                                       const float *freq_factors, const float *q_norm,
+                                       const float *k_norm, float eps, const int32_t *pos,
+                                       void *kpool, void *vpool, int64_t n_cells,
+                                       const int64_t *cells, float *q_out, void *stream) {
+  return qkv_rope_store_dev(qkv, n, n_head, n_head_kv, head_dim, n_rot, neox, freq_base,
+                            freq_factors, q_norm, k_norm, eps, pos, kpool, vpool, n_cells, cells,
+                            q_out, stream, Pending{}, Pending{}, 0, nullptr, LGMLH_Q4_0);
 }
 
 extern "C" int lgmlh_swiglu(const float *gu, int64_t n, int64_t F, void *out, int out_type,

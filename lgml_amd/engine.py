@@ -59,6 +59,9 @@ evicts (new_block's grow branch, transformer.lua:934-958, pool_grow
 
 With prefix_cache, a request that ends publishes the keys of its prompt and
 reply blocks, so a follow-up turn that repeats them attaches them.
+
+Beyond the reference: sequences fork (PoolSeqs.fork), and a pool that grew for
+a peak is compacted and cut to the blocks in use (Engine.compact).
 """
 import ctypes as C
 
@@ -142,18 +145,20 @@ class PoolSeqs:
             c.blocks[first:] = sorted(c.blocks[first:])
 
     def copy_block(self, src, dst, n):
-        """M.copy_block (transformer.lua:989-1007) on the device, every layer."""
+        """M.copy_block (transformer.lua:989-1007) on the device, every layer in
+        one launch."""
         m = self.model
-        if getattr(m, "kv_type", hip.F16) == hip.Q8_0:
-            cells = np.arange(n, dtype=np.int64)
-            m.move_cells(src * BLOCK + cells, dst * BLOCK + cells)
+        if src == dst or n == 0:
             return
-        D, Hkv = getattr(m, "paged_dims", (m.hp["head_dim"], m.hp["n_head_kv"]))
+        if m.kv_type != hip.F16 or not torch.cuda.is_current_stream_capturing():
+            m.copy_blocks([src], [dst], n)
+            return
+        # under capture: the f16 copy whose blocks are the launch's own arguments
+        D, Hkv = m.paged_dims
         for il, (kp, vp) in enumerate(zip(m.kpools, m.vpools)):
-            if getattr(m, "swa", None) and m.swa[il]:
-                continue  # ring pools hold no pool blocks
-            check(hip.lib().lgmlh_kv_copy_block(kp.data_ptr(), vp.data_ptr(), m.n_cells, Hkv, D,
-                                                src, dst, n, stream()))
+            if not m.swa[il]:  # ring pools hold no pool blocks
+                check(hip.lib().lgmlh_kv_copy_block(kp.data_ptr(), vp.data_ptr(), m.n_cells, Hkv, D,
+                                                    src, dst, n, stream()))
 
     def truncate(self, c, n):
         """transformer.lua:1084-1108."""
@@ -185,6 +190,54 @@ class PoolSeqs:
     def free(self, c):
         """M:free_seq (transformer.lua:784-803): give the blocks back."""
         self.truncate(c, 0)
+
+    def fork(self, c, n=1):
+        """n sequences that go on from c's cells, each on its own from here: the
+        full blocks are shared (M:share, transformer.lua:1116-1123), the cells of
+        the partial one are copied into a block of each, all in one launch. For
+        several replies to one prompt. PoolFull leaves the sequences as they were."""
+        full, part = divmod(c.n_past, BLOCK)
+        made = []
+        try:
+            for _ in range(n):
+                d = Seq(self, c.prio)
+                made.append(d)
+                for b in c.blocks[:full]:  # (M:share takes keyed blocks only)
+                    self.alloc.ref(b, d.prio)
+                    d.blocks.append(b)
+                d.keys[:] = c.keys[:full]
+                d.n_past = c.n_past
+                if part:
+                    self.reserve(d, c.n_past)
+        except PoolFull:
+            for d in made:
+                self.free(d)
+            raise
+        if part and made:
+            self.model.copy_blocks([c.blocks[full]] * n, [d.blocks[full] for d in made], part)
+        return made
+
+    def compact(self, seqs):
+        """The blocks in use or kept move into the lowest places: cells, references,
+        keys and the tables of seqs, which are all the sequences that hold blocks.
+        Returns how many blocks there are then: those behind them are free."""
+        held = [b for b in range(self.alloc.cap) if self.alloc.in_use(b)]
+        refs = {}
+        for b in (b for c in seqs for b in c.blocks):
+            refs[b] = refs.get(b, 0) + 1
+        for b in held:
+            if self.alloc.refs_of(b) != refs.get(b, 0):
+                raise ValueError("block %d has %d references, the sequences' tables hold %d" % (
+                    b, self.alloc.refs_of(b), refs.get(b, 0)))
+        places = sorted(set(range(len(held))) - set(held))
+        moves = dict(zip(reversed(held), places))  # from above, into the free places below
+        if moves:
+            self.model.copy_blocks(list(moves), list(moves.values()))
+            for src, dst in moves.items():
+                self.alloc.relocate(src, dst)
+            for c in seqs:
+                c.blocks[:] = [moves.get(b, b) for b in c.blocks]
+        return len(held)
 
 
 def seq_cells(c, frm, n):
@@ -375,6 +428,23 @@ class Engine:
         self._submitted = 0
         if self.ram is not None:
             self.seqs.on_evict = self.spill_block
+
+    def compact(self, shrink=True, keep_cached=True):
+        """The pool's blocks in use or kept for their keys move into its lowest
+        places (keep_cached False: those kept for their keys alone are evicted
+        first, to the RAM store if there is one); with shrink, its tensors are cut
+        to them (one block at least; they grow again as needed, grow_pool), which
+        gives the rest of their memory back to the allocator. For after a peak.
+        Between steps; a pass in flight has read its cells before they move.
+        Returns the pool's cells."""
+        if not keep_cached:
+            while (b := self.seqs.evict()) is not None:
+                self.seqs.alloc.unref(b)
+        blocks = self.seqs.compact([r.seq for r in self.active])
+        if shrink:
+            self.model.shrink_pool(max(blocks, 1) * BLOCK)
+            self.seqs.alloc.set_cap(self.model.pool_blocks)
+        return self.model.n_cells
 
     def submit(self, req):
         if len(self.active) >= self.n_slots:

@@ -11,7 +11,7 @@ import os
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "liblgml_hip.so")
 
-F32, F16, Q8_0, Q4_K, Q6_K = 0, 1, 8, 12, 14
+F32, F16, Q4_0, Q8_0, Q4_K, Q6_K = 0, 1, 2, 8, 12, 14
 OK, EINVAL, ENOMEM, EHIP, EFULL, ERANGE = 0, -1, -2, -3, -4, -5
 EPI_NONE, EPI_ADD = 0, 1
 ACT_EXACT, ACT_GGML = 0, 1
@@ -37,6 +37,9 @@ SYMBOLS = (
     "lgmlh_plan_tree", "lgmlh_paged_attention_q8", "lgmlh_kv_q8_layer_bytes", "lgmlh_kv_store_q8",
     "lgmlh_kv_gather_q8", "lgmlh_kv_move", "lgmlh_log_probs_workspace", "lgmlh_log_probs",
     "lgmlh_qkv_rope_store_q8", "lgmlh_forward_q8",
+    "lgmlh_kv_q4_layer_bytes", "lgmlh_kv_store_q4", "lgmlh_kv_gather_q4", "lgmlh_paged_attention_q4",
+    "lgmlh_qkv_rope_store_q4", "lgmlh_forward_q4", "lgmlh_kv_copy_blocks", "lgmlh_kvpool_relocate",
+    "lgmlh_qkv_rope_store_axes",
 )
 PLAN_TREE, TREE_MAX = -1, 1024
 GATING_SOFTMAX, GATING_SIGMOID = 1, 2
@@ -201,8 +204,16 @@ def _declare(L):
         "lgmlh_log_probs_workspace": ([i64, i64, i32], sz),
         "lgmlh_log_probs": ([vp, i64, i64, vp, i32, vp, vp, i32, vp, vp, vp, sz, vp], i32),
     }
-    sig["lgmlh_qkv_rope_store_q8"] = sig["lgmlh_qkv_rope_store"]
-    sig["lgmlh_forward_q8"] = sig["lgmlh_forward"]
+    sig["lgmlh_kv_copy_blocks"] = ([i32, vp, i32, i64, i32, i32, vp, vp, i64, vp], i32)
+    sig["lgmlh_kvpool_relocate"] = ([vp, C.c_int32, C.c_int32], i32)
+    sig["lgmlh_qkv_rope_store_axes"] = ([i32, vp, i64, i32, i32, i32, i32, vp, i32, C.c_float, vp, vp,
+                                         vp, C.c_float, vp, vp, vp, i64, vp, vp, vp], i32)
+    for q in ("_q8", "_q4"):
+        sig["lgmlh_qkv_rope_store" + q] = sig["lgmlh_qkv_rope_store"]
+        sig["lgmlh_forward" + q] = sig["lgmlh_forward"]
+    for name in ("lgmlh_kv_q%d_layer_bytes", "lgmlh_kv_store_q%d", "lgmlh_kv_gather_q%d",
+                 "lgmlh_paged_attention_q%d"):
+        sig[name % 4] = sig[name % 8]
     for name, (args, res) in sig.items():
         f = getattr(L, name)
         f.argtypes = args

@@ -112,3 +112,12 @@ class Pool:
 
     def set_cap(self, cap):
         hip.check(hip.lib().lgmlh_kvpool_set_cap(self.mem, cap))
+
+    def relocate(self, src, dst):
+        """Block src becomes the free block dst, with its references, key and
+        tokens (the caller moves the cells and puts its block tables right)."""
+        hip.check(hip.lib().lgmlh_kvpool_relocate(self.mem, src, dst))
+
+    def in_use(self, b):
+        """Whether block b has a reference or is kept for its key."""
+        return self.refs_of(b) > 0 or self.key_of(b) is not None

@@ -123,8 +123,8 @@ def generated_weights(hp, seed, policy):
 def load_gguf(path, n_cells, ring_cells=0, kv_type=hip.F16):
     """A DeviceModel from a gguf file (lgml_amd.gguf.load: llama, qwen3,
     qwen3moe, gemma4; a gemma4 model's sliding and global layers keep their
-    own head sizes and KV head counts). kv_type: of its KV pools, hip.F16 or
-    hip.Q8_0."""
+    own head sizes and KV head counts). kv_type: of its KV pools, hip.F16,
+    hip.Q8_0 or hip.Q4_0."""
     from . import gguf
     hp, w = gguf.load(path)
     return DeviceModel(hp, w, n_cells, ring_cells, kv_type=kv_type)
@@ -277,8 +277,9 @@ class DeviceModel:
         paged pool starts at this many cells and grows (grow_pool) up to
         n_cells, as the reference's pool starts at KV_INITIAL and doubles
         (engine.lua:49, transformer.lua:831-908); 0: n_cells from the start.
-        kv_type: hip.F16, or hip.Q8_0 for pools (and rings) of 8-bit values
-        with a scale per 32 (heads of 64, 128 and 256; 17/32 of the bytes)."""
+        kv_type: hip.F16, or hip.Q8_0 or hip.Q4_0 for pools (and rings) of 8-
+        or 4-bit values with a scale per 32 (heads of 64, 128 and 256; 17/32 or
+        9/32 of the bytes)."""
         from . import workload
         L = hip.lib()
         self.hp = hp
@@ -287,8 +288,8 @@ class DeviceModel:
         self.max_cells = int(n_cells)
         self.n_cells = int(kv_initial) if kv_initial else self.max_cells
         self.ring_cells = int(ring_cells)
-        if kv_type not in (hip.F16, hip.Q8_0):
-            raise ValueError("kv_type %r: hip.F16 or hip.Q8_0" % (kv_type,))
+        if kv_type not in (hip.F16, hip.Q8_0, hip.Q4_0):
+            raise ValueError("kv_type %r: hip.F16, hip.Q8_0 or hip.Q4_0" % (kv_type,))
         self.kv_type = kv_type
         assert self.n_cells % 64 == 0 and self.ring_cells % 64 == 0
         assert self.max_cells % 64 == 0 and self.n_cells <= self.max_cells
@@ -398,10 +399,11 @@ class DeviceModel:
                 Ly.wdown, Ly.wdown_type = keep(t).data_ptr(), ty
             # the pool tensors live in kpools / vpools (grow_pool replaces them)
             nc = self.ring_cells if Ly.swa else self.n_cells
-            kvb_l = (L.lgmlh_kv_q8_layer_bytes if kv_type == hip.Q8_0 else
-                     L.lgmlh_kv_layer_bytes)(nc, Hl, Dl)
-            if kvb_l < 0 and kv_type == hip.Q8_0 and nc:
-                raise ValueError("a Q8_0 pool takes heads of 64, 128 or 256, not %d" % Dl)
+            kvb_l = {hip.Q8_0: L.lgmlh_kv_q8_layer_bytes, hip.Q4_0: L.lgmlh_kv_q4_layer_bytes}.get(
+                kv_type, L.lgmlh_kv_layer_bytes)(nc, Hl, Dl)
+            if kvb_l < 0 and kv_type != hip.F16 and nc:
+                raise ValueError("a %s pool takes heads of 64, 128 or 256, not %d" % (
+                    "Q8_0" if kv_type == hip.Q8_0 else "Q4_0", Dl))
             kp = _zeros(kvb_l)
             vp = _zeros(kvb_l)
             self.kpools.append(kp)
@@ -473,8 +475,8 @@ class DeviceModel:
     def block_dim(self, head_dim):
         """The f16 head size whose blocks have the bytes of the pools' blocks,
         for the entry points that copy whole blocks: a Q8_0 block is 17/32 of
-        an f16 one."""
-        return head_dim * 17 // 32 if self.kv_type == hip.Q8_0 else head_dim
+        an f16 one, a Q4_0 block 9/32."""
+        return head_dim * {hip.Q8_0: 17, hip.Q4_0: 9}.get(self.kv_type, 32) // 32
 
     @property
     def pool_blocks(self):
@@ -506,16 +508,43 @@ class DeviceModel:
                                       stream()))
                 pools[il] = new
                 setattr(self.layers[il], attr, new.data_ptr())
+        self._resized(cells)
+        return cells
+
+    def shrink_pool(self, cells):
+        """The paged pool tensors of every layer cut to their first `cells`
+        cells (a multiple of 64, at least one block), for a pool whose blocks
+        behind them are free (Engine.compact); the memory goes back to the
+        allocator. The pool may grow again, up to max_cells. Returns the new
+        cell count. The counterpart of grow_pool; the reference's pools only
+        grow (transformer.lua:831-908)."""
+        cells = int(cells)
+        if cells % 64 or cells <= 0:
+            raise ValueError("%d cells: whole blocks of 64, at least one" % cells)
+        if cells >= self.n_cells:
+            return self.n_cells
+        Hkv, D = self.paged_dims[1], self.block_dim(self.paged_dims[0])
+        nb = hip.lib().lgmlh_kv_layer_bytes(cells, Hkv, D)
+        for il in range(self.hp["n_layer"]):
+            if self.swa[il]:
+                continue
+            for pools, attr in ((self.kpools, "kpool"), (self.vpools, "vpool")):
+                pools[il] = pools[il][:nb].clone()
+                setattr(self.layers[il], attr, pools[il].data_ptr())
+        self._resized(cells)
+        return cells
+
+    def _resized(self, cells):
+        """The paged pool tensors were replaced by ones of `cells` cells."""
         # the old tensors are freed once the copies are done
         torch.cuda.current_stream().synchronize()
         self.n_cells = cells
         self.m.n_cells = cells
         ptrs = []
-        for il in range(hp["n_layer"]):
+        for il in range(self.hp["n_layer"]):
             if not self.swa[il]:
                 ptrs += [self.kpools[il].data_ptr(), self.vpools[il].data_ptr()]
         self.pools_dev = torch.tensor(ptrs or [0], dtype=torch.int64, device=DEV)
-        return cells
 
     ring_blocks_per_split = 0  # the ring plans' run length (0: as blocks_per_split; 12 for heads of 256)
 
@@ -584,7 +613,8 @@ class DeviceModel:
         ws, ws_bytes = self.workspace(plan, n_out, slot)
         if logits is None:
             logits = torch.empty((n_out, self.hp["n_vocab"]), dtype=torch.float32, device=DEV)
-        fn = hip.lib().lgmlh_forward_q8 if self.kv_type == hip.Q8_0 else hip.lib().lgmlh_forward
+        L = hip.lib()
+        fn = {hip.Q8_0: L.lgmlh_forward_q8, hip.Q4_0: L.lgmlh_forward_q4}.get(self.kv_type, L.lgmlh_forward)
         check(fn(C.byref(self.m), C.byref(plan.ub),
                  C.byref(plan.ring.ub) if plan.ring is not None else None, ptr(rows), n_out,
                  logits.data_ptr(), ws.data_ptr(), ws_bytes,
@@ -610,6 +640,35 @@ class DeviceModel:
                                       self.n_cells, Hkv, D, both[0].data_ptr(), both[1].data_ptr(),
                                       ptr(src), ptr(dst), len(src), stream()))
 
+    def copy_blocks(self, src, dst, cells=64):
+        """Blocks src to dst in every paged layer's K and V, their first `cells`
+        cells (one number, or one for each block; lgmlh_kv_copy_blocks). A source
+        of -1 clears the cells; a block may be the source of several, a target is
+        no source. Queued on the current stream; the host waits for nothing; a
+        captured stream is refused."""
+        src, dst = (np.asarray(a).reshape(-1) for a in (src, dst))
+        if len(src) != len(dst):
+            raise ValueError("%d blocks to %d places" % (len(src), len(dst)))
+        copies = np.empty((len(src), 3), np.int32)
+        for i, a in enumerate((src, dst, np.broadcast_to(np.asarray(cells).reshape(-1), src.shape))):
+            copies[:, i] = a
+            if (copies[:, i] != a).any():
+                raise ValueError("blocks and cells: whole numbers of 32 bits")
+        if not len(copies) or not self.n_pools:
+            return
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("copy_blocks takes its blocks from the host: capture lgmlh_kv_copy_blocks instead")
+        dev = _dev_behind(copies)
+        D, Hkv = self.paged_dims
+        check(hip.lib().lgmlh_kv_copy_blocks(self.kv_type, self.pools_dev.data_ptr(), self.n_pools,
+                                             self.n_cells, Hkv, D, dev.data_ptr(), ptr(copies),
+                                             len(copies), stream()))
+
+    def clear_blocks(self, blocks):
+        """Zeros in the blocks' cells, in every paged layer's K and V: as new
+        cells start (a freed block holds its last sequence's until then)."""
+        self.copy_blocks(np.full(len(np.reshape(blocks, -1)), -1), blocks)
+
     def gather_kv(self, layer, cells, which=0):
         """Cells of a layer's K (0) or V (1) as (n, Hkv*D) f16 bits (uint16)
         (ring cells for a sliding layer)."""
@@ -619,9 +678,10 @@ class DeviceModel:
         out = torch.empty((len(cells), Hkv * D), dtype=torch.int16, device=DEV)
         pool = (self.kpools if which == 0 else self.vpools)[layer]
         n = self.ring_cells if self.swa[layer] else self.n_cells
-        if self.kv_type == hip.Q8_0:  # the f16 of the values held
-            check(hip.lib().lgmlh_kv_gather_q8(pool.data_ptr(), which, n, Hkv, D, dc.data_ptr(),
-                                               len(cells), out.data_ptr(), hip.F16, stream()))
+        if self.kv_type != hip.F16:  # the f16 of the values held
+            fn = hip.lib().lgmlh_kv_gather_q8 if self.kv_type == hip.Q8_0 else hip.lib().lgmlh_kv_gather_q4
+            check(fn(pool.data_ptr(), which, n, Hkv, D, dc.data_ptr(), len(cells), out.data_ptr(),
+                     hip.F16, stream()))
             return out.cpu().numpy().view(np.uint16)
         check(hip.lib().lgmlh_kv_gather(pool.data_ptr(), which, n, Hkv, D,
                                         dc.data_ptr(), len(cells), out.data_ptr(), stream()))
