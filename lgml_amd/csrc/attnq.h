@@ -32,9 +32,6 @@
 
 namespace lgmlh {
 
-constexpr float QP = 8192.0f;  // the scale of P in its halves
-constexpr int SHARED_MAX = ATTN_SHARED;  // the most items of a shared run
-
 __device__ __forceinline__ f32x4 mfma16q(f16x8 a, f16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
@@ -56,31 +53,6 @@ __device__ __forceinline__ float quads_max(float v) {
   return fmaxf(__builtin_bit_cast(float, (uint32_t)q[0]), __builtin_bit_cast(float, (uint32_t)q[1]));
 }
 
-// q row pieces -> B operands, hi and lo, of the row scaled by 2^(15 - e); the
-// factor of the scores that undoes it.
-template <int NB>
-__device__ __forceinline__ float split_q(const f32x4 (&qa)[2 * NB], bool rvalid, float scale_log2,
-                                         f16x8 (&hi)[NB], f16x8 (&lo)[NB]) {
-  float mx = 0.0f;
-#pragma unroll
-  for (int i = 0; i < 2 * NB; i++)
-#pragma unroll
-    for (int j = 0; j < 4; j++) mx = fmaxf(mx, fabsf(qa[i][j]));
-  mx = quads_max(mx);
-  int e = __builtin_amdgcn_frexp_expf(mx);
-  e = e < -110 ? -110 : e;
-  const float up = rvalid ? pow2(15 - e) : 0.0f;
-#pragma unroll
-  for (int b = 0; b < NB; b++)
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-      const float x = rvalid ? qa[2 * b + (i >> 2)][i & 3] * up : 0.0f;
-      hi[b][i] = (f16)x;
-      lo[b][i] = (f16)(x - (float)hi[b][i]);
-    }
-  return scale_log2 * pow2(e - 15);
-}
-
 // The lane, of which what follows is made anew where it is used: held over a loop, it
 // takes registers that heads of 256 do not have.
 __device__ __forceinline__ int lane_anew() {
@@ -91,50 +63,6 @@ __device__ __forceinline__ int lane_anew() {
 
 // A block's word from the lane's first cell, 8 quad, on.
 __device__ __forceinline__ uint64_t lane_cells(uint64_t word) { return word >> (lane_anew() >> 1 & 24); }
-
-// Scores (scaled, in units of log2) -> P in place, the running maximum and sum,
-// the rescale of O^T. masked: cells without a bit in word are dropped. l is of the
-// lane's own cells; the quads' add up at the end.
-template <int DT>
-__device__ __forceinline__ void softmax_q(f32x4 (&st)[4], float rscale, bool masked, uint64_t word,
-                                           float &m, float &l, f32x4 (&o)[DT]) {
-#pragma unroll
-  for (int ct = 0; ct < 4; ct++)
-#pragma unroll
-    for (int i = 0; i < 4; i++) st[ct][i] *= rscale;  // (of vectors: the factor would be held four times)
-  if (masked) {  // wave-uniform
-    word = lane_cells(word);  // s_cell(ct, 4 quad + i) = 8 quad + s_cell(ct, i)
-#pragma unroll
-    for (int ct = 0; ct < 4; ct++)
-#pragma unroll
-      for (int i = 0; i < 4; i++)
-        if (!(word >> s_cell(ct, i) & 1)) st[ct][i] = -INFINITY;
-  }
-  float mx = -INFINITY;
-#pragma unroll
-  for (int ct = 0; ct < 4; ct++)
-#pragma unroll
-    for (int i = 0; i < 4; i++) mx = fmaxf(mx, st[ct][i]);
-  mx = quads_max(mx);
-  const float m_new = fmaxf(m, mx);
-  const float m_use = m_new == -INFINITY ? 0.0f : m_new;
-  float rs = 0.0f;
-#pragma unroll
-  for (int ct = 0; ct < 4; ct++)
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      st[ct][i] = __builtin_amdgcn_exp2f(st[ct][i] - m_use);  // exp2(-inf) = 0
-      rs += st[ct][i];
-    }
-  if (__builtin_amdgcn_ballot_w64(m_new != m)) {
-    const float alpha = __builtin_amdgcn_exp2f(m - m_use);
-    l *= alpha;
-#pragma unroll
-    for (int dt = 0; dt < DT; dt++) o[dt] *= alpha;
-  }
-  l += rs;
-  m = m_new;
-}
 
 // |scale| as the f16's bits, where NaN is above the infinity: the largest of 8,
 // and the least but for zeros, less 1 (none: 0xffff). Floats of the numbers go
@@ -161,13 +89,6 @@ __device__ __forceinline__ bool plain_range(float low, float high) {
   constexpr int ONE = 15 - __builtin_ctz(F::DV);  // the exponent's bits of 1 / DV
   return high < (float)((ONE + 2) << 10) && low >= (float)(((ONE - 8) << 10) - 1);
 }
-// Whether a lane's 8 scales of a group of 32 dims (the group's 64 in 8 aligned
-// lanes) leave the group to the packed products.
-template <typename F>
-__device__ __forceinline__ bool plain_scales(u32x4 sc) {
-  return plain_range<F>(-group_max<8>(-low_bits(sc)), group_max<8>(high_bits(sc)));
-}
-
 // The scales of a lane's cells (32 h + 8 quad + e) of one block of 32 dims, those
 // of cells that word leaves out as zeros.
 __device__ __forceinline__ void seen_scales(u32x4 &s0, u32x4 &s1, uint64_t word) {
@@ -202,46 +123,6 @@ __device__ __forceinline__ void packed_pdv(H ph, H pl, H dv, H &hi, H &lo) {
   hi = ph * dv;
   lo = __builtin_elementwise_fma(pl, dv, __builtin_elementwise_fma(ph, dv, -hi));
 }
-// P of the cells 32 h + 8 quad + e, QP times as large.
-__device__ __forceinline__ void split_p(const f32x4 (&st)[4], int h, f16x8 &hi, f16x8 &lo) {
-#pragma unroll
-  for (int e = 0; e < 8; e += 2) {
-    const f32x4 &s = st[2 * h + (e >> 2)];
-    f16x2 a, b;
-    split2(s[e & 3] * QP, s[(e & 3) + 1] * QP, a, b);
-    hi[e] = a[0];
-    hi[e + 1] = a[1];
-    lo[e] = b[0];
-    lo[e + 1] = b[1];
-  }
-}
-// P dv of those cells times up, or (MASKED) of a plain row as the packed products
-// make it. (What other calls make alike is not held for this one: the copies are
-// opaque.)
-template <typename F, bool MASKED>
-__device__ __forceinline__ void weigh_p(const f32x4 (&st)[4], int h, f16x8 dv, bool plain, float up, f16x8 &hi,
-                                        f16x8 &lo) {
-  float qp = QP;
-  asm volatile("" : "+s"(qp), "+v"(dv));
-#pragma unroll
-  for (int e = 0; e < 8; e += 2) {
-    const float p0 = st[2 * h + (e >> 2)][e & 3], p1 = st[2 * h + (e >> 2)][(e & 3) + 1];
-    f16x2 a, b;
-    split2(p0 * (float)dv[e] * up, p1 * (float)dv[e + 1] * up, a, b);
-    if constexpr (MASKED) {
-      f16x2 c, d, ph, pl;
-      split2(p0 * qp, p1 * qp, ph, pl);
-      packed_pdv(ph, pl, f16x2{dv[e], dv[e + 1]} * (f16)(float)F::DV, c, d);
-      a = plain ? c : a;
-      b = plain ? d : b;
-    }
-    hi[e] = a[0];
-    hi[e + 1] = a[1];
-    lo[e] = b[0];
-    lo[e + 1] = b[1];
-  }
-}
-
 // S^T of a block: read(b, p, k, d) gives the K operands of tiles 2 p and 2 p + 1
 // and the lane's cells' dk for block b of dims, query(b, hi, lo) the row's. A step
 // reads the next step's operands and issues this one's products, and adds the
@@ -280,105 +161,6 @@ __device__ __forceinline__ void scores_q(f32x4 (&st)[4], R read, Q query) {
   add(1);
 }
 
-// V's scales as the packed products take them.
-template <typename F>
-__device__ __forceinline__ u32x4 times_dv(u32x4 s) {
-  if (F::DV == 1) return s;
-  f16x8 v = __builtin_bit_cast(f16x8, s);
-  v *= (f16)(float)F::DV;
-  return __builtin_bit_cast(u32x4, v);
-}
-
-// O^T += V^T (P dv)^T over a block. scale(b, h): the lane's cells' dv; frag(t, kc):
-// V's operand. plain (the same for the wave): plain_scales of all the block's cells,
-// whose scales are F::DV times as large here. Which way a row's part is made goes
-// by the scales of the cells it sees, and by nothing else, so that a row has the
-// same bits in any group of rows: in a plain block all its rows' cells are plain.
-template <typename F, typename S, typename V>
-__device__ __forceinline__ void values_q(f32x4 (&o)[F::D / 16], const f32x4 (&st)[4], bool plain,
-                                          bool masked, uint64_t word, S scale, V frag) {
-  constexpr int D = F::D, NB = D / 32;
-  if (plain) {
-    // a step reads the next 16 dims' V (and makes the next block's P dv) while
-    // the products of this one run
-    f16x8 ph[2], pl[2], hi[2], lo[2], v[2][2];
-    split_p(st, 0, ph[0], pl[0]);
-    split_p(st, 1, ph[1], pl[1]);
-    auto fetch = [&](int t) {
-#pragma unroll
-      for (int kc = 0; kc < 2; kc++) v[t & 1][kc] = frag(t, kc);
-    };
-    auto weigh = [&](int b) {
-#pragma unroll
-      for (int h = 0; h < 2; h++) packed_pdv(ph[h], pl[h], __builtin_bit_cast(f16x8, scale(b, h)), hi[h], lo[h]);
-    };
-    fetch(0);
-    weigh(0);
-    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int t = 0; t < D / 16; t++) {
-#pragma unroll
-      for (int kc = 0; kc < 2; kc++) {
-        o[t] = mfma16q(v[t & 1][kc], hi[kc], o[t]);
-        o[t] = mfma16q(v[t & 1][kc], lo[kc], o[t]);
-      }
-      if (t + 1 < D / 16) fetch(t + 1);
-      if (t % 2 == 1 && t / 2 + 1 < NB) weigh(t / 2 + 1);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    return;
-  }
-  auto weighed = [&](auto some_hidden, bool row_plain) __attribute__((always_inline)) {
-    constexpr bool MASKED = decltype(some_hidden)::value;
-#pragma unroll
-    for (int b = 0; b < NB; b++) {
-      u32x4 s0 = scale(b, 0), s1 = scale(b, 1);
-      if constexpr (MASKED) seen_scales(s0, s1, word);
-      const f16x8 dv[2] = {__builtin_bit_cast(f16x8, s0), __builtin_bit_cast(f16x8, s1)};
-      const int ex = largest_pdv(st, dv);
-      const float up = pow2(15 - ex), back = QP * F::DV * pow2(ex - 15);
-      f32x4 acc[2];
-#pragma unroll
-      for (int t = 0; t < 2; t++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) acc[t][i] = row_plain ? o[2 * b + t][i] : 0.0f;
-#pragma unroll
-      for (int h = 0; h < 2; h++) {
-        f16x8 hi, lo;
-        weigh_p<F, MASKED>(st, h, dv[h], row_plain, up, hi, lo);
-#pragma unroll
-        for (int t = 0; t < 2; t++) {
-          const f16x8 v = frag(2 * b + t, h);
-          acc[t] = mfma16q(v, hi, acc[t]);
-          acc[t] = mfma16q(v, lo, acc[t]);
-        }
-      }
-#pragma unroll
-      for (int t = 0; t < 2; t++) {
-        f32x4 &ot = o[2 * b + t];
-#pragma unroll
-        for (int i = 0; i < 4; i++) ot[i] = row_plain ? acc[t][i] : fmaf(acc[t][i], back, ot[i]);
-        here(ot);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-    }
-  };
-  if (!masked) {  // wave-uniform: all rows see all of the block, none is plain
-    weighed(std::false_type{}, false);
-    return;
-  }
-  // each row takes its own way
-  float low = 65535.0f, high = 0.0f;
-#pragma unroll 1
-  for (int b = 0; b < NB; b++) {
-    u32x4 s0 = scale(b, 0), s1 = scale(b, 1);
-    seen_scales(s0, s1, word);
-    low = fminf(low, fminf(low_bits(s0), low_bits(s1)));
-    high = fmaxf(high, fmaxf(high_bits(s0), high_bits(s1)));
-  }
-  weighed(std::true_type{}, plain_range<F>(-quads_max(-low), quads_max(high)));
-}
-
 // A lane's row of an item: its token of the item, its head among the G (1, 2, 4, 8
 // or 16) of the KV head, and whether the item has it.
 struct RowOf {
@@ -395,6 +177,11 @@ struct Sight {
   int b_tree;
   int G, ntok;
   const uint64_t *vis;  // the mask words of the item's first token
+  Sight() = default;
+  __device__ __forceinline__ Sight(int seq_off, int npast, int tok0, int n, int G, int ring, int window,
+                                   const uint64_t *vis)
+      : ring(ring), window(window), p_first(npast + (tok0 - seq_off)), p_last(p_first + n - 1), b_tree(npast / KV_BLOCK),
+        G(G), ntok(n), vis(ring < 0 ? vis + (int64_t)tok0 * window : nullptr) {}
   // Whether some row of the item does not see all of a block (the same for the
   // wave, and for every plan that shows the rows the same cells), and the lane's
   // row's word then (0 of a row that the item does not have).
