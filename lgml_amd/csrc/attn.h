@@ -224,6 +224,9 @@ inline const uint64_t *plan_vis(const lgmlh_ubatch *ub) {
 // that leave partial states of the same form.
 void merge_dev(int head_dim, const lgmlh_ubatch *ub, int H, int Hkv, const float *part, float *out,
                f16 *planes, int64_t npad, int xf, hipStream_t st);
+// The same with many splits merged in slices side by side (heads of 64, 128 and 256).
+void merge_slices_dev(int head_dim, const lgmlh_ubatch *ub, int H, int Hkv, const float *part, float *out,
+                      f16 *planes, int64_t npad, int xf, hipStream_t st);
 bool attn_q8k_fits(int head_dim, int G);
 int attn_check(const char *what, const float *q, int n_head, int n_head_kv, int head_dim,
                const void *kpool, const void *vpool, const lgmlh_ubatch *ub, const float *out,

@@ -578,13 +578,18 @@ paged_attn_shared_kernel(const float *__restrict__ q, int H, int Hkv, float scal
 // of a row agree), adding the outputs weighted, in split order. A merge of
 // up to SC splits is one round trip; with 4 or fewer SC is 4, else 16 (the loads
 // past the last split repeat it).
-constexpr int MERGE_THREADS = 256;
-template <int D, int SC>
+// SPREAD (Q4_0 pools): the positions are gridDim.z workgroups', one a thread; SLICES > 1
+// (more than 16 splits): a wave's positions, their splits in as many runs, a wave each,
+// with a maximum of its own as it goes (one round trip per SC splits), and the runs join
+// in order. A step of 4 sequences at 32768 to 131072 cells, 32 / 4 heads of 128, 43 to 171
+// splits: 9 us, where one workgroup for all positions and splits took 24.
+constexpr int MERGE_THREADS = 256, MERGE_SLICES = 4;
+template <int D, int SC, bool SPREAD = false, int SLICES = 1>
 __device__ __forceinline__ void merge_group(const int32_t *__restrict__ merge, int H, int Hkv,
                                             const float *__restrict__ part, float *__restrict__ out,
                                             f16 *__restrict__ planes, int64_t npad, int xf) {
-  constexpr int MT = MERGE_THREADS;
-  const int tid = threadIdx.x, lane = tid & 63, mg = blockIdx.x, kvh = blockIdx.y;
+  constexpr int MT = MERGE_THREADS / SLICES, NJ = SPREAD ? 1 : 4;
+  const int tid = SLICES > 1 ? threadIdx.x % MT : threadIdx.x, lane = tid & 63, mg = blockIdx.x, kvh = blockIdx.y;
   const int first = merge[4 * mg + 0], ns = merge[4 * mg + 1];
   const int tok0 = merge[4 * mg + 2], ntok = merge[4 * mg + 3] & 0xff;
   const int stride = merge[4 * mg + 3] >> 8;  // items from one split to the next
@@ -593,13 +598,14 @@ __device__ __forceinline__ void merge_group(const int32_t *__restrict__ merge, i
   const int64_t pstride = (int64_t)stride * Hkv * Partial<D>::floats;
   const float *ml = p0 + ROWS * D;  // m of row r at ml[r], l at ml[ROWS + r]
   const int n4 = nrows * (D / 4);
-  for (int base = 0; base < n4; base += 4 * MT) {
-    const int nj = min(4, (n4 - base + MT - 1) / MT);  // workgroup-uniform
-    int rr[4], dd[4];
-    f32x4 acc[4];
-    float M[4], L[4];
+  const int base0 = SPREAD ? blockIdx.z * MT : 0;
+  for (int base = base0; base < n4; base += SPREAD ? gridDim.z * MT : NJ * MT) {
+    const int nj = min(NJ, (n4 - base + MT - 1) / MT);  // workgroup-uniform
+    int rr[NJ], dd[NJ];
+    f32x4 acc[NJ];
+    float M[NJ], L[NJ];
 #pragma unroll
-    for (int jj = 0; jj < 4; jj++) {
+    for (int jj = 0; jj < NJ; jj++) {
       const int e4 = min(base + tid + MT * jj, n4 - 1);
       rr[jj] = e4 / (D / 4);
       dd[jj] = 4 * (e4 % (D / 4));
@@ -607,46 +613,96 @@ __device__ __forceinline__ void merge_group(const int32_t *__restrict__ merge, i
       M[jj] = -INFINITY;
       L[jj] = 0.0f;
     }
-    // More than SC splits: the maxima first, over every split's m.
-    if (ns > SC)
+    if constexpr (SLICES > 1) {
+      __shared__ f32x4 slice_acc[SLICES - 1][MT];
+      __shared__ float slice_m[SLICES - 1][MT], slice_l[SLICES - 1][MT];
+      const int slice = threadIdx.x / MT, run = (ns + SLICES - 1) / SLICES;
+      const int last = min(ns, (slice + 1) * run);
+      for (int s0 = slice * run; s0 < last; s0 += SC) {
+        f32x4 a[SC];
+        float mv[SC], lv[SC];
+#pragma unroll
+        for (int i = 0; i < SC; i++) {
+          const int64_t o = (int64_t)min(s0 + i, last - 1) * pstride;
+          a[i] = *(const f32x4 *)(p0 + o + rr[0] * D + dd[0]);
+          mv[i] = ml[o + rr[0]];
+          lv[i] = ml[o + ROWS + rr[0]];
+        }
+        float top = M[0];
+#pragma unroll
+        for (int i = 0; i < SC; i++) top = fmaxf(top, mv[i]);
+        if (top == -INFINITY) continue;  // splits that saw no cell
+        const float w = exp2f(M[0] - top);
+        L[0] *= w;
+        acc[0] *= w;
+#pragma unroll
+        for (int i = 0; i < SC; i++)
+          if (s0 + i < last) {
+            const float w = exp2f(mv[i] - top);
+            L[0] += lv[i] * w;
+            acc[0] += a[i] * w;
+          }
+        M[0] = top;
+      }
+      if (base > base0) __syncthreads();  // the last positions' are read
+      if (slice > 0) {
+        slice_acc[slice - 1][tid] = acc[0];
+        slice_m[slice - 1][tid] = M[0];
+        slice_l[slice - 1][tid] = L[0];
+      }
+      __syncthreads();
+      if (slice > 0) continue;
+#pragma unroll
+      for (int i = 0; i < SLICES - 1; i++) {
+        const float m = slice_m[i][tid], top = fmaxf(M[0], m);
+        if (top == -INFINITY) continue;
+        const float w = exp2f(M[0] - top), w1 = exp2f(m - top);
+        L[0] = L[0] * w + slice_l[i][tid] * w1;
+        acc[0] = acc[0] * w + slice_acc[i][tid] * w1;
+        M[0] = top;
+      }
+    } else {
+      // More than SC splits: the maxima first, over every split's m.
+      if (ns > SC)
+        for (int s0 = 0; s0 < ns; s0 += SC) {
+#pragma unroll
+          for (int jj = 0; jj < 4; jj++)
+            if (jj < nj) {
+              float mv[SC];
+#pragma unroll
+              for (int i = 0; i < SC; i++) mv[i] = ml[(int64_t)min(s0 + i, ns - 1) * pstride + rr[jj]];
+#pragma unroll
+              for (int i = 0; i < SC; i++) M[jj] = fmaxf(M[jj], mv[i]);  // repeats: same max
+            }
+        }
       for (int s0 = 0; s0 < ns; s0 += SC) {
 #pragma unroll
         for (int jj = 0; jj < 4; jj++)
           if (jj < nj) {
-            float mv[SC];
+            f32x4 a[SC];
+            float mv[SC], lv[SC];
 #pragma unroll
-            for (int i = 0; i < SC; i++) mv[i] = ml[(int64_t)min(s0 + i, ns - 1) * pstride + rr[jj]];
+            for (int i = 0; i < SC; i++) {
+              const int64_t o = (int64_t)min(s0 + i, ns - 1) * pstride;
+              a[i] = *(const f32x4 *)(p0 + o + rr[jj] * D + dd[jj]);
+              mv[i] = ml[o + rr[jj]];
+              lv[i] = ml[o + ROWS + rr[jj]];
+            }
+            if (ns <= SC)
 #pragma unroll
-            for (int i = 0; i < SC; i++) M[jj] = fmaxf(M[jj], mv[i]);  // repeats: same max
+              for (int i = 0; i < SC; i++) M[jj] = fmaxf(M[jj], mv[i]);
+#pragma unroll
+            for (int i = 0; i < SC; i++)
+              if (s0 + i < ns) {
+                const float w = exp2f(mv[i] - M[jj]);  // 0 for a split that saw no cell
+                L[jj] += lv[i] * w;
+                acc[jj] += a[i] * w;
+              }
           }
       }
-    for (int s0 = 0; s0 < ns; s0 += SC) {
-#pragma unroll
-      for (int jj = 0; jj < 4; jj++)
-        if (jj < nj) {
-          f32x4 a[SC];
-          float mv[SC], lv[SC];
-#pragma unroll
-          for (int i = 0; i < SC; i++) {
-            const int64_t o = (int64_t)min(s0 + i, ns - 1) * pstride;
-            a[i] = *(const f32x4 *)(p0 + o + rr[jj] * D + dd[jj]);
-            mv[i] = ml[o + rr[jj]];
-            lv[i] = ml[o + ROWS + rr[jj]];
-          }
-          if (ns <= SC)
-#pragma unroll
-            for (int i = 0; i < SC; i++) M[jj] = fmaxf(M[jj], mv[i]);
-#pragma unroll
-          for (int i = 0; i < SC; i++)
-            if (s0 + i < ns) {
-              const float w = exp2f(mv[i] - M[jj]);  // 0 for a split that saw no cell
-              L[jj] += lv[i] * w;
-              acc[jj] += a[i] * w;
-            }
-        }
     }
 #pragma unroll
-    for (int jj = 0; jj < 4; jj++) {
+    for (int jj = 0; jj < NJ; jj++) {
       const int e4 = base + tid + MT * jj;
       // groups of 8 lanes (D / 4 is a multiple of 8) leave together, and
       // whole waves where a wave holds a Q8_K block (n4 a multiple of 64)
@@ -719,6 +775,18 @@ merge_kernel(const int32_t *__restrict__ merge, int H, int Hkv, const float *__r
   else
     merge_group<D, 16>(merge, H, Hkv, part, out, planes, npad, xf);
 }
+template <int D>
+__global__ void __launch_bounds__(MERGE_THREADS)
+merge_slices_kernel(const int32_t *__restrict__ merge, int H, int Hkv, const float *__restrict__ part,
+                    float *__restrict__ out, f16 *__restrict__ planes, int64_t npad, int xf) {
+  const int ns = merge[4 * blockIdx.x + 1];
+  if (ns <= 4)
+    merge_group<D, 4, true>(merge, H, Hkv, part, out, planes, npad, xf);
+  else if (ns <= 16)
+    merge_group<D, 16, true>(merge, H, Hkv, part, out, planes, npad, xf);
+  else
+    merge_group<D, 16, true, MERGE_SLICES>(merge, H, Hkv, part, out, planes, npad, xf);
+}
 
 }  // namespace lgmlh
 
@@ -734,6 +802,16 @@ static void launch_merge(const lgmlh_ubatch *ub, int H, int Hkv, const float *pa
                          f16 *planes, int64_t npad, int xf, hipStream_t st) {
   hipLaunchKernelGGL(merge_kernel<D>, dim3(ub->n_merge, Hkv), dim3(MERGE_THREADS), 0, st, ub->merge,
                      H, Hkv, part, out, planes, npad, xf);
+}
+
+void lgmlh::merge_slices_dev(int head_dim, const lgmlh_ubatch *ub, int H, int Hkv, const float *part,
+                             float *out, f16 *planes, int64_t npad, int xf, hipStream_t st) {
+  if (ub->n_merge <= 0) return;
+  const auto kern = head_dim == 64 ? merge_slices_kernel<64> : head_dim == 128 ? merge_slices_kernel<128>
+                                                                               : merge_slices_kernel<256>;
+  // (for 8 rows' positions in slices in one turn; other groups' are a half of that)
+  hipLaunchKernelGGL(kern, dim3(ub->n_merge, Hkv, head_dim / 32), dim3(MERGE_THREADS), 0, st, ub->merge, H, Hkv, part, out,
+                     planes, npad, xf);
 }
 
 void lgmlh::merge_dev(int head_dim, const lgmlh_ubatch *ub, int H, int Hkv, const float *part,

@@ -462,7 +462,7 @@ static void launch_attn_q4(const float *q, int H, int Hkv, float scale_log2, con
                        scale_log2, (const uint8_t *)kp, (const uint8_t *)vp, ub->items, ub->seq_off, ub->seq_npast,
                        ub->block_tab, ub->max_blocks, ub->ring, ub->window, out, planes, npad, xf, part, ub->order,
                        ub->order ? ub->n_single : 0, vis);
-  merge_dev(D, ub, H, Hkv, part, out, planes, npad, xf, st);
+  merge_slices_dev(D, ub, H, Hkv, part, out, planes, npad, xf, st);
 }
 
 // paged_attention_dev over Q4_0 pools.

@@ -256,6 +256,18 @@ def test_causal_attention(L, H, kv, D, seq_n, npast, bps):
     check_attention(L, H, kv, D, seq_n, npast, None, bps, 11)
 
 
+@pytest.mark.parametrize("H,kv,D", [(8, 2, 64), (16, 2, 128), (8, 8, 128), (8, 4, 256)])
+@pytest.mark.parametrize("is_tree", [False, True])
+def test_many_splits(L, H, kv, D, is_tree):
+    """Groups of 4 splits, 5, 16, 17 and more, of one row to sixteen, alone and together;
+    in the tree, rows that see nothing of some."""
+    seq_n, npast = [1, 1, 2, 16, 1, 7], [200, 300, 900, 1000, 1087, 4500]
+    rng = np.random.default_rng(37)
+    parents = [[-1] + [int(rng.integers(0, j)) for j in range(1, n)] for n in seq_n] if is_tree else None
+    all_ = check_attention(L, H, kv, D, seq_n, npast, parents, 1, 41)
+    assert np.isfinite(all_).all()
+
+
 @pytest.mark.parametrize("H,kv,D", [(4, 2, 64), (16, 8, 128), (8, 4, 256)])
 def test_ring_attention(L, H, kv, D):
     check_attention(L, H, kv, D, [1, 20, 1, 90], [1000, 37, 0, 100], None, 1, 13, window=100, ring=3)
