@@ -178,11 +178,12 @@ int lgmlh_kv_gather_q4(const void *pool, int which, int64_t n_cells, int n_head_
  * Copies of blocks in every layer at once: forks of a sequence, copy-on-write,
  * compaction, cleared blocks. copies (n, 3) i32: {src, dst, cells}, the first
  * `cells` (0 .. 64) cells of block dst become those of block src, or zeros where
- * src is -1; the others of dst stay. A source may serve several targets; a target
- * twice, or one that is a source of the call, is LGMLH_EINVAL (a block outside the
- * pool LGMLH_ERANGE). type LGMLH_F16 (heads of a multiple of 8 up to 1024),
- * LGMLH_Q8_0 or LGMLH_Q4_0; pools as in lgmlh_kv_move, their tensors 16-byte
- * aligned; h_copies is the host copy for the checks.
+ * src is -1; the others of dst stay (they are read and written back: nothing else may
+ * write block dst meanwhile). A source may serve several targets; a target twice, or
+ * one that is a source of the call, is LGMLH_EINVAL (a block outside the pool
+ * LGMLH_ERANGE). type LGMLH_F16 (heads of a multiple of 8 up to 1024), LGMLH_Q8_0 or
+ * LGMLH_Q4_0; pools as in lgmlh_kv_move, their tensors 16-byte aligned; h_copies is
+ * the host copy for the checks.
  * ===================================================================== */
 int lgmlh_kv_copy_blocks(int type, void *const *pools, int n_pools, int64_t n_cells, int n_head_kv,
     int head_dim, const int32_t *copies, const int32_t *h_copies, int64_t n, void *stream);
