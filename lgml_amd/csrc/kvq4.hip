@@ -72,26 +72,33 @@ kv_store_q4_kernel(uint8_t *__restrict__ kp, uint8_t *__restrict__ vp, int64_t n
   }
 }
 
-// Four values of a row: f32 or f16 of (n - 8) d, n the low halves of a word's bytes.
+// 16 bytes of a row, f32 or f16 of (n - 8) d, n the low halves of the bytes of one or two
+// words.
 template <typename OutT>
-__device__ __forceinline__ void put4_q4(OutT *out, uint32_t n, float d) {
-  typedef OutT o4 __attribute__((ext_vector_type(4), aligned(sizeof(OutT))));
-  o4 y;
+struct RowPiece {
+  static constexpr int N = 16 / sizeof(OutT);
+  typedef OutT T __attribute__((ext_vector_type(N), aligned(sizeof(OutT))));
+  T y;
+  __device__ __forceinline__ RowPiece(uint32_t n0, uint32_t n1, float d) {
 #pragma unroll
-  for (int e = 0; e < 4; e++) y[e] = (OutT)(d * ((float)(n >> 8 * e & 15) - 8.0f));
-  *(o4 *)out = y;
-}
+    for (int e = 0; e < N; e++) y[e] = (OutT)(d * ((float)((e < 4 ? n0 : n1) >> 8 * (e & 3) & 15) - 8.0f));
+  }
+};
 
-// K's cells as rows (n, Hkv D): a thread has a cell's 8 dims of U blocks of 32, a
-// load's, and writes them from its registers.
+// K's cells as rows (n, Hkv D): a thread has 16 bytes of a row's, in U blocks of 32 dims,
+// from a load's words (of f32 the low or the high ones' half). The rows pass the caches
+// by, whole 128-byte lines a store. The context of 8 sequences of 4096 tokens, 8 heads of
+// 128, as f16 rows of K and V: 37 us, 4.7 TB/s (cached stores of 8 bytes 49; 16 bytes
+// past the caches, but 32 bytes of a line at a time, took f32 rows longer than cached).
 template <int D, typename OutT>
 __global__ void __launch_bounds__(Q4_THREADS)
 kv_gather_q4_k_kernel(const uint8_t *__restrict__ pool, int64_t n_cells,
                       const int64_t *__restrict__ cells, int64_t n, int Hkv, OutT *__restrict__ out) {
-  constexpr int U = q4_k_words(D), PER = D / (8 * U);  // threads of a cell
+  typedef RowPiece<OutT> Piece;
+  constexpr int N = Piece::N, U = q4_k_words(D), PER = D / (N * U);  // threads of a cell
   const int h = blockIdx.x % (uint32_t)Hkv;
   const int64_t t = (int64_t)(blockIdx.x / (uint32_t)Hkv) * (Q4_THREADS / PER) + threadIdx.x / PER;
-  const int k = threadIdx.x % PER, j = k / 4, q = k % 4;
+  const int k = threadIdx.x % PER, j = k / (32 / N), dim = k % (32 / N) * N;
   if (t >= n) return;
   const int64_t c = cells[t];
   const bool in = (uint64_t)c < (uint64_t)n_cells;
@@ -106,25 +113,25 @@ kv_gather_q4_k_kernel(const uint8_t *__restrict__ pool, int64_t n_cells,
   if (in) {
     const uint8_t *tile = q4_tile<D>(pool + (int64_t)h * q4_tile_bytes(D), c, Hkv);
     typedef uint32_t uU __attribute__((ext_vector_type(U)));
-    const uU r = *(const uU *)(tile + q4_k_at(D, cell, 32 * U * j + 8 * q));
+    const uU r = *(const uU *)(tile + q4_k_at(D, cell, 32 * U * j + dim / 8 * 8));
 #pragma unroll
     for (int u = 0; u < U; u++) {
       w[u] = r[u];
       d[u] = h2f(*(const uint16_t *)(tile + q4_scale_at(D, U * j + u, cell)));
     }
   }
-  OutT *row = out + (t * Hkv + h) * (int64_t)D + 32 * U * j + 8 * q;
+  OutT *row = out + (t * Hkv + h) * (int64_t)D + 32 * U * j + dim;
 #pragma unroll
   for (int u = 0; u < U; u++) {
     // dim e at bits 4 (e / 2) + 16 (e % 2): in order, a byte each
-    uint32_t v[2];
+    uint32_t v[N / 4];
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
-      const uint32_t s = w[u] >> 8 * i;
+    for (int i = 0; i < N / 4; i++) {
+      const uint32_t s = w[u] >> (8 * i + 2 * (dim % 8));
       v[i] = (s & 15) | (s >> 16 & 15) << 8 | (s >> 4 & 15) << 16 | (s >> 20 & 15) << 24;
     }
-    put4_q4(row + 32 * u, v[0], d[u]);
-    put4_q4(row + 32 * u + 4, v[1], d[u]);
+    const Piece y(v[0], v[N / 4 - 1], d[u]);
+    __builtin_nontemporal_store(y.y, (typename Piece::T *)(row + 32 * u));
   }
 }
 
@@ -134,7 +141,8 @@ template <int D, int W, typename OutT>
 __global__ void __launch_bounds__(Q4_THREADS)
 kv_gather_q4_v_kernel(const uint8_t *__restrict__ pool, int64_t n_cells,
                       const int64_t *__restrict__ cells, int64_t n, int Hkv, OutT *__restrict__ out) {
-  constexpr int G4 = D / 8, STEP = Q4_THREADS / G4, PAD = D / 2 + 4;  // 4 bytes, 8 dims a thread
+  typedef RowPiece<OutT> Piece;  // of a thread and step, the halves of N bytes
+  constexpr int N = Piece::N, GN = D / N, STEP = Q4_THREADS / GN, PAD = D / 2 + 4;
   constexpr int ROWS = W + CELL_HALO, NS = W + 8, GROUPS = W / CELL_GROUP;
   __shared__ CellWindow<W> win;
   __shared__ __align__(4) uint8_t turn[ROWS * PAD];
@@ -187,17 +195,16 @@ kv_gather_q4_v_kernel(const uint8_t *__restrict__ pool, int64_t n_cells,
     for (int p = tid >> sh; p < D / 2; p += Q4_THREADS >> sh) turn[t * PAD + p] = tile[64 * p];
   }
   __syncthreads();
-  const int g4 = tid % G4, j = g4 / 4;
+  const int dim = tid % GN * N, j = dim / 32, high = dim / 16 % 2 * 4;  // dims 32 j + 16 of the bytes' high halves
   const int left = n - j0 < ROWS ? (int)(n - j0) : ROWS;
 #pragma unroll 4
-  for (int t = tid / G4; t < left; t += STEP) {
+  for (int t = tid / GN; t < left; t += STEP) {
     if (!mine[t]) continue;
     const bool in = win.cell(t) >= 0;
-    const uint32_t w = in ? *(const uint32_t *)(turn + t * PAD + 4 * g4) : 0;
+    const uint32_t *w = (const uint32_t *)(turn + t * PAD + 16 * j + dim % 16);
     const float d = in ? h2f(scale[j * NS + t]) : 0.0f;
-    OutT *row = out + ((j0 + t) * Hkv + h) * (int64_t)D + 32 * j + g4 % 4 * 4;
-    put4_q4(row, w & 0x0f0f0f0fu, d);
-    put4_q4(row + 16, w >> 4 & 0x0f0f0f0fu, d);
+    const Piece y(in ? w[0] >> high : 0, in && N == 8 ? w[N / 8] >> high : 0, d);
+    __builtin_nontemporal_store(y.y, (typename Piece::T *)(out + ((j0 + t) * Hkv + h) * (int64_t)D + dim));
   }
 }
 
@@ -250,7 +257,7 @@ extern "C" int lgmlh_kv_gather_q4(const void *pool, int which, int64_t n_cells, 
                                   int out_type, void *stream) {
   if (!pool || !cells || !out || n < 0 || (which != 0 && which != 1) || n_cells <= 0 ||
       n_cells > CELLS_MAX || n_cells % KV_BLOCK || n_head_kv <= 0 || n_head_kv > Q4_HEADS ||
-      n >= CELL_ROWS / n_head_kv || !q4_head(head_dim) ||
+      n >= CELL_ROWS / (head_dim == 256 && out_type == LGMLH_F32 ? 2 : 1) / n_head_kv || !q4_head(head_dim) ||
       (out_type != LGMLH_F32 && out_type != LGMLH_F16)) {
     set_error("kv_gather_q4: bad arguments (heads of 64, 128 or 256; out f32 or f16)");
     return LGMLH_EINVAL;
@@ -273,7 +280,7 @@ extern "C" int lgmlh_kv_gather_q4(const void *pool, int which, int64_t n_cells, 
       if (which)
         small ? launch(kv_gather_q4_v_kernel<D, 16, T>, 16) : launch(kv_gather_q4_v_kernel<D, big, T>, big);
       else
-        launch(kv_gather_q4_k_kernel<D, T>, Q4_THREADS * 8 * q4_k_words(D) / D);
+        launch(kv_gather_q4_k_kernel<D, T>, Q4_THREADS * (16 / (int)sizeof(T)) * q4_k_words(D) / D);
     };
     if (head_dim == 64)
       of(std::integral_constant<int, 64>{});
