@@ -49,7 +49,8 @@ __device__ __forceinline__ void wave_lds() { asm volatile("s_waitcnt lgkmcnt(0)"
 // lane: lane l of a head's D / 8 has the pairs from 4 l on (4 dims of each half), or
 // 8 dims behind the rotated ones. The token's angles are made once, a thread each,
 // while the rows of STEPS steps are on their way. K rows turn in LDS into 8 dims in a
-// row a lane, as they are stored.
+// row a lane, as they are stored. q's rows pass the caches by: 4096 tokens of 32 / 4
+// heads of 128, 159 MB, take 31 us, 5.1 TB/s, with cached stores 34; 64 tokens 5 either way.
 constexpr int AXES_STEPS = 4;
 template <int TYPE, int D>
 __device__ __forceinline__ void turn_heads(const float *__restrict__ qkv, int64_t n, int H, int Hkv, const AxesRope &r,
@@ -120,8 +121,8 @@ __device__ __forceinline__ void turn_heads(const float *__restrict__ qkv, int64_
       }
       if (has && !is_k) {
         float *out = q_out + (t * H + h) * (int64_t)D;
-        *(f32x4_u *)(out + at0) = x;
-        *(f32x4_u *)(out + at1) = y;
+        __builtin_nontemporal_store(x, (f32x4_u *)(out + at0));
+        __builtin_nontemporal_store(y, (f32x4_u *)(out + at1));
       }
       if (h0 + AT <= H) continue;  // the same for the wave: q heads alone
       float *mine = rows[wave] + lane / L * D;
