@@ -150,15 +150,17 @@ class PoolSeqs:
         m = self.model
         if src == dst or n == 0:
             return
-        if m.kv_type != hip.F16 or not torch.cuda.is_current_stream_capturing():
+        kv_type = getattr(m, "kv_type", hip.F16)
+        if kv_type != hip.F16 or hasattr(m, "copy_blocks") and not torch.cuda.is_current_stream_capturing():
             m.copy_blocks([src], [dst], n)
             return
         # under capture: the f16 copy whose blocks are the launch's own arguments
-        D, Hkv = m.paged_dims
+        D, Hkv = getattr(m, "paged_dims", (m.hp["head_dim"], m.hp["n_head_kv"]))
         for il, (kp, vp) in enumerate(zip(m.kpools, m.vpools)):
-            if not m.swa[il]:  # ring pools hold no pool blocks
-                check(hip.lib().lgmlh_kv_copy_block(kp.data_ptr(), vp.data_ptr(), m.n_cells, Hkv, D,
-                                                    src, dst, n, stream()))
+            if getattr(m, "swa", None) and m.swa[il]:
+                continue  # ring pools hold no pool blocks
+            check(hip.lib().lgmlh_kv_copy_block(kp.data_ptr(), vp.data_ptr(), m.n_cells, Hkv, D,
+                                                src, dst, n, stream()))
 
     def truncate(self, c, n):
         """transformer.lua:1084-1108."""
