@@ -19,6 +19,15 @@
 // for a set's eight waves in LDS, as Q8_0's are, they were slower at every size: heads of
 // 128, 32 / 8, 512 tokens after 2048 cells 110 us against 95, 4096 from none 639 against
 // 583; heads of 256, 8 / 4, 133 against 55 and 318 against 288.
+//
+// Bounds. One token of 64 sequences at 128 to 4096 cells, 32 / 8 heads of 128, is 48 to 51
+// + 5 us: 159 MB, 3.2 TB/s. A block of 64 cells is 650 vector operations a wave (288 of
+// them the unpacking; a decode step's 4 rows use a quarter of the columns of the others),
+// which take the three waves of a SIMD 3.8 us, its bytes of all the waves 5.6 at the
+// copy's rate; a workgroup of 12 blocks starts with 4 us until its first bytes are there,
+// and the 1688 workgroups of the step are 2.2 times what the card holds. A chunk of 512
+// tokens after 2048, 8 / 4 heads of 256, is 51 + 5 us, half of them vector operations of
+// its 2048 waves, two a SIMD.
 #include "attnq.h"
 #include "kvq4.h"
 

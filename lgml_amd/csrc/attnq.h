@@ -1,6 +1,6 @@
 // What the attention kernels over quantised KV blocks share (formats of an f16 scale
-// per 32 values): q, P and V's scales as f16 halves, the softmax, the products of a
-// block. F is the format: its head size D, and DV, the factor of V's scales in the
+// per 32 values): the arithmetic, scores, V's scales and P dv, and what the rows of an
+// item see of a block. F is the format: its head size D, and DV, the factor of V's scales in the
 // packed products.
 //
 // s_rc = q_r . k_c = sum_b dk_cb (q_rb . kn_cb) over the blocks b of 32 dims: the
@@ -9,7 +9,7 @@
 // S^T. q rows are scaled by a power of two to just below 2^15, so that hi + lo
 // carries 22 bits of every element down to 2^-17 of the row's largest.
 // o_rd = sum_c (p_rc dv_cb) vn_cd, b = d / 32: dv goes into P, per block of 32
-// dims, and P dv enters the MFMAs as f16 hi + lo; O and l are QP DV times as large.
+// dims, and P dv enters the MFMAs as f16 hi + lo; O and l are 2^13 DV times as large.
 // Where each dv that a row sees of the block is 0 or in [2^-8, 2^2) / DV (largest
 // values of 0.03 to 31), P is split once and multiplied by DV dv in packed f16,
 // the product's rounding caught by an fma: hi = P_hi dv, lo = P_lo dv + (P_hi dv -
@@ -42,8 +42,7 @@ __device__ __forceinline__ void here(f32x4 &v) { asm volatile("" : "+v"(v)); }
 __device__ __forceinline__ float pow2(int e) { return __builtin_amdgcn_ldexpf(1.0f, e); }
 
 // The largest v of a row's four quads: lanes 16, then 32 apart change places on
-// the vector ALU (a shuffle goes through the LDS unit, which the shared kernel's
-// operands fill).
+// the vector ALU (a shuffle goes through the LDS unit, which operands fill).
 __device__ __forceinline__ float quads_max(float v) {
   const uint32_t a = __builtin_bit_cast(uint32_t, v);
   const auto p = __builtin_amdgcn_permlane16_swap(a, a, false, false);

@@ -50,7 +50,7 @@ __device__ __forceinline__ void wave_lds() { asm volatile("s_waitcnt lgkmcnt(0)"
 // 8 dims behind the rotated ones. The token's angles are made once, a thread each,
 // while the rows of STEPS steps are on their way. K rows turn in LDS into 8 dims in a
 // row a lane, as they are stored. q's rows pass the caches by: 4096 tokens of 32 / 4
-// heads of 128, 159 MB, take 31 us, 5.1 TB/s, with cached stores 34; 64 tokens 5 either way.
+// heads of 128, 159 MB, take 28 us, 5.6 TB/s, with cached stores 31; 64 tokens 5 either way.
 constexpr int AXES_STEPS = 4;
 template <int TYPE, int D>
 __device__ __forceinline__ void turn_heads(const float *__restrict__ qkv, int64_t n, int H, int Hkv, const AxesRope &r,
@@ -229,6 +229,8 @@ extern "C" int lgmlh_qkv_rope_store_axes(int kv_type, const float *qkv, int64_t 
   r.log2_step = -2.0 / n_rot * log2((double)freq_base);
   r.ff = freq_factors;
   r.pos = pos;
+  // (V's tokens of a workgroup: 64 tokens of 32 / 8 heads of 128 take 5.3 us with
+  // 16, 8.5 with 64; 4096 of 32 / 4 heads 29.2 and 28.4)
   const int big = D > 128 ? 32 : 64;
   const bool small = (n + big - 1) / big * n_head_kv < 256;
   const int w = small ? 16 : big;
