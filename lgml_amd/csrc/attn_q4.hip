@@ -20,13 +20,13 @@
 // 128, 32 / 8, 512 tokens after 2048 cells 110 us against 95, 4096 from none 639 against
 // 583; heads of 256, 8 / 4, 133 against 55 and 318 against 288.
 //
-// Bounds. One token of 64 sequences at 128 to 4096 cells, 32 / 8 heads of 128, is 48 to 51
-// + 5 us: 159 MB, 3.2 TB/s. A block of 64 cells is 650 vector operations a wave (288 of
+// Bounds. One token of 64 sequences at 128 to 4096 cells, 32 / 8 heads of 128, is 45 to 47
+// + 5 us: 159 MB, 3.5 TB/s (34 with the loads alone). A block of 64 cells is 650 vector operations a wave (288 of
 // them the unpacking; a decode step's 4 rows use a quarter of the columns of the others),
 // which take the three waves of a SIMD 3.8 us, its bytes of all the waves 5.6 at the
 // copy's rate; a workgroup of 12 blocks starts with 4 us until its first bytes are there,
 // and the 1688 workgroups of the step are 2.2 times what the card holds. A chunk of 512
-// tokens after 2048, 8 / 4 heads of 256, is 51 + 5 us, half of them vector operations of
+// tokens after 2048, 8 / 4 heads of 256, is 50 + 5 us, half of them vector operations of
 // its 2048 waves, two a SIMD.
 #include "attnq.h"
 #include "kvq4.h"
@@ -324,9 +324,9 @@ __device__ __forceinline__ bool plain_lane(u32x4 sc) {
   return plain_range<F>(low_bits(sc), high_bits(sc));
 }
 
-// An item: a workgroup, a wave each part. Each wave reads its blocks from the
-// pool into registers, the next while one is used; q's operands are in LDS, made once,
-// and the states join there. Items first_item + blockIdx.x / Hkv, or by order.
+// An item: a workgroup, a wave each part. Each wave reads its blocks from the pool into
+// registers, the next one's K and scales while one is used; q's operands are in LDS, made
+// once, and the states join there.
 template <int D>
 __global__ void __launch_bounds__(64 * PARTS, D == 256 ? 2 : 3)
 paged_attn_q4_kernel(const float *__restrict__ q, int H, int Hkv, float scale_log2,
@@ -402,7 +402,6 @@ paged_attn_q4_kernel(const float *__restrict__ q, int H, int Hkv, float scale_lo
     if (lo < hi) {
       load_s(lo);
       load_k(lo);
-      load_v(lo);
     }
     up = split_q4<NB>(qa, r.valid, scale_log2, [&](int b, f16x8 h, f16x8 l) {
       qsh[b * 64 + lane] = h;
@@ -423,6 +422,7 @@ paged_attn_q4_kernel(const float *__restrict__ q, int H, int Hkv, float scale_lo
                                                     (SR == 2 || (lane >= SL && lane < 2 * SL)));
     if (SR == 2) scl[lane] = sreg[0];
     if (SR == 2 || lane < 2 * SL) scl[(SR - 1) * 64 + lane] = sreg[SR - 1];
+    load_v(blk);  // (with the next block's K it kept that waiting: 64 sequences' step 56 us, so 52)
     if (more) load_s(blk + PARTS);
     scores_q<NB>(
         st,
@@ -442,7 +442,6 @@ paged_attn_q4_kernel(const float *__restrict__ q, int H, int Hkv, float scale_lo
     __builtin_amdgcn_sched_barrier(0);
     values_q4<F>(s, st, plain, word, [&](int b, int h) { return scale_of(1, b, h); },
                  [&](int t, int kc) { return F::v_frag(nib, vq, t, kc); });
-    if (more) load_v(blk + PARTS);
   }
   s.finish();
   if (wave > 0) {
