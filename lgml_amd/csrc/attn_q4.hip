@@ -20,11 +20,11 @@
 // 128, 32 / 8, 512 tokens after 2048 cells 110 us against 95, 4096 from none 639 against
 // 583; heads of 256, 8 / 4, 133 against 55 and 318 against 288.
 //
-// Bounds. One token of 64 sequences at 128 to 4096 cells, 32 / 8 heads of 128, is 45 to 47
-// + 5 us: 159 MB, 3.5 TB/s (34 with the loads alone). A block of 64 cells is 650 vector operations a wave (288 of
-// them the unpacking; a decode step's 4 rows use a quarter of the columns of the others),
-// which take the three waves of a SIMD 3.8 us, its bytes of all the waves 5.6 at the
-// copy's rate; a workgroup of 12 blocks starts with 4 us until its first bytes are there,
+// Bounds. One token of 64 sequences at 128 to 4096 cells, 32 / 8 heads of 128, is 43 to 45
+// + 5 us: 159 MB, 3.6 TB/s (34 us with the loads alone). A block of 64 cells is 650 vector
+// operations a wave (288 of them the unpacking; a decode step's 4 rows use a quarter of the
+// columns of the others), which take the three waves of a SIMD 3.8 us, its bytes of all the
+// waves 5.6 at the copy's rate; a workgroup of 12 blocks starts with 4 us until its first bytes are there,
 // and the 1688 workgroups of the step are 2.2 times what the card holds. A chunk of 512
 // tokens after 2048, 8 / 4 heads of 256, is 50 + 5 us, half of them vector operations of
 // its 2048 waves, two a SIMD.
@@ -326,8 +326,10 @@ __device__ __forceinline__ bool plain_lane(u32x4 sc) {
 
 // An item: a workgroup, a wave each part. Each wave reads its blocks from the pool into
 // registers, the next one's K and scales while one is used; q's operands are in LDS, made
-// once, and the states join there.
-template <int D>
+// once, and the states join there. ONCE (plans without shared sets): values are read past
+// the caches. The step of 64 sequences takes 51 us so, 53 through them; a chunk, whose
+// items read the same blocks, 52 and 50.
+template <int D, bool ONCE>
 __global__ void __launch_bounds__(64 * PARTS, D == 256 ? 2 : 3)
 paged_attn_q4_kernel(const float *__restrict__ q, int H, int Hkv, float scale_log2,
                      const uint8_t *__restrict__ kpool, const uint8_t *__restrict__ vpool,
@@ -362,18 +364,19 @@ paged_attn_q4_kernel(const float *__restrict__ q, int H, int Hkv, float scale_lo
   u32x4 vq[F::VJ], sreg[SR];
   constexpr int KC = 4 * sizeof(typename F::KUnit);  // bytes of a cell's units
   const uint32_t koff = (8 * (row >> 2) + (row & 3)) * KC + quad * (KC / 4), voff = row * 64 + quad * 16;
+  auto read = [](auto *from) { return ONCE ? __builtin_nontemporal_load(from) : *from; };
   auto load_k = [&](int blk) {
     const uint8_t *t = tile(kpool, blk);
 #pragma unroll
     for (int ct = 0; ct < 4; ct++)
 #pragma unroll
       for (int j = 0; j < F::KJ; j++)
-        kq[ct][j] = *(const typename F::KUnit *)(t + (j * 4096 + s_cell(ct, 0) * KC) + koff);
+        kq[ct][j] = read((const typename F::KUnit *)(t + (j * 4096 + s_cell(ct, 0) * KC) + koff));
   };
   auto load_v = [&](int blk) {
     const uint8_t *t = tile(vpool, blk);
 #pragma unroll
-    for (int j = 0; j < F::VJ; j++) vq[j] = *(const u32x4 *)(t + j * 1024 + voff);
+    for (int j = 0; j < F::VJ; j++) vq[j] = read((const u32x4 *)(t + j * 1024 + voff));
   };
   auto load_s = [&](int blk) {
     const uint8_t *k = tile(kpool, blk) + F::SCALES, *v = tile(vpool, blk) + F::SCALES;
@@ -465,8 +468,9 @@ static void launch_attn_q4(const float *q, int H, int Hkv, float scale_log2, con
                            const lgmlh_ubatch *ub, float *out, f16 *planes, int64_t npad, int xf,
                            float *part, hipStream_t st) {
   const uint64_t *vis = ub->ring == LGMLH_PLAN_TREE ? plan_vis(ub) : nullptr;
+  const auto kern = ub->n_shared > 0 ? paged_attn_q4_kernel<D, false> : paged_attn_q4_kernel<D, true>;
   if (ub->n_items > 0)
-    hipLaunchKernelGGL(paged_attn_q4_kernel<D>, dim3((uint32_t)ub->n_items * Hkv), dim3(64 * PARTS), 0, st, q, H, Hkv,
+    hipLaunchKernelGGL(kern, dim3((uint32_t)ub->n_items * Hkv), dim3(64 * PARTS), 0, st, q, H, Hkv,
                        scale_log2, (const uint8_t *)kp, (const uint8_t *)vp, ub->items, ub->seq_off, ub->seq_npast,
                        ub->block_tab, ub->max_blocks, ub->ring, ub->window, out, planes, npad, xf, part, ub->order,
                        ub->order ? ub->n_single : 0, vis);
