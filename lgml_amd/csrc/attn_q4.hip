@@ -426,7 +426,6 @@ paged_attn_q4_kernel(const float *__restrict__ q, int H, int Hkv, float scale_lo
     if (SR == 2) scl[lane] = sreg[0];
     if (SR == 2 || lane < 2 * SL) scl[(SR - 1) * 64 + lane] = sreg[SR - 1];
     load_v(blk);  // (with the next block's K it kept that waiting: 64 sequences' step 56 us, so 52)
-    if (more) load_s(blk + PARTS);
     scores_q<NB>(
         st,
         [&](int b, int p, f16x8(&k)[2], f16x8 &d) {
@@ -438,6 +437,7 @@ paged_attn_q4_kernel(const float *__restrict__ q, int H, int Hkv, float scale_lo
           h = qsh[b * 64 + ql_at];
           l = qsl[b * 64 + ql_at];
         });
+    if (more) load_s(blk + PARTS);
     if (more) load_k(blk + PARTS);
     uint64_t word = ~(uint64_t)0;
     const bool masked = see.masks(blk, word);
