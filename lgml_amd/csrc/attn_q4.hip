@@ -21,11 +21,12 @@
 // 583; heads of 256, 8 / 4, 133 against 55 and 318 against 288.
 //
 // Bounds. One token of 64 sequences at 128 to 4096 cells, 32 / 8 heads of 128, is 45 us, the
-// merge's 5 with them: 159 MB, 3.9 TB/s in the first (34 us with the loads alone). A block of 64 cells is 650 vector
-// operations a wave (288 of them the unpacking; a decode step's 4 rows use a quarter of the
-// columns of the others), which take the three waves of a SIMD 3.8 us, its bytes of all the
-// waves 5.6 at the copy's rate; a workgroup of 12 blocks starts with 4 us until its first bytes are there,
-// and the 1688 workgroups of the step are 2.2 times what the card holds. A chunk of 512
+// merge's 5 with them: 159 MB, 3.9 TB/s in the first (34 us with the loads alone). A block
+// of 64 cells is 650 vector operations a wave (288 of them the unpacking; a decode step's 4
+// rows use a quarter of the columns of the others), which take the three waves of a SIMD
+// 3.8 us, its bytes of all the waves 5.6 at the copy's rate; a workgroup of 12 blocks starts
+// with 4 us until its first bytes are there, and the 1688 workgroups of the step are 2.2
+// times what the card holds. A chunk of 512
 // tokens after 2048, 8 / 4 heads of 256, is 50 us, half of them vector operations of its
 // 2048 waves, two a SIMD.
 #include "attnq.h"
@@ -327,8 +328,9 @@ __device__ __forceinline__ bool plain_lane(u32x4 sc) {
 // An item: a workgroup, a wave each part. Each wave reads its blocks from the pool into
 // registers, the next one's K and scales while one is used; q's operands are in LDS, made
 // once, and the states join there. ONCE (plans without shared sets): values are read past
-// the caches. The step of 64 sequences takes 51 us so, 53 through them; a chunk, whose
-// items read the same blocks, 52 and 50.
+// the caches. The step of 64 sequences takes 45 us so, 49 through them (77 either way after
+// a prefix of 4000 cells that all share); a chunk, whose items read the same blocks, 52
+// and 50.
 template <int D, bool ONCE>
 __global__ void __launch_bounds__(64 * PARTS, D == 256 ? 2 : 3)
 paged_attn_q4_kernel(const float *__restrict__ q, int H, int Hkv, float scale_log2,
@@ -425,7 +427,7 @@ paged_attn_q4_kernel(const float *__restrict__ q, int H, int Hkv, float scale_lo
                                                     (SR == 2 || (lane >= SL && lane < 2 * SL)));
     if (SR == 2) scl[lane] = sreg[0];
     if (SR == 2 || lane < 2 * SL) scl[(SR - 1) * 64 + lane] = sreg[SR - 1];
-    load_v(blk);  // (a block ahead, it kept the next block's K waiting: 64 sequences' step 54 us instead of 49)
+    load_v(blk);  // (a block ahead, it kept the next one's K waiting: 64 sequences' step 54 us, so 49)
     scores_q<NB>(
         st,
         [&](int b, int p, f16x8(&k)[2], f16x8 &d) {
