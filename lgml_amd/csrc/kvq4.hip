@@ -7,9 +7,10 @@ namespace lgmlh {
 
 // A workgroup takes W consecutive tokens (64, or 16 of a call of few) of one head
 // of K or V, 8 values a thread and step: K's are the word they are stored as, V's
-// turn in LDS (kvstore.h). Bound by the rows: 8192 of 8 heads of 128, 76 MB, take 18 us;
-// 64 rows 4.8 us, dependent reads.
+// turn in LDS (kvstore.h), or of few tokens go byte by byte. Bound by the rows: 8192 of 8
+// heads of 128, 76 MB, take 18 us; 64 rows 3.7 us, dependent reads.
 constexpr int Q4_THREADS = KV_THREADS;
+constexpr int Q4_FEW = 16;  // W of a call of few tokens, whose V goes byte by byte, without a turn
 // KV heads: the bytes of a block, 36 D for each, are counted in 31 bits.
 constexpr int Q4_HEADS = 65535;
 static_assert((int64_t)Q4_HEADS * q4_tile_bytes(256) < INT32_MAX, "tile_of");
@@ -28,17 +29,20 @@ kv_store_q4_kernel(uint8_t *__restrict__ kp, uint8_t *__restrict__ vp, int64_t n
   const int h = blockIdx.x % (uint32_t)Hkv;
   const int64_t j0 = (int64_t)(blockIdx.x / (uint32_t)Hkv) * W;
   const float *src = (blockIdx.y ? vs : ks) + (j0 * Hkv + h) * D;
-  if (blockIdx.y) {
-    __shared__ VTurn<LGMLH_Q4_0, D, W> turn;
-    turn.store(src, (int64_t)Hkv * D, vp, h, Hkv, cells, j0, n, n_cells);
-    return;
+  const bool is_v = blockIdx.y;
+  if constexpr (W > Q4_FEW) {
+    if (is_v) {
+      __shared__ VTurn<LGMLH_Q4_0, D, W> turn;
+      turn.store(src, (int64_t)Hkv * D, vp, h, Hkv, cells, j0, n, n_cells);
+      return;
+    }
   }
   constexpr int G8 = D / 8, STEP = Q4_THREADS / G8, IT = (W + STEP - 1) / STEP;
   __shared__ uint16_t scale[D / 32 * W];
   __shared__ int64_t cell[W];
   const int tid = threadIdx.x, g8 = tid % G8, t0 = tid / G8;
   const int left = (int)(n - j0 < W ? n - j0 : W);
-  uint8_t *pool = kp + (int64_t)h * q4_tile_bytes(D);
+  uint8_t *pool = (is_v ? vp : kp) + (int64_t)h * q4_tile_bytes(D);
   f32x4 x[IT][2];
 #pragma unroll
   for (int i = 0; i < IT; i++) {
@@ -62,8 +66,22 @@ kv_store_q4_kernel(uint8_t *__restrict__ kp, uint8_t *__restrict__ vp, int64_t n
     const float d = quant8<LGMLH_Q4_0>(v, q);
     if (t >= left) continue;  // whole blocks of lanes leave together
     if (g8 % 4 == 0) scale[g8 / 4 * W + t] = f2h(d);
-    if (const int64_t c = cell[t]; c >= 0)
-      *(uint32_t *)(q4_tile<D>(pool, c, Hkv) + q4_k_at(D, (int)c & 63, 8 * g8)) = q4_k_word(q);
+    const int64_t c = cell[t];
+    if (W > Q4_FEW || !is_v) {
+      if (c >= 0) *(uint32_t *)(q4_tile<D>(pool, c, Hkv) + q4_k_at(D, (int)c & 63, 8 * g8)) = q4_k_word(q);
+      continue;
+    }
+    // dims r and r + 16 share a byte: of the eight of a lane and the one two on, each writes four
+    uint32_t w = 0;
+#pragma unroll
+    for (int e = 0; e < 8; e++) w |= q[e] << 4 * e;
+    const uint32_t other = __shfl_xor(w, 2);
+    const int high = g8 & 2, r = 8 * (g8 & 1) + 2 * high;
+    const uint32_t lo = (high ? other : w) >> 8 * high, hi = (high ? w : other) >> 8 * high;
+    uint8_t *to = q4_tile<D>(pool, c < 0 ? 0 : c, Hkv) + q4_v_at(16 * (g8 / 4) + r, (int)c & 63);
+    if (c >= 0)
+#pragma unroll
+      for (int e = 0; e < 4; e++) to[64 * e] = (uint8_t)((lo >> 4 * e & 15) | (hi >> 4 * e & 15) << 4);
   }
   __syncthreads();
   // the scales with tokens along the lanes, as a tile has them
@@ -134,6 +152,32 @@ kv_gather_q4_k_kernel(const uint8_t *__restrict__ pool, int64_t n_cells,
     const Piece y(v[0], v[N / 4 - 1], d[u]);
     __builtin_nontemporal_store(y.y, (typename Piece::T *)(row + 32 * u));
   }
+}
+
+// V's cells as rows, of few tokens: each value from its own byte, behind nothing but the
+// cell's number.
+template <int D, typename OutT>
+__global__ void __launch_bounds__(Q4_THREADS)
+kv_gather_q4_v_few_kernel(const uint8_t *__restrict__ pool, int64_t n_cells,
+                          const int64_t *__restrict__ cells, int64_t n, int Hkv, OutT *__restrict__ out) {
+  typedef RowPiece<OutT> Piece;
+  constexpr int N = Piece::N, PER = D / N;
+  const int h = blockIdx.x % (uint32_t)Hkv;
+  const int64_t t = (int64_t)(blockIdx.x / (uint32_t)Hkv) * (Q4_THREADS / PER) + threadIdx.x / PER;
+  const int dim = threadIdx.x % PER * N;
+  if (t >= n) return;
+  const int64_t c = cells[t];
+  uint32_t v[2] = {0, 0};
+  float d = 0.0f;
+  if ((uint64_t)c < (uint64_t)n_cells) {
+    const int cell = (int)c & 63;
+    const uint8_t *tile = q4_tile<D>(pool + (int64_t)h * q4_tile_bytes(D), c, Hkv);
+    const uint8_t *from = tile + q4_v_at(dim / 32 * 16 + dim % 16, cell);
+    d = h2f(*(const uint16_t *)(tile + q4_scale_at(D, dim / 32, cell)));
+#pragma unroll
+    for (int e = 0; e < N; e++) v[e / 4] |= (uint32_t)(from[64 * e] >> dim % 32 / 16 * 4) << 8 * (e % 4);
+  }
+  *(typename Piece::T *)(out + (t * Hkv + h) * (int64_t)D + dim) = Piece(v[0], v[1], d).y;
 }
 
 // V's cells as rows: whole groups of 8 cells through LDS, as the store the other way
@@ -210,9 +254,9 @@ kv_gather_q4_v_kernel(const uint8_t *__restrict__ pool, int64_t n_cells,
 }
 
 // Tokens of a workgroup: 64 (32 of heads of 256), but 16 where that makes fewer than 256
-// workgroups. 64 rows of 8 heads of 128: 4.9 us stored, V read back in 4.7 (with 64 tokens
-// 7.9 and 7.6); 8192 rows stored and read back 39 us with 16, 35 with 64; 32768 as f16 rows
-// 47 and 37.
+// workgroups, whose V goes without a turn in LDS. 64 rows of 8 heads of 128: 3.7 us stored, V
+// read back in 2.7 (16 tokens with turns 4.7 and 4.5, 64 7.9 and 7.6); with turns 8192 rows
+// stored and read back took 39 us with 16, 35 with 64; 32768 as f16 rows 47 and 37.
 constexpr int q4_tokens(int D) { return D > 128 ? 32 : 64; }
 static bool q4_small(int64_t n, int n_head_kv, int kinds, int D) {
   return (n + q4_tokens(D) - 1) / q4_tokens(D) * n_head_kv * kinds < 256;
@@ -245,12 +289,12 @@ extern "C" int lgmlh_kv_store_q4(void *kpool, void *vpool, int64_t n_cells, int 
   LGMLH_TRY(check_write_cells(h_cells, n, n_cells, "kv_store_q4"));
   if (n == 0) return LGMLH_OK;
   const bool small = q4_small(n, n_head_kv, 2, head_dim);
-  const int w = small ? 16 : q4_tokens(head_dim);
+  const int w = small ? Q4_FEW : q4_tokens(head_dim);
   // heads fastest: those of the same rows run together
   const dim3 grid((unsigned)((n + w - 1) / w * n_head_kv), 2);
-  const auto kern = head_dim == 64    ? (small ? kv_store_q4_kernel<64, 16> : kv_store_q4_kernel<64, 64>)
-                    : head_dim == 128 ? (small ? kv_store_q4_kernel<128, 16> : kv_store_q4_kernel<128, 64>)
-                                      : (small ? kv_store_q4_kernel<256, 16> : kv_store_q4_kernel<256, 32>);
+  const auto kern = head_dim == 64    ? (small ? kv_store_q4_kernel<64, Q4_FEW> : kv_store_q4_kernel<64, 64>)
+                    : head_dim == 128 ? (small ? kv_store_q4_kernel<128, Q4_FEW> : kv_store_q4_kernel<128, 64>)
+                                      : (small ? kv_store_q4_kernel<256, Q4_FEW> : kv_store_q4_kernel<256, 32>);
   hipLaunchKernelGGL(kern, grid, dim3(Q4_THREADS), 0, as_stream(stream), (uint8_t *)kpool,
                      (uint8_t *)vpool, n_cells, k_src, v_src, cells, n, n_head_kv);
   return hip_check(hipGetLastError(), "kv_store_q4");
@@ -282,7 +326,8 @@ extern "C" int lgmlh_kv_gather_q4(const void *pool, int which, int64_t n_cells, 
     auto of = [&](auto d) {
       constexpr int D = decltype(d)::value, big = q4_tokens(D);
       if (which)
-        small ? launch(kv_gather_q4_v_kernel<D, 16, T>, 16) : launch(kv_gather_q4_v_kernel<D, big, T>, big);
+        small ? launch(kv_gather_q4_v_few_kernel<D, T>, Q4_THREADS * (16 / (int)sizeof(T)) / D)
+              : launch(kv_gather_q4_v_kernel<D, big, T>, big);
       else
         launch(kv_gather_q4_k_kernel<D, T>, Q4_THREADS * (16 / (int)sizeof(T)) * q4_k_words(D) / D);
     };

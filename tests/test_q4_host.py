@@ -252,7 +252,7 @@ def test_new_kernels_use_no_scratch():
     from tests.test_kernel_resources import kernels
     all_ = kernels()
     for name in ("paged_attn_q4_kernel", "kv_store_q4_kernel", "kv_gather_q4_k_kernel", "kv_gather_q4_v_kernel",
-                 "kv_copy_blocks_kernel", "qkv_rope_axes_kernel"):
+                 "kv_gather_q4_v_few_kernel", "merge_slices_kernel", "kv_copy_blocks_kernel", "qkv_rope_axes_kernel"):
         got = {n: k for n, k in all_.items() if name in n}
         assert got, name
         for n, k in got.items():
