@@ -104,53 +104,59 @@ struct RowPiece {
   }
 };
 
-// K's cells as rows (n, Hkv D): a thread has 16 bytes of a row's, in U blocks of 32 dims,
-// from a load's words (of f32 the low or the high ones' half). The rows pass the caches
-// by, whole 128-byte lines a store. The context of 8 sequences of 4096 tokens, 8 heads of
-// 128, as f16 rows of K and V: 37 us, 4.7 TB/s (cached stores of 8 bytes 49; 16 bytes
-// past the caches, but 32 bytes of a line at a time, took f32 rows longer than cached).
+// Threads of a cell in the read back of K: 16 bytes of a row's in each of U blocks of 32
+// dims, or of f16 in every other one, so that eight write a line's 128 bytes.
+template <typename OutT>
+__host__ __device__ constexpr int q4_k_threads(int D) {
+  return D * sizeof(OutT) / 16 / q4_k_words(D) * (4 / sizeof(OutT));
+}
+
+// K's cells as rows (n, Hkv D), from a load's U words (of f32 the low or the high ones'
+// half). The rows pass the caches by, whole 128-byte lines a store. The context of 8
+// sequences of 4096 tokens, 8 heads of 128, as f16 rows of K and V: 31 us, 5.5 TB/s (64
+// bytes of a line at a time 37; cached stores of 8 bytes a thread 49).
 template <int D, typename OutT>
 __global__ void __launch_bounds__(Q4_THREADS)
 kv_gather_q4_k_kernel(const uint8_t *__restrict__ pool, int64_t n_cells,
                       const int64_t *__restrict__ cells, int64_t n, int Hkv, OutT *__restrict__ out) {
   typedef RowPiece<OutT> Piece;
-  constexpr int N = Piece::N, U = q4_k_words(D), PER = D / (N * U);  // threads of a cell
+  constexpr int N = Piece::N, U = q4_k_words(D), L = 32 / N, S = N / 4, PER = q4_k_threads<OutT>(D);
   const int h = blockIdx.x % (uint32_t)Hkv;
   const int64_t t = (int64_t)(blockIdx.x / (uint32_t)Hkv) * (Q4_THREADS / PER) + threadIdx.x / PER;
-  const int k = threadIdx.x % PER, j = k / (32 / N), dim = k % (32 / N) * N;
+  const int k = threadIdx.x % PER, j = k / (L * S), odd = k / L % S, dim = k % L * N;
   if (t >= n) return;
   const int64_t c = cells[t];
   const bool in = (uint64_t)c < (uint64_t)n_cells;
   const int cell = (int)c & 63;
-  uint32_t w[U];
-  float d[U];
+  uint32_t w[U / S];
+  float d[U / S];
 #pragma unroll
-  for (int u = 0; u < U; u++) {
-    w[u] = 0;
-    d[u] = 0.0f;
+  for (int i = 0; i < U / S; i++) {
+    w[i] = 0;
+    d[i] = 0.0f;
   }
   if (in) {
     const uint8_t *tile = q4_tile<D>(pool + (int64_t)h * q4_tile_bytes(D), c, Hkv);
     typedef uint32_t uU __attribute__((ext_vector_type(U)));
     const uU r = *(const uU *)(tile + q4_k_at(D, cell, 32 * U * j + dim / 8 * 8));
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-      w[u] = r[u];
-      d[u] = h2f(*(const uint16_t *)(tile + q4_scale_at(D, U * j + u, cell)));
+    for (int i = 0; i < U / S; i++) {
+      w[i] = odd ? r[S * i + S - 1] : r[S * i];
+      d[i] = h2f(*(const uint16_t *)(tile + q4_scale_at(D, U * j + S * i + odd, cell)));
     }
   }
-  OutT *row = out + (t * Hkv + h) * (int64_t)D + 32 * U * j + dim;
+  OutT *row = out + (t * Hkv + h) * (int64_t)D + 32 * (U * j + odd) + dim;
 #pragma unroll
-  for (int u = 0; u < U; u++) {
+  for (int i = 0; i < U / S; i++) {
     // dim e at bits 4 (e / 2) + 16 (e % 2): in order, a byte each
     uint32_t v[N / 4];
 #pragma unroll
-    for (int i = 0; i < N / 4; i++) {
-      const uint32_t s = w[u] >> (8 * i + 2 * (dim % 8));
-      v[i] = (s & 15) | (s >> 16 & 15) << 8 | (s >> 4 & 15) << 16 | (s >> 20 & 15) << 24;
+    for (int b = 0; b < N / 4; b++) {
+      const uint32_t s = w[i] >> (8 * b + 2 * (dim % 8));
+      v[b] = (s & 15) | (s >> 16 & 15) << 8 | (s >> 4 & 15) << 16 | (s >> 20 & 15) << 24;
     }
-    const Piece y(v[0], v[N / 4 - 1], d[u]);
-    __builtin_nontemporal_store(y.y, (typename Piece::T *)(row + 32 * u));
+    const Piece y(v[0], v[N / 4 - 1], d[i]);
+    __builtin_nontemporal_store(y.y, (typename Piece::T *)(row + 32 * S * i));
   }
 }
 
@@ -256,7 +262,8 @@ kv_gather_q4_v_kernel(const uint8_t *__restrict__ pool, int64_t n_cells,
 // Tokens of a workgroup: 64 (32 of heads of 256), but 16 where that makes fewer than 256
 // workgroups, whose V goes without a turn in LDS. 64 rows of 8 heads of 128: 3.7 us stored, V
 // read back in 2.7 (16 tokens with turns 4.7 and 4.5, 64 7.9 and 7.6); with turns 8192 rows
-// stored and read back took 39 us with 16, 35 with 64; 32768 as f16 rows 47 and 37.
+// stored and read back took 39 us with 16, 35 with 64; 32768 as f16 rows 47 and 37 (before K's
+// lines went whole).
 constexpr int q4_tokens(int D) { return D > 128 ? 32 : 64; }
 static bool q4_small(int64_t n, int n_head_kv, int kinds, int D) {
   return (n + q4_tokens(D) - 1) / q4_tokens(D) * n_head_kv * kinds < 256;
@@ -305,7 +312,7 @@ extern "C" int lgmlh_kv_gather_q4(const void *pool, int which, int64_t n_cells, 
                                   int out_type, void *stream) {
   if (!pool || !cells || !out || n < 0 || (which != 0 && which != 1) || n_cells <= 0 ||
       n_cells > CELLS_MAX || n_cells % KV_BLOCK || n_head_kv <= 0 || n_head_kv > Q4_HEADS ||
-      n >= CELL_ROWS / (head_dim == 256 && out_type == LGMLH_F32 ? 2 : 1) / n_head_kv || !q4_head(head_dim) ||
+      n >= CELL_ROWS / (head_dim == 256 ? 2 : 1) / n_head_kv || !q4_head(head_dim) ||
       (out_type != LGMLH_F32 && out_type != LGMLH_F16)) {
     set_error("kv_gather_q4: bad arguments (heads of 64, 128 or 256; out f32 or f16)");
     return LGMLH_EINVAL;
@@ -329,7 +336,7 @@ extern "C" int lgmlh_kv_gather_q4(const void *pool, int which, int64_t n_cells, 
         small ? launch(kv_gather_q4_v_few_kernel<D, T>, Q4_THREADS * (16 / (int)sizeof(T)) / D)
               : launch(kv_gather_q4_v_kernel<D, big, T>, big);
       else
-        launch(kv_gather_q4_k_kernel<D, T>, Q4_THREADS * (16 / (int)sizeof(T)) * q4_k_words(D) / D);
+        launch(kv_gather_q4_k_kernel<D, T>, Q4_THREADS / q4_k_threads<T>(D));
     };
     if (head_dim == 64)
       of(std::integral_constant<int, 64>{});
