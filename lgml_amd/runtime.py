@@ -559,9 +559,11 @@ class DeviceModel:
         window's few blocks over more waves; with the longest runs started
         first, C4 7172 -> 7462 tok/s against 32 and 16; 24 / 26 / 30 and
         10 / 14 are no better); else runs of 12 (C2 decode 7263 -> 7407
-        tok/s against 16; 10: 7383, 8: 7088). The run length is fixed per
-        model, so split points still depend on a sequence's own length
-        only."""
+        tok/s against 16; 10: 7383, 8: 7088), over Q4_0 pools of 20 (a
+        workgroup of four waves each: a decode step of 64 sequences 48 us of
+        attention a layer against 50 with 12 and 51 with 40, a chunk of 512
+        after 2048 83 against 90). The run length is fixed per model, so split
+        points still depend on a sequence's own length only."""
         ids = np.ascontiguousarray(ids, np.int32)
         ring_bps = self.ring_blocks_per_split or blocks_per_split
         if not ring_bps and self.hp["head_dim"] >= 256:
@@ -569,7 +571,7 @@ class DeviceModel:
         if not blocks_per_split and self.hp["head_dim"] >= 256:
             blocks_per_split = 28
         elif not blocks_per_split:
-            blocks_per_split = 12
+            blocks_per_split = 20 if self.kv_type == hip.Q4_0 else 12
         if len(ids) and (ids.min() < 0 or ids.max() >= self.hp["n_vocab"]):
             raise ValueError("token id out of range [0, %d)" % self.hp["n_vocab"])
         p = Plan(seq_n, seq_npast, block_tab, ids, self.hp["n_head"], self.paged_dims[1],
