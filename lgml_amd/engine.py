@@ -444,8 +444,10 @@ class Engine:
                 self.seqs.alloc.unref(b)
         blocks = self.seqs.compact([r.seq for r in self.active])
         if shrink:
-            self.model.shrink_pool(max(blocks, 1) * BLOCK)
-            self.seqs.alloc.set_cap(self.model.pool_blocks)
+            try:
+                self.model.shrink_pool(max(blocks, 1) * BLOCK)
+            finally:  # (cut also where memory for a shorter tensor failed)
+                self.seqs.alloc.set_cap(self.model.pool_blocks)
         return self.model.n_cells
 
     def submit(self, req):

@@ -498,17 +498,21 @@ class DeviceModel:
         L, hp = hip.lib(), self.hp
         Hkv, D = self.paged_dims[1], self.block_dim(self.paged_dims[0])
         nb = L.lgmlh_kv_layer_bytes(cells, Hkv, D)
-        for il in range(hp["n_layer"]):
-            if self.swa[il]:
-                continue
-            for pools, attr in ((self.kpools, "kpool"), (self.vpools, "vpool")):
-                old = pools[il]
-                new = _empty(nb)
-                check(L.lgmlh_kv_grow(old.data_ptr(), self.n_cells, new.data_ptr(), cells, Hkv, D,
-                                      stream()))
-                pools[il] = new
-                setattr(self.layers[il], attr, new.data_ptr())
-        self._resized(cells)
+        have = self.n_cells  # of every tensor, also when not all could grow
+        try:
+            for il in range(hp["n_layer"]):
+                if self.swa[il]:
+                    continue
+                for pools, attr in ((self.kpools, "kpool"), (self.vpools, "vpool")):
+                    old = pools[il]
+                    new = _empty(nb)
+                    check(L.lgmlh_kv_grow(old.data_ptr(), self.n_cells, new.data_ptr(), cells, Hkv, D,
+                                          stream()))
+                    pools[il] = new
+                    setattr(self.layers[il], attr, new.data_ptr())
+            have = cells
+        finally:
+            self._resized(have)
         return cells
 
     def shrink_pool(self, cells):
@@ -516,26 +520,32 @@ class DeviceModel:
         cells (a multiple of 64, at least one block), for a pool whose blocks
         behind them are free (Engine.compact); the memory goes back to the
         allocator. The pool may grow again, up to max_cells. Returns the new
-        cell count. The counterpart of grow_pool; the reference's pools only
-        grow (transformer.lua:831-908)."""
+        cell count. Where memory for a shorter tensor fails, the pool has `cells`
+        cells all the same; the next call cuts what this one left long. The
+        counterpart of grow_pool; the reference's pools only grow
+        (transformer.lua:831-908)."""
         cells = int(cells)
         if cells % 64 or cells <= 0:
             raise ValueError("%d cells: whole blocks of 64, at least one" % cells)
-        if cells >= self.n_cells:
+        if cells > self.n_cells:
             return self.n_cells
         Hkv, D = self.paged_dims[1], self.block_dim(self.paged_dims[0])
         nb = hip.lib().lgmlh_kv_layer_bytes(cells, Hkv, D)
-        for il in range(self.hp["n_layer"]):
-            if self.swa[il]:
-                continue
-            for pools, attr in ((self.kpools, "kpool"), (self.vpools, "vpool")):
+        longer = [(pools, attr, il) for il in range(self.hp["n_layer"]) if not self.swa[il]
+                  for pools, attr in ((self.kpools, "kpool"), (self.vpools, "vpool")) if pools[il].numel() > nb]
+        if not longer:
+            return cells
+        try:
+            for pools, attr, il in longer:
                 pools[il] = pools[il][:nb].clone()
                 setattr(self.layers[il], attr, pools[il].data_ptr())
-        self._resized(cells)
+        finally:
+            self._resized(cells)
         return cells
 
     def _resized(self, cells):
-        """The paged pool tensors were replaced by ones of `cells` cells."""
+        """The paged pool tensors, or some of them, were replaced, by ones of `cells`
+        cells or more."""
         # the old tensors are freed once the copies are done
         torch.cuda.current_stream().synchronize()
         self.n_cells = cells
@@ -544,7 +554,8 @@ class DeviceModel:
         for il in range(self.hp["n_layer"]):
             if not self.swa[il]:
                 ptrs += [self.kpools[il].data_ptr(), self.vpools[il].data_ptr()]
-        self.pools_dev = torch.tensor(ptrs or [0], dtype=torch.int64, device=DEV)
+        # in place: it needs no memory, and what holds its address goes on with it
+        self.pools_dev.copy_(torch.tensor(ptrs or [0], dtype=torch.int64))
 
     ring_blocks_per_split = 0  # the ring plans' run length (0: as blocks_per_split; 12 for heads of 256)
 
