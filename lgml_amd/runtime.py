@@ -187,7 +187,7 @@ class Plan:
         bt = np.ascontiguousarray(block_tab, np.int32)
         if bt.ndim == 1:
             bt = bt.reshape(len(self.seq_n), -1)
-        self.block_tab = bt
+        self.block_tab, self.pool_blocks = bt, int(pool_blocks)
         self.ids = np.ascontiguousarray(ids, np.int32)
         assert len(self.ids) == int(self.seq_n.sum())
         self.info = hip.PlanInfo()
@@ -519,7 +519,8 @@ class DeviceModel:
         """The paged pool tensors of every layer cut to their first `cells`
         cells (a multiple of 64, at least one block), for a pool whose blocks
         behind them are free (Engine.compact); the memory goes back to the
-        allocator. The pool may grow again, up to max_cells. Returns the new
+        allocator. Plans of other blocks are refused from then on; a captured
+        pass holds the tensors' addresses, and is captured anew. The pool may grow again, up to max_cells. Returns the new
         cell count. Where memory for a shorter tensor fails, the pool has `cells`
         cells all the same; the next call cuts what this one left long. The
         counterpart of grow_pool; the reference's pools only grow
@@ -618,6 +619,8 @@ class DeviceModel:
         indices; default the last token of each sequence), on the current
         stream. trace: an EventTrace to time launch groups with HIP events.
         slot: the workspace (see workspace())."""
+        if plan.pool_blocks > self.pool_blocks:
+            self._check_blocks(plan)
         if out_rows is None:
             n_out, rows = plan.info.n_seq, None
         else:
@@ -633,6 +636,14 @@ class DeviceModel:
                  logits.data_ptr(), ws.data_ptr(), ws_bytes,
                  C.byref(trace.c) if trace is not None else None, stream()))
         return logits
+
+    def _check_blocks(self, plan):
+        """The blocks of a plan made before the pool was cut are still in it."""
+        need = (plan.seq_npast + plan.seq_n + 63) // 64
+        used = plan.block_tab[np.arange(plan.block_tab.shape[1]) < need[:, None]]
+        if used.size and used.max() >= self.pool_blocks:
+            raise ValueError("the plan takes block %d, made before the pool was cut to %d" % (
+                used.max(), self.pool_blocks))
 
     def move_cells(self, src, dst):
         """Cells src to dst in every paged layer's K and V, each dst as its

@@ -3,6 +3,7 @@ part-way (no GPU work)."""
 import ctypes as C
 import types
 
+import numpy as np
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -109,6 +110,39 @@ def test_a_pool_that_could_not_all_grow_stays_as_it_was(runtime, after):
     runtime.fail.after = 1 << 30
     assert m.grow_pool() == 64 * 12
     holds(m, was, 64 * 12)
+
+
+def test_a_plan_of_blocks_that_were_cut_off_is_refused(runtime):
+    """Such a pass would read behind the tensors."""
+    m = pool(runtime, 6, 12)
+    m.m = types.SimpleNamespace(n_cells=64 * 6)
+
+    def plan(tab):
+        return types.SimpleNamespace(seq_n=np.array([1, 2], np.int32), seq_npast=np.array([127, 63], np.int32),
+                                     block_tab=np.array(tab, np.int32), pool_blocks=6)
+
+    class Reached(Exception):
+        pass
+
+    def workspace(*_):
+        raise Reached
+
+    m.workspace = workspace
+    rows = np.zeros(1, np.int32)
+    high, low = plan([[0, 3], [1, 2]]), plan([[0, 1], [1, 2]])
+    behind = plan([[0, 1, 5], [1, 2, -1]])  # (a place that no token takes)
+    for p in (high, low, behind):
+        with pytest.raises(Reached):
+            m.forward(p, rows)
+    m.shrink_pool(64 * 3)
+    with pytest.raises(ValueError, match="block 3"):
+        m.forward(high, rows)
+    for p in (low, behind):
+        with pytest.raises(Reached):
+            m.forward(p, rows)
+    m.grow_pool(64 * 6)
+    with pytest.raises(Reached):
+        m.forward(high, rows)
 
 
 def test_sizes_that_change_nothing(runtime):
