@@ -197,26 +197,36 @@ class PoolSeqs:
         """n sequences that go on from c's cells, each on its own from here: the
         full blocks are shared (M:share, transformer.lua:1116-1123), the cells of
         the partial one are copied into a block of each, all in one launch. For
-        several replies to one prompt. PoolFull leaves the sequences as they were."""
+        several replies to one prompt. What fails (PoolFull, memory, a captured
+        stream) leaves the sequences as they were. Models with sliding layers are
+        refused: their cells stand in the rings of a slot, which no block holds."""
+        if any(getattr(self.model, "swa", [])):
+            raise ValueError("a fork takes the blocks of the paged pool only, not the rings")
         full, part = divmod(c.n_past, BLOCK)
+        held, keys, past = c.blocks[:full + (part > 0)], c.keys[:full], c.n_past
         made = []
+        for b in held:  # (pressure may free c while blocks are taken)
+            self.alloc.ref(b, c.prio)
         try:
             for _ in range(n):
                 d = Seq(self, c.prio)
                 made.append(d)
-                for b in c.blocks[:full]:  # (M:share takes keyed blocks only)
+                for b in held[:full]:  # (M:share takes keyed blocks only)
                     self.alloc.ref(b, d.prio)
                     d.blocks.append(b)
-                d.keys[:] = c.keys[:full]
-                d.n_past = c.n_past
+                d.keys[:] = keys
+                d.n_past = past
                 if part:
-                    self.reserve(d, c.n_past)
-        except PoolFull:
+                    self.reserve(d, past)
+            if part and made:
+                self.model.copy_blocks([held[full]] * n, [d.blocks[full] for d in made], part)
+        except BaseException:
             for d in made:
                 self.free(d)
             raise
-        if part and made:
-            self.model.copy_blocks([c.blocks[full]] * n, [d.blocks[full] for d in made], part)
+        finally:
+            for b in held:
+                self.alloc.unref(b)
         return made
 
     def compact(self, seqs):
