@@ -175,7 +175,11 @@ class PoolSeqs:
             b = self.new_block(c, None if prev is None else prev + 1)
             if b is None:
                 raise PoolFull("kv pool full")
-            self.copy_block(last, b, n % BLOCK)
+            try:
+                self.copy_block(last, b, n % BLOCK)
+            except BaseException:
+                self.alloc.unref(b)
+                raise
             c.blocks[keep - 1] = b
             self.alloc.unref(last)
         c.n_past = min(c.n_past, n)
@@ -548,7 +552,8 @@ class Engine:
                 except PoolFull:
                     part = 0
                     c.n_past = m
-                alloc.unref(kid)
+                finally:
+                    alloc.unref(kid)
             self.hits += 1
             self.hit_blocks += len(blocks)
             return m + part

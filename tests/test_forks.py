@@ -1,5 +1,5 @@
-"""CPU checks of forks of sequences: models they refuse, what a fork that fails leaves
-behind, a source that goes while blocks are taken (no GPU work)."""
+"""CPU checks of forks of sequences: models they refuse, what a fork or another copy that
+fails leaves behind, a source that goes while blocks are taken (no GPU work)."""
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -94,3 +94,42 @@ def test_a_source_that_pressure_frees_is_there_until_it_is_copied():
     kids = seqs.fork(c, 2)
     assert [d.blocks for d in kids] == [[0, 1, 4], [0, 1, 3]] and seqs.model.calls == [([2, 2], [4, 3], 22)]
     assert [seqs.alloc.refs_of(b) for b in range(5)] == [2, 2, 0, 1, 1]
+
+
+def test_a_cut_whose_copy_fails_leaves_no_references():
+    """A shared block is copied before a sequence goes on in it."""
+    from lgml_amd import engine
+    m = Model(8)
+    seqs, c = sequence(m, 128)
+    d = seqs.fork(c)[0]
+    m.fail, m.kv_type = RuntimeError("captured"), None
+    with pytest.raises(RuntimeError):
+        seqs.truncate(d, 100)
+    assert seqs.alloc.used == 2 and [seqs.alloc.refs_of(b) for b in range(3)] == [2, 2, 0]
+    m.fail = None
+    seqs.truncate(d, 100)
+    assert d.blocks == [0, 2] and m.calls == [([1], [2], 36)]
+    assert isinstance(d, engine.Seq) and seqs.compact([c, d]) == 3
+
+
+def test_an_attached_block_whose_copy_fails_is_let_go():
+    from lgml_amd import engine
+    m = Model(8, RuntimeError("captured"))
+    m.kv_type = None
+    seqs, c = sequence(m, 100)
+    toks = list(range(100))
+    eng = object.__new__(engine.Engine)
+    eng.model, eng.seqs, eng.ram, eng.infos, eng.hits, eng.hit_blocks = m, seqs, None, {}, 0, 0
+    req = engine.Request(toks, 1)
+    req.seq = c
+    eng.publish_tail(req, toks)
+    seqs.free(c)
+    assert (seqs.alloc.used, seqs.alloc.cached) == (0, 2)
+    req = engine.Request(toks + [7], 1)
+    req.seq = engine.Seq(seqs)
+    with pytest.raises(RuntimeError):
+        eng.attach(req)
+    seqs.free(req.seq)
+    assert (seqs.alloc.used, seqs.alloc.cached) == (0, 2)
+    m.fail = None
+    assert eng.attach(req) == 100 and m.calls == [([1], [2], 36)]
