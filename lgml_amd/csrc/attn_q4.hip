@@ -496,6 +496,10 @@ int paged_attention_q4_dev(const float *q, int n_head, int n_head_kv, int head_d
   LGMLH_TRY(attn_check("paged_attention_q4", q, n_head, n_head_kv, head_dim, kpool, vpool, ub, out,
                        planes, xf, workspace, workspace_bytes, &run));
   if (!run) return LGMLH_OK;
+  if ((int64_t)ub->n_items * n_head_kv >= ((int64_t)1 << 32) / (64 * PARTS)) {  // fewer than 2^32 threads a launch
+    set_error("paged_attention_q4: %d items x %d KV heads in one launch", ub->n_items, n_head_kv);
+    return LGMLH_EINVAL;
+  }
   const float sl = scale * LOG2E;
   float *part = (float *)workspace;
   switch (head_dim) {

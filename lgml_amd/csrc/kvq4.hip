@@ -293,12 +293,14 @@ extern "C" int lgmlh_kv_store_q4(void *kpool, void *vpool, int64_t n_cells, int 
     set_error("kv_store_q4: pools are 16-byte aligned");
     return LGMLH_EINVAL;
   }
-  LGMLH_TRY(check_write_cells(h_cells, n, n_cells, "kv_store_q4"));
-  if (n == 0) return LGMLH_OK;
   const bool small = q4_small(n, n_head_kv, 2, head_dim);
   const int w = small ? Q4_FEW : q4_tokens(head_dim);
+  const int64_t groups = (n + w - 1) / w * n_head_kv;
+  LGMLH_TRY(check_groups(groups, "kv_store_q4"));
+  LGMLH_TRY(check_write_cells(h_cells, n, n_cells, "kv_store_q4"));
+  if (n == 0) return LGMLH_OK;
   // heads fastest: those of the same rows run together
-  const dim3 grid((unsigned)((n + w - 1) / w * n_head_kv), 2);
+  const dim3 grid((unsigned)groups, 2);
   const auto kern = head_dim == 64    ? (small ? kv_store_q4_kernel<64, Q4_FEW> : kv_store_q4_kernel<64, 64>)
                     : head_dim == 128 ? (small ? kv_store_q4_kernel<128, Q4_FEW> : kv_store_q4_kernel<128, 64>)
                                       : (small ? kv_store_q4_kernel<256, Q4_FEW> : kv_store_q4_kernel<256, 32>);
@@ -324,11 +326,15 @@ extern "C" int lgmlh_kv_gather_q4(const void *pool, int which, int64_t n_cells, 
   if (n == 0) return LGMLH_OK;
   const bool small = q4_small(n, n_head_kv, 1, head_dim);
   hipStream_t st = as_stream(stream);
+  int rc = LGMLH_OK;
   auto go = [&](auto out_t) {
     typedef decltype(out_t) T;
     auto launch = [&](auto kern, int w) {
-      hipLaunchKernelGGL(kern, dim3((unsigned)((n + w - 1) / w * n_head_kv)), dim3(Q4_THREADS), 0, st,
-                         (const uint8_t *)pool, n_cells, cells, n, n_head_kv, (T *)out);
+      const int64_t groups = (n + w - 1) / w * n_head_kv;
+      rc = check_groups(groups, "kv_gather_q4");
+      if (rc == LGMLH_OK)
+        hipLaunchKernelGGL(kern, dim3((unsigned)groups), dim3(Q4_THREADS), 0, st, (const uint8_t *)pool, n_cells,
+                           cells, n, n_head_kv, (T *)out);
     };
     auto of = [&](auto d) {
       constexpr int D = decltype(d)::value, big = q4_tokens(D);
@@ -349,5 +355,6 @@ extern "C" int lgmlh_kv_gather_q4(const void *pool, int which, int64_t n_cells, 
     go(float{});
   else
     go(f16{});
+  LGMLH_TRY(rc);
   return hip_check(hipGetLastError(), "kv_gather_q4");
 }

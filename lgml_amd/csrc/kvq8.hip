@@ -410,12 +410,14 @@ extern "C" int lgmlh_kv_store_q8(void *kpool, void *vpool, int64_t n_cells, int 
     set_error("kv_store_q8: pools are 16-byte aligned");
     return LGMLH_EINVAL;
   }
-  LGMLH_TRY(check_write_cells(h_cells, n, n_cells, "kv_store_q8"));
-  if (n == 0) return LGMLH_OK;
   const bool small = q8_small(n, n_head_kv, 2, head_dim);
   const int w = small ? 16 : q8_tokens(head_dim);
+  const int64_t groups = (n + w - 1) / w * n_head_kv;
+  LGMLH_TRY(check_groups(groups, "kv_store_q8"));
+  LGMLH_TRY(check_write_cells(h_cells, n, n_cells, "kv_store_q8"));
+  if (n == 0) return LGMLH_OK;
   // heads fastest: those of the same rows run together
-  const dim3 grid((unsigned)((n + w - 1) / w * n_head_kv), 2);
+  const dim3 grid((unsigned)groups, 2);
   hipStream_t st = as_stream(stream);
   const auto kern = head_dim == 64    ? (small ? kv_store_q8_kernel<64, 16> : kv_store_q8_kernel<64, 64>)
                     : head_dim == 128 ? (small ? kv_store_q8_kernel<128, 16> : kv_store_q8_kernel<128, 64>)
@@ -442,7 +444,9 @@ extern "C" int lgmlh_kv_gather_q8(const void *pool, int which, int64_t n_cells, 
   if (n == 0) return LGMLH_OK;
   const bool small = q8_small(n, n_head_kv, 1, head_dim);
   const int w = small ? 16 : q8_tokens(head_dim);
-  const dim3 grid((unsigned)((n + w - 1) / w * n_head_kv));
+  const int64_t groups = (n + w - 1) / w * n_head_kv;
+  LGMLH_TRY(check_groups(groups, "kv_gather_q8"));
+  const dim3 grid((unsigned)groups);
   hipStream_t st = as_stream(stream);
   auto go = [&](auto out_t) {
     typedef decltype(out_t) T;

@@ -8,9 +8,15 @@ namespace lgmlh {
 
 constexpr int CELL_GROUP = 8, CELL_HALO = 7;
 constexpr int64_t CELLS_MAX = (int64_t)1 << 36;  // a block's number has 31 bits
-// Heads of cells in one call: a launch has fewer than 2^32 threads, 256 for 32 or
-// more of them.
-constexpr int64_t CELL_ROWS = int64_t(1) << 29;
+// Heads of cells in one call, and its workgroups of 256: a launch has fewer than 2^32
+// threads. (CELL_ROWS of 32 a workgroup are as many; a last one in part for each head may
+// be one too many.)
+constexpr int64_t CELL_ROWS = int64_t(1) << 29, CELL_GROUPS = int64_t(1) << 24;
+inline int check_groups(int64_t groups, const char *what) {
+  if (groups < CELL_GROUPS) return LGMLH_OK;
+  set_error("%s: %lld workgroups in one launch", what, (long long)groups);
+  return LGMLH_EINVAL;
+}
 
 // Range and distinctness of cells that a call writes (kvq8.hip).
 int check_write_cells(const int64_t *h, int64_t n, int64_t n_cells, const char *what);
