@@ -666,7 +666,7 @@ __device__ __forceinline__ void merge_group(const int32_t *__restrict__ merge, i
       if (ns > SC)
         for (int s0 = 0; s0 < ns; s0 += SC) {
 #pragma unroll
-          for (int jj = 0; jj < 4; jj++)
+          for (int jj = 0; jj < NJ; jj++)
             if (jj < nj) {
               float mv[SC];
 #pragma unroll
@@ -677,7 +677,7 @@ __device__ __forceinline__ void merge_group(const int32_t *__restrict__ merge, i
         }
       for (int s0 = 0; s0 < ns; s0 += SC) {
 #pragma unroll
-        for (int jj = 0; jj < 4; jj++)
+        for (int jj = 0; jj < NJ; jj++)
           if (jj < nj) {
             f32x4 a[SC];
             float mv[SC], lv[SC];
