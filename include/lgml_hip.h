@@ -227,8 +227,8 @@ int32_t lgmlh_kvpool_lookup(void *pool, const char *key);
  * the shared token count in *shared. */
 int32_t lgmlh_kvpool_longest_kid(void *pool, const char *parent, const int32_t *tokens,
     int32_t max, int32_t *shared);
-/* Block src becomes block dst, a free one: its references, priority, key, tokens and
- * age go along, src is free. For compaction, after the owner of the tensors copied
+/* Block src becomes block dst, a free one below the cap: its references, priority,
+ * key, tokens and age go along, src is free. For compaction, after the owner of the tensors copied
  * the cells (lgmlh_kv_copy_blocks) and with the block tables that name src put
  * right. It has no counterpart in the reference, whose blocks stay where they are. */
 int lgmlh_kvpool_relocate(void *pool, int32_t src, int32_t dst);

@@ -377,9 +377,9 @@ extern "C" int32_t lgmlh_kvpool_longest_kid(void *pool, const char *parent, cons
 // Block src's record becomes the free block dst's.
 extern "C" int lgmlh_kvpool_relocate(void *pool, int32_t src, int32_t dst) {
   View v;
-  if (!view_of(pool, v) || src < 0 || src >= v.h->n || dst < 0 || dst >= v.h->n || is_free(v, src) ||
+  if (!view_of(pool, v) || src < 0 || src >= v.h->n || dst < 0 || dst >= v.h->cap || is_free(v, src) ||
       !is_free(v, dst)) {
-    set_error("kvpool_relocate: block %d to %d: from a block in use or kept to a free one", src, dst);
+    set_error("kvpool_relocate: block %d to %d: from a block in use or kept to a free one below the cap", src, dst);
     return LGMLH_EINVAL;
   }
   Block *k = v.blk(src);

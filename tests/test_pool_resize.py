@@ -173,3 +173,15 @@ def test_an_engine_whose_pool_could_not_all_be_cut_gives_out_its_blocks_alone():
         eng.compact()
     assert eng.seqs.alloc.cap == 1
     assert eng.seqs.alloc.take() == 0 and eng.seqs.alloc.take() is None
+
+
+def test_a_block_does_not_go_behind_the_cap():
+    """The tensors hold no such block."""
+    from lgml_amd import hip, kvpool
+    p = kvpool.Pool(8, 64, cap=4)
+    a, b = p.take(), p.take()
+    for dst in (4, 7):
+        with pytest.raises(hip.LgmlhError):
+            p.relocate(a, dst)
+    p.relocate(a, 3)
+    assert p.refs_of(3) == 1 and p.take() == a and b == 1
