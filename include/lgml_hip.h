@@ -228,9 +228,9 @@ int32_t lgmlh_kvpool_lookup(void *pool, const char *key);
 int32_t lgmlh_kvpool_longest_kid(void *pool, const char *parent, const int32_t *tokens,
     int32_t max, int32_t *shared);
 /* Block src becomes block dst, a free one below the cap: its references, priority,
- * key, tokens and age go along, src is free. For compaction, after the owner of the tensors copied
- * the cells (lgmlh_kv_copy_blocks) and with the block tables that name src put
- * right. It has no counterpart in the reference, whose blocks stay where they are. */
+ * key, tokens and age go along, src is free. For compaction, after the owner of the
+ * tensors copied the cells (lgmlh_kv_copy_blocks) and with the block tables that name
+ * src put right. It has no counterpart in the reference, whose blocks stay where they are. */
 int lgmlh_kvpool_relocate(void *pool, int32_t src, int32_t dst);
 /* P:set_cap (kvpool.lua:289-293). */
 int lgmlh_kvpool_set_cap(void *pool, int32_t cap);

@@ -695,13 +695,16 @@ class DeviceModel:
 
     def gather_kv(self, layer, cells, which=0):
         """Cells of a layer's K (0) or V (1) as (n, Hkv*D) f16 bits (uint16)
-        (ring cells for a sliding layer)."""
+        (ring cells for a sliding layer). A cell outside a quantised pool reads as
+        zeros, of an f16 one it is refused."""
         cells = np.ascontiguousarray(cells, np.int64)
+        n = self.ring_cells if self.swa[layer] else self.n_cells
+        if self.kv_type == hip.F16 and len(cells) and (cells.min() < 0 or cells.max() >= n):
+            raise ValueError("cells %d to %d of a pool of %d" % (cells.min(), cells.max(), n))
         dc = torch.from_numpy(cells).to(DEV)
         D, Hkv = self.dims[layer]
         out = torch.empty((len(cells), Hkv * D), dtype=torch.int16, device=DEV)
         pool = (self.kpools if which == 0 else self.vpools)[layer]
-        n = self.ring_cells if self.swa[layer] else self.n_cells
         if self.kv_type != hip.F16:  # the f16 of the values held
             fn = hip.lib().lgmlh_kv_gather_q8 if self.kv_type == hip.Q8_0 else hip.lib().lgmlh_kv_gather_q4
             check(fn(pool.data_ptr(), which, n, Hkv, D, dc.data_ptr(), len(cells), out.data_ptr(),

@@ -145,6 +145,23 @@ def test_a_plan_of_blocks_that_were_cut_off_is_refused(runtime):
         m.forward(high, rows)
 
 
+def test_cells_that_were_cut_off_are_not_read_back(runtime):
+    """The f16 read back takes the cells it is given."""
+    m = pool(runtime, 6, 12)
+    m.dims, m.ring_cells = [(D, KV)] * LAYERS, 128
+
+    def gather(*_):
+        raise AssertionError("the device is reached")
+
+    runtime.mod.hip.lib().lgmlh_kv_gather = gather
+    m.shrink_pool(128)
+    for layer, cells in ((0, [0, 128]), (0, [-1, 5]), (1, [128])):
+        with pytest.raises(ValueError, match="of a pool of 128"):
+            m.gather_kv(layer, cells)
+    with pytest.raises(AssertionError, match="reached"):
+        m.gather_kv(0, [0, 127])
+
+
 def test_sizes_that_change_nothing(runtime):
     m = pool(runtime, 6, 12)
     was = [[t + 0 for t in p] for p in (m.kpools, m.vpools)]
