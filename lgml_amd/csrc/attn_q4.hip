@@ -16,19 +16,24 @@
 // states join in order.
 //
 // Sets of items over the same blocks (a chunk's) are taken one by one, too. Unpacked once
-// for a set's eight waves in LDS, as Q8_0's are, they were slower at every size: heads of
-// 128, 32 / 8, 512 tokens after 2048 cells 110 us against 95, 4096 from none 639 against
-// 583; heads of 256, 8 / 4, 133 against 55 and 318 against 288.
+// for a set's eight waves in LDS, as Q8_0's are, they were slower at every size, in runs of
+// 12 (28) and with what this kernel was then: heads of 128, 32 / 8, 512 tokens after 2048
+// cells 110 us against 95 (90 since), 4096 from none 639 against 583 (561); heads of 256, 8 /
+// 4, 133 against 55 (50) and 318 against 288 (277).
 //
-// Bounds. One token of 64 sequences at 128 to 4096 cells, 32 / 8 heads of 128, is 45 us, the
-// merge's 5 with them: 159 MB, 3.9 TB/s in the first (34 us with the loads alone). A block
+// Bounds. One token of 64 sequences at 128 to 4096 cells, 32 / 8 heads of 128, is 46 us in
+// runs of 12 blocks and 42 in runs of 20 (968 workgroups), the merge's 5 with them: 159 MB,
+// 3.9 and 4.3 TB/s in the first kernel (34 us with the loads alone). In runs of 12, a block
 // of 64 cells is 650 vector operations a wave (288 of them the unpacking; a decode step's 4
 // rows use a quarter of the columns of the others), which take the three waves of a SIMD
 // 3.8 us, its bytes of all the waves 5.6 at the copy's rate; a workgroup of 12 blocks starts
 // with 4 us until its first bytes are there, and the 1688 workgroups of the step are 2.2
-// times what the card holds. A chunk of 512
-// tokens after 2048, 8 / 4 heads of 256, is 50 us, half of them vector operations of its
-// 2048 waves, two a SIMD.
+// times what the card holds. A chunk of 512 tokens after 2048, 8 / 4 heads of 256, is 50
+// us, half of them vector operations of its 2048 waves, two a SIMD; over 32 / 8 heads of
+// 128, in runs of 20, 83. One sequence leaves most of the card idle, and the blocks of a
+// wave go one after another: 8192 cells, 32 / 8 heads of 128, are 16 us in runs of 12 and
+// 21 in runs of 20 (56 workgroups, five blocks a wave), 8 / 4 heads of 256 40 in runs of
+// 28 (Q8_0 34 and 113, f16 20 and 55).
 #include "attnq.h"
 #include "kvq4.h"
 
@@ -328,9 +333,9 @@ __device__ __forceinline__ bool plain_lane(u32x4 sc) {
 // An item: a workgroup, a wave each part. Each wave reads its blocks from the pool into
 // registers, the next one's K and scales while one is used; q's operands are in LDS, made
 // once, and the states join there. ONCE (plans without shared sets): values are read past
-// the caches. The step of 64 sequences takes 45 us so, 49 through them (77 either way after
-// a prefix of 4000 cells that all share); a chunk, whose items read the same blocks, 52
-// and 50.
+// the caches. The step of 64 sequences, in runs of 12, takes 45 us so, 49 through them (77
+// either way after a prefix of 4000 cells that all share); a chunk, whose items read the
+// same blocks, 52 and 50.
 template <int D, bool ONCE>
 __global__ void __launch_bounds__(64 * PARTS, D == 256 ? 2 : 3)
 paged_attn_q4_kernel(const float *__restrict__ q, int H, int Hkv, float scale_log2,

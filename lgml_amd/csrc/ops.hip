@@ -236,9 +236,11 @@ __global__ void rope_table_kernel(const int32_t *__restrict__ pos, int n_rot, fl
 // rope for q and k heads, and the store: q to q_out, k and v to their pool
 // cell. With QKV_V_FROM_K a V head is the raw K head (transformer.lua:1779).
 // TYPE Q8_0 or Q4_0: the pool is quantised (kvq8.h, kvq4.h); a block of 32 values is half a wave's. 64, 512
-// and 2048 tokens of 32 / 8 heads of 128 take 6.6, 20 and 65 us, 6.3, 19.5 and 63
-// over f16 (18 and 59 of the 20 and 65 with V left out): the rows, angles and q
-// bound it, not V's single bytes.
+// and 2048 tokens of 32 / 8 heads of 128 take 6.4, 20 and 65 us over Q8_0, 6.6, 21 and 67
+// over Q4_0, 6.2, 20 and 63 over f16 (18 and 59 of Q8_0's 20 and 65 with V left out): the
+// rows, angles and q bound it, not V's single bytes. That is a quarter of the rate that
+// the rows' bytes could have: qkv_rope_axes_kernel, whose workgroups take whole tokens,
+// takes 16 us for the 2048.
 constexpr int QKV_HEADS = 8;
 template <int TYPE>
 __global__ void __launch_bounds__(64 * QKV_HEADS)

@@ -572,9 +572,11 @@ class DeviceModel:
         first, C4 7172 -> 7462 tok/s against 32 and 16; 24 / 26 / 30 and
         10 / 14 are no better); else runs of 12 (C2 decode 7263 -> 7407
         tok/s against 16; 10: 7383, 8: 7088), over Q4_0 pools of 20 (a
-        workgroup of four waves each: a decode step of 64 sequences 48 us of
-        attention a layer against 50 with 12 and 51 with 40, a chunk of 512
-        after 2048 83 against 90). The run length is fixed per model, so split
+        workgroup of four waves each: a decode step of 64 sequences 42 us of
+        attention a layer against 46 with 12 and 43 with 40, a chunk of 512
+        after 2048 83 against 90 and 75; one sequence of 8192 cells, which
+        leaves most of the card idle either way, 21 against 16 and 30, 5% of
+        its pass of the 8B shape). The run length is fixed per model, so split
         points still depend on a sequence's own length only."""
         ids = np.ascontiguousarray(ids, np.int32)
         ring_bps = self.ring_blocks_per_split or blocks_per_split
