@@ -235,8 +235,9 @@ class PoolSeqs:
 
     def compact(self, seqs):
         """The blocks in use or kept move into the lowest places: cells, references,
-        keys and the tables of seqs, which are all the sequences that hold blocks.
-        Returns how many blocks there are then: those behind them are free."""
+        keys and the tables of seqs, which are all the sequences that hold blocks
+        (plans made before name the old places: make them anew). Returns how many
+        blocks there are then: those behind them are free."""
         held = [b for b in range(self.alloc.cap) if self.alloc.in_use(b)]
         refs = {}
         for b in (b for c in seqs for b in c.blocks):
