@@ -520,11 +520,11 @@ class DeviceModel:
         cells (a multiple of 64, at least one block), for a pool whose blocks
         behind them are free (Engine.compact); the memory goes back to the
         allocator. Plans of other blocks are refused from then on; a captured
-        pass holds the tensors' addresses, and is captured anew. The pool may grow again, up to max_cells. Returns the new
-        cell count. Where memory for a shorter tensor fails, the pool has `cells`
-        cells all the same; the next call cuts what this one left long. The
-        counterpart of grow_pool; the reference's pools only grow
-        (transformer.lua:831-908)."""
+        pass holds the tensors' addresses, and is captured anew. The pool may grow
+        again, up to max_cells. Returns the new cell count. Where memory for a
+        shorter tensor fails, the pool has `cells` cells all the same; the next
+        call cuts what this one left long. The counterpart of grow_pool; the
+        reference's pools only grow (transformer.lua:831-908)."""
         cells = int(cells)
         if cells % 64 or cells <= 0:
             raise ValueError("%d cells: whole blocks of 64, at least one" % cells)
