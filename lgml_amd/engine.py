@@ -558,6 +558,9 @@ class Engine:
             self.hits += 1
             self.hit_blocks += len(blocks)
             return m + part
+        except BaseException:  # the request runs all of its tokens then
+            self.seqs.free(c)
+            raise
         finally:
             for b in blocks:  # E:drop_held
                 alloc.unref(b)

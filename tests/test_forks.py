@@ -133,3 +133,24 @@ def test_an_attached_block_whose_copy_fails_is_let_go():
     assert (seqs.alloc.used, seqs.alloc.cached) == (0, 2)
     m.fail = None
     assert eng.attach(req) == 100 and m.calls == [([1], [2], 36)]
+
+
+def test_a_request_whose_attach_fails_starts_from_nothing():
+    """Blocks shared before the failure would put its first token behind them."""
+    from lgml_amd import engine
+    m = Model(8, RuntimeError("captured"))
+    m.kv_type = None
+    seqs, c = sequence(m, 100)
+    toks = list(range(100))
+    eng = object.__new__(engine.Engine)
+    eng.model, eng.seqs, eng.ram, eng.infos, eng.hits, eng.hit_blocks = m, seqs, None, {}, 0, 0
+    eng.active, eng.n_slots, eng.free_slots, eng._submitted, eng.prefix_cache = [], 2, [0, 1], 0, True
+    req = engine.Request(toks, 1)
+    req.seq = c
+    eng.publish_tail(req, toks)
+    seqs.free(c)
+    req = engine.Request(toks + [7], 1)
+    with pytest.raises(RuntimeError):
+        eng.submit(req)
+    assert (req.fed, req.seq.n_past, req.seq.blocks, req.seq.keys) == (0, 0, [], [])
+    assert (seqs.alloc.used, seqs.alloc.cached) == (0, 2)
